@@ -358,6 +358,69 @@ int bi_rope_cache(const void* q, int64_t q_row, const void* k, int64_t k_row, co
                   int64_t Hq, int64_t Hkv, int64_t D, int64_t pos, int64_t max_len, const int64_t* strides, int dtype,
                   void* stream);
 
+/* ---- Filling a paged K/V cache ---------------------------------------------
+ * Pages and slots of a step's new tokens, in one launch. Request b holds
+ * kv_lens[b] tokens in pages block_table[b * table_stride + i] of page_size
+ * tokens (a power of two, 1 .. 2^24) and gets new_lens[b] more (0 .. T; device
+ * int32 [B] both, negative ones count as 0, lengths past max_pages * page_size
+ * as that). Its new pages come from free_pages[c ..], c = cursor[0] (clamped to
+ * [0, num_free]; null: 0) plus the pages of the requests before it, and are
+ * written into its row of block_table behind the ones it holds. A request whose
+ * pages do not fit its row (max_pages) or the free list, or with more than T new
+ * tokens, is refused: nothing of it is written and its length stays; requests
+ * behind one that the free list cannot serve get only what needs no new page.
+ * Outputs: slots [B, T] int64, block_table page * page_size + row of each new
+ * token, in the LAST new_lens[b] of the T rows, as the bottom-right aligned
+ * causal attention counts them, and -1 in the others; positions [B, T] int32,
+ * the new tokens' places in their sequences, 0 in the others; out_lens [B];
+ * out_cursor [1], behind the last page taken. out_lens and out_cursor must not
+ * be the inputs. Page numbers are taken as they are (a negative one gives slot
+ * -1). B <= 2^20, T <= 2^24, max_pages * page_size + T < 2^31.
+ * Replaces: nothing in the reference (its caches are contiguous,
+ * kernels/attention.py:87-254). */
+int bi_paged_slots(const int32_t* kv_lens, const int32_t* new_lens, int32_t* block_table, int64_t table_stride,
+                   int64_t max_pages, const int32_t* free_pages, int64_t num_free, const int32_t* cursor,
+                   int64_t* slots, int32_t* positions, int32_t* out_lens, int32_t* out_cursor, int64_t B, int64_t T,
+                   int64_t page_size, void* stream);
+
+/* Rotary embedding of queries and keys with positions of 1 to 4 axes, and the
+ * write of keys and values into the pages of a paged cache, in one launch.
+ * q [B, T, Hq, D], k / v [B, T, Hkv, D] with heads contiguous and q_row / k_row
+ * / v_row elements between tokens. cos / sin contiguous [table_rows, R] of dtype
+ * table_dtype (the operands' or BI_F32); sections (host, int64[axes]) cut the R
+ * pairs of dims (their sum, a multiple of 8, at most D / 2) into one run for
+ * each axis, and pair d of axis x is turned by row positions[x, b, t] of column
+ * d (device int32 [axes, B, T]; clamped into the table). With the halves x1, x2
+ * of a head's first 2 R dims y1 = T(x1 cos - x2 sin), y2 = T(x2 cos + x1 sin),
+ * in fp32, rounded once; the other dims are copied. q_out contiguous [B, Hq, T,
+ * D]. Key and value of token (b, t) go to row slots[b, t] % page_size of page
+ * slots[b, t] / page_size (device int64 [B, T]) of the pools, whose (page, head,
+ * row) element strides are strides[0..2] (k) and strides[3..5] (v), d
+ * contiguous; a slot outside [0, num_pages * page_size) writes nothing. Of
+ * several tokens with one slot, each 16 bytes of the row keep some one's.
+ * D % 16 == 0, 16-byte aligned rows; outputs must not overlap inputs.
+ * Replaces: nothing in the reference's kernels (its models rotate through
+ * mx.fast.rope, harness/model_sweep.py:62-108). */
+int bi_rope_paged_cache(const void* q, int64_t q_row, const void* k, int64_t k_row, const void* v, int64_t v_row,
+                        const void* cos, const void* sin, int64_t table_rows, int table_dtype,
+                        const int32_t* positions, const int64_t* sections, int64_t axes, const int64_t* slots,
+                        void* q_out, void* k_pages, void* v_pages, int64_t num_pages, int64_t page_size, int64_t B,
+                        int64_t T, int64_t Hq, int64_t Hkv, int64_t D, const int64_t* strides, int dtype, void* stream);
+
+/* ---- The norms around a block ------------------------------------------------
+ * u = x * inv(x) * w_post (post == 0: u = x), y = res + u * gate * scale,
+ * h = y * inv(y) * w_pre (pre == 0: no h), inv(z) = 1 / sqrt(ss(z) / D + eps)
+ * with ss in bi_rms_norm's order; all in fp32, y and h rounded once (h is taken
+ * from the unrounded y). w_post, w_pre [D] and gate may be null (ones). x and
+ * res rows are x_row_stride / res_row_stride >= D elements apart; row r's gate
+ * starts (r / gate_group) * gate_row_stride elements into gate (gate_group =
+ * rows: one gate for all). y and h contiguous [rows, D], not overlapping inputs.
+ * Replaces: nothing in the reference (RMSNorm alone: kernels/rmsnorm.py:19-79). */
+int bi_residual_rms_norm(const void* x, int64_t x_row_stride, const void* res, int64_t res_row_stride,
+                         const void* gate, int64_t gate_row_stride, int64_t gate_group, const void* w_post,
+                         const void* w_pre, void* y, void* h, int64_t rows, int64_t D, float eps, float scale,
+                         int post, int pre, int dtype, void* stream);
+
 /* Diagnostic, no counterpart in the reference: y[i] = the hardware base-2
  * exponential (v_exp_f32) of x[i], n >= 0 floats, device pointers, on the
  * stream. It is the instruction the matrix-core attention kernels compute

@@ -20,7 +20,11 @@ from .kernels import (
     batch_invariant_layer_norm,
     batch_invariant_matmul,
     batch_invariant_quantized_matmul,
+    batch_invariant_residual_rms_norm,
     batch_invariant_rms_norm,
+    PagedSlots,
+    paged_slots,
+    rope_paged_cache,
 )
 from .kernels.quantized import (quantize, dequantize, pack, unpack, cache_dequantized, drop_dequantized,
                                 cache_packed, drop_packed)
@@ -36,11 +40,15 @@ __all__ = [
     "batch_invariant_bmm",
     "batch_invariant_rms_norm",
     "batch_invariant_layer_norm",
+    "batch_invariant_residual_rms_norm",
     "batch_invariant_quantized_matmul",
     "batch_invariant_decode_attention",
     "batch_invariant_prefill_attention",
     "batch_invariant_attention",
     "batch_invariant_paged_attention",
+    "PagedSlots",
+    "paged_slots",
+    "rope_paged_cache",
     "quantize",
     "dequantize",
     "cache_dequantized",

@@ -10,6 +10,7 @@ as the reference does (mlx_batch_invariant/ops.py:36-39).
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 import threading
@@ -78,6 +79,15 @@ _SIGNATURES = {
     "bi_rope_cache": (ctypes.c_int, [_vp, _c_i64, _vp, _c_i64, _vp, _c_i64, _vp, _vp, _vp, _vp, _vp, _c_i64, _c_i64,
                                      _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, ctypes.POINTER(_c_i64), ctypes.c_int,
                                      _vp]),
+    "bi_paged_slots": (ctypes.c_int, [_vp, _vp, _vp, _c_i64, _c_i64, _vp, _c_i64, _vp, _vp, _vp, _vp, _vp, _c_i64,
+                                      _c_i64, _c_i64, _vp]),
+    "bi_rope_paged_cache": (ctypes.c_int, [_vp, _c_i64, _vp, _c_i64, _vp, _c_i64, _vp, _vp, _c_i64, ctypes.c_int,
+                                           _vp, ctypes.POINTER(_c_i64), _c_i64, _vp, _vp, _vp, _vp, _c_i64, _c_i64,
+                                           _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, ctypes.POINTER(_c_i64),
+                                           ctypes.c_int, _vp]),
+    "bi_residual_rms_norm": (ctypes.c_int, [_vp, _c_i64, _vp, _c_i64, _vp, _c_i64, _c_i64, _vp, _vp, _vp, _vp,
+                                            _c_i64, _c_i64, ctypes.c_float, ctypes.c_float, ctypes.c_int,
+                                            ctypes.c_int, ctypes.c_int, _vp]),
     "bi_exp2_f32": (ctypes.c_int, [_vp, _vp, _c_i64, _vp]),
     "bi_stream_read": (ctypes.c_int, [_vp, _c_i64, _vp, ctypes.c_uint32, _vp]),
     "bi_quantized_dequantize": (ctypes.c_int, [_vp, _vp, _vp, _vp, _c_i64, _c_i64, ctypes.c_int, ctypes.c_int,
@@ -181,6 +191,44 @@ def stream_of(t: torch.Tensor) -> int:
     if _raw_stream is not None:
         return _raw_stream(t.get_device())
     return torch.cuda.current_stream(t.device).cuda_stream
+
+
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
+_no_switch = contextlib.nullcontext()
+
+
+def on_device(t: torch.Tensor):
+    """A context in which ``t``'s device is the current one (a launch takes the
+    current device's code): nothing to do where it is already."""
+    return _no_switch if t.get_device() == _current_device() else torch.cuda.device(t.device)
+
+
+def one_device(what: str, *tensors) -> None:
+    """Every tensor (None aside) on the GPU, and on the first one's device."""
+    require_gpu(what, *tensors)
+    dev = tensors[0].get_device()
+    for t in tensors[1:]:
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"{what}: tensors on {tensors[0].device} and {t.device}")
+
+
+def in_place(what: str, *tensors) -> None:
+    """Refuse what torch's own in-place operations refuse: rows that share
+    memory, an inference tensor outside inference mode, a leaf that needs a
+    gradient."""
+    for t in tensors:
+        if any(s <= 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
+            raise ValueError(f"{what}: written tensor with rows that share memory (shape {tuple(t.shape)}, "
+                             f"strides {t.stride()})")
+        if t.is_inference() and not torch.is_inference_mode_enabled():
+            raise ValueError(f"{what}: an inference tensor cannot be written outside inference mode")
+        if t.requires_grad and torch.is_grad_enabled():
+            raise ValueError(f"{what}: a tensor that needs a gradient cannot be written in place")
+
+
+def written(*tensors) -> None:
+    """Count the tensors as changed in place (their version counters)."""
+    torch.autograd.graph.increment_version([t for t in tensors if not t.is_inference()])
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

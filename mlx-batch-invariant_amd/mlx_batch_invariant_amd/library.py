@@ -19,7 +19,13 @@ Operators (each the same computation, and bits, as the Python function named):
 * ``attention(q, k, v, scale, causal, kv_lens)``: decode for one query token,
   prefill otherwise (``mask="causal"`` is bottom-right aligned);
 * ``paged_attention(q, k_pages, v_pages, block_table, kv_lens, scale, causal)``:
-  the same over a paged K/V pool (``batch_invariant_paged_attention``).
+  the same over a paged K/V pool (``batch_invariant_paged_attention``);
+* ``residual_rms_norm(x, residual, post_weight, pre_weight, eps, gate, scale)``:
+  both norms (``batch_invariant_residual_rms_norm``); returns (y, h);
+* ``paged_slots(kv_lens, new_lens, block_table!, free_pages, cursor, page_size,
+  max_new)``: (slots, positions, kv_lens, cursor), the table changed in place;
+* ``rope_paged_cache(q, k, v, cos, sin, positions, slots, k_pages!, v_pages!,
+  sections)``: the rotated queries, the pools changed in place.
 
 The ops have no autograd formula (inference kernels, as in the reference).
 """
@@ -100,3 +106,40 @@ def paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_table: Te
 @paged_attention.register_fake
 def _paged_attention_fake(q, k_pages, v_pages, block_table, kv_lens, scale, causal):
     return q.new_empty((*q.shape[:-1], v_pages.shape[-1]))
+
+
+@torch.library.custom_op(f"{NAMESPACE}::residual_rms_norm", mutates_args=())
+def residual_rms_norm(x: Tensor, residual: Tensor, post_weight: Optional[Tensor], pre_weight: Optional[Tensor],
+                      eps: float, gate: Optional[Tensor], scale: float) -> tuple[Tensor, Tensor]:
+    return _k.batch_invariant_residual_rms_norm(x, residual, post_weight, pre_weight, eps, gate=gate, scale=scale)
+
+
+@residual_rms_norm.register_fake
+def _residual_rms_norm_fake(x, residual, post_weight, pre_weight, eps, gate, scale):
+    return x.new_empty(x.shape), x.new_empty(x.shape)
+
+
+@torch.library.custom_op(f"{NAMESPACE}::paged_slots", mutates_args=("block_table",))
+def paged_slots(kv_lens: Tensor, new_lens: Tensor, block_table: Tensor, free_pages: Tensor,
+                cursor: Optional[Tensor], page_size: int, max_new: int) -> tuple[Tensor, Tensor, Tensor, Tensor]:
+    p = _k.paged_slots(kv_lens, new_lens, block_table, free_pages, page_size=page_size, max_new=max_new, cursor=cursor)
+    return p.slots, p.positions, p.kv_lens.clone(), p.cursor.clone()       # (outputs that share no memory)
+
+
+@paged_slots.register_fake
+def _paged_slots_fake(kv_lens, new_lens, block_table, free_pages, cursor, page_size, max_new):
+    new = lambda dt, *shape: block_table.new_empty(shape, dtype=dt)
+    B = block_table.shape[0]
+    return new(torch.int64, B, max_new), new(torch.int32, B, max_new), new(torch.int32, B), new(torch.int32, 1)
+
+
+@torch.library.custom_op(f"{NAMESPACE}::rope_paged_cache", mutates_args=("k_pages", "v_pages"))
+def rope_paged_cache(q: Tensor, k: Tensor, v: Tensor, cos: Tensor, sin: Tensor, positions: Tensor, slots: Tensor,
+                     k_pages: Tensor, v_pages: Tensor, sections: Optional[list[int]]) -> Tensor:
+    return _k.rope_paged_cache(q, k, v, cos, sin, positions, slots, k_pages, v_pages, sections=sections)
+
+
+@rope_paged_cache.register_fake
+def _rope_paged_cache_fake(q, k, v, cos, sin, positions, slots, k_pages, v_pages, sections):
+    B, T, H, D = q.shape
+    return q.new_empty((B, H, T, D))
