@@ -316,6 +316,38 @@ int bi_attn_prefill_paged(const void* q, const void* k_pages, const void* v_page
                           int64_t Tq, int64_t L, int64_t D, const int64_t* strides, int causal,
                           float scale, int dtype, void* stream);
 
+/* ---- Attention with changed scores and masks ---------------------------------
+ * bi_attn_decode (Tq == 1) and bi_attn_prefill, contiguous (block_table null) or
+ * paged, with what bi_score_mod asks for; fields of 0 / null ask for nothing.
+ * Query t of sequence b stands at position p = len_b - Tq + t; its score with
+ * key j is
+ *   s = softcap tanh(q.k scale / softcap) - slopes[h] |p - j|
+ * and it sees the keys j < len_b with, causal: j <= p or j < prefix_lens[b], and
+ * with doc_ids: doc_ids[b][j] == doc_ids[b][p]. Queries with p < 0 see nothing
+ * (causal, or with doc_ids); a query that sees no key, or none of a score above
+ * -inf, gets zeros. What hidden keys' K and V rows hold (infinities, NaN) does
+ * not matter. slopes fp32 [Hq], doc_ids int32 rows doc_stride >= L apart, prefix_lens
+ * int32 [B]: device pointers. softcap >= 0; a prefix needs causal (decode sees
+ * every key of its sequence); slopes need L <= 2^24. strides[0..8] as for
+ * bi_attn_prefill (strides[2] unused at Tq == 1). Same order of operations as
+ * bi_attn_decode / bi_attn_prefill, so the same invariances hold, and where no
+ * score or mask is changed (slopes 0, one document, no prefix) the same bits.
+ * Workspace: bi_attn_scored_workspace_bytes; calls that overlap must not share it.
+ * Replaces: nothing in the reference (its masks are none and causal,
+ * kernels/attention.py:299-310). */
+typedef struct bi_score_mod {
+  float softcap;
+  const float* slopes;
+  const int32_t* doc_ids;
+  int64_t doc_stride;
+  const int32_t* prefix_lens;
+} bi_score_mod;
+size_t bi_attn_scored_workspace_bytes(int64_t B, int64_t Hq, int64_t Tq, int64_t L, int64_t D, int has_docs);
+int bi_attn_scored(const void* q, const void* k, const void* v, const int32_t* block_table, int64_t table_stride,
+                   int64_t page_size, int64_t num_pages, const int32_t* kv_lens, void* out, int64_t B, int64_t Hq,
+                   int64_t Hkv, int64_t Tq, int64_t L, int64_t D, const int64_t* strides, int causal, float scale,
+                   const bi_score_mod* score_mod, int dtype, void* ws, size_t ws_bytes, void* stream);
+
 /* ---- Attention in the reference's per-key order ----------------------------
  * The arguments, validation and invariance properties of bi_attn_decode /
  * bi_attn_prefill plus split_size, in the reference kernels' own order of

@@ -136,7 +136,8 @@ int check_pages(const char* what, const int32_t* table, int64_t table_stride, in
 int decode_impl(const char* what, const void* q, const void* k, const void* v, const int32_t* kv_lens, void* out,
                 int64_t B, int64_t Hq, int64_t Hkv, int64_t L, int64_t D, const int64_t* strides, float scale,
                 int dtype, void* ws, size_t ws_bytes, void* stream, const int32_t* table, int64_t table_stride,
-                int page_shift, int64_t num_pages, bool per_key = false, int64_t split = bi::kSplit) {
+                int page_shift, int64_t num_pages, bool per_key = false, int64_t split = bi::kSplit,
+                const bi::ScoreMod* mod = nullptr) {
   using namespace bi_host;
   if (per_key && (split <= 0 || split > kMaxSplit))
     return fail(BI_E_INVALID_ARG, "%s: split_size %lld must be in [1, 2^20]", what, (long long)split);
@@ -160,7 +161,7 @@ int decode_impl(const char* what, const void* q, const void* k, const void* v, c
   if (!table && !per_key && strides[7] * (int64_t)es >= ((int64_t)1 << 23))
     return fail(BI_E_UNSUPPORTED, "%s: V position stride (%lld elements) must stay below 2^23 bytes", what,
                 (long long)strides[7]);
-  bi::DecodeArgs a;
+  bi::ModDecodeArgs a;
   a.q = q; a.k = k; a.v = v; a.kv_lens = kv_lens; a.out = out;
   a.table = table; a.table_stride = table_stride; a.page_shift = page_shift; a.num_pages = (int)num_pages;
   a.B = (int)B; a.Hq = (int)Hq; a.Hkv = (int)Hkv; a.L = (int)L;
@@ -184,6 +185,14 @@ int decode_impl(const char* what, const void* q, const void* k, const void* v, c
       (per_key && bh / a.GU > ((int64_t)1 << 27)))  // per-key: 32 threads per unit, < 2^32 threads
     return fail(BI_E_UNSUPPORTED, "%s: grid too large", what);
   hipStream_t st = static_cast<hipStream_t>(stream);
+  if (mod) {
+    a.mod = *mod;
+    switch (dtype) {
+      case BI_BF16: return bi::with_head_dim((int)D, [&](auto dd) { return bi::launch_decode_mod<bi::bf16, dd.value>(a, st); });
+      case BI_F16: return bi::with_head_dim((int)D, [&](auto dd) { return bi::launch_decode_mod<bi::f16, dd.value>(a, st); });
+      default: return bi::with_head_dim((int)D, [&](auto dd) { return bi::launch_decode_mod<float, dd.value>(a, st); });
+    }
+  }
 #define BI_DEC(TY)                                                                                          \
   if (per_key)                                                                                              \
     return bi::with_head_dim_per_key((int)D, [&](auto dd) { return bi::launch_decode_perkey<TY, dd.value>(a, st); }); \
@@ -197,11 +206,24 @@ int decode_impl(const char* what, const void* q, const void* k, const void* v, c
 #undef BI_DEC
 }
 
+// The instantiation with the score terms of a.mod.
+template <typename T>
+int launch_prefill_scored(int D, bi::ModPrefillArgs& a, hipStream_t st) {
+  const bool cap = a.mod.cap_log2 != 0.0f, bias = a.mod.slopes != nullptr;
+  return bi::with_head_dim(D, [&](auto dd) {
+    constexpr int kD = dd.value;
+    if (cap && bias) return bi::launch_prefill_mod<T, kD, (bi::kModAny | bi::kModCap | bi::kModBias)>(a, st);
+    if (cap) return bi::launch_prefill_mod<T, kD, (bi::kModAny | bi::kModCap)>(a, st);
+    if (bias) return bi::launch_prefill_mod<T, kD, (bi::kModAny | bi::kModBias)>(a, st);
+    return bi::launch_prefill_mod<T, kD, bi::kModAny>(a, st);
+  });
+}
+
 int prefill_impl(const char* what, const void* q, const void* k, const void* v, const int32_t* kv_lens,
                  void* out, int64_t B, int64_t Hq, int64_t Hkv, int64_t Tq, int64_t L, int64_t D,
                  const int64_t* strides, int causal, float scale, int dtype, void* stream, const int32_t* table,
                  int64_t table_stride, int page_shift, int64_t num_pages, bool per_key = false,
-                 int64_t split = bi::kSplit) {
+                 int64_t split = bi::kSplit, const bi::ScoreMod* mod = nullptr) {
   using namespace bi_host;
   if (per_key && (split <= 0 || split > kMaxSplit))
     return fail(BI_E_INVALID_ARG, "%s: split_size %lld must be in [1, 2^20]", what, (long long)split);
@@ -231,7 +253,7 @@ int prefill_impl(const char* what, const void* q, const void* k, const void* v, 
       (!per_key && wgs * Hkv * B > 0x7fffffffLL - 8) ||
       (per_key && B * Hq * ((Tq + bi::pk_prefill_qb(D) - 1) / bi::pk_prefill_qb(D)) > ((int64_t)1 << 27)))
     return fail(BI_E_UNSUPPORTED, "%s: grid too large", what);
-  bi::PrefillArgs a;
+  bi::ModPrefillArgs a;
   a.q = q; a.k = k; a.v = v; a.kv_lens = kv_lens; a.out = out;
   a.table = table; a.table_stride = table_stride; a.page_shift = page_shift; a.num_pages = (int)num_pages;
   a.B = (int)B; a.Hq = (int)Hq; a.Hkv = (int)Hkv; a.Tq = (int)Tq; a.L = (int)L;
@@ -243,6 +265,14 @@ int prefill_impl(const char* what, const void* q, const void* k, const void* v, 
   a.scale = scale;
   a.split = (int)split;
   hipStream_t st = static_cast<hipStream_t>(stream);
+  if (mod) {
+    a.mod = *mod;
+    switch (dtype) {
+      case BI_BF16: return launch_prefill_scored<bi::bf16>((int)D, a, st);
+      case BI_F16: return launch_prefill_scored<bi::f16>((int)D, a, st);
+      default: return launch_prefill_scored<float>((int)D, a, st);
+    }
+  }
 #define BI_PRE(TY)                                                                                            \
   if (per_key)                                                                                                \
     return bi::with_head_dim_per_key((int)D, [&](auto dd) { return bi::launch_prefill_perkey<TY, dd.value>(a, st); }); \
@@ -328,6 +358,80 @@ extern "C" int bi_attn_prefill_per_key(const void* q, const void* k, const void*
   if (rc) return rc;
   return prefill_impl("bi_attn_prefill_per_key", q, k, v, kv_lens, out, B, Hq, Hkv, Tq, L, D, strides, causal,
                       scale, dtype, stream, nullptr, 0, 0, 0, true, split_size);
+}
+
+// ---------------------------------------------------------------------------
+// Attention with ScoreMod: capped scores, a distance bias, a document mask, a
+// prefix mask (bi_attn_mod.h), over a contiguous or a paged cache.
+// ---------------------------------------------------------------------------
+namespace {
+
+int check_score_mod(const char* what, const bi_score_mod* m, int64_t L, float scale, int dtype, bool prefill,
+                    int causal, bi::ScoreMod* out) {
+  using namespace bi_host;
+  if (dtype != BI_BF16 && dtype != BI_F16 && dtype != BI_F32)
+    return fail(BI_E_UNSUPPORTED, "%s: unknown dtype %d", what, dtype);
+  if (!m) return fail(BI_E_INVALID_ARG, "%s: null bi_score_mod", what);
+  if (!(m->softcap >= 0.0f) || m->softcap > 3e38f)
+    return fail(BI_E_INVALID_ARG, "%s: softcap %g (a positive number, or 0 for none)", what, (double)m->softcap);
+  if (m->doc_ids && m->doc_stride < L)
+    return fail(BI_E_INVALID_ARG, "%s: document rows of %lld for %lld keys", what, (long long)m->doc_stride,
+                (long long)L);
+  if (m->prefix_lens && prefill && !causal)
+    return fail(BI_E_INVALID_ARG, "%s: a prefix without the causal mask", what);
+  if (m->slopes && L > ((int64_t)1 << 24))  // distances are exact in fp32 up to there
+    return fail(BI_E_UNSUPPORTED, "%s: a distance bias over %lld keys (at most 2^24)", what, (long long)L);
+  out->cap_log2 = m->softcap * bi::kLog2e;
+  out->cap_in = m->softcap == 0.0f ? 0.0f : (dtype == BI_F32 ? 1.0f : 2.0f * bi::kLog2e) * (scale / m->softcap);
+  out->slopes = m->slopes;
+  out->docs = m->doc_ids;
+  out->docs_sb = m->doc_stride;
+  out->ranges = nullptr;
+  out->prefix = m->prefix_lens;
+  return BI_OK;
+}
+
+}  // namespace
+
+extern "C" size_t bi_attn_scored_workspace_bytes(int64_t B, int64_t Hq, int64_t Tq, int64_t L, int64_t D,
+                                                 int has_docs) {
+  if (B <= 0 || Hq <= 0 || Tq <= 0 || L <= 0 || D <= 0) return 0;
+  if (Tq == 1) return decode_ws_bytes(B, Hq, L, D, bi::kSplit);
+  return has_docs ? (size_t)(B * ((L + bi::kSplit - 1) / bi::kSplit)) * sizeof(int2) : 0;
+}
+
+extern "C" int bi_attn_scored(const void* q, const void* k, const void* v, const int32_t* block_table,
+                              int64_t table_stride, int64_t page_size, int64_t num_pages, const int32_t* kv_lens,
+                              void* out, int64_t B, int64_t Hq, int64_t Hkv, int64_t Tq, int64_t L, int64_t D,
+                              const int64_t* strides, int causal, float scale, const bi_score_mod* score_mod,
+                              int dtype, void* ws, size_t ws_bytes, void* stream) {
+  const char* what = "bi_attn_scored";
+  int rc = check_attn_shape(what, B, Hq, Hkv, L, D);
+  if (rc) return rc;
+  if (Tq <= 0) return bi_host::fail(BI_E_INVALID_ARG, "%s: Tq=%lld", what, (long long)Tq);
+  bi::ScoreMod mod;
+  if ((rc = check_score_mod(what, score_mod, L, scale, dtype, Tq > 1, causal, &mod))) return rc;
+  int shift = 0;
+  if (B > 0 && block_table && (rc = check_pages(what, block_table, table_stride, page_size, num_pages, L, &shift)))
+    return rc;
+  if (!strides) return bi_host::fail(BI_E_INVALID_ARG, "%s: null pointer argument", what);
+  if (Tq == 1) {
+    const int64_t st8[8] = {strides[0], strides[1], strides[3], strides[4], strides[5],
+                            strides[6], strides[7], strides[8]};
+    return decode_impl(what, q, k, v, kv_lens, out, B, Hq, Hkv, L, D, st8, scale, dtype, ws, ws_bytes, stream,
+                       block_table, table_stride, shift, num_pages, false, bi::kSplit, &mod);
+  }
+  if (B > 0 && mod.docs) {
+    const size_t need = bi_attn_scored_workspace_bytes(B, Hq, Tq, L, D, 1);
+    if (!ws || ws_bytes < need || !bi_host::aligned16(ws))
+      return bi_host::fail(BI_E_WORKSPACE, "%s: 16-byte aligned workspace of %zu bytes required, got %zu", what, need,
+                           ws ? ws_bytes : (size_t)0);
+    if (B * ((L + bi::kSplit - 1) / bi::kSplit) > 0x7fffffffLL)
+      return bi_host::fail(BI_E_UNSUPPORTED, "%s: grid too large", what);
+    mod.ranges = static_cast<const int2*>(ws);
+  }
+  return prefill_impl(what, q, k, v, kv_lens, out, B, Hq, Hkv, Tq, L, D, strides, causal, scale, dtype, stream,
+                      block_table, table_stride, shift, num_pages, false, bi::kSplit, &mod);
 }
 
 // ---------------------------------------------------------------------------

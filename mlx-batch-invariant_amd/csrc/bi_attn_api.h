@@ -33,6 +33,11 @@ template <typename T, int D>
 int launch_decode(DecodeArgs& a, hipStream_t st);
 template <typename T, int D>
 int launch_prefill(PrefillArgs& a, hipStream_t st);
+// The same with ScoreMod (bi_attn_mod_{bf16,f16,f32}.hip).
+template <typename T, int D>
+int launch_decode_mod(ModDecodeArgs& a, hipStream_t st);
+template <typename T, int D, int MOD>
+int launch_prefill_mod(ModPrefillArgs& a, hipStream_t st);
 // The reference's per-key order on the vector ALUs (bi_attn_perkey.h).
 template <typename T, int D>
 int launch_decode_perkey(DecodeArgs& a, hipStream_t st);

@@ -84,6 +84,64 @@ struct PrefillArgs {
   int num_pages;
 };
 
+// What changes a score before the softmax, and which keys a query sees, beyond
+// the plain kernels: s = cap tanh(q.k scale / cap) - slope_h |pos_q - key|, a
+// document mask and a prefix that every query sees. Positions are bottom-right
+// aligned: query t of Tq stands at pos_q = len - Tq + t.
+struct ScoreMod {
+  float cap_log2;         // cap log2(e); 0: scores are not capped
+  float cap_in;           // scale / cap (fp32 scores), 2 log2(e) scale / cap (16-bit)
+  const float* slopes;    // [Hq]; null: no distance bias
+  const int32_t* docs;    // document of key j of sequence b: docs[b docs_sb + j]; null: one document
+  int64_t docs_sb;
+  const int2* ranges;     // smallest and largest document of each split, [B, nsplit] (prefill with docs)
+  const int32_t* prefix;  // keys below prefix[b] are seen by every query (causal prefill); null: none
+};
+struct ModDecodeArgs : DecodeArgs { ScoreMod mod; };
+struct ModPrefillArgs : PrefillArgs { ScoreMod mod; };
+
+// Score variants of a kernel instantiation: 0 the plain ones; kModAny reads
+// ScoreMod's masks, and the other bits its score terms.
+enum { kModAny = 1, kModCap = 2, kModBias = 4 };
+template <int MOD> using DecodeArgsOf = std::conditional_t<MOD != 0, ModDecodeArgs, DecodeArgs>;
+
+// cap log2(e) tanh(dot scale / cap). For 16-bit operands 1 - 2 / (exp(2 z) + 1)
+// by the hardware exp2 and reciprocal (44 cycles a wave): off by at most about 3
+// 2^-24 cap log2(e) in absolute terms, 2^-16 of a weight at cap = 50, where
+// their own rounding is 2^-9 (bf16) or 2^-11 (f16) of the output. For fp32
+// operands the same above |z| = 0.6 and below it, where the difference cancels,
+// z P(z^2) with P fitted to tanh(z) / z at Chebyshev points (1.7 2^-24).
+template <typename T>
+__device__ __forceinline__ float cap_score(float dot, const ScoreMod& m) {
+  if constexpr (sizeof(T) == 2) {
+    const float x = __builtin_amdgcn_exp2f(dot * m.cap_in);
+    return __builtin_fmaf(-2.0f * m.cap_log2, __builtin_amdgcn_rcpf(x + 1.0f), m.cap_log2);
+  } else {
+    const float z = dot * m.cap_in, u = z * z;
+    float p = -0.00584964407607913f;
+    p = __builtin_fmaf(p, u, 0.02075134962797165f);
+    p = __builtin_fmaf(p, u, -0.05376798287034035f);
+    p = __builtin_fmaf(p, u, 0.1333167999982834f);
+    p = __builtin_fmaf(p, u, -0.3333328366279602f);
+    const float small = z * __builtin_fmaf(p, u, 1.0f);
+    const float x = __builtin_amdgcn_exp2f(2.0f * kLog2e * fabsf(z));
+    const float large = __builtin_copysignf(__builtin_fmaf(-2.0f, __builtin_amdgcn_rcpf(x + 1.0f), 1.0f), z);
+    return (fabsf(z) < 0.6f ? small : large) * m.cap_log2;
+  }
+}
+
+// A visible key's score in log2 units from its dot product: `slope2` the head's
+// slope times log2(e), `far` the distance |pos_q - key| (exact below 2^24). With
+// no cap and slope 0 these are the plain kernels' bits.
+template <typename T, int MOD, class Args>
+__device__ __forceinline__ float mod_score(float dot, const Args& a, float slope2, float far) {
+  float y;
+  if constexpr ((MOD & kModCap) != 0) y = cap_score<T>(dot, a.mod);
+  else y = dot * a.scale_log2;
+  if constexpr ((MOD & kModBias) != 0) y = __builtin_fmaf(-slope2, fabsf(far), y);
+  return y;
+}
+
 // Element offset of key `pos` of (sequence b, kv head hk) in a K or V cache
 // with strides (sb, sh, sl). Contiguous (a.table null): b sb + hk sh + pos sl.
 // Paged: the cache is a pool of pages of 2^page_shift keys, sb the page

@@ -173,8 +173,12 @@ constexpr int decode_v_slices() {
   return kSplit * D * (int)sizeof(T) <= (128 << 10) ? 1 : 2;
 }
 
-template <typename T, int D, int GU, bool DYN, int MODE>
-__global__ __launch_bounds__(256) void attn_decode_mfma(DecodeArgs a) {
+// MOD (kModAny, ScoreMod): the score terms are chosen at run time, since decode
+// waits for memory. A document mask hides a key from every head of the item, so
+// its V row is cleared in LDS and its weight 0 meets no infinity or NaN; a split
+// without a key of the query's document writes an empty partial (l = 0).
+template <typename T, int D, int GU, bool DYN, int MODE, int MOD = 0>
+__global__ __launch_bounds__(256) void attn_decode_mfma(DecodeArgsOf<MOD> a) {
   constexpr bool ROWPAGED = MODE == kKvRowPaged;
   typedef typename Frag<T>::type F;
   constexpr int NVP = decode_v_slices<T, D>();
@@ -246,6 +250,31 @@ __global__ __launch_bounds__(256) void attn_decode_mfma(DecodeArgs a) {
   const int G = a.Hq / a.Hkv;
   const int h0 = hk * G + chunk * GU;
   const int r = lane % 16, qq = lane / 16;
+  unsigned seen = ~0u;                                  // MOD: bit 4 t + i: the document mask leaves that key
+  float slope2 = 0.0f;
+  bool hidden = false;                                  // MOD: key tid of the split is another document's
+  if constexpr (MOD != 0) {
+    if (a.mod.docs) {
+      const int32_t* docs = a.mod.docs + (int64_t)b * a.mod.docs_sb;
+      const int mine = docs[len - 1];
+      hidden = tid >= n_act || docs[j0 + min(tid, n_act - 1)] != mine;
+      if (!__syncthreads_or(!hidden)) {
+        const int64_t po = ((int64_t)b * a.Hq + h0) * a.nsplit + split;
+        if (tid < GU) {
+          a.pm[po + (int64_t)tid * a.nsplit] = -INFINITY;
+          a.pl[po + (int64_t)tid * a.nsplit] = 0.0f;
+        }
+        continue;
+      }
+      seen = 0;
+#pragma unroll
+      for (int t = 0; t < KT; ++t)
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          seen |= (docs[j0 + min(64 * wave + 16 * t + 4 * qq + i, n_act - 1)] == mine ? 1u : 0u) << (4 * t + i);
+    }
+    if (a.mod.slopes) slope2 = a.mod.slopes[h0 + (r < GU ? r : 0)] * kLog2e;
+  }
 
   const T* qb = static_cast<const T*>(a.q) + (int64_t)b * a.q_sb;
   const T* kbase = static_cast<const T*>(a.k);
@@ -347,7 +376,14 @@ __global__ __launch_bounds__(256) void attn_decode_mfma(DecodeArgs a) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int key = 64 * wave + 16 * t + 4 * qq + i;
-      s[t][i] = key < n_act ? acc[i] * a.scale_log2 : -INFINITY;
+      if constexpr (MOD != 0) {
+        const float far = (float)(len - 1 - j0 - key);
+        const float y = a.mod.cap_log2 != 0.0f ? mod_score<T, MOD | kModCap | kModBias>(acc[i], a, slope2, far)
+                                               : mod_score<T, MOD | kModBias>(acc[i], a, slope2, far);
+        s[t][i] = key < n_act && (seen >> (4 * t + i) & 1u) ? y : -INFINITY;
+      } else {
+        s[t][i] = key < n_act ? acc[i] * a.scale_log2 : -INFINITY;
+      }
       mloc = fmaxf(mloc, s[t][i]);
     }
   }
@@ -362,7 +398,12 @@ __global__ __launch_bounds__(256) void attn_decode_mfma(DecodeArgs a) {
       const int key0 = 64 * wave + 16 * t + 4 * qq;
       f32x4 p;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) p[i] = split_weight(s[t][i], m, key0 + i < n_act);
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (MOD != 0)                         // (all visible scores -inf: weights 0, as in prefill)
+          p[i] = split_weight(s[t][i], m == -INFINITY ? 0.0f : m, key0 + i < n_act && (seen >> (4 * t + i) & 1u));
+        else
+          p[i] = split_weight(s[t][i], m, key0 + i < n_act);
+      }
       *reinterpret_cast<f32x4*>(&Ps[r][key0]) = p;
     }
   }
@@ -380,6 +421,17 @@ __global__ __launch_bounds__(256) void attn_decode_mfma(DecodeArgs a) {
       vdim0 = vp * DV;
       copy_v();
       stage_barrier<0>();
+    }
+    if constexpr (MOD != 0) {
+      // (copies by row repeat the last key's row past the end; the others leave zeros)
+      if (a.mod.docs || (!kVFixed && !TILED && n_act < kSplit)) {
+        if (hidden || tid >= n_act) {
+#pragma unroll
+          for (int c = 0; c < KV::kCPR; ++c)
+            *reinterpret_cast<u32x4*>(Vs + tid * KV::kRowBytes + 16 * c) = u32x4{0u, 0u, 0u, 0u};
+        }
+        __syncthreads();
+      }
     }
     f32x4 acc[(NDTV + 3) / 4];
 #pragma unroll

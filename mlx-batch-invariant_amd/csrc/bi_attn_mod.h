@@ -1,0 +1,503 @@
+// bi_attn_mod.h — prefill attention whose scores are capped by a tanh or get a
+// distance bias, under a document mask or a prefix mask (ScoreMod,
+// bi_attn_common.h). Layouts, tiles and the order of every sum are those of
+// attn_prefill_mfma (bi_attn_mfma.h): with nothing to change a score or a mask
+// the results are its bits, and a token's are those of the decode kernel. It is
+// a text of its own so that the plain kernel's registers stay as they are.
+//
+//   scores     s = cap tanh(dot scale / cap) - slope |pos_q - key| in log2 units
+//              (mod_score). Compiled in, since a branch at every score would
+//              stop the pipelined body's MFMAs.
+//   prefix     a row's key limit is max(pos_q + 1, prefix): limits still grow
+//              with the token, so nothing else changes.
+//   documents  the split's document numbers come to LDS with its first K chunk;
+//              splits whose range of numbers misses the workgroup's are skipped
+//              (64 of them tested by one ballot), and one with a single number,
+//              the workgroup's own, runs unmasked. Any numbers are right; sorted
+//              ones (documents packed one after another) skip the most.
+//   masked V   a hidden key's weight 0 times an infinity or NaN in its V row
+//              would be NaN. Such rows are as good as never there, so the kernel
+//              looks at its sums instead: if one is not finite, the workgroup
+//              runs again with every split masked, clears such elements in LDS
+//              and notes in `poison` for which rows and dims one was seen (1: inf,
+//              2: -inf, 4: NaN); those get it back at the end.
+#pragma once
+
+#include "bi_attn_mfma.h"
+
+namespace bi {
+
+// Keys per ring chunk: as in the plain kernel's forms without FEW.
+template <typename T, int D, int MODE>
+constexpr int mod_chunk() {
+  return prefill_chunk<T, D, MODE, false>();
+}
+// Workgroups per CU the registers are held to (see prefill_min_blocks).
+template <typename T, int D, int MODE>
+constexpr int mod_min_blocks() {
+  return sizeof(T) != 2 || D > 128 || MODE == kKvRowPaged ? 1 : 2;
+}
+
+// A wave-uniform pointer held in scalar registers, whatever the compiler can prove.
+template <typename P>
+__device__ __forceinline__ const P* uniform_ptr(const P* p) {
+  const uint64_t u = reinterpret_cast<uint64_t>(p);
+  const uint64_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)u);
+  const uint64_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(u >> 32));
+  return reinterpret_cast<const P*>(hi << 32 | lo);
+}
+
+template <typename T, int D, int MODE, int MOD>
+__global__ __launch_bounds__(256, (mod_min_blocks<T, D, MODE>())) void attn_prefill_mod(ModPrefillArgs a) {
+  constexpr bool ROWPAGED = MODE == kKvRowPaged, TILED = MODE == kKvTilePaged;
+  constexpr bool PIPE = sizeof(T) == 2 && !ROWPAGED;
+  constexpr int CH = mod_chunk<T, D, MODE>();
+  typedef typename Frag<T>::type F;
+  typedef KVTile<T, D> KV;
+  constexpr int KC = kSplit / CH;                       // chunks per split (of K, then of V)
+  constexpr int TPC = CH / 16;                          // 16-key score tiles per chunk
+  constexpr int CHB = CH * KV::kRowBytes;               // bytes per chunk
+  constexpr int CPW = KV::copies(CH) / 4;               // copy instructions per wave per chunk
+  constexpr int NDT = D / 16, KS = D / 32;
+  static_assert(CPW >= 1 && (CH == 64 || (CH == 128 && MODE == kKvContig)), "attn_prefill_mod: chunk size");
+  __shared__ __attribute__((aligned(1024))) char ring[2 * CHB];
+  __shared__ __attribute__((aligned(16))) int split_docs[kSplit];
+  __shared__ int doc_range[2][4];
+  __shared__ uint32_t poison[16 * D];                   // a byte for each of 64 rows and D dims
+
+  const int tid = threadIdx.x;
+  const int lane = tid % kWave;
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int r = lane % 16, qq = lane / 16;
+  const int G = a.Hq / a.Hkv;
+  const int npairs = a.Tq * G;
+  // Work items and their order over the XCDs as in the plain kernel.
+  const int wgs = (npairs + 63) / 64;
+  const int64_t items = (int64_t)wgs * a.Hkv * a.B;
+  const int64_t per_xcd = (items + 7) / 8;
+  const int64_t item = (int64_t)(blockIdx.x % 8) * per_xcd + blockIdx.x / 8;
+  if (item >= items) return;                            // uniform per workgroup, before any barrier
+  const int wg = wgs - 1 - (int)(item % wgs);
+  const int hk = __builtin_amdgcn_readfirstlane((int)(item / wgs % a.Hkv));
+  const int b = __builtin_amdgcn_readfirstlane((int)(item / wgs / a.Hkv));
+  const int len = __builtin_amdgcn_readfirstlane(a.kv_lens ? min(max(a.kv_lens[b], 0), a.L) : a.L);
+  const int prefix = a.mod.prefix ? min(max(a.mod.prefix[b], 0), len) : 0;
+  const int32_t* docs = a.mod.docs ? a.mod.docs + (int64_t)b * a.mod.docs_sb : nullptr;
+  // Keys [0, n) that a (token, head) row may see; the document mask comes on top.
+  auto nkeys_of = [&](int pair) -> int {
+    if (pair >= npairs) return 0;
+    const int end = len - a.Tq + pair / G + 1;          // keys up to the row's own position
+    if (end <= 0 && (a.causal || docs)) return 0;
+    return a.causal ? max(end, prefix) : len;
+  };
+  const int maxkeys = nkeys_of(min(64 * wg + 63, npairs - 1));
+  const int my_pair = 64 * wg + 16 * wave + r;          // score-layout row of this lane
+  const int my_nkeys = nkeys_of(my_pair);
+  const int my_pos = len - a.Tq + my_pair / G;
+  // Every row of the wave sees all keys below this limit (the first row's).
+  const int wave_min_nkeys = __builtin_amdgcn_readfirstlane(nkeys_of(64 * wg + 16 * wave));
+  float slope2 = 0.0f;
+  if constexpr ((MOD & kModBias) != 0) {
+    if (a.mod.slopes && my_pair < npairs) slope2 = a.mod.slopes[hk * G + my_pair % G] * kLog2e;
+  }
+  // The lane's document, and the workgroup's smallest and largest.
+  int my_doc = 0, doc_lo = 0x7fffffff, doc_hi = -0x7fffffff - 1;
+  if (docs) {
+    if (my_nkeys > 0) doc_lo = doc_hi = my_doc = docs[my_pos];
+#pragma unroll
+    for (int off = 1; off < 16; off <<= 1) {
+      doc_lo = min(doc_lo, __shfl_xor(doc_lo, off, kWave));
+      doc_hi = max(doc_hi, __shfl_xor(doc_hi, off, kWave));
+    }
+    if (lane == 0) {
+      doc_range[0][wave] = doc_lo;
+      doc_range[1][wave] = doc_hi;
+    }
+    __syncthreads();
+    doc_lo = __builtin_amdgcn_readfirstlane(
+        min(min(doc_range[0][0], doc_range[0][1]), min(doc_range[0][2], doc_range[0][3])));
+    doc_hi = __builtin_amdgcn_readfirstlane(
+        max(max(doc_range[1][0], doc_range[1][1]), max(doc_range[1][2], doc_range[1][3])));
+  }
+
+  const T* kbase = static_cast<const T*>(a.k);
+  const T* vbase = static_cast<const T*>(a.v);
+  const T* kb = kbase + (int64_t)b * a.k_sb + (int64_t)hk * a.k_sh;   // contiguous caches
+  const T* vb = vbase + (int64_t)b * a.v_sb + (int64_t)hk * a.v_sh;
+  F qf[KS];
+  {
+    const bool ok = my_pair < npairs;
+    const T* qrow = static_cast<const T*>(a.q) + (int64_t)b * a.q_sb +
+                    (ok ? (int64_t)(hk * G + my_pair % G) * a.q_sh + (int64_t)(my_pair / G) * a.q_st : 0);
+#pragma unroll
+    for (int st = 0; st < KS; ++st) qf[st] = ok ? frag_load(qrow + 32 * st + 8 * qq) : frag_zero<F>();
+  }
+
+  // A split's chunks: K 0 .. n - 1, then V 0 .. n - 1, in alternating buffers
+  // from buffer 0; n = KC but for the last split, which has enough for maxkeys.
+  const int nsplit = maxkeys > 0 ? (maxkeys + kSplit - 1) / kSplit : 0;
+  const int nkc_last = nsplit > 0 ? (maxkeys - (nsplit - 1) * kSplit + CH - 1) / CH : 0;
+  // Copy offsets as in the plain kernel: a per-lane byte offset that is the same
+  // for every chunk, the rest a wave-uniform row step.
+  constexpr bool kFixed = 64 % KV::kCPR == 0;
+  constexpr int kRPC = kFixed ? 64 / KV::kCPR : 1;
+  constexpr auto period = [](int key_rows) {
+    return !kFixed || TILED ? CPW : kRPC >= key_rows ? 1 : key_rows / kRPC < CPW ? key_rows / kRPC : CPW;
+  };
+  constexpr int kKPeriod = period(KV::template kKeyRows<false>), kVPeriod = period(KV::template kKeyRows<true>);
+  constexpr bool kRowPerCopy = KV::kCPR == 64 && !TILED && !ROWPAGED;
+  int koff[kKPeriod], voff[kVPeriod];
+  if constexpr (!ROWPAGED && !kRowPerCopy) {
+    const int c0 = TILED ? 0 : wave * CPW;              // a tile's offsets start at its own first row
+#pragma unroll
+    for (int i = 0; i < kKPeriod; ++i) koff[i] = KV::template tile_off<false>(c0 + i, lane, a.k_sl);
+#pragma unroll
+    for (int i = 0; i < kVPeriod; ++i) voff[i] = KV::template tile_off<true>(c0 + i, lane, a.v_sl);
+  }
+  // Requests the chunk of keys key0 .. key0 + CH - 1 of K (or V) into buffer `slot`,
+  // and a split's document numbers with its first K chunk (every wave is past the
+  // scores of the split before it then).
+  auto request = [&](auto is_v, int at, int slot) __attribute__((always_inline)) {
+    constexpr bool V = decltype(is_v)::value;
+    const int key0 = __builtin_amdgcn_readfirstlane(at);
+    const int64_t sl = V ? a.v_sl : a.k_sl;
+    char* buf = ring + slot * CHB;
+    if (!V && docs && key0 % kSplit == 0) copy_to_lds4(docs + min(key0 + tid, len - 1), split_docs + 64 * wave);
+    if constexpr (MODE == kKvContig || MODE == kKvPaged) {
+      const int rows = min(CH, len - key0);             // >= 1: chunks start below maxkeys <= len
+      const T* base = MODE == kKvContig
+                          ? (V ? vb : kb) + (int64_t)key0 * sl
+                          : kv_segment<MODE>(a, V ? vbase : kbase, V ? a.v_sb : a.k_sb, V ? a.v_sh : a.k_sh, sl, b, hk, key0);
+      const auto rs = buffer_rsrc(base, (int)(rows * sl * (int64_t)sizeof(T)));
+      char* dst = buf + 1024 * wave * CPW;
+      constexpr int kP = V ? kVPeriod : kKPeriod;
+      const int rows_b = kP * kRPC * (int)(sl * (int64_t)sizeof(T));
+      if constexpr (kRowPerCopy) {
+        int row_b = (int)(sl * (int64_t)sizeof(T)), l = lane;
+        asm volatile("" : "+v"(l), "+s"(row_b));        // (not kept live across chunks)
+#pragma unroll
+        for (int i = 0; i < CPW; ++i)
+          copy_to_lds16(rs, ((l ^ KV::template key<V>(wave * CPW + i)) << 4) + (wave * CPW + i) * row_b, dst + 1024 * i);
+        return;
+      }
+#pragma unroll
+      for (int i = 0; i < kP; ++i) {
+        int o = V ? voff[i % kVPeriod] : koff[i % kKPeriod];
+        asm volatile("" : "+v"(o));                     // the stepped offsets are not kept live across chunks
+#pragma unroll
+        for (int i2 = i; i2 < CPW; i2 += kP) copy_to_lds16(rs, o + i2 / kP * rows_b, dst + 1024 * i2);
+      }
+    } else if constexpr (TILED) {
+      // Wave w copies the chunk's 16-key tile w; a tile past the sequence
+      // reads as zero (and its table entry is the last tile's).
+      static_assert(!TILED || (CH == 64 && CPW == KV::kTileCopies), "attn_prefill_mod: a tile per wave");
+      const int pos = __builtin_amdgcn_readfirstlane(min(key0 + 16 * wave, (len - 1) & ~15));
+      const int rows = uniform_clamp(len - key0 - 16 * wave, 16);
+      const int e = load_uniform_i32(uniform_ptr(kv_entry(a, b, pos)));
+      const auto rs = buffer_rsrc(uniform_ptr(kv_tile(a, V ? vbase : kbase, V ? a.v_sb : a.k_sb, V ? a.v_sh : a.k_sh, sl,
+                                                      e, hk, pos)),
+                                  (int)(rows * sl * (int64_t)sizeof(T)));
+      char* dst = buf + 1024 * wave * CPW;
+#pragma unroll
+      for (int i = 0; i < CPW; ++i) copy_to_lds16(rs, V ? voff[i % kVPeriod] : koff[i % kKPeriod], dst + 1024 * i);
+    } else {
+      auto row = [&](int i) {
+        return (V ? vbase : kbase) + kv_row_off(a, V ? a.v_sb : a.k_sb, V ? a.v_sh : a.k_sh, sl, b, hk, key0 + i);
+      };
+#pragma unroll
+      for (int i = 0; i < CPW; ++i) KV::template copy<V>(buf, wave * CPW + i, row, len - key0, lane);
+    }
+  };
+
+  // The split to run next, and whether its only document is the workgroup's.
+  int next = 0;
+  bool next_own = true;
+  uint64_t hit = 0, lone = 0;                           // splits 64 g .. 64 g + 63: one of our documents; only ours
+  int group = -1;
+  auto advance = [&](int sp) __attribute__((always_inline)) {
+    if (docs) {
+      while (sp < nsplit) {
+        if (sp / 64 != group) {
+          group = sp / 64;
+          int2 range = {0x7fffffff, -0x7fffffff - 1};
+          if (64 * group + lane < nsplit)
+            range = a.mod.ranges[(int64_t)b * ((a.L + kSplit - 1) / kSplit) + 64 * group + lane];
+          hit = __ballot(range.y >= doc_lo && range.x <= doc_hi);
+          lone = __ballot(range.x == doc_lo && range.y == doc_lo && doc_lo == doc_hi);
+        }
+        const uint64_t left = hit >> (sp % 64);
+        sp = left ? sp + __builtin_ctzll(left) : 64 * (group + 1);
+        if (left) break;
+      }
+      next_own = lone >> (sp % 64) & 1;
+    }
+    next = __builtin_amdgcn_readfirstlane(sp);          // (known to be one for the wave: copies take it so)
+  };
+  // The keys of a chunk that the document mask leaves to this lane's row, bit
+  // 4 t + i for key 16 t + 4 qq + i.
+  auto doc_bits = [&](int kc) __attribute__((always_inline)) {
+    uint32_t ok = ~0u;
+    if (docs) {
+      ok = 0;
+#pragma unroll
+      for (int t = 0; t < TPC; ++t) {
+        const int4 d = *reinterpret_cast<const int4*>(split_docs + CH * kc + 16 * t + 4 * qq);
+        ok |= ((d.x == my_doc ? 1u : 0u) | (d.y == my_doc ? 2u : 0u) | (d.z == my_doc ? 4u : 0u) |
+               (d.w == my_doc ? 8u : 0u)) << (4 * t);
+      }
+    }
+    return ok;
+  };
+  // The second run: clears the infinities and NaN in the V chunk of keys key0 ..
+  // and notes the rows that see them.
+  bool careful = false;
+  auto clean_v = [&](char* buf, int key0) __attribute__((always_inline)) {
+    constexpr int kPer = 16 / (int)sizeof(T);
+    for (int f = tid; f < CH * KV::kCPR; f += 256) {
+      const int row = f / KV::kCPR, slot = f % KV::kCPR, key = key0 + row;
+      T e[kPer];
+      u32x4 raw = *reinterpret_cast<u32x4*>(buf + 16 * f);
+      __builtin_memcpy(e, &raw, 16);
+      bool changed = false;
+      for (int j = 0; j < kPer; ++j) {
+        const float x = to_f32(e[j]);
+        if (fabsf(x) < INFINITY) continue;
+        changed = true;
+        e[j] = (T)0.0f;
+        const int dim = (slot ^ KV::template key<true>(row)) * kPer + j;
+        const uint32_t bit = (x != x ? 4u : x > 0.0f ? 1u : 2u) << (8 * (dim % 4));
+        for (int p = 0; p < 64; ++p) {
+          if (key >= nkeys_of(64 * wg + p)) continue;
+          if (docs && docs[len - a.Tq + (64 * wg + p) / G] != docs[key]) continue;
+          atomicOr(&poison[(p * D + dim) / 4], bit);
+        }
+      }
+      if (changed) {
+        __builtin_memcpy(&raw, e, 16);
+        *reinterpret_cast<u32x4*>(buf + 16 * f) = raw;
+      }
+    }
+    __syncthreads();
+  };
+
+  float M[4], Lsum[4];
+  f32x4 A[NDT];
+  const int kbase0 = KV::kbase(r, qq), vbase0 = KV::vbase(lane);
+  // One split: scores of the wave's 16 rows (kept in registers), their maximum
+  // and weights, P.V and the weight sum, the merge. PIPE: software-pipelined
+  // inside the wave as attn_prefill_mfma's split_body_pipe, whose comment says how.
+  auto split_body = [&](const int sp, auto masked) __attribute__((always_inline)) {
+    constexpr bool MASKED = decltype(masked)::value;
+    const int j0 = sp * kSplit;
+    const int nkc = !MASKED || sp + 1 < nsplit ? KC : nkc_last;
+    float s[16][4];
+    float m = -INFINITY;
+#pragma unroll
+    for (int kc = 0; kc < KC; ++kc) {
+      if (kc >= nkc) {
+#pragma unroll
+        for (int t = 0; t < TPC; ++t)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) s[TPC * kc + t][i] = -INFINITY;
+        continue;
+      }
+      // Chunk landed (everyone's: the barrier); the next one goes into the
+      // other buffer, which every wave is done with.
+      stage_barrier<0>();
+      if (kc + 1 < nkc) request(std::false_type(), j0 + CH * (kc + 1), (kc + 1) % 2);
+      else request(std::true_type(), j0, nkc % 2);
+      const char* buf = ring + kc % 2 * CHB;
+      const int lim = my_nkeys - (j0 + CH * kc + 4 * qq);
+      const uint32_t seen = MASKED ? doc_bits(kc) : ~0u;
+      const float far = (MOD & kModBias) != 0 ? (float)(my_pos - (j0 + CH * kc + 4 * qq)) : 0.0f;
+      auto finish = [&](int t, f32x4 dot) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float y = mod_score<T, MOD>(dot[i], a, slope2, far - (float)(16 * t + i));
+          const float x = (!MASKED || (16 * t + i < lim && (seen >> (4 * t + i) & 1u))) ? y : -INFINITY;
+          s[TPC * kc + t][i] = x;
+          m = fmaxf(m, x);
+        }
+      };
+      if constexpr (PIPE) {
+        int ko = kbase0;
+        asm volatile("" : "+v"(ko));                    // recomputed per chunk, not kept live across them
+        F kf[2][KS];
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+          for (int st = 0; st < KS; ++st) kf[t][st] = KV::kfrag_at(buf, ko, 16 * t, st);
+        f32x4 prev = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int t = 0; t < TPC; ++t) {
+          f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int st = 0; st < KS; ++st) {
+            acc = mfma_step(kf[t & 1][st], qf[st], acc);
+            if (t + 2 < TPC) kf[t & 1][st] = KV::kfrag_at(buf, ko, 16 * (t + 2), st);
+          }
+          if (t > 0) finish(t - 1, prev);
+          prev = acc;
+          __builtin_amdgcn_sched_barrier(0);
+        }
+        finish(TPC - 1, prev);
+      } else {
+#pragma unroll
+        for (int t = 0; t < TPC; ++t) {
+          f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int st = 0; st < KS; ++st) acc = mfma_step(KV::kfrag(buf, 16 * t + r, st, qq), qf[st], acc);
+          finish(t, acc);
+        }
+      }
+    }
+    m = quarter_max(m);
+    // Weights exp2(s - m): exactly +0 for a hidden key (s = -inf). A row without a
+    // visible key in the split subtracts 0 instead, so that they are 0, not NaN.
+    const float msub = m == -INFINITY ? 0.0f : m;
+    float mi[4];                                        // accumulator-layout rows' maxima
+#pragma unroll
+    for (int i = 0; i < 4; ++i) mi[i] = __shfl(m, 4 * qq + i, kWave);
+    auto weight_pair = [&](PFrag<T>& pf, int ks, int j) __attribute__((always_inline)) {
+      const int t = 2 * ks + j / 2, i = 2 * (j % 2);
+      const float p0 = __builtin_amdgcn_exp2f(s[t][i] - msub), p1 = __builtin_amdgcn_exp2f(s[t][i + 1] - msub);
+      if constexpr (sizeof(T) == 2) {
+        pfrag_pair<T>(pf, j, p0, p1);
+      } else {
+        f32x4& half = j < 2 ? pf.f.lo : pf.f.hi;
+        half[i] = p0;
+        half[i + 1] = p1;
+      }
+    };
+    f32x4 acc[NDT];
+    f32x4 lsum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt) acc[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    PFrag<T> pf;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) weight_pair(pf, 0, j);
+    constexpr int HS = CH / 32, NB = NDT / 2;           // 32-key steps per chunk, dim-tile pairs
+#pragma unroll
+    for (int kc = 0; kc < KC; ++kc) {
+      if (kc >= nkc) continue;
+      stage_barrier<0>();
+      char* buf = ring + (nkc + kc) % 2 * CHB;
+      if constexpr (MASKED) {
+        if (careful) clean_v(buf, j0 + CH * kc);
+      }
+      if (kc + 1 < nkc) request(std::true_type(), j0 + CH * (kc + 1), (nkc + kc + 1) % 2);
+      else if (next < nsplit) request(std::false_type(), kSplit * next, 0);
+      if constexpr (PIPE) {
+        int vo = vbase0;
+        asm volatile("" : "+v"(vo));
+        F vf[NDT];
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt) vf[dt] = KV::vfrag_at(buf, vo, 0, dt);
+        __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+        for (int h = 0; h < HS; ++h) {
+          const int ks = HS * kc + h;
+          PFrag<T> after = pf;
+#pragma unroll
+          for (int b2 = 0; b2 < NB; ++b2) {
+            const int d0 = 2 * b2, d1 = 2 * b2 + 1;
+            acc[d0] = mfma_step(pf.hi, vf[d0], acc[d0]);
+            acc[d1] = mfma_step(pf.hi, vf[d1], acc[d1]);
+            acc[d0] = mfma_step(pf.lo, vf[d0], acc[d0]);
+            if (h + 1 < HS) vf[d0] = KV::vfrag_at(buf, vo, 32 * (h + 1), d0);
+            acc[d1] = mfma_step(pf.lo, vf[d1], acc[d1]);
+            if (h + 1 < HS) vf[d1] = KV::vfrag_at(buf, vo, 32 * (h + 1), d1);
+            if (b2 == 0) lsum = pv_step<T>(pf, ones_frag<T>(), lsum);
+            if (ks + 1 < kSplit / 32) {
+#pragma unroll
+              for (int j = 4 * b2 / NB; j < 4 * (b2 + 1) / NB; ++j) weight_pair(after, ks + 1, j);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+          }
+          pf = after;
+        }
+        __builtin_amdgcn_s_setprio(0);
+      } else {
+#pragma unroll
+        for (int h = 0; h < HS; ++h) {
+          const int ks = HS * kc + h;
+          if (ks > 0) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j) weight_pair(pf, ks, j);
+          }
+          __builtin_amdgcn_s_setprio(1);
+#pragma unroll
+          for (int dt = 0; dt < NDT; ++dt) acc[dt] = pv_step<T>(pf, KV::vfrag(buf, 32 * h, dt, lane), acc[dt]);
+          __builtin_amdgcn_s_setprio(0);
+          lsum = pv_step<T>(pf, ones_frag<T>(), lsum);
+        }
+      }
+    }
+    // Merge into the running state (accumulator layout: rows 4 qq + i). A row
+    // that sees no key of the split skips it.
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (mi[i] > -INFINITY || lsum[i] != 0.0f) {
+        float ai[NDT];
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt) ai[dt] = A[dt][i];
+        float acci[NDT];
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt) acci[dt] = acc[dt][i];
+        merge_split<NDT>(M[i], Lsum[i], ai, mi[i], lsum[i], acci);
+#pragma unroll
+        for (int dt = 0; dt < NDT; ++dt) A[dt][i] = ai[dt];
+      }
+    }
+  };
+
+  for (;;) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      M[i] = -INFINITY;
+      Lsum[i] = 0.0f;
+    }
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt) A[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    advance(0);
+    if (next < nsplit) request(std::false_type(), kSplit * next, 0);
+    while (next < nsplit) {
+      const int sp = next;
+      const bool own = next_own;
+      advance(sp + 1);
+      if (sp * kSplit + kSplit <= wave_min_nkeys && own && !careful) split_body(sp, std::false_type());
+      else split_body(sp, std::true_type());
+    }
+    bool finite = true;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      if (64 * wg + 16 * wave + 4 * qq + i >= npairs) continue;
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt) finite = finite && fabsf(A[dt][i]) < INFINITY;
+    }
+    if (careful || !__builtin_amdgcn_readfirstlane(__syncthreads_or(!finite))) break;
+    careful = true;
+    for (int i = tid; i < 16 * D; i += 256) poison[i] = 0;
+    __syncthreads();
+  }
+
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int row = 16 * wave + 4 * qq + i, pair = 64 * wg + row;
+    if (pair >= npairs) continue;
+    T* o = static_cast<T*>(a.out) +
+           ((((int64_t)b * a.Hq + hk * G + pair % G) * a.Tq) + pair / G) * D + r;
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt) {
+      float x = Lsum[i] != 0.0f ? A[dt][i] / Lsum[i] : 0.0f;   // no key: 0
+      if (careful) {
+        const int at = row * D + 16 * dt + r;
+        const uint32_t bad = poison[at / 4] >> (8 * (at % 4)) & 7u;
+        if (bad) x = bad == 1 ? INFINITY : bad == 2 ? -INFINITY : NAN;
+      }
+      o[16 * dt] = to_store<T>(x);
+    }
+  }
+}
+
+}  // namespace bi

@@ -1,0 +1,7 @@
+// bi_attn_mod_bias_bf16.hip — prefill attention with ScoreMod for bf16 elements: a distance bias.
+#include "bi_attn_mod_launch.h"
+
+namespace bi {
+#define BI_MOD(T, D) template int launch_prefill_mod<T, D, (kModAny | kModBias)>(ModPrefillArgs&, hipStream_t);
+BI_ATTN_MOD_D(BI_MOD, bf16)
+}  // namespace bi

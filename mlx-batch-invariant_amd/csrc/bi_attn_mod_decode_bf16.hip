@@ -1,0 +1,6 @@
+// bi_attn_mod_decode_bf16.hip — decode attention with ScoreMod for bf16 elements, every head dim.
+#include "bi_attn_mod_launch.h"
+
+namespace bi {
+BI_ATTN_MOD_D(BI_ATTN_MOD_DECODE, bf16)
+}  // namespace bi

@@ -1,0 +1,135 @@
+// bi_attn_mod_launch.h — host launchers of the attention kernels with ScoreMod
+// (capped scores, distance bias, document and prefix masks), included by the
+// translation units bi_attn_mod_*.hip, which instantiate them per element type
+// and score variant. Kernels: bi_attn_mfma.h (decode), bi_attn_mod.h (prefill).
+#pragma once
+
+#include "bi_attn_launch.h"
+#include "bi_attn_mod.h"
+
+namespace bi {
+
+// attn_combine_kernel, but a split without a visible key (l = 0 at m = -inf) is
+// not merged: its m would make the factors NaN. (A split whose scores are all
+// NaN has l = NaN and is merged.)
+template <typename T, int D>
+__global__ __launch_bounds__(256) void attn_combine_mod_kernel(DecodeArgs a) {
+  const int64_t gid0 = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const bool live = gid0 < (int64_t)a.B * a.Hq * D;
+  const int64_t gid = live ? gid0 : 0;
+  const int64_t bh = gid / D;
+  const int d = (int)(gid % D), b = (int)(bh / a.Hq);
+  const int len = a.kv_lens ? min(max(a.kv_lens[b], 0), a.L) : a.L;
+  const int ns = (len + kSplit - 1) / kSplit;
+  float M = -INFINITY, Ls = 0.0f, A = 0.0f;
+  auto merge = [&](float m, float l, float acc) {
+    if (m > -INFINITY || l != 0.0f) merge_split<1>(M, Ls, &A, m, l, &acc);
+  };
+  int i = 0;
+  for (; i + 8 <= ns; i += 8) {                         // partials loaded eight splits ahead, merged in order
+    float pm[8], pl[8], pa[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      const int64_t po = bh * a.nsplit + i + j;
+      pm[j] = a.pm[po];
+      pl[j] = a.pl[po];
+      pa[j] = a.pacc[po * D + d];
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j) merge(pm[j], pl[j], pa[j]);
+  }
+  for (; i < ns; ++i) {
+    const int64_t po = bh * a.nsplit + i;
+    merge(a.pm[po], a.pl[po], a.pacc[po * D + d]);
+  }
+  if (live) static_cast<T*>(a.out)[bh * D + d] = to_store<T>(Ls != 0.0f ? A / Ls : 0.0f);
+}
+
+// One item order (dynamic) for every cache: the extra launch that zeroes the
+// counter costs what the second instantiation would save.
+template <typename T, int D, int GU, int MODE>
+static int launch_decode_mod_gu(ModDecodeArgs& a, hipStream_t st) {
+  static int cache[kMaxDev] = {};
+  const int64_t most = (int64_t)a.B * a.nsplit * a.Hkv * a.nchunk;
+  const int grid = resident_grid(attn_decode_mfma<T, D, GU, true, MODE, kModAny>, cache);
+  if (grid <= 0) return bi_host::fail(BI_E_UNSUPPORTED, "bi_attn_scored: device occupancy query failed");
+  zero_counter_kernel<<<1, 1, 0, st>>>(a.ctr);
+  attn_decode_mfma<T, D, GU, true, MODE, kModAny><<<(int)std::min<int64_t>(grid, most), 256, 0, st>>>(a);
+  return 0;
+}
+
+template <typename T, int D, int GU>
+static int launch_decode_mod_mode(ModDecodeArgs& a, hipStream_t st) {
+  switch (kv_mode<T>(a)) {
+    case kKvPaged: return launch_decode_mod_gu<T, D, GU, kKvPaged>(a, st);
+    case kKvTilePaged: return launch_decode_mod_gu<T, D, GU, kKvTilePaged>(a, st);
+    case kKvRowPaged: return launch_decode_mod_gu<T, D, GU, kKvRowPaged>(a, st);
+    default: return launch_decode_mod_gu<T, D, GU, kKvContig>(a, st);
+  }
+}
+
+template <typename T, int D>
+int launch_decode_mod(ModDecodeArgs& a, hipStream_t st) {
+  int rc = 0;
+  switch (a.GU) {
+    case 16: rc = launch_decode_mod_mode<T, D, 16>(a, st); break;
+    case 8: rc = launch_decode_mod_mode<T, D, 8>(a, st); break;
+    case 4: rc = launch_decode_mod_mode<T, D, 4>(a, st); break;
+    case 2: rc = launch_decode_mod_mode<T, D, 2>(a, st); break;
+    default: rc = launch_decode_mod_mode<T, D, 1>(a, st); break;
+  }
+  if (rc) return rc;
+  if ((rc = bi_host::launch_status("bi_attn_scored"))) return rc;
+  const int64_t n = (int64_t)a.B * a.Hq * D;
+  attn_combine_mod_kernel<T, D><<<(unsigned)((n + 255) / 256), 256, 0, st>>>(a);
+  return bi_host::launch_status("bi_attn_scored(combine)");
+}
+
+// Smallest and largest document number of each split's keys below the sequence's
+// length: one wave per split.
+static __global__ __launch_bounds__(64) void doc_ranges_kernel(const int32_t* __restrict__ docs, int64_t docs_sb,
+                                                               const int32_t* kv_lens, int L, int nsplit,
+                                                               int2* ranges) {
+  const int b = blockIdx.x / nsplit, sp = blockIdx.x % nsplit;
+  const int len = kv_lens ? min(max(kv_lens[b], 0), L) : L;
+  int lo = 0x7fffffff, hi = -0x7fffffff - 1;
+#pragma unroll
+  for (int j = 0; j < kSplit / 64; ++j) {
+    const int key = kSplit * sp + 64 * j + (int)threadIdx.x;
+    if (key < len) {
+      const int d = docs[b * docs_sb + key];
+      lo = min(lo, d);
+      hi = max(hi, d);
+    }
+  }
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) {
+    lo = min(lo, __shfl_xor(lo, off, kWave));
+    hi = max(hi, __shfl_xor(hi, off, kWave));
+  }
+  if (threadIdx.x == 0) ranges[blockIdx.x] = int2{lo, hi};
+}
+
+template <typename T, int D, int MOD>
+int launch_prefill_mod(ModPrefillArgs& a, hipStream_t st) {
+  const int64_t wgs = ((int64_t)a.Tq * (a.Hq / a.Hkv) + 63) / 64;
+  const int64_t items = wgs * a.Hkv * a.B;
+  dim3 grid((unsigned)(8 * ((items + 7) / 8)));
+  if (a.mod.docs) {
+    const int ns = (a.L + kSplit - 1) / kSplit;
+    doc_ranges_kernel<<<(unsigned)(a.B * ns), 64, 0, st>>>(a.mod.docs, a.mod.docs_sb, a.kv_lens, a.L, ns,
+                                                           const_cast<int2*>(a.mod.ranges));
+  }
+  switch (kv_mode<T>(a)) {
+    case kKvPaged: attn_prefill_mod<T, D, kKvPaged, MOD><<<grid, 256, 0, st>>>(a); break;
+    case kKvTilePaged: attn_prefill_mod<T, D, kKvTilePaged, MOD><<<grid, 256, 0, st>>>(a); break;
+    case kKvRowPaged: attn_prefill_mod<T, D, kKvRowPaged, MOD><<<grid, 256, 0, st>>>(a); break;
+    default: attn_prefill_mod<T, D, kKvContig, MOD><<<grid, 256, 0, st>>>(a); break;
+  }
+  return bi_host::launch_status("bi_attn_scored");
+}
+
+#define BI_ATTN_MOD_D(X, T) X(T, 32) X(T, 64) X(T, 96) X(T, 128) X(T, 192) X(T, 256)
+#define BI_ATTN_MOD_DECODE(T, D) template int launch_decode_mod<T, D>(ModDecodeArgs&, hipStream_t);
+
+}  // namespace bi

@@ -172,7 +172,12 @@ __device__ __forceinline__ void copy_to_lds16(const void* src, void* lds_block) 
   __builtin_amdgcn_global_load_lds((gbl_void_t*)src, (lds_void_t*)lds_block, 16, 0, 0);
 }
 
-// The same copy through a buffer resource over [base, base + bytes): lane l
+// One dword per lane; lane l lands at lds_block + 4 l.
+__device__ __forceinline__ void copy_to_lds4(const void* src, void* lds_block) {
+  __builtin_amdgcn_global_load_lds((gbl_void_t*)src, (lds_void_t*)lds_block, 4, 0, 0);
+}
+
+// The 16-byte copy through a buffer resource over [base, base + bytes): lane l
 // reads base + voffset (zero past the range) and lands at lds_block + 16 l.
 __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer_rsrc(const void* base, int bytes) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(base), (short)0, bytes, 0x00020000);

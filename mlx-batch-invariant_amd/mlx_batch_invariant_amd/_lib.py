@@ -33,6 +33,13 @@ DECODE_SCRATCH_BYTES = 64 << 20   # BI_DECODE_SCRATCH_BYTES: static scratch of b
 _c_i64 = ctypes.c_int64
 _vp = ctypes.c_void_p
 
+
+class ScoreMod(ctypes.Structure):
+    """``bi_score_mod`` of include/bi_kernels.h."""
+    _fields_ = [("softcap", ctypes.c_float), ("slopes", _vp), ("doc_ids", _vp), ("doc_stride", _c_i64),
+                ("prefix_lens", _vp)]
+
+
 # name -> (restype, argtypes); must match include/bi_kernels.h
 _SIGNATURES = {
     "bi_abi_version": (ctypes.c_int, []),
@@ -76,6 +83,10 @@ _SIGNATURES = {
     "bi_attn_prefill_paged": (ctypes.c_int, [_vp, _vp, _vp, _vp, _c_i64, _c_i64, _c_i64, _vp, _vp, _c_i64, _c_i64,
                                              _c_i64, _c_i64, _c_i64, _c_i64, ctypes.POINTER(_c_i64), ctypes.c_int,
                                              ctypes.c_float, ctypes.c_int, _vp]),
+    "bi_attn_scored_workspace_bytes": (ctypes.c_size_t, [_c_i64, _c_i64, _c_i64, _c_i64, _c_i64, ctypes.c_int]),
+    "bi_attn_scored": (ctypes.c_int, [_vp, _vp, _vp, _vp, _c_i64, _c_i64, _c_i64, _vp, _vp, _c_i64, _c_i64, _c_i64,
+                                      _c_i64, _c_i64, _c_i64, ctypes.POINTER(_c_i64), ctypes.c_int, ctypes.c_float,
+                                      ctypes.POINTER(ScoreMod), ctypes.c_int, _vp, ctypes.c_size_t, _vp]),
     "bi_rope_cache": (ctypes.c_int, [_vp, _c_i64, _vp, _c_i64, _vp, _c_i64, _vp, _vp, _vp, _vp, _vp, _c_i64, _c_i64,
                                      _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, ctypes.POINTER(_c_i64), ctypes.c_int,
                                      _vp]),

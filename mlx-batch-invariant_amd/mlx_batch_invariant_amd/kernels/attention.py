@@ -39,6 +39,21 @@ result): ``split_size != 256`` runs them.
 ``kv_lens`` (int32 [B], optional) is an extension the reference does not have:
 sequence b uses only its first ``kv_lens[b]`` keys, and its output is bit-for-bit
 what it would be alone with K/V cut to that length.
+
+``softcap``, ``slopes``, ``doc_ids`` and ``prefix_lens`` (extensions too) change
+the scores and the mask in the matrix-core order: with query t at position
+``p = len - T_q + t``,
+
+* the score with key j is ``softcap * tanh(q.k * scale / softcap) - slopes[h] *
+  |p - j|``;
+* key j is visible if ``j < len`` and, with the causal mask, ``j <= p`` or
+  ``j < prefix_lens[b]``, and with ``doc_ids[b]`` of one number per key position,
+  ``doc_ids[b, j] == doc_ids[b, p]``.
+
+Hidden keys take no part whatever their rows hold; a query that sees none (one
+in front of a padded prompt, p < 0) gets zeros. The invariances above hold, and
+where nothing is changed (slopes of 0, one document, no prefix) the bits of the
+plain call.
 """
 
 from __future__ import annotations
@@ -216,16 +231,85 @@ def batch_invariant_prefill_attention(q, k, v, *, scale: float, causal: bool,
     return out
 
 
+def _scored(what, q, k, v, table, num_pages, page_size, L, kl, scale, causal, softcap, slopes, doc_ids,
+            prefix_lens) -> torch.Tensor:
+    """One call of ``bi_attn_scored`` on checked operands: K / V contiguous
+    (``table`` None) or pools of pages. Host-side checks of what changes the
+    scores and masks; see the module's text for their meaning."""
+    B, Hq, Tq, D = q.shape
+    mod = _lib.ScoreMod()
+    if softcap is not None:
+        softcap = float(softcap)
+        if not 0.0 < softcap < 3e38:
+            raise ValueError(f"{what}: softcap must be a positive number; got {softcap}")
+        mod.softcap = softcap
+    if slopes is not None:
+        slopes = torch.as_tensor(slopes, dtype=torch.float32, device=q.device).contiguous()
+        if tuple(slopes.shape) != (Hq,):
+            raise ValueError(f"{what}: slopes {tuple(slopes.shape)}, expected one for each of {Hq} heads")
+        mod.slopes = slopes.data_ptr()
+    if doc_ids is not None:
+        if doc_ids.is_floating_point() or doc_ids.ndim != 2 or doc_ids.shape[0] != B or doc_ids.shape[1] < L:
+            raise ValueError(f"{what}: doc_ids {doc_ids.dtype} {tuple(doc_ids.shape)}; need whole numbers, {B} rows "
+                             f"of at least {L}")
+        _lib.one_device(what, q, doc_ids)
+        doc_ids = doc_ids.to(torch.int32)
+        if doc_ids.stride(1) != 1 or doc_ids.stride(0) < L:
+            doc_ids = doc_ids.contiguous()
+        mod.doc_ids, mod.doc_stride = doc_ids.data_ptr(), max(doc_ids.stride(0), L)
+    if prefix_lens is not None:
+        if not causal:
+            raise ValueError(f"{what}: prefix_lens goes with mask='causal'")
+        prefix_lens = _lens(prefix_lens, B, L, q.device)
+        mod.prefix_lens = prefix_lens.data_ptr()
+    q = _fix(q)
+    out = torch.empty((B, Hq, Tq, D), dtype=q.dtype, device=q.device)
+    if B == 0 or Tq == 0:
+        return out
+    n = _lib.ws_bytes("bi_attn_scored_workspace_bytes", B, Hq, Tq, L, D, int(doc_ids is not None))
+    ws = _lib.workspace(n, q.device)
+    strides = (_lib._c_i64 * 9)(q.stride(0), q.stride(1), q.stride(2), k.stride(0), k.stride(1), k.stride(2),
+                                v.stride(0), v.stride(1), v.stride(2))
+    with _lib.on_device(q):
+        rc = _lib.load().bi_attn_scored(q.data_ptr(), k.data_ptr(), v.data_ptr(), _lib.ptr(table),
+                                        0 if table is None else table.stride(0), page_size, num_pages, _lib.ptr(kl),
+                                        out.data_ptr(), B, Hq, v.shape[1], Tq, L, D, strides, 1 if causal else 0,
+                                        float(scale), mod, _lib.DTYPE_CODE[q.dtype], _lib.ptr(ws), n,
+                                        _lib.stream_of(q))
+    _lib.check(rc, "bi_attn_scored")
+    return out
+
+
 def batch_invariant_attention(q, k, v, *, scale: float | None = None, mask=None, kv_lens=None,
-                              order: str | None = None, split_size: int = SPLIT_SIZE) -> torch.Tensor:
+                              order: str | None = None, split_size: int = SPLIT_SIZE, softcap: float | None = None,
+                              slopes=None, doc_ids=None, prefix_lens=None) -> torch.Tensor:
     """Dispatch: decode path for T_q == 1, prefill otherwise (reference:
     kernels/attention.py:393-397). ``mask`` is None or "causal"; ``order`` is
     "mfma" (matrix cores), "per_key" (the reference's own order) or None (the
-    matrix cores for split_size 256, else per-key)."""
+    matrix cores for split_size 256, else per-key). ``softcap`` (a number),
+    ``slopes`` (fp32 ``[Hq]``), ``doc_ids`` (int32 ``[B, L]``) and ``prefix_lens``
+    (int32 ``[B]``) cap the scores, add a bias that grows with the distance, and
+    mask by document and prefix (matrix-core order only)."""
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])
     if mask is not None and mask != "causal":
         raise ValueError("batch_invariant_attention: mask must be None or 'causal'")
+    if softcap is not None or slopes is not None or doc_ids is not None or prefix_lens is not None:
+        what = "batch_invariant_attention"
+        B, Hq, Tq, D = q.shape
+        if k.ndim != 4 or k.shape != v.shape or k.shape[0] != B or k.shape[3] != D or k.shape[1] == 0 or Hq % k.shape[1]:
+            raise ValueError(f"{what}: unsupported shapes q {tuple(q.shape)} k {tuple(k.shape)} v {tuple(v.shape)}")
+        if _per_key(order, split_size, D):
+            raise ValueError(f"{what}: softcap, slopes, doc_ids and prefix_lens need the matrix-core order (head dims "
+                             f"{MFMA_HEAD_DIMS}, split_size {SPLIT_SIZE}); got D={D}, order={order!r}, "
+                             f"split_size={split_size}")
+        L, causal = k.shape[2], mask == "causal"
+        if causal and Tq > L:
+            raise ValueError(f"causal prefill needs T_q <= L (T_q={Tq}, L={L})")
+        _, k, v = _prep(q, k, v)
+        _lib.one_device(what, q, k, v)
+        return _scored(what, q, _fix(k), _fix(v), None, 0, 0, L, _lens(kv_lens, B, L, q.device), scale, causal,
+                       softcap, slopes, doc_ids, prefix_lens)
     if q.shape[2] == 1:
         return batch_invariant_decode_attention(q, k, v, scale=scale, kv_lens=kv_lens, order=order,
                                                 split_size=split_size)
@@ -234,7 +318,8 @@ def batch_invariant_attention(q, k, v, *, scale: float | None = None, mask=None,
 
 
 def batch_invariant_paged_attention(q, k_pages, v_pages, block_table, kv_lens=None, *, scale: float | None = None,
-                                    mask=None) -> torch.Tensor:
+                                    mask=None, softcap: float | None = None, slopes=None, doc_ids=None,
+                                    prefix_lens=None) -> torch.Tensor:
     """Attention over a paged K/V cache: decode for T_q == 1, prefill otherwise.
 
     ``k_pages`` / ``v_pages``: ``[num_pages, Hkv, page_size, D]`` (any strides
@@ -248,7 +333,9 @@ def batch_invariant_paged_attention(q, k_pages, v_pages, block_table, kv_lens=No
     row that sees no key, gets an all-zero output. The output is bit for bit the
     contiguous call on the same keys: paging changes addresses only. The
     reference reads one contiguous cache (kernels/attention.py:87-254); paged
-    KV is an item of its roadmap of adjacent ops.
+    KV is an item of its roadmap of adjacent ops. ``softcap``, ``slopes``,
+    ``doc_ids`` (int32 ``[B, max_pages * page_size]``, by key position) and
+    ``prefix_lens`` as in ``batch_invariant_attention``.
     """
     if scale is None:
         scale = 1.0 / math.sqrt(q.shape[-1])
@@ -272,6 +359,11 @@ def batch_invariant_paged_attention(q, k_pages, v_pages, block_table, kv_lens=No
     causal = mask == "causal"
     if causal and Tq > L:
         raise ValueError(f"causal prefill needs T_q <= L (T_q={Tq}, L={L})")
+    if softcap is not None or slopes is not None or doc_ids is not None or prefix_lens is not None:
+        what = "batch_invariant_paged_attention"
+        _lib.one_device(what, q, k_pages, v_pages, table)
+        return _scored(what, q, k_pages, v_pages, table, num_pages, page_size, L, kl, scale, causal, softcap, slopes,
+                       doc_ids, prefix_lens)
     out = torch.empty((B, Hq, Tq, D), dtype=dt, device=q.device)
     if B == 0 or Tq == 0:
         return out

@@ -20,6 +20,10 @@ Operators (each the same computation, and bits, as the Python function named):
   prefill otherwise (``mask="causal"`` is bottom-right aligned);
 * ``paged_attention(q, k_pages, v_pages, block_table, kv_lens, scale, causal)``:
   the same over a paged K/V pool (``batch_invariant_paged_attention``);
+* ``scored_attention(q, k, v, scale, causal, kv_lens, softcap, slopes, doc_ids,
+  prefix_lens)`` and ``scored_paged_attention(q, k_pages, v_pages, block_table,
+  kv_lens, scale, causal, softcap, ...)``: the two with capped scores, a distance
+  bias, a document mask or a prefix mask;
 * ``residual_rms_norm(x, residual, post_weight, pre_weight, eps, gate, scale)``:
   both norms (``batch_invariant_residual_rms_norm``); returns (y, h);
 * ``paged_slots(kv_lens, new_lens, block_table!, free_pages, cursor, page_size,
@@ -143,3 +147,32 @@ def rope_paged_cache(q: Tensor, k: Tensor, v: Tensor, cos: Tensor, sin: Tensor, 
 def _rope_paged_cache_fake(q, k, v, cos, sin, positions, slots, k_pages, v_pages, sections):
     B, T, H, D = q.shape
     return q.new_empty((B, H, T, D))
+
+
+@torch.library.custom_op(f"{NAMESPACE}::scored_attention", mutates_args=())
+def scored_attention(q: Tensor, k: Tensor, v: Tensor, scale: float, causal: bool, kv_lens: Optional[Tensor],
+                     softcap: Optional[float], slopes: Optional[Tensor], doc_ids: Optional[Tensor],
+                     prefix_lens: Optional[Tensor]) -> Tensor:
+    return _k.batch_invariant_attention(q, k, v, scale=scale, mask="causal" if causal else None, kv_lens=kv_lens,
+                                        softcap=softcap, slopes=slopes, doc_ids=doc_ids, prefix_lens=prefix_lens)
+
+
+@scored_attention.register_fake
+def _scored_attention_fake(q, k, v, scale, causal, kv_lens, softcap, slopes, doc_ids, prefix_lens):
+    return q.new_empty(q.shape)
+
+
+@torch.library.custom_op(f"{NAMESPACE}::scored_paged_attention", mutates_args=())
+def scored_paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_table: Tensor,
+                           kv_lens: Optional[Tensor], scale: float, causal: bool, softcap: Optional[float],
+                           slopes: Optional[Tensor], doc_ids: Optional[Tensor],
+                           prefix_lens: Optional[Tensor]) -> Tensor:
+    return _k.batch_invariant_paged_attention(q, k_pages, v_pages, block_table, kv_lens, scale=scale,
+                                              mask="causal" if causal else None, softcap=softcap, slopes=slopes,
+                                              doc_ids=doc_ids, prefix_lens=prefix_lens)
+
+
+@scored_paged_attention.register_fake
+def _scored_paged_attention_fake(q, k_pages, v_pages, block_table, kv_lens, scale, causal, softcap, slopes, doc_ids,
+                                 prefix_lens):
+    return q.new_empty(q.shape)

@@ -62,12 +62,15 @@ def residual_norm(x, res, w1, w2, eps, gate=None, scale=1.0, post=True, pre=True
 
 
 def attention(q, k, v, scale, lens, causal, softcap=None, slopes=None, docs=None, prefix=None):
-    """q [B, Hq, T, D], k / v [B, Hkv, L, D] in 64 bits. Masked keys take no
-    part, whatever K and V hold there; a row that sees none is 0."""
+    """q [B, Hq, T, D], k / v [B, Hkv, L, D] in 64 bits: the outputs, and per
+    output the softmax of |v| and the row's largest score terms (for the bounds:
+    sum |q k| scale, slope x distance). Masked keys take no part, whatever K and
+    V hold there; a row that sees none is 0."""
     q, k, v = q.double(), k.double(), v.double()
     B, Hq, T, D = q.shape
     L, G = k.shape[2], Hq // k.shape[1]
-    out = torch.zeros(B, Hq, T, D, dtype=torch.float64)
+    out, absv = (torch.zeros(B, Hq, T, D, dtype=torch.float64) for _ in range(2))
+    dot, bias = (torch.zeros(B, Hq, T, 1, dtype=torch.float64) for _ in range(2))
     for b in range(B):
         n = L if lens is None else min(max(int(lens[b]), 0), L)
         for t in range(T):
@@ -78,11 +81,33 @@ def attention(q, k, v, scale, lens, causal, softcap=None, slopes=None, docs=None
                 keys = keys[docs[b, :end] == docs[b, p]] if p >= 0 else keys[:0]
             if not len(keys):
                 continue
-            for h in range(Hq):
-                s = k[b, h // G, keys] @ q[b, h, t] * scale
-                if softcap is not None:
-                    s = softcap * torch.tanh(s / softcap)
-                if slopes is not None:
-                    s = s - slopes[h].double() * (p - keys).abs()
-                out[b, h, t] = torch.softmax(s, 0) @ v[b, h // G, keys]
-    return out
+            kk, vv = (x[b, :, keys].repeat_interleave(G, 0) for x in (k, v))
+            qq = q[b, :, t, :, None]
+            s = (kk @ qq)[..., 0] * scale
+            dot[b, :, t, 0] = (kk.abs() @ qq.abs()).amax((1, 2)) * scale
+            if softcap is not None:
+                s = softcap * torch.tanh(s / softcap)
+            if slopes is not None:
+                far = slopes[:, None].double() * (p - keys).abs()
+                bias[b, :, t, 0] = far.abs().amax(1)
+                s = s - far
+            w = torch.softmax(s, 1)[:, None]
+            out[b, :, t], absv[b, :, t] = (w @ vv)[:, 0], (w @ vv.abs())[:, 0]
+    return out, absv, dot, bias
+
+
+def attention_allowance(want, absv, dot, bias, dtype, D, nsplit, softcap=None):
+    """How far an output may be from the 64-bit one. Half a step of the result, and
+    2 A (e_p + e_acc + 2 e_s) with A the softmax of |v|:
+      e_p   = 2^-17 (bf16) / 2^-21 (f16) / 0: a weight is carried as hi + lo;
+      e_acc = (2 x 256 + 2 nsplit) 2^-24: one rounding per MFMA block and merge;
+      e_s     a score's error: (D + 2) 2^-24 of sum |q k| scale; 12 2^-24 softcap
+              for the cap (of 1 - 2 / (x + 1): 2 from x = exp2, 6 from the
+              reciprocal and its argument, 1 from the difference, 2 from the
+              factor and its rounding); 4 2^-24 of the largest slope x distance
+              (slope, its factor, the sum)."""
+    e = 2.0 ** -24
+    e_p = {torch.bfloat16: 2.0 ** -17, torch.float16: 2.0 ** -21, torch.float32: 0.0}[dtype]
+    e_s = (D + 2) * e * dot + 12 * e * (softcap or 0.0) + 4 * e * bias
+    fi = torch.finfo(dtype)
+    return fi.eps / 2 * want.abs() + fi.smallest_normal * fi.eps + 2 * absv * (e_p + (512 + 2 * nsplit) * e + 2 * e_s)
