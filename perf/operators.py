@@ -220,10 +220,13 @@ def prepare(case, seed):
 # ---- one pass: the library's calls -----------------------------------------------------
 
 def _library():
-    pkg = os.path.join(os.getcwd(), "mlx-batch-invariant_amd")
-    if pkg not in sys.path:
-        sys.path.insert(0, pkg)
-    import mlx_batch_invariant_amd as bi
+    """The package, imported by the first pass: a pass is the library's call alone."""
+    bi = sys.modules.get("mlx_batch_invariant_amd")
+    if bi is None:
+        pkg = os.path.join(os.getcwd(), "mlx-batch-invariant_amd")
+        if pkg not in sys.path:
+            sys.path.insert(0, pkg)
+        import mlx_batch_invariant_amd as bi
     return bi
 
 
