@@ -280,7 +280,7 @@ extern "C" int bi_paged_slots(const int32_t* kv_lens, const int32_t* new_lens, i
   if ((B > 0 && (!kv_lens || !new_lens || !block_table || !slots || !positions || !out_lens)) || !out_cursor ||
       (num_free > 0 && !free_pages))
     return fail(BI_E_INVALID_ARG, "%s: null pointer argument", what);
-  if (out_lens == kv_lens || out_lens == new_lens || out_cursor == cursor)
+  if ((B > 0 && (out_lens == kv_lens || out_lens == new_lens)) || out_cursor == cursor)
     return fail(BI_E_INVALID_ARG, "%s: outputs must not be the inputs (every workgroup reads all of them)", what);
   bi::SlotArgs a;
   a.lens = kv_lens; a.news = new_lens; a.free_pages = free_pages; a.cursor = cursor;

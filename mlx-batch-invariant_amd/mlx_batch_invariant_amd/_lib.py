@@ -10,7 +10,6 @@ as the reference does (mlx_batch_invariant/ops.py:36-39).
 
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import os
 import threading
@@ -151,26 +150,43 @@ def load() -> ctypes.CDLL:
         return lib
 
 
-# The three most frequently called entry points go through the CPython binding
-# _bi_pycall when it is built (csrc/bi_pycall.c: the same C functions, about
-# 3 us less host time per call than ctypes' argument conversion), else
-# through ctypes. Same arguments either way; each returns the ABI status code.
+# The most frequently called entry points go through the CPython binding
+# _bi_pycall when it is built (csrc/bi_pycall.c: the same C functions, 3 us
+# less host time per call than ctypes' argument conversion for 15 arguments),
+# else through ctypes. Same arguments either way (host arrays and structs as
+# their values one by one); each returns the ABI status code.
 qmm_call = None
 matmul_call = None
 rms_norm_call = None
+slots_call = None
+rope_paged_call = None
+scored_call = None
+residual_norm_call = None
 
 
 def _bind_fast(lib) -> None:
-    global qmm_call, matmul_call, rms_norm_call
+    global qmm_call, matmul_call, rms_norm_call, slots_call, rope_paged_call, scored_call, residual_norm_call
     qmm_call, matmul_call, rms_norm_call = lib.bi_quantized_matmul, lib.bi_matmul, lib.bi_rms_norm
+    slots_call, residual_norm_call = lib.bi_paged_slots, lib.bi_residual_rms_norm
+
+    def rope_paged_call(*a):
+        return lib.bi_rope_paged_cache(*a[:11], (_c_i64 * 4)(*a[12:16]), a[11], *a[16:27], (_c_i64 * 6)(*a[27:33]),
+                                       *a[33:])
+
+    def scored_call(*a):
+        return lib.bi_attn_scored(*a[:15], (_c_i64 * 9)(*a[15:24]), a[24], a[25], ScoreMod(*a[26:31]), *a[31:])
+
     try:
-        from . import _bi_pycall
+        from . import _bi_pycall as fast
     except ImportError:
         return
     addr = [ctypes.cast(getattr(lib, n), ctypes.c_void_p).value
-            for n in ("bi_quantized_matmul", "bi_matmul", "bi_rms_norm")]
-    _bi_pycall.bind(*addr)
-    qmm_call, matmul_call, rms_norm_call = _bi_pycall.quantized_matmul, _bi_pycall.matmul, _bi_pycall.rms_norm
+            for n in ("bi_quantized_matmul", "bi_matmul", "bi_rms_norm", "bi_paged_slots", "bi_rope_paged_cache",
+                      "bi_attn_scored", "bi_residual_rms_norm")]
+    fast.bind(*addr)
+    qmm_call, matmul_call, rms_norm_call = fast.quantized_matmul, fast.matmul, fast.rms_norm
+    slots_call, rope_paged_call = fast.paged_slots, fast.rope_paged_cache
+    scored_call, residual_norm_call = fast.attn_scored, fast.residual_rms_norm
 
 
 def exported_symbols() -> list[str]:
@@ -205,22 +221,28 @@ def stream_of(t: torch.Tensor) -> int:
 
 
 _current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
-_no_switch = contextlib.nullcontext()
 
 
-def on_device(t: torch.Tensor):
-    """A context in which ``t``'s device is the current one (a launch takes the
-    current device's code): nothing to do where it is already."""
-    return _no_switch if t.get_device() == _current_device() else torch.cuda.device(t.device)
+def launch(dev: int, fn, *args) -> int:
+    """``fn(*args)`` with device ``dev`` current (a launch takes the current
+    device's code)."""
+    if dev == _current_device():
+        return fn(*args)
+    with torch.cuda.device(dev):
+        return fn(*args)
 
 
-def one_device(what: str, *tensors) -> None:
-    """Every tensor (None aside) on the GPU, and on the first one's device."""
-    require_gpu(what, *tensors)
+def one_device(what: str, *tensors) -> int:
+    """Every tensor (None aside) on the GPU, and on the first one's device;
+    returns its index."""
     dev = tensors[0].get_device()
-    for t in tensors[1:]:
-        if t is not None and t.get_device() != dev:
+    for t in tensors:
+        if t is not None and (t.get_device() != dev or not t.is_cuda):
+            require_gpu(what, *tensors)
             raise ValueError(f"{what}: tensors on {tensors[0].device} and {t.device}")
+    if _lib is None:
+        load()
+    return dev
 
 
 def in_place(what: str, *tensors) -> None:
@@ -228,7 +250,7 @@ def in_place(what: str, *tensors) -> None:
     memory, an inference tensor outside inference mode, a leaf that needs a
     gradient."""
     for t in tensors:
-        if any(s <= 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
+        if 0 in t.stride() and any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
             raise ValueError(f"{what}: written tensor with rows that share memory (shape {tuple(t.shape)}, "
                              f"strides {t.stride()})")
         if t.is_inference() and not torch.is_inference_mode_enabled():
@@ -239,7 +261,9 @@ def in_place(what: str, *tensors) -> None:
 
 def written(*tensors) -> None:
     """Count the tensors as changed in place (their version counters)."""
-    torch.autograd.graph.increment_version([t for t in tensors if not t.is_inference()])
+    if any(t.is_inference() for t in tensors):
+        tensors = [t for t in tensors if not t.is_inference()]
+    torch.autograd.graph.increment_version(tensors)
 
 
 def ptr(t: torch.Tensor | None) -> int | None:

@@ -237,17 +237,17 @@ def _scored(what, q, k, v, table, num_pages, page_size, L, kl, scale, causal, so
     (``table`` None) or pools of pages. Host-side checks of what changes the
     scores and masks; see the module's text for their meaning."""
     B, Hq, Tq, D = q.shape
-    mod = _lib.ScoreMod()
+    slope_p = doc_p = prefix_p = None
+    doc_stride = 0
     if softcap is not None:
         softcap = float(softcap)
         if not 0.0 < softcap < 3e38:
             raise ValueError(f"{what}: softcap must be a positive number; got {softcap}")
-        mod.softcap = softcap
     if slopes is not None:
         slopes = torch.as_tensor(slopes, dtype=torch.float32, device=q.device).contiguous()
         if tuple(slopes.shape) != (Hq,):
             raise ValueError(f"{what}: slopes {tuple(slopes.shape)}, expected one for each of {Hq} heads")
-        mod.slopes = slopes.data_ptr()
+        slope_p = slopes.data_ptr()
     if doc_ids is not None:
         if doc_ids.is_floating_point() or doc_ids.ndim != 2 or doc_ids.shape[0] != B or doc_ids.shape[1] < L:
             raise ValueError(f"{what}: doc_ids {doc_ids.dtype} {tuple(doc_ids.shape)}; need whole numbers, {B} rows "
@@ -256,27 +256,25 @@ def _scored(what, q, k, v, table, num_pages, page_size, L, kl, scale, causal, so
         doc_ids = doc_ids.to(torch.int32)
         if doc_ids.stride(1) != 1 or doc_ids.stride(0) < L:
             doc_ids = doc_ids.contiguous()
-        mod.doc_ids, mod.doc_stride = doc_ids.data_ptr(), max(doc_ids.stride(0), L)
+        doc_p, doc_stride = doc_ids.data_ptr(), max(doc_ids.stride(0), L)
     if prefix_lens is not None:
         if not causal:
             raise ValueError(f"{what}: prefix_lens goes with mask='causal'")
         prefix_lens = _lens(prefix_lens, B, L, q.device)
-        mod.prefix_lens = prefix_lens.data_ptr()
+        prefix_p = prefix_lens.data_ptr()
     q = _fix(q)
     out = torch.empty((B, Hq, Tq, D), dtype=q.dtype, device=q.device)
     if B == 0 or Tq == 0:
         return out
     n = _lib.ws_bytes("bi_attn_scored_workspace_bytes", B, Hq, Tq, L, D, int(doc_ids is not None))
     ws = _lib.workspace(n, q.device)
-    strides = (_lib._c_i64 * 9)(q.stride(0), q.stride(1), q.stride(2), k.stride(0), k.stride(1), k.stride(2),
-                                v.stride(0), v.stride(1), v.stride(2))
-    with _lib.on_device(q):
-        rc = _lib.load().bi_attn_scored(q.data_ptr(), k.data_ptr(), v.data_ptr(), _lib.ptr(table),
-                                        0 if table is None else table.stride(0), page_size, num_pages, _lib.ptr(kl),
-                                        out.data_ptr(), B, Hq, v.shape[1], Tq, L, D, strides, 1 if causal else 0,
-                                        float(scale), mod, _lib.DTYPE_CODE[q.dtype], _lib.ptr(ws), n,
-                                        _lib.stream_of(q))
-    _lib.check(rc, "bi_attn_scored")
+    rc = _lib.launch(q.get_device(), _lib.scored_call, q.data_ptr(), k.data_ptr(), v.data_ptr(), _lib.ptr(table),
+                     0 if table is None else table.stride(0), page_size, num_pages, _lib.ptr(kl), out.data_ptr(), B,
+                     Hq, v.shape[1], Tq, L, D, *q.stride()[:3], *k.stride()[:3], *v.stride()[:3], bool(causal),
+                     float(scale), softcap or 0.0, slope_p, doc_p, doc_stride, prefix_p, _lib.DTYPE_CODE[q.dtype],
+                     _lib.ptr(ws), n, _lib.stream_of(q))
+    if rc:
+        _lib.check(rc, "bi_attn_scored")
     return out
 
 

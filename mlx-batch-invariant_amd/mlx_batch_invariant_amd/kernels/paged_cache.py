@@ -35,12 +35,13 @@ class PagedSlots(NamedTuple):
 
 def _int32(what: str, name: str, t, device, shape=None) -> torch.Tensor:
     """``t`` (a tensor of whole numbers, or a list) as contiguous int32 on ``device``."""
-    if isinstance(t, torch.Tensor) and t.dtype not in _INTS:
-        raise ValueError(f"{what}: {name} must hold whole numbers; got {t.dtype}")
-    if isinstance(t, torch.Tensor) and t.is_cuda and t.device != device:
-        raise ValueError(f"{what}: {name} on {t.device}, expected {device}")
-    t = torch.as_tensor(t, dtype=torch.int32, device=device).contiguous()
-    if shape is not None and tuple(t.shape) != tuple(shape):
+    if not (isinstance(t, torch.Tensor) and t.dtype == torch.int32 and t.device == device and t.is_contiguous()):
+        if isinstance(t, torch.Tensor) and t.dtype not in _INTS:
+            raise ValueError(f"{what}: {name} must hold whole numbers; got {t.dtype}")
+        if isinstance(t, torch.Tensor) and t.is_cuda and t.device != device:
+            raise ValueError(f"{what}: {name} on {t.device}, expected {device}")
+        t = torch.as_tensor(t, dtype=torch.int32, device=device).contiguous()
+    if shape is not None and t.shape != shape:
         raise ValueError(f"{what}: {name} {tuple(t.shape)}, expected {tuple(shape)}")
     return t
 
@@ -85,9 +86,10 @@ def paged_slots(kv_lens, new_lens, block_table: torch.Tensor, free_pages, *, pag
     B, max_pages = block_table.shape
     if B > 0 and max_pages == 0:
         raise ValueError(f"{what}: block table without columns")
-    if block_table.stride(1) != 1 and max_pages > 1 or B > 1 and block_table.stride(0) < max_pages:
+    stride, one = block_table.stride()
+    if one != 1 and max_pages > 1 or B > 1 and stride < max_pages:
         raise ValueError(f"{what}: block table rows must be contiguous and apart; got strides {block_table.stride()}")
-    _lib.one_device(what, block_table)
+    index = _lib.one_device(what, block_table)
     _lib.in_place(what, block_table)
     dev = block_table.device
     lens = _int32(what, "kv_lens", kv_lens, dev, (B,))
@@ -97,22 +99,25 @@ def paged_slots(kv_lens, new_lens, block_table: torch.Tensor, free_pages, *, pag
         raise ValueError(f"{what}: free_pages must be one list; got {tuple(free.shape)}")
     cur = None if cursor is None else _int32(what, "cursor", cursor, dev, (1,))
     slots = torch.empty((B, max_new), dtype=torch.int64, device=dev)
-    positions = torch.empty((B, max_new), dtype=torch.int32, device=dev)
-    out = torch.empty(B + 1, dtype=torch.int32, device=dev)
-    stride = block_table.stride(0) if B > 1 else max_pages
-    with _lib.on_device(block_table):
-        rc = _lib.load().bi_paged_slots(lens.data_ptr(), news.data_ptr(), block_table.data_ptr(), max(stride, 1),
-                                        max(max_pages, 1), free.data_ptr(), free.numel(), _lib.ptr(cur),
-                                        slots.data_ptr(), positions.data_ptr(), out.data_ptr(),
-                                        out.data_ptr() + 4 * B, B, max_new, page_size, _lib.stream_of(block_table))
-    _lib.check(rc, "bi_paged_slots")
+    positions = torch.empty_like(slots, dtype=torch.int32)
+    out = torch.empty_like(lens)
+    end = lens.new_empty(1) if cur is None else torch.empty_like(cur)
+    max_pages = max(max_pages, 1)
+    rc = _lib.launch(index, _lib.slots_call, lens.data_ptr(), news.data_ptr(), block_table.data_ptr(),
+                     stride if B > 1 else max_pages, max_pages, free.data_ptr(), free.numel(), _lib.ptr(cur),
+                     slots.data_ptr(), positions.data_ptr(), out.data_ptr(), end.data_ptr(), B, max_new, page_size,
+                     _lib.stream_of(block_table))
+    if rc:
+        _lib.check(rc, "bi_paged_slots")
     _lib.written(block_table)
-    return PagedSlots(slots, positions, out[:B], out[B:])
+    return PagedSlots(slots, positions, out, end)
 
 
 def _rows(t: torch.Tensor) -> torch.Tensor:
     """``t`` [B, T, H, D] with contiguous heads and all tokens at one stride of
     whole 16-byte pieces (such as a slice of a joint projection), else a copy."""
+    if t.is_contiguous() and t.data_ptr() % 16 == 0:
+        return t
     B, T, H, D = t.shape
     unit = 16 // t.element_size()
     s = t.stride()
@@ -122,6 +127,11 @@ def _rows(t: torch.Tensor) -> torch.Tensor:
     if not ok:
         t = t.contiguous()
     return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _packed(t: torch.Tensor) -> torch.Tensor:
+    """``t`` contiguous and 16-byte aligned, or a copy that is."""
+    return t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
 
 
 def _row_stride(t: torch.Tensor) -> int:
@@ -150,14 +160,15 @@ def rope_paged_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: tor
     product and sum is in fp32, the result rounded once.
     """
     what = "rope_paged_cache"
-    if q.ndim != 4 or k.ndim != 4 or k.shape != v.shape or q.shape[:2] != k.shape[:2] or q.shape[3] != k.shape[3]:
+    qs, ks, ps = q.shape, k.shape, k_pages.shape
+    if len(qs) != 4 or len(ks) != 4 or ks != v.shape or qs[:2] != ks[:2] or qs[3] != ks[3]:
         raise ValueError(f"{what}: shapes q {tuple(q.shape)} k {tuple(k.shape)} v {tuple(v.shape)}")
-    B, T, Hq, D = q.shape
-    Hkv = k.shape[2]
-    if k_pages.ndim != 4 or k_pages.shape != v_pages.shape or k_pages.shape[1] != Hkv or k_pages.shape[3] != D:
+    B, T, Hq, D = qs
+    Hkv = ks[2]
+    if len(ps) != 4 or ps != v_pages.shape or ps[1] != Hkv or ps[3] != D:
         raise ValueError(f"{what}: pools {tuple(k_pages.shape)} and {tuple(v_pages.shape)} for {Hkv} heads of {D}")
     dt = q.dtype
-    if dt not in _lib.FLOAT_DTYPES or any(t.dtype != dt for t in (k, v, k_pages, v_pages)):
+    if dt not in _lib.FLOAT_DTYPES or not dt == k.dtype == v.dtype == k_pages.dtype == v_pages.dtype:
         raise ValueError(f"{what}: q, k, v and the pools must have one type of {_lib.FLOAT_DTYPES}; got "
                          f"{[str(t.dtype) for t in (q, k, v, k_pages, v_pages)]}")
     if cos.ndim != 2 or cos.shape != sin.shape or cos.dtype != sin.dtype or cos.dtype not in (dt, torch.float32):
@@ -165,41 +176,41 @@ def rope_paged_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: tor
                          f"one shape [n, R] in {dt} or float32")
     if slots.dtype not in (torch.int64, torch.int32) or tuple(slots.shape) != (B, T):
         raise ValueError(f"{what}: slots {slots.dtype} {tuple(slots.shape)}, expected int64 {(B, T)}")
-    page_size = k_pages.shape[2]
+    page_size = ps[2]
     _page_size(what, page_size)
     half = cos.shape[1]
-    sections = (half,) if sections is None else tuple(int(s) for s in sections)
-    if not 1 <= len(sections) <= 4 or any(s < 0 for s in sections) or sum(sections) != half:
+    sections = (half,) if sections is None else tuple(map(int, sections))
+    if not 1 <= len(sections) <= 4 or min(sections) < 0 or sum(sections) != half:
         raise ValueError(f"{what}: sections {sections} of tables with {half} columns (1 to 4 axes)")
     if D % 16 or half % 8 or not 0 < half <= D // 2 or cos.shape[0] == 0:
         raise ValueError(f"{what}: head dim {D} with tables {tuple(cos.shape)}: need D % 16 == 0 and a positive "
                          "multiple of 8 columns, at most D / 2")
-    _lib.one_device(what, q, k, v, cos, sin, slots, k_pages, v_pages)
+    index = _lib.one_device(what, q, k, v, cos, sin, slots, k_pages, v_pages)
     _lib.in_place(what, k_pages, v_pages)
     unit = 16 // q.element_size()
-    for t in (k_pages, v_pages):
-        if t.stride(3) != 1 or any(s % unit for s in t.stride()[:3]) or t.data_ptr() % 16:
-            raise ValueError(f"{what}: pool rows must be contiguous and 16-byte aligned; got strides {t.stride()}")
-    A = len(sections)
-    pos = _int32(what, "positions", positions, q.device)
-    if tuple(pos.shape) not in (((A, B, T), (B, T)) if A == 1 else ((A, B, T),)):
+    kst, vst = k_pages.stride(), v_pages.stride()
+    kp, vp = k_pages.data_ptr(), v_pages.data_ptr()
+    for s, p in ((kst, kp), (vst, vp)):
+        if s[3] != 1 or s[0] % unit or s[1] % unit or s[2] % unit or p % 16:
+            raise ValueError(f"{what}: pool rows must be contiguous and 16-byte aligned; got strides {s}")
+    A, dev = len(sections), q.device
+    pos = _int32(what, "positions", positions, dev)
+    if pos.shape != (A, B, T) and (A > 1 or pos.shape != (B, T)):
         raise ValueError(f"{what}: positions {tuple(pos.shape)}, expected {(A, B, T)}")
-    out = torch.empty((B, Hq, T, D), dtype=dt, device=q.device)
-    if B == 0 or T == 0 or k_pages.shape[0] == 0 and Hq == 0:
+    out = torch.empty((B, Hq, T, D), dtype=dt, device=dev)
+    if B == 0 or T == 0:
         return out
-    if k_pages.shape[0] == 0:
+    if ps[0] == 0:
         raise ValueError(f"{what}: a pool without pages")
-    q, k, v = _rows(q), _rows(k), _rows(v)
-    cos, sin = (t if t.is_contiguous() and t.data_ptr() % 16 == 0 else t.clone(memory_format=torch.contiguous_format)
-                for t in (cos, sin))
-    slots = slots.to(torch.int64).contiguous()
-    strides = (_lib._c_i64 * 6)(*k_pages.stride()[:3], *v_pages.stride()[:3])
-    with _lib.on_device(q):
-        rc = _lib.load().bi_rope_paged_cache(
-            q.data_ptr(), _row_stride(q), k.data_ptr(), _row_stride(k), v.data_ptr(), _row_stride(v), cos.data_ptr(),
-            sin.data_ptr(), cos.shape[0], _lib.DTYPE_CODE[cos.dtype], pos.data_ptr(), (_lib._c_i64 * A)(*sections), A,
-            slots.data_ptr(), out.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), k_pages.shape[0], page_size, B,
-            T, Hq, Hkv, D, strides, _lib.DTYPE_CODE[dt], _lib.stream_of(q))
-    _lib.check(rc, "bi_rope_paged_cache")
+    q, k, v, cos, sin = _rows(q), _rows(k), _rows(v), _packed(cos), _packed(sin)
+    if slots.dtype != torch.int64 or not slots.is_contiguous():
+        slots = slots.to(torch.int64).contiguous()
+    rc = _lib.launch(index, _lib.rope_paged_call, q.data_ptr(), _row_stride(q), k.data_ptr(), _row_stride(k),
+                     v.data_ptr(), _row_stride(v), cos.data_ptr(), sin.data_ptr(), cos.shape[0],
+                     _lib.DTYPE_CODE[cos.dtype], pos.data_ptr(), A, *sections, *(0,) * (4 - A), slots.data_ptr(),
+                     out.data_ptr(), kp, vp, ps[0], page_size, B, T, Hq, Hkv, D, *kst[:3], *vst[:3],
+                     _lib.DTYPE_CODE[dt], _lib.stream_of(q))
+    if rc:
+        _lib.check(rc, "bi_rope_paged_cache")
     _lib.written(k_pages, v_pages)
     return out

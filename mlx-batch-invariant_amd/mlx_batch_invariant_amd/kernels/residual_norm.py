@@ -16,8 +16,8 @@ from .. import _lib
 
 def _weight(what: str, name: str, w, x):
     """A weight vector as contiguous elements of x's type (None stays None)."""
-    if w is None:
-        return None
+    if w is None or w.dtype == x.dtype and w.ndim == 1 and w.is_contiguous() and w.shape[0] == x.shape[-1]:
+        return w
     if w.numel() != x.shape[-1]:
         raise ValueError(f"{what}: {name} has {w.numel()} elements, expected {x.shape[-1]}")
     w = w.reshape(-1)
@@ -29,9 +29,9 @@ def _gate(what: str, gate, x):
     and a gate of x's shape are read in place, and so is one that is constant
     over the last token dims ([B, 1, D] for x [B, T, D]); other broadcasts are
     laid out first."""
-    D, rows = x.shape[-1], x.numel() // x.shape[-1]
     if gate is None:
         return None, 0, 1
+    D, rows = x.shape[-1], x.numel() // x.shape[-1]
     if gate.ndim == 0 or gate.ndim > x.ndim or gate.shape[-1] != D or any(
             a != b and a != 1 for a, b in zip(reversed(gate.shape), reversed(x.shape))):
         raise ValueError(f"{what}: gate {tuple(gate.shape)} does not broadcast over rows of {tuple(x.shape)}")
@@ -51,6 +51,16 @@ def _gate(what: str, gate, x):
     return gate.expand(x.shape).contiguous().reshape(rows, D), D, 1
 
 
+def _rows(t, rows: int, D: int):
+    """t as rows of D contiguous elements, and the elements between rows."""
+    if t.is_contiguous():
+        return t, D
+    t = t.reshape(rows, D)
+    if t.stride(1) != 1 and D > 1 or t.stride(0) < D and rows > 1:
+        t = t.contiguous()
+    return t, max(t.stride(0), D)
+
+
 def batch_invariant_residual_rms_norm(x: torch.Tensor, residual: torch.Tensor, post_weight: torch.Tensor | None,
                                       pre_weight: torch.Tensor | None, eps: float, *,
                                       gate: torch.Tensor | None = None, scale: float = 1.0, post_norm: bool = True,
@@ -64,32 +74,30 @@ def batch_invariant_residual_rms_norm(x: torch.Tensor, residual: torch.Tensor, p
     weights and gate are converted to x's type. ``h`` is taken from y before its
     rounding, so it is not the bits of ``batch_invariant_rms_norm(y, ...)``."""
     what = "batch_invariant_residual_rms_norm"
-    if x.dtype not in _lib.FLOAT_DTYPES or residual.dtype != x.dtype:
+    dt, shape = x.dtype, x.shape
+    if dt not in _lib.FLOAT_DTYPES or residual.dtype != dt:
         raise ValueError(f"{what}: unsupported dtypes {x.dtype} and {residual.dtype}")
-    if x.ndim == 0 or x.shape != residual.shape:
+    if not shape or residual.shape != shape:
         raise ValueError(f"{what}: shapes {tuple(x.shape)} and {tuple(residual.shape)}")
     if not post_norm and not pre_norm:
         raise ValueError(f"{what}: neither post_norm nor pre_norm")
     if not post_norm and post_weight is not None or not pre_norm and pre_weight is not None:
         raise ValueError(f"{what}: a weight for a norm that is not asked for")
-    _lib.one_device(what, x, residual, post_weight, pre_weight, gate)
-    D = x.shape[-1]
-    y = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-    h = torch.empty(x.shape, dtype=x.dtype, device=x.device) if pre_norm else None
+    dev = _lib.one_device(what, x, residual, post_weight, pre_weight, gate)
+    D = shape[-1]
+    y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    h = torch.empty_like(y) if pre_norm else None
     w1, w2 = _weight(what, "post_weight", post_weight, x), _weight(what, "pre_weight", pre_weight, x)
-    if x.numel() == 0:
+    n = x.numel()
+    if n == 0:
         return y, h
-    rows = x.numel() // D
+    rows = n // D
     g, g_stride, g_group = _gate(what, gate, x)
-    x2, r2 = (t if t.ndim == 2 else t.reshape(rows, D) for t in (x, residual))
-    if x2.stride(-1) != 1 or x2.stride(0) < D:
-        x2 = x2.contiguous()
-    if r2.stride(-1) != 1 or r2.stride(0) < D:
-        r2 = r2.contiguous()
-    with _lib.on_device(x):
-        rc = _lib.load().bi_residual_rms_norm(x2.data_ptr(), max(x2.stride(0), D), r2.data_ptr(),
-                                              max(r2.stride(0), D), _lib.ptr(g), g_stride, g_group,
-                                              _lib.ptr(w1), _lib.ptr(w2), y.data_ptr(), _lib.ptr(h), rows, D, float(eps), float(scale), int(post_norm),
-                                              int(pre_norm), _lib.DTYPE_CODE[x.dtype], _lib.stream_of(x))
-    _lib.check(rc, "bi_residual_rms_norm")
+    x2, x_stride = _rows(x, rows, D)
+    r2, r_stride = _rows(residual, rows, D)
+    rc = _lib.launch(dev, _lib.residual_norm_call, x2.data_ptr(), x_stride, r2.data_ptr(), r_stride, _lib.ptr(g),
+                     g_stride, g_group, _lib.ptr(w1), _lib.ptr(w2), y.data_ptr(), _lib.ptr(h), rows, D, float(eps),
+                     float(scale), bool(post_norm), bool(pre_norm), _lib.DTYPE_CODE[dt], _lib.stream_of(x))
+    if rc:
+        _lib.check(rc, "bi_residual_rms_norm")
     return y, h

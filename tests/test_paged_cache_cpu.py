@@ -163,3 +163,34 @@ def test_operators_are_registered():
         assert s.shape == pos.shape == (5, 3) and s.dtype == torch.int64 and lens.shape == (5,) and cur.shape == (1,)
         o = _rope_operands()
         assert torch.ops.mlx_bi.rope_paged_cache(*o.values(), None).shape == (2, 4, 3, 32)
+
+
+def test_bindings_agree():
+    """The CPython binding and ctypes hand the same arguments over: each refuses
+    what the other does, with the same text."""
+    from mlx_batch_invariant_amd import _bi_pycall as fast
+    lib = _lib.load()
+    assert _lib.slots_call is fast.paged_slots and _lib.rope_paged_call is fast.rope_paged_cache
+    assert _lib.scored_call is fast.attn_scored and _lib.residual_norm_call is fast.residual_rms_norm
+
+    slots = [16, 16, 16, 4, 4, 16, 9, None, 16, 16, 32, 32, 2, 3, 24, None]
+    rope = [16, 512, 16, 256, 16, 256, 16, 16, 9, 0, 16, 2, 16, 24, 7, 7, 16, 16, 16, 16, 5, 16, 2, 3, 4, 2, 128,
+            *(128, 256, 384, 512, 640, 100), 2, None]
+    scored = [256] * 3 + [None, 0, 0, 0, None, 256, 1, 4, 2, 4, 300, 128, *(128 * i for i in range(1, 10)), 1, 0.5, 2.0,
+              None, 256, 299, None, 2, None, 0, None]
+    norm = [16, 16, 16, 15, None, 0, 1, 16, 16, 16, 16, 2, 16, 1e-6, 2.0, 1, 1, 2, None]
+    for calls in (((fast.paged_slots, lib.bi_paged_slots), slots), ((fast.residual_rms_norm, lib.bi_residual_rms_norm), norm),
+                  ((fast.rope_paged_cache, lambda *a: lib.bi_rope_paged_cache(
+                      *a[:11], (ctypes.c_int64 * 4)(*a[12:16]), a[11], *a[16:27], (ctypes.c_int64 * 6)(*a[27:33]),
+                      *a[33:])), rope),
+                  ((fast.attn_scored, lambda *a: lib.bi_attn_scored(
+                      *a[:15], (ctypes.c_int64 * 9)(*a[15:24]), a[24], a[25], _lib.ScoreMod(*a[26:31]), *a[31:])),
+                   scored)):
+        (f, g), args = calls
+        got = f(*args)
+        text = _err(lib)
+        assert got == g(*args) < 0 and _err(lib) == text and text
+        with pytest.raises(TypeError, match="arguments"):
+            f(*args, 0)
+        with pytest.raises(TypeError):
+            f("x", *args[1:])
