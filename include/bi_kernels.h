@@ -342,7 +342,8 @@ typedef struct bi_score_mod {
   int64_t doc_stride;
   const int32_t* prefix_lens;
 } bi_score_mod;
-size_t bi_attn_scored_workspace_bytes(int64_t B, int64_t Hq, int64_t Tq, int64_t L, int64_t D, int has_docs);
+size_t bi_attn_scored_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t Tq, int64_t L, int64_t D,
+                                      int causal, int has_docs, int dtype);
 int bi_attn_scored(const void* q, const void* k, const void* v, const int32_t* block_table, int64_t table_stride,
                    int64_t page_size, int64_t num_pages, const int32_t* kv_lens, void* out, int64_t B, int64_t Hq,
                    int64_t Hkv, int64_t Tq, int64_t L, int64_t D, const int64_t* strides, int causal, float scale,

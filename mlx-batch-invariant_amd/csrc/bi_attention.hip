@@ -206,9 +206,11 @@ int decode_impl(const char* what, const void* q, const void* k, const void* v, c
 #undef BI_DEC
 }
 
-// The instantiation with the score terms of a.mod.
+// Few rows: the split-parallel kernel, its partials in the workspace. Else the
+// instantiation with the score terms of a.mod.
 template <typename T>
-int launch_prefill_scored(int D, bi::ModPrefillArgs& a, hipStream_t st) {
+int launch_prefill_scored(int D, bi::ModRowsArgs& a, hipStream_t st) {
+  if (a.pm) return bi::with_head_dim(D, [&](auto dd) { return bi::launch_rows_mod<T, dd.value>(a, st); });
   const bool cap = a.mod.cap_log2 != 0.0f, bias = a.mod.slopes != nullptr;
   return bi::with_head_dim(D, [&](auto dd) {
     constexpr int kD = dd.value;
@@ -223,7 +225,7 @@ int prefill_impl(const char* what, const void* q, const void* k, const void* v, 
                  void* out, int64_t B, int64_t Hq, int64_t Hkv, int64_t Tq, int64_t L, int64_t D,
                  const int64_t* strides, int causal, float scale, int dtype, void* stream, const int32_t* table,
                  int64_t table_stride, int page_shift, int64_t num_pages, bool per_key = false,
-                 int64_t split = bi::kSplit, const bi::ScoreMod* mod = nullptr) {
+                 int64_t split = bi::kSplit, const bi::ScoreMod* mod = nullptr, float* partials = nullptr) {
   using namespace bi_host;
   if (per_key && (split <= 0 || split > kMaxSplit))
     return fail(BI_E_INVALID_ARG, "%s: split_size %lld must be in [1, 2^20]", what, (long long)split);
@@ -253,7 +255,7 @@ int prefill_impl(const char* what, const void* q, const void* k, const void* v, 
       (!per_key && wgs * Hkv * B > 0x7fffffffLL - 8) ||
       (per_key && B * Hq * ((Tq + bi::pk_prefill_qb(D) - 1) / bi::pk_prefill_qb(D)) > ((int64_t)1 << 27)))
     return fail(BI_E_UNSUPPORTED, "%s: grid too large", what);
-  bi::ModPrefillArgs a;
+  bi::ModRowsArgs a;
   a.q = q; a.k = k; a.v = v; a.kv_lens = kv_lens; a.out = out;
   a.table = table; a.table_stride = table_stride; a.page_shift = page_shift; a.num_pages = (int)num_pages;
   a.B = (int)B; a.Hq = (int)Hq; a.Hkv = (int)Hkv; a.Tq = (int)Tq; a.L = (int)L;
@@ -267,6 +269,13 @@ int prefill_impl(const char* what, const void* q, const void* k, const void* v, 
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (mod) {
     a.mod = *mod;
+    a.nsplit = (int)((L + bi::kSplit - 1) / bi::kSplit);
+    const int64_t n = B * Hq * Tq * a.nsplit, up = (n + 3) / 4 * 4;
+    a.pm = partials;
+    a.pl = partials ? partials + up : nullptr;
+    a.pacc = partials ? partials + 2 * up : nullptr;
+    if (partials && ((Tq * (Hq / Hkv) + 15) / 16 * a.nsplit * Hkv * B > 0x7fffffffLL - 8 || n > ((int64_t)1 << 36)))
+      return fail(BI_E_UNSUPPORTED, "%s: grid too large", what);
     switch (dtype) {
       case BI_BF16: return launch_prefill_scored<bi::bf16>((int)D, a, st);
       case BI_F16: return launch_prefill_scored<bi::f16>((int)D, a, st);
@@ -393,10 +402,11 @@ int check_score_mod(const char* what, const bi_score_mod* m, int64_t L, float sc
 
 }  // namespace
 
-extern "C" size_t bi_attn_scored_workspace_bytes(int64_t B, int64_t Hq, int64_t Tq, int64_t L, int64_t D,
-                                                 int has_docs) {
-  if (B <= 0 || Hq <= 0 || Tq <= 0 || L <= 0 || D <= 0) return 0;
+extern "C" size_t bi_attn_scored_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t Tq, int64_t L, int64_t D,
+                                                 int causal, int has_docs, int dtype) {
+  if (B <= 0 || Hq <= 0 || Hkv <= 0 || Hq % Hkv || Tq <= 0 || L <= 0 || D <= 0) return 0;
   if (Tq == 1) return decode_ws_bytes(B, Hq, L, D, bi::kSplit);
+  if (bi::few_rows(B, Hq, Hkv, Tq, L, D, causal, dtype)) return (size_t)bi::rows_partial_bytes(B, Hq, Tq, L, D);
   return has_docs ? (size_t)(B * ((L + bi::kSplit - 1) / bi::kSplit)) * sizeof(int2) : 0;
 }
 
@@ -414,24 +424,30 @@ extern "C" int bi_attn_scored(const void* q, const void* k, const void* v, const
   int shift = 0;
   if (B > 0 && block_table && (rc = check_pages(what, block_table, table_stride, page_size, num_pages, L, &shift)))
     return rc;
-  if (!strides) return bi_host::fail(BI_E_INVALID_ARG, "%s: null pointer argument", what);
+  if (B > 0 && (!q || !k || !v || !out || !strides))
+    return bi_host::fail(BI_E_INVALID_ARG, "%s: null pointer argument", what);
+  if (B == 0) return BI_OK;
+  if (Tq > 1 && causal && Tq > L)
+    return bi_host::fail(BI_E_INVALID_ARG, "%s: causal needs Tq (%lld) <= L (%lld)", what, (long long)Tq, (long long)L);
   if (Tq == 1) {
     const int64_t st8[8] = {strides[0], strides[1], strides[3], strides[4], strides[5],
                             strides[6], strides[7], strides[8]};
     return decode_impl(what, q, k, v, kv_lens, out, B, Hq, Hkv, L, D, st8, scale, dtype, ws, ws_bytes, stream,
                        block_table, table_stride, shift, num_pages, false, bi::kSplit, &mod);
   }
-  if (B > 0 && mod.docs) {
-    const size_t need = bi_attn_scored_workspace_bytes(B, Hq, Tq, L, D, 1);
+  const size_t need = bi_attn_scored_workspace_bytes(B, Hq, Hkv, Tq, L, D, causal, mod.docs != nullptr, dtype);
+  float* partials = nullptr;
+  if (need > 0) {
     if (!ws || ws_bytes < need || !bi_host::aligned16(ws))
       return bi_host::fail(BI_E_WORKSPACE, "%s: 16-byte aligned workspace of %zu bytes required, got %zu", what, need,
                            ws ? ws_bytes : (size_t)0);
     if (B * ((L + bi::kSplit - 1) / bi::kSplit) > 0x7fffffffLL)
       return bi_host::fail(BI_E_UNSUPPORTED, "%s: grid too large", what);
-    mod.ranges = static_cast<const int2*>(ws);
+    if (bi::few_rows(B, Hq, Hkv, Tq, L, D, causal, dtype)) partials = static_cast<float*>(ws);
+    else mod.ranges = static_cast<const int2*>(ws);
   }
   return prefill_impl(what, q, k, v, kv_lens, out, B, Hq, Hkv, Tq, L, D, strides, causal, scale, dtype, stream,
-                      block_table, table_stride, shift, num_pages, false, bi::kSplit, &mod);
+                      block_table, table_stride, shift, num_pages, false, bi::kSplit, &mod, partials);
 }
 
 // ---------------------------------------------------------------------------

@@ -2,6 +2,8 @@
 // per (element type, head dim) in bi_attn_{bf16,f16,f32}.hip.
 #pragma once
 
+#include <algorithm>
+
 #include "bi_attn_common.h"
 
 namespace bi {
@@ -38,6 +40,31 @@ template <typename T, int D>
 int launch_decode_mod(ModDecodeArgs& a, hipStream_t st);
 template <typename T, int D, int MOD>
 int launch_prefill_mod(ModPrefillArgs& a, hipStream_t st);
+template <typename T, int D>
+int launch_rows_mod(ModRowsArgs& a, hipStream_t st);
+
+// Bytes of the partials (m, l, acc) of every row and split of a chunk of Tq tokens.
+inline int64_t rows_partial_bytes(int64_t B, int64_t Hq, int64_t Tq, int64_t L, int64_t D) {
+  const int64_t n = B * Hq * Tq * ((L + kSplit - 1) / kSplit);
+  return ((n + 3) / 4 * 4 * 2 + n * D) * (int64_t)sizeof(float);
+}
+// Whether attn_rows_mod takes a chunk (a workgroup per split and 16 rows) or
+// attn_prefill_mod (one that walks the splits of 64 rows). Walking costs the
+// longest row's splits, whatever the rows, while these leave CUs idle; per split
+// and 16 rows K and V come from the cache again. With R the 16-row chunks, less
+// the half that a causal chunk's own triangle leaves out, and N the splits, 32 /
+// 8 heads of 128 in bf16 (us, walk / split): R = 32, N = 16: 104 / 32; R = 192,
+// N = 3: 22 / 23; N = 16: 114 / 75; R = 384, N = 16: 123 / 138; R = 512, N = 7: 46
+// / 154; N = 1 always slower (a second launch merges). fp32, 8 / 8 heads: R = 64,
+// N = 16: 571 / 28; R = 300, N = 3: 93 / 81; R = 520, N = 9: 292 / 297; 32 / 8
+// heads R = 400, N = 2: 59 / 82. Heads of 64 turn at about the same R (420 and
+// 680). The partials stay below 256 MB.
+inline bool few_rows(int64_t B, int64_t Hq, int64_t Hkv, int64_t Tq, int64_t L, int64_t D, int causal, int dtype) {
+  const int64_t n = (L + kSplit - 1) / kSplit;
+  const int64_t chunks = (Tq * (Hq / Hkv) + 15) / 16 * Hkv * B;
+  const int64_t r = causal ? chunks - chunks * std::min(Tq, L) / (2 * L) : chunks;
+  return r <= (dtype == BI_F32 ? 380 : 300 - 320 / n) && rows_partial_bytes(B, Hq, Tq, L, D) <= ((int64_t)256 << 20);
+}
 // The reference's per-key order on the vector ALUs (bi_attn_perkey.h).
 template <typename T, int D>
 int launch_decode_perkey(DecodeArgs& a, hipStream_t st);

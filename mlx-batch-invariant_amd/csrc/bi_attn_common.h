@@ -99,6 +99,12 @@ struct ScoreMod {
 };
 struct ModDecodeArgs : DecodeArgs { ScoreMod mod; };
 struct ModPrefillArgs : PrefillArgs { ScoreMod mod; };
+struct ModRowsArgs : ModPrefillArgs {     // partials of every (b, head, token) row and split
+  float* pm;
+  float* pl;
+  float* pacc;
+  int nsplit;
+};
 
 // Score variants of a kernel instantiation: 0 the plain ones; kModAny reads
 // ScoreMod's masks, and the other bits its score terms.

@@ -27,6 +27,33 @@
 
 namespace bi {
 
+// Keys [0, n) that a (token, head) row may see; a document mask comes on top.
+// Grows with the row, so a tile's last row has its largest limit.
+template <class Args>
+__device__ __forceinline__ int mod_nkeys(const Args& a, const int32_t* docs, int len, int prefix, int G, int npairs,
+                                         int pair) {
+  if (pair >= npairs) return 0;
+  const int end = len - a.Tq + pair / G + 1;            // keys up to the row's own position
+  if (end <= 0 && (a.causal || docs)) return 0;
+  return a.causal ? max(end, prefix) : len;
+}
+
+// Infinities and NaN of a fragment as 0.
+template <typename F>
+__device__ __forceinline__ F finite_frag(F v) {
+  if constexpr (std::is_same_v<F, f32x8>) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      v.lo[e] = fabsf(v.lo[e]) < INFINITY ? v.lo[e] : 0.0f;
+      v.hi[e] = fabsf(v.hi[e]) < INFINITY ? v.hi[e] : 0.0f;
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = fabsf((float)v[e]) < INFINITY ? v[e] : (decltype(v[e] + v[e]))0;
+  }
+  return v;
+}
+
 // Keys per ring chunk: as in the plain kernel's forms without FEW.
 template <typename T, int D, int MODE>
 constexpr int mod_chunk() {
@@ -83,13 +110,7 @@ __global__ __launch_bounds__(256, (mod_min_blocks<T, D, MODE>())) void attn_pref
   const int len = __builtin_amdgcn_readfirstlane(a.kv_lens ? min(max(a.kv_lens[b], 0), a.L) : a.L);
   const int prefix = a.mod.prefix ? min(max(a.mod.prefix[b], 0), len) : 0;
   const int32_t* docs = a.mod.docs ? a.mod.docs + (int64_t)b * a.mod.docs_sb : nullptr;
-  // Keys [0, n) that a (token, head) row may see; the document mask comes on top.
-  auto nkeys_of = [&](int pair) -> int {
-    if (pair >= npairs) return 0;
-    const int end = len - a.Tq + pair / G + 1;          // keys up to the row's own position
-    if (end <= 0 && (a.causal || docs)) return 0;
-    return a.causal ? max(end, prefix) : len;
-  };
+  auto nkeys_of = [&](int pair) -> int { return mod_nkeys(a, docs, len, prefix, G, npairs, pair); };
   const int maxkeys = nkeys_of(min(64 * wg + 63, npairs - 1));
   const int my_pair = 64 * wg + 16 * wave + r;          // score-layout row of this lane
   const int my_nkeys = nkeys_of(my_pair);
@@ -498,6 +519,319 @@ __global__ __launch_bounds__(256, (mod_min_blocks<T, D, MODE>())) void attn_pref
       o[16 * dt] = to_store<T>(x);
     }
   }
+}
+
+// ---------------------------------------------------------------------------
+// Few rows: one 256-thread workgroup per (sequence, kv head, 16 (token, head)
+// rows, split), so that a short chunk against a long cache has as many
+// workgroups as there are splits instead of walking them one after another.
+// Wave w scores keys 64 w .. 64 w + 63 (K in registers), the split's maximum is
+// exchanged through LDS, each wave writes its keys' weights there, and wave w
+// computes P.V of dims 16 dt, dt = w, w + 4, ..., from the split's V in LDS
+// (attn_decode_mfma's scheme with rows for heads). Writes (m, l, acc) of its
+// split; attn_rows_combine merges them in order, so the results are the bits of
+// attn_prefill_mod. LDS is the split's V and 16 KB of weights, the wave maxima
+// inside them: 80 KB for 16-bit D = 128, two workgroups per CU.
+// ---------------------------------------------------------------------------
+template <typename T, int D, int MODE>
+__global__ __launch_bounds__(256) void attn_rows_mod(ModRowsArgs a) {
+  constexpr bool ROWPAGED = MODE == kKvRowPaged, TILED = MODE == kKvTilePaged;
+  typedef typename Frag<T>::type F;
+  constexpr int NVP = decode_v_slices<T, D>();
+  constexpr int DV = D / NVP;                           // dims per V slice
+  typedef KVTile<T, DV> KV;
+  constexpr int KT = 4, KS = D / 32;                    // score tiles per wave
+  constexpr int NDTV = DV / 16, NJ = (NDTV + 3) / 4;    // P.V dim tiles per slice, per wave
+  constexpr int CPW = KV::copies(kSplit) / 4;           // V copy instructions per wave and slice
+  static_assert(DV % 16 == 0 && CPW >= 1 && CPW < 64, "attn_rows_mod: V slice tiling");
+  __shared__ __attribute__((aligned(1024))) char Vs[kSplit * KV::kRowBytes];
+  __shared__ __attribute__((aligned(16))) float Ps[16][kSplit];
+
+  const int tid = threadIdx.x;
+  const int lane = tid % kWave;
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int r = lane % 16, qq = lane / 16;
+  const int G = a.Hq / a.Hkv, npairs = a.Tq * G;
+  // Items (b, hk, split, row chunk) in that nesting order, a contiguous range of
+  // them per XCD: the row chunks that read one split's K and V share an L2.
+  const int nchunks = (npairs + 15) / 16;
+  const int64_t items = (int64_t)nchunks * a.nsplit * a.Hkv * a.B;
+  const int64_t per_xcd = (items + 7) / 8;
+  const int64_t item = (int64_t)(blockIdx.x % 8) * per_xcd + blockIdx.x / 8;
+  if (blockIdx.x / 8 >= per_xcd || item >= items) return;
+  const int chunk = __builtin_amdgcn_readfirstlane((int)(item % nchunks));
+  const int split = __builtin_amdgcn_readfirstlane((int)(item / nchunks % a.nsplit));
+  const int hk = __builtin_amdgcn_readfirstlane((int)(item / nchunks / a.nsplit % a.Hkv));
+  const int b = __builtin_amdgcn_readfirstlane((int)(item / nchunks / a.nsplit / a.Hkv));
+  const int len = __builtin_amdgcn_readfirstlane(a.kv_lens ? min(max(a.kv_lens[b], 0), a.L) : a.L);
+  const int prefix = a.mod.prefix ? min(max(a.mod.prefix[b], 0), len) : 0;
+  const int32_t* docs = a.mod.docs ? a.mod.docs + (int64_t)b * a.mod.docs_sb : nullptr;
+  auto nkeys_of = [&](int pair) -> int { return mod_nkeys(a, docs, len, prefix, G, npairs, pair); };
+  const int j0 = split * kSplit;
+  const int maxkeys = nkeys_of(min(16 * chunk + 15, npairs - 1));
+  if (j0 >= maxkeys) return;                            // the merge reads no such split of these rows
+  const int n_act = __builtin_amdgcn_readfirstlane(min(kSplit, maxkeys - j0));
+  const int pair = 16 * chunk + r;                      // score-layout row of this lane
+  const int lim = nkeys_of(pair) - j0;                  // keys of the split it may see
+  const int pos = len - a.Tq + pair / G;
+  float slope2 = 0.0f;
+  if (a.mod.slopes && pair < npairs) slope2 = a.mod.slopes[hk * G + pair % G] * kLog2e;
+  // Index of a row's partial: rows in the output's order, splits inside them.
+  auto partial = [&](int p) -> int64_t {
+    return ((((int64_t)b * a.Hq + hk * G + p % G) * a.Tq) + p / G) * a.nsplit + split;
+  };
+
+  // Document mask: bit 4 t + i: the lane's row is of key 64 wave + 16 t + 4 qq + i's document.
+  unsigned seen = ~0u;
+  if (docs) {
+    seen = 0;
+    const bool row = lim > -j0;                         // a row that exists (its position has a document)
+    const int mine = row ? docs[pos] : 0;
+#pragma unroll
+    for (int t = 0; t < KT; ++t)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        seen |= (row && docs[j0 + min(64 * wave + 16 * t + 4 * qq + i, n_act - 1)] == mine ? 1u : 0u) << (4 * t + i);
+    // (the vote goes through Ps: the library's own would take LDS past 80 KB)
+    const bool hit = __ballot(seen != 0) != 0;
+    if (lane == 0) Ps[0][wave] = hit ? 1.0f : 0.0f;
+    __syncthreads();
+    const float any = Ps[0][0] + Ps[0][1] + Ps[0][2] + Ps[0][3];
+    __syncthreads();
+    if (any == 0.0f) {
+      if (tid < 16 && 16 * chunk + tid < npairs) {
+        a.pm[partial(16 * chunk + tid)] = -INFINITY;
+        a.pl[partial(16 * chunk + tid)] = 0.0f;
+      }
+      return;
+    }
+  }
+
+  // Memory requests, in this order: Q^T, this wave's K rows, its V copies. A
+  // wave's keys are one 64-key segment or four 16-key tiles, clamped to the last
+  // active one (attn_decode_mfma).
+  F qf[KS];
+  {
+    const bool ok = pair < npairs;
+    const T* qrow = static_cast<const T*>(a.q) + (int64_t)b * a.q_sb +
+                    (ok ? (int64_t)(hk * G + pair % G) * a.q_sh + (int64_t)(pair / G) * a.q_st : 0);
+#pragma unroll
+    for (int st = 0; st < KS; ++st) qf[st] = ok ? frag_load(qrow + 32 * st + 8 * qq) : frag_zero<F>();
+  }
+  const T* kbase = static_cast<const T*>(a.k);
+  const T* vbase = static_cast<const T*>(a.v);
+  const int seg = __builtin_amdgcn_readfirstlane(min(wave, (n_act - 1) >> 6));
+  const T* kseg = kbase;
+  const T* vseg = vbase;
+  int ktile[4], entry[4];                               // TILED: first key and table entry of each tile
+  if constexpr (TILED) {
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      ktile[t] = __builtin_amdgcn_readfirstlane(min(64 * wave + 16 * t, (n_act - 1) & ~15));
+      entry[t] = load_uniform_i32(uniform_ptr(kv_entry(a, b, j0 + ktile[t])));
+    }
+  } else if constexpr (MODE == kKvPaged) {
+    const int key0 = j0 + 64 * seg;
+    const int64_t page = clamp_page(load_uniform_i32(uniform_ptr(kv_entry(a, b, key0))), a.num_pages);
+    const int64_t row = key0 & ((1 << a.page_shift) - 1);
+    kseg = uniform_ptr(kbase + page * a.k_sb + hk * a.k_sh + row * a.k_sl);
+    vseg = uniform_ptr(vbase + page * a.v_sb + hk * a.v_sh + row * a.v_sl);
+  } else if constexpr (MODE == kKvContig) {
+    kseg = uniform_ptr(kv_segment<MODE>(a, kbase, a.k_sb, a.k_sh, a.k_sl, b, hk, j0 + 64 * seg));
+    vseg = uniform_ptr(kv_segment<MODE>(a, vbase, a.v_sb, a.v_sh, a.v_sl, b, hk, j0 + 64 * seg));
+  }
+  F kf[KT][KS];
+#pragma unroll
+  for (int t = 0; t < KT; ++t) {
+    const int key = min(64 * wave + 16 * t + r, n_act - 1);
+    const T* kr;
+    if constexpr (TILED)
+      kr = kv_tile(a, kbase, a.k_sb, a.k_sh, a.k_sl, entry[t], hk, j0 + ktile[t]) +
+           (int64_t)min(r, n_act - 1 - ktile[t]) * a.k_sl;
+    else if constexpr (ROWPAGED) kr = kbase + kv_row_off(a, a.k_sb, a.k_sh, a.k_sl, b, hk, j0 + key);
+    else kr = kseg + (int64_t)(key - 64 * seg) * a.k_sl;
+#pragma unroll
+    for (int st = 0; st < KS; ++st) kf[t][st] = frag_load(kr + 32 * st + 8 * qq);
+  }
+  asm volatile("" ::: "memory");
+  constexpr bool kVFixed = (MODE == kKvContig || MODE == kKvPaged) && (64 % KV::kCPR) == 0;
+  constexpr int kRowsPerCopy = kVFixed ? 64 / KV::kCPR : 1;
+  constexpr int kKeyRows = KV::template kKeyRows<true>;
+  constexpr int kVPeriod = TILED ? KV::kTileCopies : kRowsPerCopy >= kKeyRows ? 1 : kKeyRows / kRowsPerCopy;
+  auto copy_v = [&](int vp) __attribute__((always_inline)) {
+    const int vbytes = vp * DV * (int)sizeof(T);
+    const int left = n_act - 64 * wave;                 // active rows from this wave's first
+    if constexpr (kVFixed) {
+      const auto rs = buffer_rsrc(vseg, (int)(uniform_clamp(left, 64) * a.v_sl * (int64_t)sizeof(T)));
+      const int v_step = kVPeriod * kRowsPerCopy * (int)(a.v_sl * (int64_t)sizeof(T));
+#pragma unroll
+      for (int c = 0; c < CPW; ++c)
+        copy_to_lds16(rs, KV::template tile_off<true>(c % kVPeriod, lane, a.v_sl) + (c / kVPeriod) * v_step + vbytes,
+                      Vs + 1024 * (wave * CPW + c));
+    } else if constexpr (TILED) {
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+        const auto rs = buffer_rsrc(uniform_ptr(kv_tile(a, vbase, a.v_sb, a.v_sh, a.v_sl, entry[t], hk, j0 + ktile[t])),
+                                    (int)(uniform_clamp(left - 16 * t, 16) * a.v_sl * (int64_t)sizeof(T)));
+#pragma unroll
+        for (int c = 0; c < KV::kTileCopies; ++c)
+          copy_to_lds16(rs, KV::template tile_off<true>(c, lane, a.v_sl) + vbytes,
+                        Vs + 1024 * (wave * CPW + KV::kTileCopies * t + c));
+      }
+    } else {
+      auto vrow = [&](int key) {
+        if constexpr (ROWPAGED) return vbase + kv_row_off(a, a.v_sb, a.v_sh, a.v_sl, b, hk, j0 + key) + vp * DV;
+        else return vseg + (int64_t)(key - 64 * seg) * a.v_sl + vp * DV;
+      };
+#pragma unroll
+      for (int c = 0; c < CPW; ++c) KV::template copy<true>(Vs, wave * CPW + c, vrow, n_act, lane);
+    }
+  };
+  copy_v(0);
+
+  float s[KT][4];
+  float m = -INFINITY;
+#pragma unroll
+  for (int t = 0; t < KT; ++t) {
+    f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int st = 0; st < KS; ++st) acc = mfma_step(kf[t][st], qf[st], acc);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int key = 64 * wave + 16 * t + 4 * qq + i;
+      const float far = (float)(pos - j0 - key);
+      const float y = a.mod.cap_log2 != 0.0f ? mod_score<T, (kModAny | kModCap | kModBias)>(acc[i], a, slope2, far)
+                                             : mod_score<T, (kModAny | kModBias)>(acc[i], a, slope2, far);
+      s[t][i] = key < lim && (seen >> (4 * t + i) & 1u) ? y : -INFINITY;
+      m = fmaxf(m, s[t][i]);
+    }
+  }
+  m = quarter_max(m);
+  if (qq == 0) Ps[0][16 * wave + r] = m;
+  stage_barrier<CPW>();                                 // the wave maxima visible; V copies may still be in flight
+  m = fmaxf(fmaxf(Ps[0][r], Ps[0][16 + r]), fmaxf(Ps[0][32 + r], Ps[0][48 + r]));
+  stage_barrier<CPW>();                                 // read by everyone: the weights go over them
+  const float msub = m == -INFINITY ? 0.0f : m;         // no visible key: weights 0, not NaN
+#pragma unroll
+  for (int t = 0; t < KT; ++t) {
+    f32x4 p;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) p[i] = __builtin_amdgcn_exp2f(s[t][i] - msub);
+    *reinterpret_cast<f32x4*>(&Ps[r][64 * wave + 16 * t + 4 * qq]) = p;
+  }
+  if (wave == 0 && qq == 0 && pair < npairs) a.pm[partial(pair)] = m;
+  stage_barrier<0>();                                   // V landed, weights visible
+
+  f32x4 lsum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int vp = 0; vp < NVP; ++vp) {
+    if (vp > 0) {
+      __syncthreads();                                  // every wave is done with the previous slice
+      copy_v(vp);
+      stage_barrier<0>();
+    }
+    f32x4 acc[NJ];
+    // P.V of this wave's dim tiles; `clean` takes infinities and NaN of V as 0.
+    auto weigh = [&](bool clean, bool sum) __attribute__((always_inline)) {
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
+      for (int ks = 0; ks < kSplit / 32; ++ks) {
+        const f32x4 x0 = *reinterpret_cast<const f32x4*>(&Ps[r][32 * ks + 4 * qq]);
+        const f32x4 x1 = *reinterpret_cast<const f32x4*>(&Ps[r][32 * ks + 16 + 4 * qq]);
+        const float p8[8] = {x0[0], x0[1], x0[2], x0[3], x1[0], x1[1], x1[2], x1[3]};
+        const PFrag<T> pf = make_pfrag<T>(p8);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+          if (wave + 4 * j >= NDTV) continue;
+          F v = KV::vfrag(Vs, 32 * ks, wave + 4 * j, lane);
+          if (clean) v = finite_frag(v);
+          acc[j] = pv_step<T>(pf, v, acc[j]);
+        }
+        if (sum) lsum = pv_step<T>(pf, ones_frag<T>(), lsum);
+      }
+    };
+    weigh(false, vp == 0 && wave == 0);
+    // A hidden key's weight 0 times an infinity or NaN of its V row is NaN: such a
+    // wave weighs again without them and adds the ones its rows see.
+    bool finite = true;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) finite = finite && (wave + 4 * j >= NDTV || fabsf(acc[j][i]) < INFINITY);
+    if (__ballot(!finite)) {
+      weigh(true, false);
+      for (int key = 0; key < n_act; ++key) {
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+          if (wave + 4 * j >= NDTV) continue;
+          const int dim = 16 * (wave + 4 * j) + r;
+          constexpr int kPer = 16 / (int)sizeof(T);
+          const float x = to_f32(reinterpret_cast<const T*>(Vs + KV::template off<true>(key, dim / kPer))[dim % kPer]);
+          if (fabsf(x) < INFINITY) continue;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int p = 16 * chunk + 4 * qq + i;
+            if (j0 + key < nkeys_of(p) && (!docs || docs[j0 + key] == docs[len - a.Tq + p / G])) acc[j][i] += x;
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      if (wave + 4 * j >= NDTV) continue;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int p = 16 * chunk + 4 * qq + i;
+        if (p < npairs) a.pacc[partial(p) * D + vp * DV + 16 * (wave + 4 * j) + r] = acc[j][i];
+      }
+    }
+  }
+  if (wave == 0 && r == 0) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int p = 16 * chunk + 4 * qq + i;
+      if (p < npairs) a.pl[partial(p)] = lsum[i];
+    }
+  }
+}
+
+// Merges the splits of every row that attn_rows_mod left, left to right, and
+// divides: one thread per four dims of a row. A split in which the row sees
+// nothing (l = 0 at m = -inf) is passed over.
+template <typename T, int D>
+__global__ __launch_bounds__(256) void attn_rows_combine(ModRowsArgs a) {
+  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t row = id / (D / 4);                     // (b, head, token), the output's order
+  if (row >= (int64_t)a.B * a.Hq * a.Tq) return;
+  const int d = (int)(id % (D / 4)) * 4;
+  const int t = (int)(row % a.Tq), b = (int)(row / a.Tq / a.Hq);
+  const int len = a.kv_lens ? min(max(a.kv_lens[b], 0), a.L) : a.L;
+  const int prefix = a.mod.prefix ? min(max(a.mod.prefix[b], 0), len) : 0;
+  const int ns = (mod_nkeys(a, a.mod.docs, len, prefix, 1, a.Tq, t) + kSplit - 1) / kSplit;
+  float M = -INFINITY, Ls = 0.0f, A[4] = {0.f, 0.f, 0.f, 0.f};
+  const int64_t p0 = row * a.nsplit;
+  for (int i0 = 0; i0 < ns; i0 += 4) {                  // four splits' partials requested together
+    float pm[4], pl[4];
+    f32x4 pa[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int64_t p = p0 + min(i0 + j, ns - 1);
+      pm[j] = a.pm[p];
+      pl[j] = a.pl[p];
+      pa[j] = *reinterpret_cast<const f32x4*>(a.pacc + p * D + d);
+    }
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      if (i0 + j < ns && (pm[j] > -INFINITY || pl[j] != 0.0f)) {
+        const float acc[4] = {pa[j][0], pa[j][1], pa[j][2], pa[j][3]};
+        merge_split<4>(M, Ls, A, pm[j], pl[j], acc);
+      }
+    }
+  }
+  T* o = static_cast<T*>(a.out) + row * D + d;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) o[e] = to_store<T>(Ls != 0.0f ? A[e] / Ls : 0.0f);
 }
 
 }  // namespace bi

@@ -129,7 +129,25 @@ int launch_prefill_mod(ModPrefillArgs& a, hipStream_t st) {
   return bi_host::launch_status("bi_attn_scored");
 }
 
+template <typename T, int D>
+int launch_rows_mod(ModRowsArgs& a, hipStream_t st) {
+  const int64_t nchunks = ((int64_t)a.Tq * (a.Hq / a.Hkv) + 15) / 16;
+  const unsigned grid = (unsigned)(8 * ((nchunks * a.nsplit * a.Hkv * a.B + 7) / 8));
+  switch (kv_mode<T>(a)) {
+    case kKvPaged: attn_rows_mod<T, D, kKvPaged><<<grid, 256, 0, st>>>(a); break;
+    case kKvTilePaged: attn_rows_mod<T, D, kKvTilePaged><<<grid, 256, 0, st>>>(a); break;
+    case kKvRowPaged: attn_rows_mod<T, D, kKvRowPaged><<<grid, 256, 0, st>>>(a); break;
+    default: attn_rows_mod<T, D, kKvContig><<<grid, 256, 0, st>>>(a); break;
+  }
+  int rc = bi_host::launch_status("bi_attn_scored");
+  if (rc) return rc;
+  const int64_t n = (int64_t)a.B * a.Hq * a.Tq * (D / 4);
+  attn_rows_combine<T, D><<<(unsigned)((n + 255) / 256), 256, 0, st>>>(a);
+  return bi_host::launch_status("bi_attn_scored(combine)");
+}
+
 #define BI_ATTN_MOD_D(X, T) X(T, 32) X(T, 64) X(T, 96) X(T, 128) X(T, 192) X(T, 256)
 #define BI_ATTN_MOD_DECODE(T, D) template int launch_decode_mod<T, D>(ModDecodeArgs&, hipStream_t);
+#define BI_ATTN_MOD_ROWS(T, D) template int launch_rows_mod<T, D>(ModRowsArgs&, hipStream_t);
 
 }  // namespace bi

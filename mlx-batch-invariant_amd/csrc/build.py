@@ -70,7 +70,7 @@ EXTRA_FLAGS = {
     "bi_attn_bf16": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "bi_attn_f16": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     **{f"bi_attn_mod_{v}_{t}": ["-mllvm", "-amdgpu-mfma-vgpr-form"]
-       for v in ("decode", "mask", "cap", "bias", "capbias") for t in ("bf16", "f16")},
+       for v in ("decode", "rows", "mask", "cap", "bias", "capbias") for t in ("bf16", "f16")},
     "bi_qmm_bf16": _CLAUSE,
     "bi_qmm_f16": _CLAUSE,
 }

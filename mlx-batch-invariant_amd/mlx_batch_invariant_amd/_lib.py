@@ -82,7 +82,8 @@ _SIGNATURES = {
     "bi_attn_prefill_paged": (ctypes.c_int, [_vp, _vp, _vp, _vp, _c_i64, _c_i64, _c_i64, _vp, _vp, _c_i64, _c_i64,
                                              _c_i64, _c_i64, _c_i64, _c_i64, ctypes.POINTER(_c_i64), ctypes.c_int,
                                              ctypes.c_float, ctypes.c_int, _vp]),
-    "bi_attn_scored_workspace_bytes": (ctypes.c_size_t, [_c_i64, _c_i64, _c_i64, _c_i64, _c_i64, ctypes.c_int]),
+    "bi_attn_scored_workspace_bytes": (ctypes.c_size_t, [_c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, ctypes.c_int,
+                                                         ctypes.c_int, ctypes.c_int]),
     "bi_attn_scored": (ctypes.c_int, [_vp, _vp, _vp, _vp, _c_i64, _c_i64, _c_i64, _vp, _vp, _c_i64, _c_i64, _c_i64,
                                       _c_i64, _c_i64, _c_i64, ctypes.POINTER(_c_i64), ctypes.c_int, ctypes.c_float,
                                       ctypes.POINTER(ScoreMod), ctypes.c_int, _vp, ctypes.c_size_t, _vp]),

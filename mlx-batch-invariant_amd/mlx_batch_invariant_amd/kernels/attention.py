@@ -266,7 +266,8 @@ def _scored(what, q, k, v, table, num_pages, page_size, L, kl, scale, causal, so
     out = torch.empty((B, Hq, Tq, D), dtype=q.dtype, device=q.device)
     if B == 0 or Tq == 0:
         return out
-    n = _lib.ws_bytes("bi_attn_scored_workspace_bytes", B, Hq, Tq, L, D, int(doc_ids is not None))
+    n = _lib.ws_bytes("bi_attn_scored_workspace_bytes", B, Hq, v.shape[1], Tq, L, D, int(causal),
+                      int(doc_ids is not None), _lib.DTYPE_CODE[q.dtype])
     ws = _lib.workspace(n, q.device)
     rc = _lib.launch(q.get_device(), _lib.scored_call, q.data_ptr(), k.data_ptr(), v.data_ptr(), _lib.ptr(table),
                      0 if table is None else table.stride(0), page_size, num_pages, _lib.ptr(kl), out.data_ptr(), B,

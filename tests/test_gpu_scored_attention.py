@@ -278,3 +278,37 @@ def test_operators_of_the_dispatcher():
     table = torch.arange(8, dtype=I32, device="cuda").reshape(2, 4)
     kp, vp = (x.reshape(2, 2, 4, 16, 64).transpose(1, 2).reshape(8, 2, 16, 64) for x in (k, v))
     assert bits(torch.ops.mlx_bi.scored_paged_attention(q, kp, vp, table, None, 0.125, True, *a)) == bits(want)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("page,D", [(0, 64), (16, 128), (64, 64), (4, 32)])
+@pytest.mark.parametrize("which", ["c", "s", "d", "p", "csdp"])
+def test_many_rows_are_the_bits_of_few(dt, page, D, which):
+    """A batch large enough for the workgroups that walk the splits against its
+    sequences alone, which take a workgroup per split; hidden infinities in both."""
+    B, Hq, Hkv, T, L = 6, 8, 4, 200, 600
+    q, k, v = _case(dt, B, Hq, Hkv, T, L, D, 21)
+    m = _mods(which, B, Hq, L, 21)
+    lens = [L, 100, 257, 513, 31, 599]
+    for b, n in enumerate(lens):
+        k[b, :, n:], v[b, :, n:] = float("inf"), float("nan")
+    if "d" in which:
+        for b in range(B):                              # another document's rows, and the last token's own
+            other = (m["doc_ids"][b] != m["doc_ids"][b, lens[b] - 1]).nonzero()[:, 0]
+            v[b, :, other[other < 20].cuda(), 3] = float("nan")
+    from mlx_batch_invariant_amd import _lib
+    size = lambda n: _lib.load().bi_attn_scored_workspace_bytes(n, Hq, Hkv, T, L, D, 1, 0, _lib.DTYPE_CODE[DT[dt]])
+    assert size(B) == 0 < size(1)
+    got = _call(q, k, v, lens, True, page, **m)
+    for b in range(B):
+        one = {n: (x[b:b + 1] if n in ("doc_ids", "prefix_lens") else x) for n, x in m.items()}
+        alone = _call(q[b:b + 1], k[b:b + 1], v[b:b + 1], lens[b:b + 1], True, page, **one)
+        same = (alone == got[b:b + 1]) | (alone.isnan() & got[b:b + 1].isnan())
+        assert same.all(), b
+    clean = [x.clone() for x in (k, v)]
+    for b, n in enumerate(lens):
+        clean[0][b, :, n:], clean[1][b, :, n:] = 0.0, 0.0
+    if which != "d" and "d" not in which:
+        assert bits(_call(q, *clean, lens, True, page, **m)) == bits(got)
+        _check(got[1:2], q[1:2], clean[0][1:2], clean[1][1:2], lens[1:2], True,
+               **{n: (x[1:2] if n == "prefix_lens" else x) for n, x in m.items()})

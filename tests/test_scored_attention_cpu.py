@@ -77,11 +77,15 @@ def test_abi():
     assert call(M(slopes=256), L=(1 << 24) + 1) == -2
     assert call(M(softcap=1.0), table=p, page=12, pages=9, stride=99) == -1
     docs = M(doc_ids=256, doc_stride=300)
-    need = lib.bi_attn_scored_workspace_bytes(1, 4, 4, 300, 128, 1)
-    assert need == 2 * 8 and call(docs) == -3 and call(docs, ws=p, n=need - 1) == -3
+    size = lib.bi_attn_scored_workspace_bytes
+    need = size(1, 4, 2, 4, 300, 128, 1, 1, 2)           # few rows: partials of 16 rows and 2 splits
+    assert need == (2 * 32 + 32 * 128) * 4 and call(docs) == -3 and call(docs, ws=p, n=need - 1) == -3
     assert call(docs, ws=ctypes.c_void_p(264), n=need) == -3
-    assert lib.bi_attn_scored_workspace_bytes(1, 4, 4, 300, 128, 0) == 0
-    assert lib.bi_attn_scored_workspace_bytes(3, 4, 1, 300, 128, 1) == lib.bi_attn_decode_workspace_bytes(3, 4, 300, 128)
+    assert size(3, 4, 2, 1, 300, 128, 0, 1, 2) == lib.bi_attn_decode_workspace_bytes(3, 4, 300, 128)
+    assert size(1, 4, 2, 4, 256, 128, 1, 1, 2) == 8 and size(1, 4, 2, 4, 256, 128, 1, 0, 2) == 0     # one split
+    assert size(4, 32, 8, 2048, 2048, 128, 1, 1, 2) == 4 * 8 * 8 and size(4, 32, 8, 2048, 2048, 128, 1, 0, 2) == 0
+    assert size(1, 32, 8, 16, 1 << 20, 128, 1, 0, 0) == 0                   # partials over 256 MB
+    assert size(1, 4, 3, 4, 300, 128, 1, 1, 2) == 0
     assert call(docs, Tq=1) == -3 and call(M(softcap=1.0), B=0) == 0 and call(M(softcap=1.0), B=0, Tq=1) == 0
 
 
