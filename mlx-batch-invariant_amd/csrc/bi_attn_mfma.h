@@ -226,7 +226,7 @@ __global__ __launch_bounds__(256) void attn_decode_mfma(DecodeArgsOf<MOD> a) {
     // 4,096 keys, pages of 16 / 256: 58 / 55 us so, now 39.) The end-of-item
     // barrier below keeps thread 0 from overwriting item_s before every thread
     // has read it.
-    if (next >= gridDim.x) {
+    if (next >= gridDim.x && (MOD == 0 || a.ctr)) {     // (MOD without a counter: the static order)
       if (tid == 0) item_s = atomicAdd(a.ctr, 1u);
       __syncthreads();
       item = (int64_t)gridDim.x + item_s;
@@ -236,7 +236,8 @@ __global__ __launch_bounds__(256) void attn_decode_mfma(DecodeArgsOf<MOD> a) {
   // outside [0, L] is clamped, so no key past the cache is ever read.
   for (; b < a.B; ++b) {
     len = a.kv_lens ? min(max(a.kv_lens[b], 0), a.L) : a.L;
-    const int64_t nb = (int64_t)((len + kSplit - 1) / kSplit) * per_split;
+    int64_t nb = (int64_t)((len + kSplit - 1) / kSplit) * per_split;
+    if constexpr (MOD != 0) nb = a.nsplit == 1 ? per_split : nb;   // (no merge: an item for an empty sequence too)
     if (item < base + nb) break;
     base += nb;
   }
@@ -250,6 +251,15 @@ __global__ __launch_bounds__(256) void attn_decode_mfma(DecodeArgsOf<MOD> a) {
   const int G = a.Hq / a.Hkv;
   const int h0 = hk * G + chunk * GU;
   const int r = lane % 16, qq = lane / 16;
+  const bool direct = MOD != 0 && a.nsplit == 1;        // the item is the whole result: nothing to merge
+  if constexpr (MOD != 0) {
+    if (n_act <= 0) {                                   // (direct only) no key: zeros
+      for (int i = tid; i < GU * D; i += 256)
+        static_cast<T*>(a.out)[((int64_t)b * a.Hq + h0) * D + i] = (T)0.0f;
+      __syncthreads();                                  // (item_s read by everyone)
+      continue;
+    }
+  }
   unsigned seen = ~0u;                                  // MOD: bit 4 t + i: the document mask leaves that key
   float slope2 = 0.0f;
   bool hidden = false;                                  // MOD: key tid of the split is another document's
@@ -408,7 +418,7 @@ __global__ __launch_bounds__(256) void attn_decode_mfma(DecodeArgsOf<MOD> a) {
     }
   }
   const int64_t pbase = ((int64_t)b * a.Hq + h0) * a.nsplit + split;
-  if (wave == 0 && qq == 0 && r < GU) a.pm[pbase + (int64_t)r * a.nsplit] = m;
+  if (!direct && wave == 0 && qq == 0 && r < GU) a.pm[pbase + (int64_t)r * a.nsplit] = m;
   stage_barrier<0>();  // V landed (own copies: vmcnt; everyone's: the barrier); weights visible
 
   // P.V over the split's 8 key steps, this wave's dim tiles of each V slice
@@ -457,7 +467,7 @@ __global__ __launch_bounds__(256) void attn_decode_mfma(DecodeArgsOf<MOD> a) {
         const int dt = wave + 4 * j;
         if (dt < NDTV) acc[j] = pv_step<T>(pf, KV::vfrag(Vs, 32 * ks, dt, lane), acc[j]);
       }
-      if (vp == 0 && wave == 0) lsum = pv_step<T>(pf, ones_frag<T>(), lsum);
+      if (vp == 0 && (wave == 0 || direct)) lsum = pv_step<T>(pf, ones_frag<T>(), lsum);
     }
 
 #pragma unroll
@@ -467,11 +477,19 @@ __global__ __launch_bounds__(256) void attn_decode_mfma(DecodeArgsOf<MOD> a) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int row = 4 * qq + i;
+        if constexpr (MOD != 0) {
+          if (direct) {                                 // (the merge's fma(0, 0, acc): no -0)
+            if (row < GU)
+              static_cast<T*>(a.out)[(pbase + row) * D + vp * DV + 16 * dt + r] =
+                  to_store<T>(lsum[i] != 0.0f ? (acc[j][i] + 0.0f) / lsum[i] : 0.0f);
+            continue;
+          }
+        }
         if (row < GU) a.pacc[(pbase + (int64_t)row * a.nsplit) * D + vp * DV + 16 * dt + r] = acc[j][i];
       }
     }
   }
-  if (wave == 0 && r == 0) {
+  if (!direct && wave == 0 && r == 0) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int row = 4 * qq + i;

@@ -569,18 +569,25 @@ __global__ __launch_bounds__(256) void attn_rows_mod(ModRowsArgs a) {
   auto nkeys_of = [&](int pair) -> int { return mod_nkeys(a, docs, len, prefix, G, npairs, pair); };
   const int j0 = split * kSplit;
   const int maxkeys = nkeys_of(min(16 * chunk + 15, npairs - 1));
-  if (j0 >= maxkeys) return;                            // the merge reads no such split of these rows
+  const bool direct = a.nsplit == 1;                    // one split: the results themselves, nothing to merge
+  // Index of a row's partial: rows in the output's order, splits inside them.
+  auto partial = [&](int p) -> int64_t {
+    return ((((int64_t)b * a.Hq + hk * G + p % G) * a.Tq) + p / G) * a.nsplit + split;
+  };
+  if (j0 >= maxkeys) {                                  // the merge reads no such split of these rows
+    if (direct) {
+      for (int i = tid; i < 16 * D; i += 256)
+        if (16 * chunk + i / D < npairs)
+          static_cast<T*>(a.out)[partial(16 * chunk + i / D) * D + i % D] = (T)0.0f;
+    }
+    return;
+  }
   const int n_act = __builtin_amdgcn_readfirstlane(min(kSplit, maxkeys - j0));
   const int pair = 16 * chunk + r;                      // score-layout row of this lane
   const int lim = nkeys_of(pair) - j0;                  // keys of the split it may see
   const int pos = len - a.Tq + pair / G;
   float slope2 = 0.0f;
   if (a.mod.slopes && pair < npairs) slope2 = a.mod.slopes[hk * G + pair % G] * kLog2e;
-  // Index of a row's partial: rows in the output's order, splits inside them.
-  auto partial = [&](int p) -> int64_t {
-    return ((((int64_t)b * a.Hq + hk * G + p % G) * a.Tq) + p / G) * a.nsplit + split;
-  };
-
   // Document mask: bit 4 t + i: the lane's row is of key 64 wave + 16 t + 4 qq + i's document.
   unsigned seen = ~0u;
   if (docs) {
@@ -599,7 +606,11 @@ __global__ __launch_bounds__(256) void attn_rows_mod(ModRowsArgs a) {
     const float any = Ps[0][0] + Ps[0][1] + Ps[0][2] + Ps[0][3];
     __syncthreads();
     if (any == 0.0f) {
-      if (tid < 16 && 16 * chunk + tid < npairs) {
+      if (direct) {
+        for (int i = tid; i < 16 * D; i += 256)
+          if (16 * chunk + i / D < npairs)
+            static_cast<T*>(a.out)[partial(16 * chunk + i / D) * D + i % D] = (T)0.0f;
+      } else if (tid < 16 && 16 * chunk + tid < npairs) {
         a.pm[partial(16 * chunk + tid)] = -INFINITY;
         a.pl[partial(16 * chunk + tid)] = 0.0f;
       }
@@ -719,7 +730,7 @@ __global__ __launch_bounds__(256) void attn_rows_mod(ModRowsArgs a) {
     for (int i = 0; i < 4; ++i) p[i] = __builtin_amdgcn_exp2f(s[t][i] - msub);
     *reinterpret_cast<f32x4*>(&Ps[r][64 * wave + 16 * t + 4 * qq]) = p;
   }
-  if (wave == 0 && qq == 0 && pair < npairs) a.pm[partial(pair)] = m;
+  if (!direct && wave == 0 && qq == 0 && pair < npairs) a.pm[partial(pair)] = m;
   stage_barrier<0>();                                   // V landed, weights visible
 
   f32x4 lsum = {0.f, 0.f, 0.f, 0.f};
@@ -751,7 +762,7 @@ __global__ __launch_bounds__(256) void attn_rows_mod(ModRowsArgs a) {
         if (sum) lsum = pv_step<T>(pf, ones_frag<T>(), lsum);
       }
     };
-    weigh(false, vp == 0 && wave == 0);
+    weigh(false, vp == 0 && (wave == 0 || direct));
     // A hidden key's weight 0 times an infinity or NaN of its V row is NaN: such a
     // wave weighs again without them and adds the ones its rows see.
     bool finite = true;
@@ -783,11 +794,16 @@ __global__ __launch_bounds__(256) void attn_rows_mod(ModRowsArgs a) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int p = 16 * chunk + 4 * qq + i;
-        if (p < npairs) a.pacc[partial(p) * D + vp * DV + 16 * (wave + 4 * j) + r] = acc[j][i];
+        if (p >= npairs) continue;
+        const int64_t at = partial(p) * D + vp * DV + 16 * (wave + 4 * j) + r;
+        if (direct)                                     // (the merge's fma(0, 0, acc): no -0)
+          static_cast<T*>(a.out)[at] = to_store<T>(lsum[i] != 0.0f ? (acc[j][i] + 0.0f) / lsum[i] : 0.0f);
+        else
+          a.pacc[at] = acc[j][i];
       }
     }
   }
-  if (wave == 0 && r == 0) {
+  if (!direct && wave == 0 && r == 0) {
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int p = 16 * chunk + 4 * qq + i;

@@ -45,15 +45,17 @@ __global__ __launch_bounds__(256) void attn_combine_mod_kernel(DecodeArgs a) {
   if (live) static_cast<T*>(a.out)[bh * D + d] = to_store<T>(Ls != 0.0f ? A / Ls : 0.0f);
 }
 
-// One item order (dynamic) for every cache: the extra launch that zeroes the
-// counter costs what the second instantiation would save.
+// One instantiation for both item orders, chosen as for the plain kernel: with at
+// most kDynMinRounds rounds of the resident grid the static order, which needs no
+// launch to zero a counter.
 template <typename T, int D, int GU, int MODE>
 static int launch_decode_mod_gu(ModDecodeArgs& a, hipStream_t st) {
   static int cache[kMaxDev] = {};
   const int64_t most = (int64_t)a.B * a.nsplit * a.Hkv * a.nchunk;
   const int grid = resident_grid(attn_decode_mfma<T, D, GU, true, MODE, kModAny>, cache);
   if (grid <= 0) return bi_host::fail(BI_E_UNSUPPORTED, "bi_attn_scored: device occupancy query failed");
-  zero_counter_kernel<<<1, 1, 0, st>>>(a.ctr);
+  if (most > (int64_t)kDynMinRounds * grid) zero_counter_kernel<<<1, 1, 0, st>>>(a.ctr);
+  else a.ctr = nullptr;
   attn_decode_mfma<T, D, GU, true, MODE, kModAny><<<(int)std::min<int64_t>(grid, most), 256, 0, st>>>(a);
   return 0;
 }
@@ -79,7 +81,7 @@ int launch_decode_mod(ModDecodeArgs& a, hipStream_t st) {
     default: rc = launch_decode_mod_mode<T, D, 1>(a, st); break;
   }
   if (rc) return rc;
-  if ((rc = bi_host::launch_status("bi_attn_scored"))) return rc;
+  if ((rc = bi_host::launch_status("bi_attn_scored")) || a.nsplit == 1) return rc;
   const int64_t n = (int64_t)a.B * a.Hq * D;
   attn_combine_mod_kernel<T, D><<<(unsigned)((n + 255) / 256), 256, 0, st>>>(a);
   return bi_host::launch_status("bi_attn_scored(combine)");
@@ -140,7 +142,7 @@ int launch_rows_mod(ModRowsArgs& a, hipStream_t st) {
     default: attn_rows_mod<T, D, kKvContig><<<grid, 256, 0, st>>>(a); break;
   }
   int rc = bi_host::launch_status("bi_attn_scored");
-  if (rc) return rc;
+  if (rc || a.nsplit == 1) return rc;
   const int64_t n = (int64_t)a.B * a.Hq * a.Tq * (D / 4);
   attn_rows_combine<T, D><<<(unsigned)((n + 255) / 256), 256, 0, st>>>(a);
   return bi_host::launch_status("bi_attn_scored(combine)");

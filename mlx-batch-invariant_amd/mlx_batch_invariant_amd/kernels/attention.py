@@ -111,10 +111,13 @@ def _aligned(t: torch.Tensor) -> bool:
     kernels address a split's or chunk's rows with 32-bit offsets). Others are
     copied."""
     es = t.element_size()
-    st = t.stride()
-    return (st[-1] == 1 and t.data_ptr() % 16 == 0
-            and all((s * es) % 16 == 0 and s >= 0 for s in st[:-1])
-            and (t.dim() < 2 or st[-2] * es < 1 << 23))
+    *lead, last = t.stride()
+    if last != 1 or t.data_ptr() % 16 or lead and lead[-1] * es >= 1 << 23:
+        return False
+    for s in lead:
+        if s * es % 16 or s < 0:
+            return False
+    return True
 
 
 def _fix(t: torch.Tensor) -> torch.Tensor:
@@ -124,7 +127,11 @@ def _fix(t: torch.Tensor) -> torch.Tensor:
 def _lens(kv_lens, B: int, L: int, device) -> torch.Tensor | None:
     if kv_lens is None:
         return None
-    kl = torch.as_tensor(kv_lens, dtype=torch.int32, device=device).reshape(-1).contiguous()
+    if (isinstance(kv_lens, torch.Tensor) and kv_lens.dtype == torch.int32 and kv_lens.ndim == 1
+            and kv_lens.device == device and kv_lens.is_contiguous()):
+        kl = kv_lens
+    else:
+        kl = torch.as_tensor(kv_lens, dtype=torch.int32, device=device).reshape(-1).contiguous()
     if kl.numel() != B:
         raise ValueError(f"kv_lens has {kl.numel()} entries for batch {B}")
     return kl

@@ -312,3 +312,23 @@ def test_many_rows_are_the_bits_of_few(dt, page, D, which):
         assert bits(_call(q, *clean, lens, True, page, **m)) == bits(got)
         _check(got[1:2], q[1:2], clean[0][1:2], clean[1][1:2], lens[1:2], True,
                **{n: (x[1:2] if n == "prefix_lens" else x) for n, x in m.items()})
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("D,page", [(64, 0), (128, 16), (256, 0), (96, 4)])
+def test_caches_of_one_split(dt, D, page):
+    """Caches of at most 256 keys need no merge: the bits of the same lengths in a
+    longer cache; empty sequences and negative zeros as there."""
+    B, Hq, Hkv = 5, 8, 2
+    lens = [256, 0, 1, 77, 255]
+    for T in (1, 9, 60):
+        q, k, v = _case(dt, B, Hq, Hkv, T, 256, D, 31)
+        v[:, :, :, 0] = -0.0
+        longer = [torch.nn.functional.pad(x, (0, 0, 0, 300), value=3.0) for x in (k, v)]
+        for which in ("c", "sd", "csdp"):
+            m = _mods(which, B, Hq, 256, 31)
+            n = {a: torch.nn.functional.pad(x, (0, 300), value=-1) if a == "doc_ids" else x for a, x in m.items()}
+            got = _call(q, k, v, lens, True, page, **m)
+            assert bits(got) == bits(_call(q, *longer, lens, True, page, **n))
+            assert not got[1].any()
+            _check(got, q, k, v, lens, True, **m)
