@@ -11,10 +11,10 @@
 //   prefix     a row's key limit is max(pos_q + 1, prefix): limits still grow
 //              with the token, so nothing else changes.
 //   documents  the split's document numbers come to LDS with its first K chunk;
-//              splits whose range of numbers misses the workgroup's are skipped
-//              (64 of them tested by one ballot), and one with a single number,
-//              the workgroup's own, runs unmasked. Any numbers are right; sorted
-//              ones (documents packed one after another) skip the most.
+//              the splits in front of and behind all whose range of numbers meets
+//              the workgroup's are skipped, and one with a single number, the
+//              workgroup's own, runs unmasked. Any numbers are right; sorted ones
+//              (documents packed one after another) skip all they can.
 //   masked V   a hidden key's weight 0 times an infinity or NaN in its V row
 //              would be NaN. Such rows are as good as never there, so the kernel
 //              looks at its sums instead: if one is not finite, the workgroup
@@ -54,10 +54,19 @@ __device__ __forceinline__ F finite_frag(F v) {
   return v;
 }
 
-// Keys per ring chunk: as in the plain kernel's forms without FEW.
+// Keys per ring chunk: 128 for contiguous caches of narrow rows, else 64.
 template <typename T, int D, int MODE>
 constexpr int mod_chunk() {
-  return prefill_chunk<T, D, MODE, false>();
+  return MODE == kKvContig && D * (int)sizeof(T) <= (sizeof(T) == 2 ? 128 : 256) ? 128 : 64;
+}
+// Chunk buffers in the ring: four if they leave the workgroups per CU that the
+// registers allow (two up to 16-bit D = 128, else one), else two. Either divides
+// the chunks of a whole split, so every split starts in buffer 0.
+template <typename T, int D, int MODE>
+constexpr int mod_ring() {
+  constexpr int budget = sizeof(T) == 2 && D <= 128 && MODE != kKvRowPaged ? 80 << 10 : 160 << 10;
+  constexpr int fit = (budget - 64 * D - (11 << 8)) / (mod_chunk<T, D, MODE>() * D * (int)sizeof(T));
+  return fit < 4 ? 2 : 4;
 }
 // Workgroups per CU the registers are held to (see prefill_min_blocks).
 template <typename T, int D, int MODE>
@@ -78,7 +87,8 @@ template <typename T, int D, int MODE, int MOD>
 __global__ __launch_bounds__(256, (mod_min_blocks<T, D, MODE>())) void attn_prefill_mod(ModPrefillArgs a) {
   constexpr bool ROWPAGED = MODE == kKvRowPaged, TILED = MODE == kKvTilePaged;
   constexpr bool PIPE = sizeof(T) == 2 && !ROWPAGED;
-  constexpr int CH = mod_chunk<T, D, MODE>();
+  constexpr int CH = mod_chunk<T, D, MODE>(), NBUF = mod_ring<T, D, MODE>();
+  static_assert(2 * (kSplit / CH) % NBUF == 0, "attn_prefill_mod: ring depth");
   typedef typename Frag<T>::type F;
   typedef KVTile<T, D> KV;
   constexpr int KC = kSplit / CH;                       // chunks per split (of K, then of V)
@@ -87,10 +97,18 @@ __global__ __launch_bounds__(256, (mod_min_blocks<T, D, MODE>())) void attn_pref
   constexpr int CPW = KV::copies(CH) / 4;               // copy instructions per wave per chunk
   constexpr int NDT = D / 16, KS = D / 32;
   static_assert(CPW >= 1 && (CH == 64 || (CH == 128 && MODE == kKvContig)), "attn_prefill_mod: chunk size");
-  __shared__ __attribute__((aligned(1024))) char ring[2 * CHB];
-  __shared__ __attribute__((aligned(16))) int split_docs[kSplit];
-  __shared__ int doc_range[2][4];
-  __shared__ uint32_t poison[16 * D];                   // a byte for each of 64 rows and D dims
+  // LDS: the ring; the document numbers of this split and the next; for each of 64
+  // rows its key limit and document (for the masked splits: a register more would
+  // spill, and its reload waits for the copies in flight); the poison, a byte for
+  // each of 64 rows and D dims. One array: of several, the compiler tells the reads
+  // of each from the copies into it and waits for those in flight at every read.
+  constexpr int kDocs = NBUF * CHB, kRows = kDocs + 2 * kSplit * 4, kPoison = kRows + 2 * 64 * 4 + 32;
+  __shared__ __attribute__((aligned(1024))) char ring[kPoison + 64 * D];
+  int* const split_docs = reinterpret_cast<int*>(ring + kDocs);
+  int* const row_nkeys = reinterpret_cast<int*>(ring + kRows);
+  int* const row_doc = row_nkeys + 64;
+  int* const doc_range = row_doc + 64;
+  uint32_t* const poison = reinterpret_cast<uint32_t*>(ring + kPoison);
 
   const int tid = threadIdx.x;
   const int lane = tid % kWave;
@@ -114,6 +132,7 @@ __global__ __launch_bounds__(256, (mod_min_blocks<T, D, MODE>())) void attn_pref
   const int maxkeys = nkeys_of(min(64 * wg + 63, npairs - 1));
   const int my_pair = 64 * wg + 16 * wave + r;          // score-layout row of this lane
   const int my_nkeys = nkeys_of(my_pair);
+  if (qq == 0) row_nkeys[16 * wave + r] = my_nkeys;     // (read by the wave that wrote it)
   const int my_pos = len - a.Tq + my_pair / G;
   // Every row of the wave sees all keys below this limit (the first row's).
   const int wave_min_nkeys = __builtin_amdgcn_readfirstlane(nkeys_of(64 * wg + 16 * wave));
@@ -121,24 +140,25 @@ __global__ __launch_bounds__(256, (mod_min_blocks<T, D, MODE>())) void attn_pref
   if constexpr ((MOD & kModBias) != 0) {
     if (a.mod.slopes && my_pair < npairs) slope2 = a.mod.slopes[hk * G + my_pair % G] * kLog2e;
   }
-  // The lane's document, and the workgroup's smallest and largest.
-  int my_doc = 0, doc_lo = 0x7fffffff, doc_hi = -0x7fffffff - 1;
+  // The workgroup's smallest and largest document.
+  int doc_lo = 0x7fffffff, doc_hi = -0x7fffffff - 1;
   if (docs) {
-    if (my_nkeys > 0) doc_lo = doc_hi = my_doc = docs[my_pos];
+    if (my_nkeys > 0) doc_lo = doc_hi = docs[my_pos];
+    if (qq == 0) row_doc[16 * wave + r] = doc_lo;
 #pragma unroll
     for (int off = 1; off < 16; off <<= 1) {
       doc_lo = min(doc_lo, __shfl_xor(doc_lo, off, kWave));
       doc_hi = max(doc_hi, __shfl_xor(doc_hi, off, kWave));
     }
     if (lane == 0) {
-      doc_range[0][wave] = doc_lo;
-      doc_range[1][wave] = doc_hi;
+      doc_range[wave] = doc_lo;
+      doc_range[4 + wave] = doc_hi;
     }
     __syncthreads();
     doc_lo = __builtin_amdgcn_readfirstlane(
-        min(min(doc_range[0][0], doc_range[0][1]), min(doc_range[0][2], doc_range[0][3])));
+        min(min(doc_range[0], doc_range[1]), min(doc_range[2], doc_range[3])));
     doc_hi = __builtin_amdgcn_readfirstlane(
-        max(max(doc_range[1][0], doc_range[1][1]), max(doc_range[1][2], doc_range[1][3])));
+        max(max(doc_range[4], doc_range[5]), max(doc_range[6], doc_range[7])));
   }
 
   const T* kbase = static_cast<const T*>(a.k);
@@ -154,8 +174,8 @@ __global__ __launch_bounds__(256, (mod_min_blocks<T, D, MODE>())) void attn_pref
     for (int st = 0; st < KS; ++st) qf[st] = ok ? frag_load(qrow + 32 * st + 8 * qq) : frag_zero<F>();
   }
 
-  // A split's chunks: K 0 .. n - 1, then V 0 .. n - 1, in alternating buffers
-  // from buffer 0; n = KC but for the last split, which has enough for maxkeys.
+  // A split's chunks: K 0 .. n - 1, then V 0 .. n - 1, through the ring; n = KC but
+  // for the last split, which has enough for maxkeys.
   const int nsplit = maxkeys > 0 ? (maxkeys + kSplit - 1) / kSplit : 0;
   const int nkc_last = nsplit > 0 ? (maxkeys - (nsplit - 1) * kSplit + CH - 1) / CH : 0;
   // Copy offsets as in the plain kernel: a per-lane byte offset that is the same
@@ -176,14 +196,17 @@ __global__ __launch_bounds__(256, (mod_min_blocks<T, D, MODE>())) void attn_pref
     for (int i = 0; i < kVPeriod; ++i) voff[i] = KV::template tile_off<true>(c0 + i, lane, a.v_sl);
   }
   // Requests the chunk of keys key0 .. key0 + CH - 1 of K (or V) into buffer `slot`,
-  // and a split's document numbers with its first K chunk (every wave is past the
-  // scores of the split before it then).
+  // and with a split's first K chunk its document numbers.
+  int docs_slot = 0;
   auto request = [&](auto is_v, int at, int slot) __attribute__((always_inline)) {
     constexpr bool V = decltype(is_v)::value;
     const int key0 = __builtin_amdgcn_readfirstlane(at);
     const int64_t sl = V ? a.v_sl : a.k_sl;
     char* buf = ring + slot * CHB;
-    if (!V && docs && key0 % kSplit == 0) copy_to_lds4(docs + min(key0 + tid, len - 1), split_docs + 64 * wave);
+    if (!V && docs && key0 % kSplit == 0) {
+      copy_to_lds4(docs + min(key0 + tid, len - 1), split_docs + kSplit * docs_slot + 64 * wave);
+      docs_slot ^= 1;
+    }
     if constexpr (MODE == kKvContig || MODE == kKvPaged) {
       const int rows = min(CH, len - key0);             // >= 1: chunks start below maxkeys <= len
       const T* base = MODE == kKvContig
@@ -230,42 +253,73 @@ __global__ __launch_bounds__(256, (mod_min_blocks<T, D, MODE>())) void attn_pref
     }
   };
 
-  // The split to run next, and whether its only document is the workgroup's.
-  int next = 0;
-  bool next_own = true;
-  uint64_t hit = 0, lone = 0;                           // splits 64 g .. 64 g + 63: one of our documents; only ours
-  int group = -1;
-  auto advance = [&](int sp) __attribute__((always_inline)) {
-    if (docs) {
-      while (sp < nsplit) {
-        if (sp / 64 != group) {
-          group = sp / 64;
-          int2 range = {0x7fffffff, -0x7fffffff - 1};
-          if (64 * group + lane < nsplit)
-            range = a.mod.ranges[(int64_t)b * ((a.L + kSplit - 1) / kSplit) + 64 * group + lane];
-          hit = __ballot(range.y >= doc_lo && range.x <= doc_hi);
-          lone = __ballot(range.x == doc_lo && range.y == doc_lo && doc_lo == doc_hi);
-        }
-        const uint64_t left = hit >> (sp % 64);
-        sp = left ? sp + __builtin_ctzll(left) : 64 * (group + 1);
-        if (left) break;
+  // Splits [sp0, sp1) hold all of the workgroup's documents' keys: 64 splits'
+  // ranges tested at once, before the first copy (a vector load inside the loop
+  // would make the compiler wait for the copies in flight).
+  int sp0 = 0, sp1 = nsplit;
+  if (docs) {
+    sp0 = nsplit;
+    sp1 = 0;
+    for (int g = 0; g < nsplit; g += 64) {
+      int2 range = {0x7fffffff, -0x7fffffff - 1};
+      if (g + lane < nsplit) range = a.mod.ranges[(int64_t)b * ((a.L + kSplit - 1) / kSplit) + g + lane];
+      const uint64_t hit = __ballot(range.y >= doc_lo && range.x <= doc_hi);
+      if (hit) {
+        sp0 = min(sp0, g + __builtin_ctzll(hit));
+        sp1 = g + 64 - __builtin_clzll(hit);
       }
-      next_own = lone >> (sp % 64) & 1;
     }
-    next = __builtin_amdgcn_readfirstlane(sp);          // (known to be one for the wave: copies take it so)
+    sp0 = __builtin_amdgcn_readfirstlane(sp0);          // (known to be one for the wave: copies take it so)
+    sp1 = __builtin_amdgcn_readfirstlane(sp1);
+  }
+  // Whether the workgroup's only document is split sp's only one.
+  auto own_doc = [&](int sp) __attribute__((always_inline)) {
+    if (!docs) return true;
+    const int32_t* at = reinterpret_cast<const int32_t*>(a.mod.ranges + (int64_t)b * ((a.L + kSplit - 1) / kSplit) + sp);
+    return doc_lo == doc_hi && load_uniform_i32(uniform_ptr(at)) == doc_lo &&
+           load_uniform_i32(uniform_ptr(at + 1)) == doc_lo;
   };
+  // The chunks in the order they are used, requested NBUF - 1 ahead: the next one
+  // to request is chunk r_i (of r_n K chunks, then r_n V chunks) of split r_sp,
+  // into buffer r_slot; `ahead` of them are requested and not yet opened.
+  int r_sp = 0, r_i = 0, r_n = 0, r_slot = 0, ahead = 0;
+  auto chunks_of = [&](int sp) { return sp + 1 < nsplit ? KC : nkc_last; };
+  auto request_next = [&]() __attribute__((always_inline)) {
+    if (r_sp >= sp1) return;
+    if (r_i < r_n) request(std::false_type(), r_sp * kSplit + r_i * CH, r_slot);
+    else request(std::true_type(), r_sp * kSplit + (r_i - r_n) * CH, r_slot);
+    r_slot = (r_slot + 1) % NBUF;
+    ++ahead;
+    if (++r_i == 2 * r_n) {
+      r_i = 0;
+      r_n = chunks_of(++r_sp);
+    }
+  };
+  // Opens the chunk in buffer `slot`: waits until it is there (the copies requested
+  // behind it may be in flight) and every wave is done with the one before it,
+  // whose buffer takes the next request (`behind`: work on this chunk before that).
+  auto open_chunk = [&](int slot, auto behind) __attribute__((always_inline)) {
+    --ahead;
+    if (NBUF >= 4 && ahead >= 2) stage_barrier<2 * CPW>();
+    else if (NBUF >= 4 && ahead >= 1) stage_barrier<CPW>();
+    else stage_barrier<0>();
+    char* buf = ring + slot * CHB;
+    behind(buf);
+    request_next();
+    return buf;
+  };
+  int doc_buf = 0;                                      // the split's document numbers
   // The keys of a chunk that the document mask leaves to this lane's row, bit
   // 4 t + i for key 16 t + 4 qq + i.
   auto doc_bits = [&](int kc) __attribute__((always_inline)) {
-    uint32_t ok = ~0u;
-    if (docs) {
-      ok = 0;
+    const int my_doc = row_doc[16 * wave + r];
+    uint32_t ok = 0;
 #pragma unroll
-      for (int t = 0; t < TPC; ++t) {
-        const int4 d = *reinterpret_cast<const int4*>(split_docs + CH * kc + 16 * t + 4 * qq);
-        ok |= ((d.x == my_doc ? 1u : 0u) | (d.y == my_doc ? 2u : 0u) | (d.z == my_doc ? 4u : 0u) |
-               (d.w == my_doc ? 8u : 0u)) << (4 * t);
-      }
+    for (int t = 0; t < TPC; ++t) {
+      // (a vector type, not int4: its reads carry type information, see lds_read_tr16)
+      const u32x4 d = *reinterpret_cast<const u32x4*>(split_docs + kSplit * doc_buf + CH * kc + 16 * t + 4 * qq);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) ok |= ((int)d[i] == my_doc ? 1u : 0u) << (4 * t + i);
     }
     return ok;
   };
@@ -308,9 +362,9 @@ __global__ __launch_bounds__(256, (mod_min_blocks<T, D, MODE>())) void attn_pref
   // and weights, P.V and the weight sum, the merge. PIPE: software-pipelined
   // inside the wave as attn_prefill_mfma's split_body_pipe, whose comment says how.
   auto split_body = [&](const int sp, auto masked) __attribute__((always_inline)) {
-    constexpr bool MASKED = decltype(masked)::value;
+    constexpr bool MASKED = decltype(masked)::value > 0, DOCS = decltype(masked)::value > 1;
     const int j0 = sp * kSplit;
-    const int nkc = !MASKED || sp + 1 < nsplit ? KC : nkc_last;
+    const int nkc = MASKED ? chunks_of(sp) : KC;
     float s[16][4];
     float m = -INFINITY;
 #pragma unroll
@@ -322,20 +376,18 @@ __global__ __launch_bounds__(256, (mod_min_blocks<T, D, MODE>())) void attn_pref
           for (int i = 0; i < 4; ++i) s[TPC * kc + t][i] = -INFINITY;
         continue;
       }
-      // Chunk landed (everyone's: the barrier); the next one goes into the
-      // other buffer, which every wave is done with.
-      stage_barrier<0>();
-      if (kc + 1 < nkc) request(std::false_type(), j0 + CH * (kc + 1), (kc + 1) % 2);
-      else request(std::true_type(), j0, nkc % 2);
-      const char* buf = ring + kc % 2 * CHB;
-      const int lim = my_nkeys - (j0 + CH * kc + 4 * qq);
-      const uint32_t seen = MASKED ? doc_bits(kc) : ~0u;
+      const char* buf = open_chunk(kc % NBUF, [](char*) {});
+      const int lim = MASKED ? row_nkeys[16 * wave + r] - (j0 + CH * kc + 4 * qq) : 0;
+      const uint32_t seen = DOCS ? doc_bits(kc) : ~0u;
       const float far = (MOD & kModBias) != 0 ? (float)(my_pos - (j0 + CH * kc + 4 * qq)) : 0.0f;
       auto finish = [&](int t, f32x4 dot) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          const float y = mod_score<T, MOD>(dot[i], a, slope2, far - (float)(16 * t + i));
-          const float x = (!MASKED || (16 * t + i < lim && (seen >> (4 * t + i) & 1u))) ? y : -INFINITY;
+          // (materialised here: left alone the compiler moves the whole split's score
+          // arithmetic behind its last K chunk, away from the MFMAs that hide it, or
+          // branches around it for every hidden key)
+          const float y = materialize(mod_score<T, MOD>(dot[i], a, slope2, far - (float)(16 * t + i)));
+          const float x = (!MASKED || 16 * t + i < lim) && (!DOCS || (seen >> (4 * t + i) & 1u)) ? y : -INFINITY;
           s[TPC * kc + t][i] = x;
           m = fmaxf(m, x);
         }
@@ -401,13 +453,9 @@ __global__ __launch_bounds__(256, (mod_min_blocks<T, D, MODE>())) void attn_pref
 #pragma unroll
     for (int kc = 0; kc < KC; ++kc) {
       if (kc >= nkc) continue;
-      stage_barrier<0>();
-      char* buf = ring + (nkc + kc) % 2 * CHB;
-      if constexpr (MASKED) {
-        if (careful) clean_v(buf, j0 + CH * kc);
-      }
-      if (kc + 1 < nkc) request(std::true_type(), j0 + CH * (kc + 1), (nkc + kc + 1) % 2);
-      else if (next < nsplit) request(std::false_type(), kSplit * next, 0);
+      const char* buf = open_chunk((nkc + kc) % NBUF, [&](char* v) __attribute__((always_inline)) {
+        if (MASKED && careful) clean_v(v, j0 + CH * kc);
+      });
       if constexpr (PIPE) {
         int vo = vbase0;
         asm volatile("" : "+v"(vo));
@@ -458,17 +506,16 @@ __global__ __launch_bounds__(256, (mod_min_blocks<T, D, MODE>())) void attn_pref
     // that sees no key of the split skips it.
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-      if (mi[i] > -INFINITY || lsum[i] != 0.0f) {
-        float ai[NDT];
+      // (merge_split's operations; a row that skips the split multiplies by 1 and
+      // adds -0 instead of branching, which leaves its state's every bit)
+      const bool sees = mi[i] > -INFINITY || lsum[i] != 0.0f;
+      const float top = sees ? fmaxf(M[i], mi[i]) : M[i];
+      const float c_old = sees ? __builtin_amdgcn_exp2f(M[i] - top) : 1.0f;
+      const float c_new = sees ? __builtin_amdgcn_exp2f(mi[i] - top) : -0.0f;
+      Lsum[i] = __builtin_fmaf(Lsum[i], c_old, lsum[i] * c_new);
 #pragma unroll
-        for (int dt = 0; dt < NDT; ++dt) ai[dt] = A[dt][i];
-        float acci[NDT];
-#pragma unroll
-        for (int dt = 0; dt < NDT; ++dt) acci[dt] = acc[dt][i];
-        merge_split<NDT>(M[i], Lsum[i], ai, mi[i], lsum[i], acci);
-#pragma unroll
-        for (int dt = 0; dt < NDT; ++dt) A[dt][i] = ai[dt];
-      }
+      for (int dt = 0; dt < NDT; ++dt) A[dt][i] = __builtin_fmaf(A[dt][i], c_old, acc[dt][i] * c_new);
+      M[i] = top;
     }
   };
 
@@ -480,14 +527,17 @@ __global__ __launch_bounds__(256, (mod_min_blocks<T, D, MODE>())) void attn_pref
     }
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt) A[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
-    advance(0);
-    if (next < nsplit) request(std::false_type(), kSplit * next, 0);
-    while (next < nsplit) {
-      const int sp = next;
-      const bool own = next_own;
-      advance(sp + 1);
-      if (sp * kSplit + kSplit <= wave_min_nkeys && own && !careful) split_body(sp, std::false_type());
-      else split_body(sp, std::true_type());
+    r_sp = sp0;
+    r_n = chunks_of(r_sp);
+    r_i = r_slot = ahead = docs_slot = doc_buf = 0;
+#pragma unroll
+    for (int c = 0; c < NBUF - 1; ++c) request_next();
+    for (int sp = sp0; sp < sp1; ++sp) {
+      if (sp * kSplit + kSplit <= wave_min_nkeys && !careful && own_doc(sp))
+        split_body(sp, std::integral_constant<int, 0>());
+      else if (!docs) split_body(sp, std::integral_constant<int, 1>());
+      else split_body(sp, std::integral_constant<int, 2>());
+      doc_buf ^= 1;
     }
     bool finite = true;
 #pragma unroll
@@ -496,7 +546,11 @@ __global__ __launch_bounds__(256, (mod_min_blocks<T, D, MODE>())) void attn_pref
 #pragma unroll
       for (int dt = 0; dt < NDT; ++dt) finite = finite && fabsf(A[dt][i]) < INFINITY;
     }
-    if (careful || !__builtin_amdgcn_readfirstlane(__syncthreads_or(!finite))) break;
+    if (careful) break;
+    const bool bad = __ballot(!finite) != 0;            // (the library's vote would be a second LDS array)
+    if (lane == 0) doc_range[wave] = bad ? 1 : 0;
+    __syncthreads();
+    if (!__builtin_amdgcn_readfirstlane(doc_range[0] | doc_range[1] | doc_range[2] | doc_range[3])) break;
     careful = true;
     for (int i = tid; i < 16 * D; i += 256) poison[i] = 0;
     __syncthreads();
@@ -505,19 +559,24 @@ __global__ __launch_bounds__(256, (mod_min_blocks<T, D, MODE>())) void attn_pref
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int row = 16 * wave + 4 * qq + i, pair = 64 * wg + row;
+#pragma unroll
+    for (int dt = 0; dt < NDT; ++dt) {
+      const float x = materialize(A[dt][i] / Lsum[i]);
+      A[dt][i] = Lsum[i] != 0.0f ? x : 0.0f;            // no key: 0
+    }
+    if (careful) {
+#pragma unroll
+      for (int dt = 0; dt < NDT; ++dt) {
+        const int at = row * D + 16 * dt + r;
+        const uint32_t bad = poison[at / 4] >> (8 * (at % 4)) & 7u;
+        if (bad) A[dt][i] = bad == 1 ? INFINITY : bad == 2 ? -INFINITY : NAN;
+      }
+    }
     if (pair >= npairs) continue;
     T* o = static_cast<T*>(a.out) +
            ((((int64_t)b * a.Hq + hk * G + pair % G) * a.Tq) + pair / G) * D + r;
 #pragma unroll
-    for (int dt = 0; dt < NDT; ++dt) {
-      float x = Lsum[i] != 0.0f ? A[dt][i] / Lsum[i] : 0.0f;   // no key: 0
-      if (careful) {
-        const int at = row * D + 16 * dt + r;
-        const uint32_t bad = poison[at / 4] >> (8 * (at % 4)) & 7u;
-        if (bad) x = bad == 1 ? INFINITY : bad == 2 ? -INFINITY : NAN;
-      }
-      o[16 * dt] = to_store<T>(x);
-    }
+    for (int dt = 0; dt < NDT; ++dt) o[16 * dt] = to_store<T>(A[dt][i]);
   }
 }
 
