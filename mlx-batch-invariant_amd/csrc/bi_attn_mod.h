@@ -434,7 +434,20 @@ __global__ __launch_bounds__(256, (mod_min_blocks<T, D, MODE>())) void attn_pref
     auto weight_pair = [&](PFrag<T>& pf, int ks, int j) __attribute__((always_inline)) {
       const int t = 2 * ks + j / 2, i = 2 * (j % 2);
       const float p0 = __builtin_amdgcn_exp2f(s[t][i] - msub), p1 = __builtin_amdgcn_exp2f(s[t][i + 1] - msub);
-      if constexpr (sizeof(T) == 2) {
+      if constexpr (std::is_same_v<T, f16>) {
+        // pfrag_pair's values: p - hi is exact, and v_fma_mix_f32 takes hi unwidened
+        // (written out, since the compiler turns the fma back into a widening and a
+        // subtraction; it follows the conversion, so nothing reads an exp too early).
+        const f16x2_t h = __builtin_convertvector(f32x2_t{p0, p1}, f16x2_t);
+        float l0, l1;
+        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel_hi:[1,0,0]" : "=v"(l0) : "v"(h), "v"(p0));
+        asm("v_fma_mix_f32 %0, %1, -1.0, %2 op_sel:[1,0,0] op_sel_hi:[1,0,0]" : "=v"(l1) : "v"(h), "v"(p1));
+        const f16x2_t l = __builtin_convertvector(f32x2_t{l0, l1}, f16x2_t);
+        pf.hi[2 * j] = h[0];
+        pf.hi[2 * j + 1] = h[1];
+        pf.lo[2 * j] = l[0];
+        pf.lo[2 * j + 1] = l[1];
+      } else if constexpr (sizeof(T) == 2) {
         pfrag_pair<T>(pf, j, p0, p1);
       } else {
         f32x4& half = j < 2 ? pf.f.lo : pf.f.hi;
