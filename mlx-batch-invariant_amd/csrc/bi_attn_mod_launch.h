@@ -23,7 +23,15 @@ __global__ __launch_bounds__(256) void attn_combine_mod_kernel(DecodeArgs a) {
   const int ns = (len + kSplit - 1) / kSplit;
   float M = -INFINITY, Ls = 0.0f, A = 0.0f;
   auto merge = [&](float m, float l, float acc) {
-    if (m > -INFINITY || l != 0.0f) merge_split<1>(M, Ls, &A, m, l, &acc);
+    // (merge_split's operations, without a branch: a split passed over multiplies
+    // by 1 and adds -0; its acc may be unwritten)
+    const bool sees = m > -INFINITY || l != 0.0f;
+    const float top = sees ? fmaxf(M, m) : M;
+    const float c_old = sees ? __builtin_amdgcn_exp2f(M - top) : 1.0f;
+    const float c_new = sees ? __builtin_amdgcn_exp2f(m - top) : -0.0f;
+    Ls = __builtin_fmaf(Ls, c_old, l * c_new);
+    A = __builtin_fmaf(A, c_old, sees ? acc * c_new : -0.0f);
+    M = top;
   };
   int i = 0;
   for (; i + 8 <= ns; i += 8) {                         // partials loaded eight splits ahead, merged in order
