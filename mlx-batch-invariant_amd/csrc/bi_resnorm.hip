@@ -20,49 +20,87 @@ struct ResNormArgs {
   const void *x, *res, *gate, *w_post, *w_pre;
   void *y, *h;
   int64_t x_row, res_row, gate_row, gate_group;   // gate row r / gate_group
+  int64_t rows;
   int D;
   float eps, scale;
 };
 
-// Sum over the workgroup in rms_norm's order; every thread gets it. The barrier
-// before the write lets a second sum use the same words.
+// How a row's 8-element chunks are read and written: rows of whole 16-byte
+// pieces; rows at any element (an odd D, a slice), whose chunks are still one
+// access each (the hardware takes any address; the last chunk may be short and
+// goes element by element); rows longer than the registers hold, element by element.
+enum RowForm { kAligned, kAnywhere, kElements };
+
+template <typename T>
+struct Any16 { uint32_t w[4]; } __attribute__((packed, aligned(alignof(T))));
+
+// Eight elements from index `base`, zeros past D.
+template <typename T, RowForm FORM>
+__device__ __forceinline__ void row_load(const T* p, int base, int D, float* out) {
+  if constexpr (FORM == kAligned) {
+    load8<T>(p + base, out);
+    return;
+  }
+  if (FORM == kAnywhere && base + 8 <= D) {
+    T e[8];
+    *reinterpret_cast<Any16<T>*>(e) = *reinterpret_cast<const Any16<T>*>(p + base);
+    if constexpr (sizeof(T) == 4)
+      *reinterpret_cast<Any16<T>*>(e + 4) = *reinterpret_cast<const Any16<T>*>(p + base + 4);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) out[i] = to_f32(e[i]);
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) out[e] = base + e < D ? to_f32(p[base + e]) : 0.0f;
+}
+template <typename T, RowForm FORM>
+__device__ __forceinline__ void row_store(T* p, int base, int D, const float* in) {
+  if constexpr (FORM == kAligned) {
+    store8<T>(p + base, in);
+    return;
+  }
+  if (FORM == kAnywhere && base + 8 <= D) {
+    T e[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) e[i] = to_store<T>(in[i]);
+    *reinterpret_cast<Any16<T>*>(p + base) = *reinterpret_cast<const Any16<T>*>(e);
+    if constexpr (sizeof(T) == 4)
+      *reinterpret_cast<Any16<T>*>(p + base + 4) = *reinterpret_cast<const Any16<T>*>(e + 4);
+    return;
+  }
+#pragma unroll
+  for (int e = 0; e < 8; ++e)
+    if (base + e < D) p[base + e] = to_store<T>(in[e]);
+}
+
+// Sum over the WPR waves of a row in rms_norm's order (waves it does not have
+// would add 0 there); every thread gets it. The barrier before the write lets a
+// second sum use the same words.
+template <int WPR>
 __device__ __forceinline__ float row_sum(float ss, float* wave_sums) {
   ss = wave_sum_butterfly(ss);
+  if constexpr (WPR == 1) return ss;
+  const int wave = threadIdx.x / kWave, first = wave / WPR * WPR;
   __syncthreads();
-  if (threadIdx.x % kWave == 0) wave_sums[threadIdx.x / kWave] = ss;
+  if (threadIdx.x % kWave == 0) wave_sums[wave] = ss;
   __syncthreads();
-  float total = wave_sums[0];
+  float total = wave_sums[first];
 #pragma unroll
-  for (int i = 1; i < kResThreads / kWave; ++i) total = total + wave_sums[i];
+  for (int i = 1; i < WPR; ++i) total = total + wave_sums[first + i];
   return total;
 }
 
-// Eight elements from index `base`, vectorised or one by one (zeros past D).
-template <typename T, bool VECTOR>
-__device__ __forceinline__ void row_load(const T* p, int base, int D, float* out) {
-  if constexpr (VECTOR) {
-    load8<T>(p + base, out);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) out[e] = base + e < D ? to_f32(p[base + e]) : 0.0f;
-  }
-}
-template <typename T, bool VECTOR>
-__device__ __forceinline__ void row_store(T* p, int base, int D, const float* in) {
-  if constexpr (VECTOR) {
-    store8<T>(p + base, in);
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (base + e < D) p[base + e] = to_store<T>(in[e]);
-  }
-}
-
-// Rows of up to NC * 2048 elements, kept in registers between the sums.
-template <typename T, int NC, bool VECTOR, bool POST, bool PRE>
+// Rows of up to NC * 512 * WPR elements, kept in registers between the sums, WPR
+// waves each: 4 / WPR rows in a workgroup.
+template <typename T, int NC, RowForm FORM, bool POST, bool PRE, int WPR>
 __global__ __launch_bounds__(kResThreads) void res_norm_kernel(ResNormArgs a) {
+  static_assert(WPR == 4 || NC == 1, "res_norm_kernel: a row's chunks are its threads'");
   __shared__ float wave_sums[kResThreads / kWave];
-  const int64_t row = blockIdx.x;
+  constexpr int kRowThreads = WPR * kWave;
+  const int t = threadIdx.x % kRowThreads;
+  const int64_t row0 = (int64_t)blockIdx.x * (kResThreads / kRowThreads) + threadIdx.x / kRowThreads;
+  const bool live = row0 < a.rows;
+  const int64_t row = live ? row0 : a.rows - 1;        // (a workgroup's spare rows repeat the last and store nothing)
   const T* x = static_cast<const T*>(a.x) + row * a.x_row;
   const T* res = static_cast<const T*>(a.res) + row * a.res_row;
   const T* gate = a.gate ? static_cast<const T*>(a.gate) + row / a.gate_group * a.gate_row : nullptr;
@@ -72,10 +110,10 @@ __global__ __launch_bounds__(kResThreads) void res_norm_kernel(ResNormArgs a) {
   float u[NC][8], y[NC][8];
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
-    const int chunk = threadIdx.x + c * kResThreads;
+    const int chunk = t + c * kRowThreads;
     if (chunk < nchunks) {
-      row_load<T, VECTOR>(x, 8 * chunk, D, u[c]);
-      row_load<T, VECTOR>(res, 8 * chunk, D, y[c]);
+      row_load<T, FORM>(x, 8 * chunk, D, u[c]);
+      row_load<T, FORM>(res, 8 * chunk, D, y[c]);
     } else {
 #pragma unroll
       for (int e = 0; e < 8; ++e) u[c][e] = y[c][e] = 0.0f;
@@ -87,12 +125,12 @@ __global__ __launch_bounds__(kResThreads) void res_norm_kernel(ResNormArgs a) {
     for (int c = 0; c < NC; ++c)
 #pragma unroll
       for (int e = 0; e < 8; ++e) ss = __builtin_fmaf(u[c][e], u[c][e], ss);
-    const float inv = 1.0f / sqrtf(row_sum(ss, wave_sums) / (float)D + a.eps);
+    const float inv = 1.0f / sqrtf(row_sum<WPR>(ss, wave_sums) / (float)D + a.eps);
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      const int chunk = threadIdx.x + c * kResThreads;
+      const int chunk = t + c * kRowThreads;
       float w[8];
-      if (w1 && chunk < nchunks) row_load<T, VECTOR>(w1, 8 * chunk, D, w);
+      if (w1 && chunk < nchunks) row_load<T, FORM>(w1, 8 * chunk, D, w);
 #pragma unroll
       for (int e = 0; e < 8; ++e) u[c][e] = w1 && chunk < nchunks ? (u[c][e] * inv) * w[e] : u[c][e] * inv;
     }
@@ -100,33 +138,33 @@ __global__ __launch_bounds__(kResThreads) void res_norm_kernel(ResNormArgs a) {
   float ss = 0.0f;
 #pragma unroll
   for (int c = 0; c < NC; ++c) {
-    const int chunk = threadIdx.x + c * kResThreads;
+    const int chunk = t + c * kRowThreads;
     if (chunk < nchunks) {
       if (gate) {
         float g[8];
-        row_load<T, VECTOR>(gate, 8 * chunk, D, g);
+        row_load<T, FORM>(gate, 8 * chunk, D, g);
 #pragma unroll
         for (int e = 0; e < 8; ++e) u[c][e] = u[c][e] * g[e];
       }
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         y[c][e] = y[c][e] + u[c][e] * a.scale;
-        if (VECTOR || 8 * chunk + e < D) ss = __builtin_fmaf(y[c][e], y[c][e], ss);
+        if (FORM == kAligned || 8 * chunk + e < D) ss = __builtin_fmaf(y[c][e], y[c][e], ss);
       }
-      row_store<T, VECTOR>(static_cast<T*>(a.y) + row * D, 8 * chunk, D, y[c]);
+      if (live) row_store<T, FORM>(static_cast<T*>(a.y) + row * D, 8 * chunk, D, y[c]);
     }
   }
   if constexpr (PRE) {
-    const float inv = 1.0f / sqrtf(row_sum(ss, wave_sums) / (float)D + a.eps);
+    const float inv = 1.0f / sqrtf(row_sum<WPR>(ss, wave_sums) / (float)D + a.eps);
 #pragma unroll
     for (int c = 0; c < NC; ++c) {
-      const int chunk = threadIdx.x + c * kResThreads;
+      const int chunk = t + c * kRowThreads;
       if (chunk < nchunks) {
         float w[8];
-        if (w2) row_load<T, VECTOR>(w2, 8 * chunk, D, w);
+        if (w2) row_load<T, FORM>(w2, 8 * chunk, D, w);
 #pragma unroll
         for (int e = 0; e < 8; ++e) y[c][e] = w2 ? (y[c][e] * inv) * w[e] : y[c][e] * inv;
-        row_store<T, VECTOR>(static_cast<T*>(a.h) + row * D, 8 * chunk, D, y[c]);
+        if (live) row_store<T, FORM>(static_cast<T*>(a.h) + row * D, 8 * chunk, D, y[c]);
       }
     }
   }
@@ -148,23 +186,23 @@ __global__ __launch_bounds__(kResThreads) void res_norm_kernel_long(ResNormArgs 
     float ss = 0.0f;
     for (int chunk = threadIdx.x; chunk < nchunks; chunk += kResThreads) {
       float u[8];
-      row_load<T, false>(x, 8 * chunk, D, u);
+      row_load<T, kElements>(x, 8 * chunk, D, u);
 #pragma unroll
       for (int e = 0; e < 8; ++e) ss = __builtin_fmaf(u[e], u[e], ss);
     }
-    inv1 = 1.0f / sqrtf(row_sum(ss, wave_sums) / (float)D + a.eps);
+    inv1 = 1.0f / sqrtf(row_sum<kResThreads / kWave>(ss, wave_sums) / (float)D + a.eps);
   }
   auto stream = [&](int chunk, float* y) {            // the chunk's y, unrounded
     float u[8], w[8];
-    row_load<T, false>(x, 8 * chunk, D, u);
-    row_load<T, false>(res, 8 * chunk, D, y);
+    row_load<T, kElements>(x, 8 * chunk, D, u);
+    row_load<T, kElements>(res, 8 * chunk, D, y);
     if (POST) {
-      if (w1) row_load<T, false>(w1, 8 * chunk, D, w);
+      if (w1) row_load<T, kElements>(w1, 8 * chunk, D, w);
 #pragma unroll
       for (int e = 0; e < 8; ++e) u[e] = w1 ? (u[e] * inv1) * w[e] : u[e] * inv1;
     }
     if (gate) {
-      row_load<T, false>(gate, 8 * chunk, D, w);
+      row_load<T, kElements>(gate, 8 * chunk, D, w);
 #pragma unroll
       for (int e = 0; e < 8; ++e) u[e] = u[e] * w[e];
     }
@@ -178,35 +216,40 @@ __global__ __launch_bounds__(kResThreads) void res_norm_kernel_long(ResNormArgs 
 #pragma unroll
     for (int e = 0; e < 8; ++e)
       if (8 * chunk + e < D) ss = __builtin_fmaf(y[e], y[e], ss);
-    if constexpr (!PRE) row_store<T, false>(static_cast<T*>(a.y) + row * D, 8 * chunk, D, y);
+    if constexpr (!PRE) row_store<T, kElements>(static_cast<T*>(a.y) + row * D, 8 * chunk, D, y);
   }
   if constexpr (PRE) {
-    const float inv = 1.0f / sqrtf(row_sum(ss, wave_sums) / (float)D + a.eps);
+    const float inv = 1.0f / sqrtf(row_sum<kResThreads / kWave>(ss, wave_sums) / (float)D + a.eps);
     for (int chunk = threadIdx.x; chunk < nchunks; chunk += kResThreads) {
       float y[8], w[8];
       stream(chunk, y);
-      row_store<T, false>(static_cast<T*>(a.y) + row * D, 8 * chunk, D, y);
-      if (w2) row_load<T, false>(w2, 8 * chunk, D, w);
+      row_store<T, kElements>(static_cast<T*>(a.y) + row * D, 8 * chunk, D, y);
+      if (w2) row_load<T, kElements>(w2, 8 * chunk, D, w);
 #pragma unroll
       for (int e = 0; e < 8; ++e) y[e] = w2 ? (y[e] * inv) * w[e] : y[e] * inv;
-      row_store<T, false>(static_cast<T*>(a.h) + row * D, 8 * chunk, D, y);
+      row_store<T, kElements>(static_cast<T*>(a.h) + row * D, 8 * chunk, D, y);
     }
   }
 }
 
 template <typename T, bool POST, bool PRE>
 static void launch_res_norm(const ResNormArgs& a, int64_t rows, bool vec, hipStream_t st) {
-  const dim3 grid((unsigned)rows);
   const int nchunks = (a.D + 7) / 8;
-#define BI_RES(NC)                                                                                      \
+#define BI_RES(NC, WPR)                                                                                 \
   do {                                                                                                  \
-    if (vec) res_norm_kernel<T, NC, true, POST, PRE><<<grid, kResThreads, 0, st>>>(a);                  \
-    else res_norm_kernel<T, NC, false, POST, PRE><<<grid, kResThreads, 0, st>>>(a);                     \
+    const unsigned grid = (unsigned)((rows + 4 / WPR - 1) / (4 / WPR));                                 \
+    if (vec) res_norm_kernel<T, NC, kAligned, POST, PRE, WPR><<<grid, kResThreads, 0, st>>>(a);         \
+    else res_norm_kernel<T, NC, kAnywhere, POST, PRE, WPR><<<grid, kResThreads, 0, st>>>(a);            \
   } while (0)
-  if (nchunks <= kResThreads) BI_RES(1);
-  else if (nchunks <= 2 * kResThreads) BI_RES(2);
-  else if (nchunks <= 4 * kResThreads) BI_RES(4);
-  else res_norm_kernel_long<T, POST, PRE><<<grid, kResThreads, 0, st>>>(a);
+  // A wave or two for rows that fill no more: all of its lanes have work, and rows
+  // of one wave meet no barrier.
+  if (nchunks <= kWave) BI_RES(1, 1);
+  else if (nchunks <= 2 * kWave) BI_RES(1, 2);
+  else if (nchunks <= kResThreads) BI_RES(1, 4);
+  else if (nchunks <= 2 * kResThreads) BI_RES(2, 4);
+  else if (nchunks <= 3 * kResThreads) BI_RES(3, 4);
+  else if (nchunks <= 4 * kResThreads) BI_RES(4, 4);
+  else res_norm_kernel_long<T, POST, PRE><<<(unsigned)rows, kResThreads, 0, st>>>(a);
 #undef BI_RES
 }
 
@@ -239,7 +282,7 @@ extern "C" int bi_residual_rms_norm(const void* x, int64_t x_row_stride, const v
                 what, (long long)x_row_stride, (long long)res_row_stride, (long long)D, (long long)gate_row_stride,
                 (long long)gate_group);
   bi::ResNormArgs a{x, res, gate, post ? w_post : nullptr, pre ? w_pre : nullptr, y, h, x_row_stride, res_row_stride,
-                    gate ? gate_row_stride : 0, gate ? gate_group : 1, (int)D, eps, scale};
+                    gate ? gate_row_stride : 0, gate ? gate_group : 1, rows, (int)D, eps, scale};
   bool vec = D % 8 == 0 && a.x_row % 8 == 0 && a.res_row % 8 == 0 && a.gate_row % 8 == 0;
   for (const void* p : {x, res, gate, a.w_post, a.w_pre, (const void*)y, (const void*)h}) vec = vec && aligned16(p);
   hipStream_t st = static_cast<hipStream_t>(stream);

@@ -236,9 +236,9 @@ def launch(dev: int, fn, *args) -> int:
 def one_device(what: str, *tensors) -> int:
     """Every tensor (None aside) on the GPU, and on the first one's device;
     returns its index."""
-    dev = tensors[0].get_device()
+    dev = tensors[0].get_device()                       # (-1: not on a GPU)
     for t in tensors:
-        if t is not None and (t.get_device() != dev or not t.is_cuda):
+        if t is not None and t.get_device() != dev or dev < 0:
             require_gpu(what, *tensors)
             raise ValueError(f"{what}: tensors on {tensors[0].device} and {t.device}")
     if _lib is None:
@@ -250,19 +250,20 @@ def in_place(what: str, *tensors) -> None:
     """Refuse what torch's own in-place operations refuse: rows that share
     memory, an inference tensor outside inference mode, a leaf that needs a
     gradient."""
+    infer, grad = torch.is_inference_mode_enabled(), torch.is_grad_enabled()
     for t in tensors:
         if 0 in t.stride() and any(s == 0 and n > 1 for s, n in zip(t.stride(), t.shape)):
             raise ValueError(f"{what}: written tensor with rows that share memory (shape {tuple(t.shape)}, "
                              f"strides {t.stride()})")
-        if t.is_inference() and not torch.is_inference_mode_enabled():
+        if not infer and t.is_inference():
             raise ValueError(f"{what}: an inference tensor cannot be written outside inference mode")
-        if t.requires_grad and torch.is_grad_enabled():
+        if grad and t.requires_grad:
             raise ValueError(f"{what}: a tensor that needs a gradient cannot be written in place")
 
 
 def written(*tensors) -> None:
     """Count the tensors as changed in place (their version counters)."""
-    if any(t.is_inference() for t in tensors):
+    if torch.is_inference_mode_enabled():
         tensors = [t for t in tensors if not t.is_inference()]
     torch.autograd.graph.increment_version(tensors)
 
