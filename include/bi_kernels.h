@@ -327,7 +327,7 @@ int bi_attn_prefill_paged(const void* q, const void* k_pages, const void* v_page
  * (causal, or with doc_ids); a query that sees no key, or none of a score above
  * -inf, gets zeros. What hidden keys' K and V rows hold (infinities, NaN) does
  * not matter. slopes fp32 [Hq], doc_ids int32 rows doc_stride >= L apart, prefix_lens
- * int32 [B]: device pointers. softcap >= 0; a prefix needs causal (decode sees
+ * int32 [B]: device pointers. softcap 0 or 1e-30 .. 1e30; a prefix needs causal (decode sees
  * every key of its sequence); slopes need L <= 2^24. strides[0..8] as for
  * bi_attn_prefill (strides[2] unused at Tq == 1). Same order of operations as
  * bi_attn_decode / bi_attn_prefill, so the same invariances hold, and where no

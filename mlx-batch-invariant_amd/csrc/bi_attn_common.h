@@ -90,7 +90,8 @@ struct PrefillArgs {
 // aligned: query t of Tq stands at pos_q = len - Tq + t.
 struct ScoreMod {
   float cap_log2;         // cap log2(e); 0: scores are not capped
-  float cap_in;           // scale / cap (fp32 scores), 2 log2(e) scale / cap (16-bit)
+  float cap_in;           // scale / cap, or 2 log2(e) scale / cap if not cap_close
+  int cap_close;          // scores close to 0 matter beside the cap: cap_score's closer form
   const float* slopes;    // [Hq]; null: no distance bias
   const int32_t* docs;    // document of key j of sequence b: docs[b docs_sb + j]; null: one document
   int64_t docs_sb;
@@ -111,15 +112,18 @@ struct ModRowsArgs : ModPrefillArgs {     // partials of every (b, head, token) 
 enum { kModAny = 1, kModCap = 2, kModBias = 4 };
 template <int MOD> using DecodeArgsOf = std::conditional_t<MOD != 0, ModDecodeArgs, DecodeArgs>;
 
-// cap log2(e) tanh(dot scale / cap). For 16-bit operands 1 - 2 / (exp(2 z) + 1)
-// by the hardware exp2 and reciprocal (44 cycles a wave): off by at most about 3
-// 2^-24 cap log2(e) in absolute terms, 2^-16 of a weight at cap = 50, where
-// their own rounding is 2^-9 (bf16) or 2^-11 (f16) of the output. For fp32
-// operands the same above |z| = 0.6 and below it, where the difference cancels,
-// z P(z^2) with P fitted to tanh(z) / z at Chebyshev points (1.7 2^-24).
-template <typename T>
+// cap log2(e) tanh(dot scale / cap). For 16-bit operands and caps up to 128 as
+// 1 - 2 / (exp(2 z) + 1) by the hardware exp2 and reciprocal (five operations):
+// off by at most 12 2^-24 cap, 2^-14 of a weight at cap = 85, where the output's
+// own rounding is 2^-9 (bf16) or 2^-11 (f16). For fp32 operands, and larger caps,
+// beside which small scores would drown in that, the same above |z| = 0.6 only
+// and below it, where the difference cancels, z P(z^2) with P fitted to tanh(z) /
+// z at Chebyshev points (1.7 2^-24). QUICK: the caller knows that it is not
+// cap_close.
+constexpr float kCapClose = 128.0f;
+template <typename T, bool QUICK>
 __device__ __forceinline__ float cap_score(float dot, const ScoreMod& m) {
-  if constexpr (sizeof(T) == 2) {
+  if (QUICK || (sizeof(T) == 2 && !m.cap_close)) {
     const float x = __builtin_amdgcn_exp2f(dot * m.cap_in);
     return __builtin_fmaf(-2.0f * m.cap_log2, __builtin_amdgcn_rcpf(x + 1.0f), m.cap_log2);
   } else {
@@ -142,7 +146,7 @@ __device__ __forceinline__ float cap_score(float dot, const ScoreMod& m) {
 template <typename T, int MOD, class Args>
 __device__ __forceinline__ float mod_score(float dot, const Args& a, float slope2, float far) {
   float y;
-  if constexpr ((MOD & kModCap) != 0) y = cap_score<T>(dot, a.mod);
+  if constexpr ((MOD & kModCap) != 0) y = cap_score<T, sizeof(T) == 2 && MOD == (kModAny | kModCap)>(dot, a.mod);
   else y = dot * a.scale_log2;
   if constexpr ((MOD & kModBias) != 0) y = __builtin_fmaf(-slope2, fabsf(far), y);
   return y;

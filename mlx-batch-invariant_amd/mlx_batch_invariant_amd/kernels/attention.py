@@ -248,8 +248,8 @@ def _scored(what, q, k, v, table, num_pages, page_size, L, kl, scale, causal, so
     doc_stride = 0
     if softcap is not None:
         softcap = float(softcap)
-        if not 0.0 < softcap < 3e38:
-            raise ValueError(f"{what}: softcap must be a positive number; got {softcap}")
+        if not 1e-30 <= softcap <= 1e30:
+            raise ValueError(f"{what}: softcap must be a positive number (1e-30 to 1e30); got {softcap}")
     if slopes is not None:
         slopes = torch.as_tensor(slopes, dtype=torch.float32, device=q.device).contiguous()
         if tuple(slopes.shape) != (Hq,):

@@ -332,3 +332,41 @@ def test_caches_of_one_split(dt, D, page):
             assert bits(got) == bits(_call(q, *longer, lens, True, page, **n))
             assert not got[1].any()
             _check(got, q, k, v, lens, True, **m)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("cap", [1e-3, 128.0, 1000.0, 1e6, 1e30])
+def test_caps_small_and_large(dt, cap):
+    """Caps far below the scores and far above them (then the plain scores)."""
+    q, k, v = _case(dt, 2, 4, 2, 24, 300, 64, 41)
+    for T in (24, 1):
+        qq = q[:, :, :T].contiguous()
+        got = _call(qq, k, v, None, True, softcap=cap)
+        c = [t.cpu() for t in (qq, k, v)]
+        want, absv, dot, bias = ref.attention(*c, 0.125, None, True, cap)
+        # past a cap of 128 (or in fp32) the error is 12 2^-24 of the score, not of the cap
+        close = cap > 128 or dt == "f32"
+        allow = ref.attention_allowance(want, absv, dot + (12 * dot if close else 0), bias, DT[dt], 64, 2,
+                                        0.0 if close else cap)
+        err = (got.double().cpu() - want).abs()
+        assert (err <= allow).all(), float((err / allow).max())
+
+
+def test_bias_of_any_sign_and_masks_at_their_ends():
+    q, k, v = _case("bf16", 2, 4, 2, 40, 290, 64, 42)
+    for m in (dict(slopes=torch.tensor([-0.01, 0.0, 3.0, 1e-6])),
+              dict(prefix_lens=torch.tensor([1000, -7], dtype=I32)),
+              dict(doc_ids=torch.tensor([[-2**31] * 250 + [2**31 - 1] * 40, list(range(290))], dtype=I32))):
+        for T in (40, 1):
+            qq = q[:, :, :T].contiguous()
+            _check(_call(qq, k, v, None, True, **m), qq, k, v, None, True, **m)
+
+
+def test_bias_over_a_long_cache():
+    """Distances of hundreds of thousands of keys (exact in fp32 up to 2^24)."""
+    L = 300_000
+    q, k, v = _case("bf16", 1, 2, 1, 3, L, 32, 43)
+    m = dict(slopes=torch.tensor([1e-5, 0.0]))
+    for T in (3, 1):
+        qq = q[:, :, :T].contiguous()
+        _check(_call(qq, k, v, None, True, **m), qq, k, v, None, True, **m)
