@@ -127,7 +127,7 @@ def _residual_rms_norm_fake(x, residual, post_weight, pre_weight, eps, gate, sca
 def paged_slots(kv_lens: Tensor, new_lens: Tensor, block_table: Tensor, free_pages: Tensor,
                 cursor: Optional[Tensor], page_size: int, max_new: int) -> tuple[Tensor, Tensor, Tensor, Tensor]:
     p = _k.paged_slots(kv_lens, new_lens, block_table, free_pages, page_size=page_size, max_new=max_new, cursor=cursor)
-    return p.slots, p.positions, p.kv_lens.clone(), p.cursor.clone()       # (outputs that share no memory)
+    return tuple(p)
 
 
 @paged_slots.register_fake
