@@ -424,6 +424,7 @@ extern "C" int bi_attn_scored(const void* q, const void* k, const void* v, const
   int rc = check_attn_shape(what, B, Hq, Hkv, L, D);
   if (rc) return rc;
   if (Tq <= 0) return bi_host::fail(BI_E_INVALID_ARG, "%s: Tq=%lld", what, (long long)Tq);
+  if (Tq > 0x7fffffffLL) return bi_host::fail(BI_E_UNSUPPORTED, "%s: grid too large", what);
   bi::ScoreMod mod;
   if ((rc = check_score_mod(what, score_mod, L, scale, dtype, Tq > 1, causal, &mod))) return rc;
   int shift = 0;

@@ -60,6 +60,7 @@ inline int64_t rows_partial_bytes(int64_t B, int64_t Hq, int64_t Tq, int64_t L, 
 // heads R = 400, N = 2: 59 / 82. Heads of 64 turn at about the same R (420 and
 // 680). The partials stay below 256 MB.
 inline bool few_rows(int64_t B, int64_t Hq, int64_t Hkv, int64_t Tq, int64_t L, int64_t D, int causal, int dtype) {
+  if ((double)Tq * Hq * B > 1e9) return false;           // (so that the products below stay in 64 bits)
   const int64_t n = (L + kSplit - 1) / kSplit;
   const int64_t chunks = (Tq * (Hq / Hkv) + 15) / 16 * Hkv * B;
   const int64_t r = causal ? chunks - chunks * std::min(Tq, L) / (2 * L) : chunks;

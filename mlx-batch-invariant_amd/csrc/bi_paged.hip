@@ -348,6 +348,7 @@ extern "C" int bi_rope_paged_cache(const void* q, int64_t q_row, const void* k, 
                 (long long)half, (long long)(D / 2));
   if (B == 0 || T == 0) return BI_OK;
   const int64_t unit = 16 / (int64_t)dtype_size(dtype);
+  if (k_pages && k_pages == v_pages) return fail(BI_E_INVALID_ARG, "%s: one pool for keys and values", what);
   bool ok = q && k && v && cos && sin && positions && slots && q_out && k_pages && v_pages && q_row >= Hq * D &&
             k_row >= Hkv * D && v_row >= Hkv * D && q_row % unit == 0 && k_row % unit == 0 && v_row % unit == 0;
   for (const void* p : {q, k, v, cos, sin, (const void*)q_out, (const void*)k_pages, (const void*)v_pages})

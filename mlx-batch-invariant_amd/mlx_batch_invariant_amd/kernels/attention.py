@@ -48,7 +48,8 @@ the scores and the mask in the matrix-core order: with query t at position
   |p - j|``;
 * key j is visible if ``j < len`` and, with the causal mask, ``j <= p`` or
   ``j < prefix_lens[b]``, and with ``doc_ids[b]`` of one number per key position,
-  ``doc_ids[b, j] == doc_ids[b, p]``.
+  ``doc_ids[b, j] == doc_ids[b, p]`` (int32; wider numbers are taken modulo
+  2^32).
 
 Hidden keys take no part whatever their rows hold; a query that sees none (one
 in front of a padded prompt, p < 0) gets zeros. The invariances above hold, and

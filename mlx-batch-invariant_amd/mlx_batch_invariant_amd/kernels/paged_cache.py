@@ -149,7 +149,8 @@ def rope_paged_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: tor
     give them; ``k_pages`` / ``v_pages`` ``[num_pages, Hkv, page_size, D]``, the
     pools of ``batch_invariant_paged_attention``, changed in place; ``slots``
     int64 ``[B, T]`` as ``paged_slots`` gives them: one outside the pool (-1: a
-    padding row) writes nothing, and each of the others should occur once.
+    padding row) writes nothing, and each of the others should occur once (of
+    rows written twice either one's values may stay, piece by piece).
 
     ``cos`` / ``sin`` ``[n, R]`` (fp32 or q's type): row p, column j turns the
     pair of dims (j, R + j) of a head at position p; dims from 2 R on are copied
@@ -190,6 +191,8 @@ def rope_paged_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: tor
     unit = 16 // q.element_size()
     kst, vst = k_pages.stride(), v_pages.stride()
     kp, vp = k_pages.data_ptr(), v_pages.data_ptr()
+    if kp == vp and ps[0] > 0:
+        raise ValueError(f"{what}: one pool for keys and values")
     for s, p in ((kst, kp), (vst, vp)):
         if s[3] != 1 or s[0] % unit or s[1] % unit or s[2] % unit or p % 16:
             raise ValueError(f"{what}: pool rows must be contiguous and 16-byte aligned; got strides {s}")

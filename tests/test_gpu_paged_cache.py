@@ -279,3 +279,9 @@ def test_operators_of_the_dispatcher():
     for x, y in zip(p, torch.ops.mlx_bi.paged_slots(i(0, 5), i(3, 1), t2, i(8, 9), None, 4, 3)):
         assert torch.equal(x, y)
     assert torch.equal(t1, t2)
+
+
+def test_rope_refuses_one_pool_for_both():
+    q, k, v, cos, sin, pos, slots, pools = _rope_case("bf16", "f32", 1, 2, (4, 2), 64, (32,), 8, 8)
+    with pytest.raises(ValueError, match="one pool"):
+        _bi().rope_paged_cache(q, k, v, cos, sin, pos, slots, pools[0], pools[0])

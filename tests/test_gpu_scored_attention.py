@@ -370,3 +370,57 @@ def test_bias_over_a_long_cache():
     for T in (3, 1):
         qq = q[:, :, :T].contiguous()
         _check(_call(qq, k, v, None, True, **m), qq, k, v, None, True, **m)
+
+
+def test_caches_past_32_bits():
+    """Pages and sequences that start behind 2^32 elements of their storage."""
+    Hkv, D, page, L = 2, 64, 16, 300
+    n = (1 << 21) + 64                                   # 2048 elements a page
+    q, k, v = _case("bf16", 2, 4, Hkv, 40, L, D, 44)
+    per = -(-L // page)
+    pools, flats = [], []
+    for x in (k, v):
+        pool = torch.empty((n, Hkv, page, D), dtype=x.dtype, device="cuda")
+        pad = torch.nn.functional.pad(x, (0, 0, 0, per * page - L))
+        # the last pages in reverse order, then (contiguous) rows 2^32 elements apart
+        at = torch.arange(n - 1, n - 1 - 2 * per, -1, device="cuda")
+        pool[at] = pad.reshape(2, Hkv, per, page, D).transpose(1, 2).reshape(-1, Hkv, page, D)
+        pools.append(pool)
+        flat = torch.as_strided(pool, (2, Hkv, L, D), (1 << 32, L * D, D, 1))
+        flats.append(flat)
+    table = torch.arange(n - 1, n - 1 - 2 * per, -1, dtype=I32, device="cuda").view(2, per)
+    lens = [L, 211]
+    m = dict(softcap=30.0, slopes=torch.tensor([0.01, 0.1, 0.0, 0.5]).cuda(),
+             doc_ids=(torch.arange(L) // 90).repeat(2, 1).cuda())
+    mp = dict(m, doc_ids=torch.nn.functional.pad(m["doc_ids"], (0, per * page - L)))
+    want = {}
+    for T in (40, 1):
+        qq = q[:, :, :T].contiguous()
+        want[T] = bits(_call(qq, k, v, lens, True, **m))
+        got = _bi().batch_invariant_paged_attention(qq, *pools, table, torch.tensor(lens, dtype=I32, device="cuda"),
+                                                    scale=D ** -0.5, mask="causal", **mp)
+        assert bits(got) == want[T]
+    for flat, x in zip(flats, (k, v)):
+        flat.copy_(x)
+    for T in (40, 1):
+        assert bits(_call(q[:, :, :T].contiguous(), *flats, lens, True, **m)) == want[T]
+    many = q.repeat(1, 4, 8, 1)[:, :, :300].contiguous()  # rows enough for the kernel that walks the splits
+    m["slopes"] = m["slopes"].repeat(4)
+    assert bits(_call(many, *flats, lens, True, **m)) == bits(_call(many, k, v, lens, True, **m))
+
+
+def test_calls_at_once_on_two_streams():
+    """Every call has a workspace of its own."""
+    q, k, v = _case("bf16", 2, 8, 2, 48, 1500, 64, 45)
+    forms = [(q[:, :, :T].contiguous(), dict(softcap=20.0 + T, slopes=torch.full((8,), 0.01 * T))) for T in (1, 5, 48)]
+    want = [bits(_call(x, k, v, None, True, **m)) for x, m in forms]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(10):
+        for s in streams:
+            with torch.cuda.stream(s):
+                got += [_call(x, k, v, None, True, **m) for x, m in forms]
+    torch.cuda.synchronize()
+    for i, g in enumerate(got):
+        assert bits(g) == want[i % 3]
