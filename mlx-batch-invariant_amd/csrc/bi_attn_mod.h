@@ -13,7 +13,8 @@
 //   documents  the split's document numbers come to LDS with its first K chunk;
 //              the splits in front of and behind all whose range of numbers meets
 //              the workgroup's are skipped, and one with a single number, the
-//              workgroup's own, runs unmasked. Any numbers are right; sorted ones
+//              workgroup's own, runs unmasked; the first one's chunks in front of the
+//              documents are skipped too. Any numbers are right; sorted ones
 //              (documents packed one after another) skip all they can.
 //   masked V   a hidden key's weight 0 times an infinity or NaN in its V row
 //              would be NaN. Such rows are as good as never there, so the kernel
@@ -195,18 +196,12 @@ __global__ __launch_bounds__(256, (mod_min_blocks<T, D, MODE>())) void attn_pref
 #pragma unroll
     for (int i = 0; i < kVPeriod; ++i) voff[i] = KV::template tile_off<true>(c0 + i, lane, a.v_sl);
   }
-  // Requests the chunk of keys key0 .. key0 + CH - 1 of K (or V) into buffer `slot`,
-  // and with a split's first K chunk its document numbers.
-  int docs_slot = 0;
+  // Requests the chunk of keys key0 .. key0 + CH - 1 of K (or V) into buffer `slot`.
   auto request = [&](auto is_v, int at, int slot) __attribute__((always_inline)) {
     constexpr bool V = decltype(is_v)::value;
     const int key0 = __builtin_amdgcn_readfirstlane(at);
     const int64_t sl = V ? a.v_sl : a.k_sl;
     char* buf = ring + slot * CHB;
-    if (!V && docs && key0 % kSplit == 0) {
-      copy_to_lds4(docs + min(key0 + tid, len - 1), split_docs + kSplit * docs_slot + 64 * wave);
-      docs_slot ^= 1;
-    }
     if constexpr (MODE == kKvContig || MODE == kKvPaged) {
       const int rows = min(CH, len - key0);             // >= 1: chunks start below maxkeys <= len
       const T* base = MODE == kKvContig
@@ -272,6 +267,22 @@ __global__ __launch_bounds__(256, (mod_min_blocks<T, D, MODE>())) void attn_pref
     sp0 = __builtin_amdgcn_readfirstlane(sp0);          // (known to be one for the wave: copies take it so)
     sp1 = __builtin_amdgcn_readfirstlane(sp1);
   }
+  auto chunks_of = [&](int sp) { return sp + 1 < nsplit ? KC : nkc_last; };
+  // The chunks of split sp0 in front of the documents' first key are left out too,
+  // as packed documents begin anywhere in a split: 8192 tokens, 32 / 8 heads of 128,
+  // bf16, documents of 100 keys on average 128 -> 112 us, of 700 252 -> 244. Its
+  // first buffer, 2 kc0 mod NBUF, lets the next split start in buffer 0.
+  int kc0 = 0;
+  if (docs && sp0 < sp1) {
+    int first = kSplit / 64 - 1;
+#pragma unroll
+    for (int j = kSplit / 64 - 1; j >= 0; --j) {
+      const int key = sp0 * kSplit + 64 * j + lane;
+      const int d = docs[min(key, len - 1)];
+      if (__ballot(key < len && d >= doc_lo && d <= doc_hi)) first = j;
+    }
+    kc0 = __builtin_amdgcn_readfirstlane(min(first / (CH / 64), chunks_of(sp0) - 1));
+  }
   // Whether the workgroup's only document is split sp's only one.
   auto own_doc = [&](int sp) __attribute__((always_inline)) {
     if (!docs) return true;
@@ -280,19 +291,29 @@ __global__ __launch_bounds__(256, (mod_min_blocks<T, D, MODE>())) void attn_pref
            load_uniform_i32(uniform_ptr(at + 1)) == doc_lo;
   };
   // The chunks in the order they are used, requested NBUF - 1 ahead: the next one
-  // to request is chunk r_i (of r_n K chunks, then r_n V chunks) of split r_sp,
-  // into buffer r_slot; `ahead` of them are requested and not yet opened.
-  int r_sp = 0, r_i = 0, r_n = 0, r_slot = 0, ahead = 0;
-  auto chunks_of = [&](int sp) { return sp + 1 < nsplit ? KC : nkc_last; };
+  // to request is chunk r_i of split r_sp's K (r_v: of its V), of which r_0 .. r_n -
+  // 1 are read, into buffer r_slot; `ahead` of them are requested and not yet
+  // opened. A split's document numbers come in front of its first K chunk.
+  int r_sp = 0, r_i = 0, r_n = 0, r_slot = 0, ahead = 0, docs_slot = 0;
+  bool r_v = false;
   auto request_next = [&]() __attribute__((always_inline)) {
     if (r_sp >= sp1) return;
-    if (r_i < r_n) request(std::false_type(), r_sp * kSplit + r_i * CH, r_slot);
-    else request(std::true_type(), r_sp * kSplit + (r_i - r_n) * CH, r_slot);
+    const int r_0 = r_sp == sp0 ? kc0 : 0, key0 = r_sp * kSplit + r_i * CH;
+    if (docs && !r_v && r_i == r_0) {
+      copy_to_lds4(docs + min(r_sp * kSplit + tid, len - 1), split_docs + kSplit * docs_slot + 64 * wave);
+      docs_slot ^= 1;
+    }
+    if (!r_v) request(std::false_type(), key0, r_slot);
+    else request(std::true_type(), key0, r_slot);
     r_slot = (r_slot + 1) % NBUF;
     ++ahead;
-    if (++r_i == 2 * r_n) {
-      r_i = 0;
-      r_n = chunks_of(++r_sp);
+    if (++r_i == r_n) {
+      r_i = r_0;
+      if (r_v) {
+        r_i = 0;
+        r_n = chunks_of(++r_sp);
+      }
+      r_v = !r_v;
     }
   };
   // Opens the chunk in buffer `slot`: waits until it is there (the copies requested
@@ -365,18 +386,19 @@ __global__ __launch_bounds__(256, (mod_min_blocks<T, D, MODE>())) void attn_pref
     constexpr bool MASKED = decltype(masked)::value > 0, DOCS = decltype(masked)::value > 1;
     const int j0 = sp * kSplit;
     const int nkc = MASKED ? chunks_of(sp) : KC;
+    const int kc_0 = DOCS && sp == sp0 ? kc0 : 0, slot_0 = DOCS && sp == sp0 ? (2 * kc0) % NBUF - kc0 : 0;
     float s[16][4];
     float m = -INFINITY;
 #pragma unroll
     for (int kc = 0; kc < KC; ++kc) {
-      if (kc >= nkc) {
+      if (kc < kc_0 || kc >= nkc) {
 #pragma unroll
         for (int t = 0; t < TPC; ++t)
 #pragma unroll
           for (int i = 0; i < 4; ++i) s[TPC * kc + t][i] = -INFINITY;
         continue;
       }
-      const char* buf = open_chunk(kc % NBUF, [](char*) {});
+      const char* buf = open_chunk((kc + slot_0) % NBUF, [](char*) {});
       const int lim = MASKED ? row_nkeys[16 * wave + r] - (j0 + CH * kc + 4 * qq) : 0;
       const uint32_t seen = DOCS ? doc_bits(kc) : ~0u;
       const float far = (MOD & kModBias) != 0 ? (float)(my_pos - (j0 + CH * kc + 4 * qq)) : 0.0f;
@@ -463,10 +485,18 @@ __global__ __launch_bounds__(256, (mod_min_blocks<T, D, MODE>())) void attn_pref
 #pragma unroll
     for (int j = 0; j < 4; ++j) weight_pair(pf, 0, j);
     constexpr int HS = CH / 32, NB = NDT / 2;           // 32-key steps per chunk, dim-tile pairs
+    if constexpr (DOCS && PIPE) {                       // (here, where the accumulators take no registers yet)
+#pragma unroll
+      for (int kc = 1; kc < KC; ++kc) {
+        if (kc != kc_0) continue;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) weight_pair(pf, HS * kc, j);
+      }
+    }
 #pragma unroll
     for (int kc = 0; kc < KC; ++kc) {
-      if (kc >= nkc) continue;
-      const char* buf = open_chunk((nkc + kc) % NBUF, [&](char* v) __attribute__((always_inline)) {
+      if ((DOCS && kc < kc_0) || kc >= nkc) continue;
+      const char* buf = open_chunk((nkc - kc_0 + kc + slot_0) % NBUF, [&](char* v) __attribute__((always_inline)) {
         if (MASKED && careful) clean_v(v, j0 + CH * kc);
       });
       if constexpr (PIPE) {
@@ -541,8 +571,11 @@ __global__ __launch_bounds__(256, (mod_min_blocks<T, D, MODE>())) void attn_pref
 #pragma unroll
     for (int dt = 0; dt < NDT; ++dt) A[dt] = f32x4{0.f, 0.f, 0.f, 0.f};
     r_sp = sp0;
+    r_i = kc0;
     r_n = chunks_of(r_sp);
-    r_i = r_slot = ahead = docs_slot = doc_buf = 0;
+    r_slot = (2 * kc0) % NBUF;
+    r_v = false;
+    ahead = docs_slot = doc_buf = 0;
 #pragma unroll
     for (int c = 0; c < NBUF - 1; ++c) request_next();
     for (int sp = sp0; sp < sp1; ++sp) {

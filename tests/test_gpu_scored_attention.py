@@ -424,3 +424,26 @@ def test_calls_at_once_on_two_streams():
     torch.cuda.synchronize()
     for i, g in enumerate(got):
         assert bits(g) == want[i % 3]
+
+
+@pytest.mark.parametrize("page", [0, 16, 4])
+@pytest.mark.parametrize("dt,D", [("bf16", 128), ("f16", 64), ("f32", 64), ("bf16", 256)])
+def test_documents_that_begin_anywhere_in_a_split(dt, D, page):
+    """Rows enough for the kernel that walks the splits; documents that begin in each
+    64 keys of a split, some shorter than 64, against the formula and one call each."""
+    L, at = 700, [0, 70, 130, 200, 256, 330, 450, 465, 480, 515, 640]
+    q, k, v = _case(dt, 2, 8, 1, L, L, D, 46)
+    doc = torch.zeros(2, L, dtype=I32)
+    for i, b in enumerate(at):
+        doc[0, b:] = i
+        doc[1, b:] = len(at) - i                         # descending numbers
+    lens = [L, 690]
+    got = _call(q, k, v, lens, True, page, doc_ids=doc)
+    _check(got, q, k, v, lens, True, doc_ids=doc)
+    ends = at[1:] + [L]
+    for b, e in zip(at, ends):
+        # (a call of the document alone counts its splits from its own start, so only
+        # those that begin a split have the same bits)
+        if b % 256 == 0:
+            alone = _call(q[:1, :, b:e].contiguous(), k[:1, :, b:e].contiguous(), v[:1, :, b:e].contiguous(), None, True)
+            assert bits(alone) == bits(got[:1, :, b:e])
