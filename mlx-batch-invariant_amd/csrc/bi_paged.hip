@@ -22,7 +22,8 @@ namespace bi {
 // Bound by latency: a decode step of 64 requests moves 3 KB. So one launch,
 // with no pass between workgroups: each workgroup adds up the needs of all
 // requests before its own (8 bytes a request from the cache; at 4,096 requests
-// the last of 16 workgroups reads 32 KB).
+// the last of 16 workgroups reads 32 KB). 64 requests of one token 3.4 us, 256 of
+// up to 2,048 (6.6 MB of slots and positions) 7.3.
 // ---------------------------------------------------------------------------
 struct SlotArgs {
   const int32_t *lens, *news, *free_pages, *cursor;
