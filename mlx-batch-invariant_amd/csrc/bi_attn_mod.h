@@ -267,9 +267,11 @@ __global__ __launch_bounds__(256, (mod_min_blocks<T, D, MODE>())) void attn_pref
     sp0 = nsplit;
     sp1 = 0;
     for (int g = 0; g < nsplit; g += 64) {
+      // (lanes past the last split have no vote: documents of both -2^31 and 2^31 - 1
+      // meet every range, an empty one too)
       int2 range = {0x7fffffff, -0x7fffffff - 1};
       if (g + lane < nsplit) range = a.mod.ranges[(int64_t)b * ((a.L + kSplit - 1) / kSplit) + g + lane];
-      const uint64_t hit = __ballot(range.y >= doc_lo && range.x <= doc_hi);
+      const uint64_t hit = __ballot(g + lane < nsplit && range.y >= doc_lo && range.x <= doc_hi);
       if (hit) {
         sp0 = min(sp0, g + __builtin_ctzll(hit));
         sp1 = g + 64 - __builtin_clzll(hit);
