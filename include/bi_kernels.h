@@ -326,12 +326,14 @@ int bi_attn_prefill_paged(const void* q, const void* k_pages, const void* v_page
  * with doc_ids: doc_ids[b][j] == doc_ids[b][p]. Queries with p < 0 see nothing
  * (causal, or with doc_ids); a query that sees no key, or none of a score above
  * -inf, gets zeros. What hidden keys' K and V rows hold (infinities, NaN) does
- * not matter. slopes fp32 [Hq], doc_ids int32 rows doc_stride >= L apart, prefix_lens
+ * not matter; an infinity or NaN that a query sees in V comes out in its dim as inf,
+ * -inf or (a NaN, or both) NaN, however small the key's weight. slopes fp32 [Hq], doc_ids int32 rows doc_stride >= L apart, prefix_lens
  * int32 [B]: device pointers. softcap 0 or 1e-30 .. 1e30; a prefix needs causal (decode sees
  * every key of its sequence); slopes need L <= 2^24. strides[0..8] as for
  * bi_attn_prefill (strides[2] unused at Tq == 1). Same order of operations as
  * bi_attn_decode / bi_attn_prefill, so the same invariances hold, and where no
- * score or mask is changed (slopes 0, one document, no prefix) the same bits.
+ * score or mask is changed (slopes 0, one document, no prefix) and V is finite the
+ * same bits (infinities in V: those give what the products do, mostly NaN).
  * Workspace: bi_attn_scored_workspace_bytes; calls that overlap must not share it.
  * Replaces: nothing in the reference (its masks are none and causal,
  * kernels/attention.py:299-310). */

@@ -23,8 +23,8 @@
 //              would be NaN. Such rows are as good as never there, so the kernel
 //              looks at its sums instead: if one is not finite, the workgroup
 //              runs again with every split masked, clears such elements in LDS
-//              and notes in `poison` for which rows and dims one was seen (1: inf,
-//              2: -inf, 4: NaN); those get it back at the end.
+//              and notes in `poison` which rows see one in which dim, and its
+//              kind (kSeenTag's low bits); those get it back at the end.
 #pragma once
 
 #include "bi_attn_mfma.h"
@@ -40,22 +40,6 @@ __device__ __forceinline__ int mod_nkeys(const Args& a, const int32_t* docs, int
   const int end = len - a.Tq + pair / G + 1;            // keys up to the row's own position
   if (end <= 0 && (a.causal || docs)) return 0;
   return a.causal ? max(end, prefix) : len;
-}
-
-// Infinities and NaN of a fragment as 0.
-template <typename F>
-__device__ __forceinline__ F finite_frag(F v) {
-  if constexpr (std::is_same_v<F, f32x8>) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      v.lo[e] = fabsf(v.lo[e]) < INFINITY ? v.lo[e] : 0.0f;
-      v.hi[e] = fabsf(v.hi[e]) < INFINITY ? v.hi[e] : 0.0f;
-    }
-  } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = fabsf((float)v[e]) < INFINITY ? v[e] : (decltype(v[e] + v[e]))0;
-  }
-  return v;
 }
 
 // Keys per ring chunk: 128 for contiguous caches of narrow rows, else 64.
@@ -374,7 +358,7 @@ __global__ __launch_bounds__(256, (mod_min_blocks<T, D, MODE>())) void attn_pref
         changed = true;
         e[j] = (T)0.0f;
         const int dim = (slot ^ KV::template key<true>(row)) * kPer + j;
-        const uint32_t bit = (x != x ? 4u : x > 0.0f ? 1u : 2u) << (8 * (dim % 4));
+        const uint32_t bit = v_kind(x) << (8 * (dim % 4));
         for (int p = 0; p < 64; ++p) {
           if (key >= nkeys_of(64 * wg + p)) continue;
           if (docs && docs[len - a.Tq + (64 * wg + p) / G] != docs[key]) continue;
@@ -627,8 +611,8 @@ __global__ __launch_bounds__(256, (mod_min_blocks<T, D, MODE>())) void attn_pref
 #pragma unroll
       for (int dt = 0; dt < NDT; ++dt) {
         const int at = row * D + 16 * dt + r;
-        const uint32_t bad = poison[at / 4] >> (8 * (at % 4)) & 7u;
-        if (bad) A[dt][i] = bad == 1 ? INFINITY : bad == 2 ? -INFINITY : NAN;
+        const uint32_t kinds = poison[at / 4] >> (8 * (at % 4)) & 7u;
+        if (kinds) A[dt][i] = seen_value(kinds, Lsum[i]);
       }
     }
     if (pair >= npairs) continue;
@@ -737,7 +721,7 @@ __global__ __launch_bounds__(256) void attn_rows_mod(ModRowsArgs a) {
           if (16 * chunk + i / D < npairs)
             static_cast<T*>(a.out)[partial(16 * chunk + i / D) * D + i % D] = (T)0.0f;
       } else if (tid < 16 && 16 * chunk + tid < npairs) {
-        a.pm[partial(16 * chunk + tid)] = -INFINITY;
+        a.pm[partial(16 * chunk + tid)] = NAN;           // (no acc is written: the merge reads none)
         a.pl[partial(16 * chunk + tid)] = 0.0f;
       }
       return;
@@ -890,7 +874,7 @@ __global__ __launch_bounds__(256) void attn_rows_mod(ModRowsArgs a) {
     };
     weigh(false, vp == 0 && (wave == 0 || direct));
     // A hidden key's weight 0 times an infinity or NaN of its V row is NaN: such a
-    // wave weighs again without them and adds the ones its rows see.
+    // wave weighs again without them and notes the ones its rows see (kSeenTag).
     bool finite = true;
 #pragma unroll
     for (int j = 0; j < NJ; ++j)
@@ -909,7 +893,8 @@ __global__ __launch_bounds__(256) void attn_rows_mod(ModRowsArgs a) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int p = 16 * chunk + 4 * qq + i;
-            if (j0 + key < nkeys_of(p) && (!docs || docs[j0 + key] == docs[len - a.Tq + p / G])) acc[j][i] += x;
+            if (j0 + key < nkeys_of(p) && (!docs || docs[j0 + key] == docs[len - a.Tq + p / G]))
+              acc[j][i] = note_seen(acc[j][i], x);
           }
         }
       }
@@ -922,8 +907,8 @@ __global__ __launch_bounds__(256) void attn_rows_mod(ModRowsArgs a) {
         const int p = 16 * chunk + 4 * qq + i;
         if (p >= npairs) continue;
         const int64_t at = partial(p) * D + vp * DV + 16 * (wave + 4 * j) + r;
-        if (direct)                                     // (the merge's fma(0, 0, acc): no -0)
-          static_cast<T*>(a.out)[at] = to_store<T>(lsum[i] != 0.0f ? (acc[j][i] + 0.0f) / lsum[i] : 0.0f);
+        if (direct)
+          static_cast<T*>(a.out)[at] = to_store<T>(only_split(acc[j][i], lsum[i]));
         else
           a.pacc[at] = acc[j][i];
       }
@@ -940,7 +925,7 @@ __global__ __launch_bounds__(256) void attn_rows_mod(ModRowsArgs a) {
 
 // Merges the splits of every row that attn_rows_mod left, left to right, and
 // divides: one thread per four dims of a row. A split in which the row sees
-// nothing (l = 0 at m = -inf) is passed over.
+// nothing (l = 0 at m = -inf) is passed over; one at m = NaN has no acc.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void attn_rows_combine(ModRowsArgs a) {
   const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -952,6 +937,7 @@ __global__ __launch_bounds__(256) void attn_rows_combine(ModRowsArgs a) {
   const int prefix = a.mod.prefix ? min(max(a.mod.prefix[b], 0), len) : 0;
   const int ns = (mod_nkeys(a, a.mod.docs, len, prefix, 1, a.Tq, t) + kSplit - 1) / kSplit;
   float M = -INFINITY, Ls = 0.0f, A[4] = {0.f, 0.f, 0.f, 0.f};
+  uint32_t kinds[4] = {0, 0, 0, 0};
   const int64_t p0 = row * a.nsplit;
   for (int i0 = 0; i0 < ns; i0 += 4) {                  // four splits' partials requested together
     float pm[4], pl[4];
@@ -969,11 +955,14 @@ __global__ __launch_bounds__(256) void attn_rows_combine(ModRowsArgs a) {
         const float acc[4] = {pa[j][0], pa[j][1], pa[j][2], pa[j][3]};
         merge_split<4>(M, Ls, A, pm[j], pl[j], acc);
       }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) kinds[e] |= pm[j] == pm[j] ? seen_kinds(pa[j][e]) : 0u;  // (the last split again: no matter)
     }
   }
   T* o = static_cast<T*>(a.out) + row * D + d;
 #pragma unroll
-  for (int e = 0; e < 4; ++e) o[e] = to_store<T>(Ls != 0.0f ? A[e] / Ls : 0.0f);
+  for (int e = 0; e < 4; ++e)
+    o[e] = to_store<T>(kinds[e] ? seen_value(kinds[e], Ls) : Ls != 0.0f ? A[e] / Ls : 0.0f);
 }
 
 }  // namespace bi

@@ -10,8 +10,9 @@
 namespace bi {
 
 // attn_combine_kernel, but a split without a visible key (l = 0 at m = -inf) is
-// not merged: its m would make the factors NaN. (A split whose scores are all
-// NaN has l = NaN and is merged.)
+// not merged: its m would make the factors NaN; one at m = NaN has no acc. (A split
+// whose scores are all NaN has l = NaN and is merged.) Infinities and NaN that the
+// row saw in V: kSeenTag.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void attn_combine_mod_kernel(DecodeArgs a) {
   const int64_t gid0 = (int64_t)blockIdx.x * 256 + threadIdx.x;
@@ -22,6 +23,7 @@ __global__ __launch_bounds__(256) void attn_combine_mod_kernel(DecodeArgs a) {
   const int len = a.kv_lens ? min(max(a.kv_lens[b], 0), a.L) : a.L;
   const int ns = (len + kSplit - 1) / kSplit;
   float M = -INFINITY, Ls = 0.0f, A = 0.0f;
+  uint32_t kinds = 0;
   auto merge = [&](float m, float l, float acc) {
     // (merge_split's operations, without a branch: a split passed over multiplies
     // by 1 and adds -0; its acc may be unwritten)
@@ -45,12 +47,19 @@ __global__ __launch_bounds__(256) void attn_combine_mod_kernel(DecodeArgs a) {
     }
 #pragma unroll
     for (int j = 0; j < 8; ++j) merge(pm[j], pl[j], pa[j]);
+    const float any = ((pa[0] + pa[1]) + (pa[2] + pa[3])) + ((pa[4] + pa[5]) + (pa[6] + pa[7]));
+    if (any != any) {                                   // (a NaN among them)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) kinds |= pm[j] == pm[j] ? seen_kinds(pa[j]) : 0u;
+    }
   }
   for (; i < ns; ++i) {
     const int64_t po = bh * a.nsplit + i;
-    merge(a.pm[po], a.pl[po], a.pacc[po * D + d]);
+    const float m = a.pm[po], acc = a.pacc[po * D + d];
+    merge(m, a.pl[po], acc);
+    kinds |= m == m ? seen_kinds(acc) : 0u;
   }
-  if (live) static_cast<T*>(a.out)[bh * D + d] = to_store<T>(Ls != 0.0f ? A / Ls : 0.0f);
+  if (live) static_cast<T*>(a.out)[bh * D + d] = to_store<T>(kinds ? seen_value(kinds, Ls) : Ls != 0.0f ? A / Ls : 0.0f);
 }
 
 // One instantiation for both item orders, chosen as for the plain kernel: with at

@@ -52,9 +52,10 @@ the scores and the mask in the matrix-core order: with query t at position
   2^32).
 
 Hidden keys take no part whatever their rows hold; a query that sees none (one
-in front of a padded prompt, p < 0) gets zeros. The invariances above hold, and
-where nothing is changed (slopes of 0, one document, no prefix) the bits of the
-plain call.
+in front of a padded prompt, p < 0) gets zeros. An infinity or NaN that a query
+sees in V comes out in its dim, as inf, -inf or (a NaN, or both) NaN, however small
+the key's weight. The invariances above hold, and where nothing is changed (slopes
+of 0, one document, no prefix) and V is finite the bits of the plain call.
 """
 
 from __future__ import annotations
