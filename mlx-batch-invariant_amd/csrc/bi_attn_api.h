@@ -35,7 +35,7 @@ template <typename T, int D>
 int launch_decode(DecodeArgs& a, hipStream_t st);
 template <typename T, int D>
 int launch_prefill(PrefillArgs& a, hipStream_t st);
-// The same with ScoreMod (bi_attn_mod_{bf16,f16,f32}.hip).
+// The same with ScoreMod (bi_attn_mod_{decode,mask,cap,bias,capbias,rows}_{bf16,f16,f32}.hip).
 template <typename T, int D>
 int launch_decode_mod(ModDecodeArgs& a, hipStream_t st);
 template <typename T, int D, int MOD>
@@ -60,7 +60,10 @@ inline int64_t rows_partial_bytes(int64_t B, int64_t Hq, int64_t Tq, int64_t L, 
 // no pipeline, 8 / 8 heads of 128: R = 426, N = 3: 102 / 79; R = 569, N = 18: 615 /
 // 454; 32 / 8: R = 623, N = 4: 124 / 131; heads of 32 to 192 turn alike (192: R = 460,
 // N = 3: 114 / 108; R = 623: 184 / 189), of 256, where the walk spills, later: R = 885,
-// N = 5: 841 / 529. The partials stay below 256 MB.
+// N = 5: 841 / 529. The partials stay below 256 MB. N is what the cache can hold (the
+// host does not know the lengths): a workgroup without keys costs 1.1 ns, so 300 keys
+// in a table of 32768 take 39 us where walking takes 21 (R = 128), and 32768 keys 380
+// where walking takes some 1000.
 inline bool few_rows(int64_t B, int64_t Hq, int64_t Hkv, int64_t Tq, int64_t L, int64_t D, int causal, int dtype) {
   if ((double)Tq * Hq * B > 1e9) return false;           // (so that the products below stay in 64 bits)
   const int64_t n = (L + kSplit - 1) / kSplit;

@@ -664,15 +664,20 @@ __global__ __launch_bounds__(256) void attn_rows_mod(ModRowsArgs a) {
   const int G = a.Hq / a.Hkv, npairs = a.Tq * G;
   // Items (b, hk, split, row chunk) in that nesting order, a contiguous range of
   // them per XCD: the row chunks that read one split's K and V share an L2.
-  const int nchunks = (npairs + 15) / 16;
-  const int64_t items = (int64_t)nchunks * a.nsplit * a.Hkv * a.B;
-  const int64_t per_xcd = (items + 7) / 8;
-  const int64_t item = (int64_t)(blockIdx.x % 8) * per_xcd + blockIdx.x / 8;
+  // (In 32 bits, as the host keeps the items below 2^31: a table wider than its
+  // sequences has many workgroups that only find out that they have no keys. 4 x 16
+  // tokens, 32 / 8 heads of 128, bf16, 300 keys in tables of 512 / 32768: 20.8 / 43.5 us
+  // with 64-bit divisions, 20.8 / 38.8 so.)
+  const unsigned nchunks = (unsigned)(npairs + 15) / 16, nsplits = (unsigned)a.nsplit, nhk = (unsigned)a.Hkv;
+  const unsigned items = nchunks * nsplits * nhk * (unsigned)a.B;
+  const unsigned per_xcd = (items + 7) / 8;
+  const unsigned item = blockIdx.x % 8 * per_xcd + blockIdx.x / 8;
   if (blockIdx.x / 8 >= per_xcd || item >= items) return;
-  const int chunk = __builtin_amdgcn_readfirstlane((int)(item % nchunks));
-  const int split = __builtin_amdgcn_readfirstlane((int)(item / nchunks % a.nsplit));
-  const int hk = __builtin_amdgcn_readfirstlane((int)(item / nchunks / a.nsplit % a.Hkv));
-  const int b = __builtin_amdgcn_readfirstlane((int)(item / nchunks / a.nsplit / a.Hkv));
+  const unsigned at = item / nchunks, pair_bh = at / nsplits;
+  const int chunk = __builtin_amdgcn_readfirstlane((int)(item - at * nchunks));
+  const int split = __builtin_amdgcn_readfirstlane((int)(at - pair_bh * nsplits));
+  const int hk = __builtin_amdgcn_readfirstlane((int)(pair_bh % nhk));
+  const int b = __builtin_amdgcn_readfirstlane((int)(pair_bh / nhk));
   const int len = __builtin_amdgcn_readfirstlane(a.kv_lens ? min(max(a.kv_lens[b], 0), a.L) : a.L);
   const int prefix = a.mod.prefix ? min(max(a.mod.prefix[b], 0), len) : 0;
   const int32_t* docs = a.mod.docs ? a.mod.docs + (int64_t)b * a.mod.docs_sb : nullptr;
@@ -955,8 +960,14 @@ __global__ __launch_bounds__(256) void attn_rows_combine(ModRowsArgs a) {
         const float acc[4] = {pa[j][0], pa[j][1], pa[j][2], pa[j][3]};
         merge_split<4>(M, Ls, A, pm[j], pl[j], acc);
       }
+    }
+    const f32x4 any = (pa[0] + pa[1]) + (pa[2] + pa[3]);  // (the last split several times: no matter)
+    const float odd = (any[0] + any[1]) + (any[2] + any[3]);
+    if (odd != odd) {                                   // a NaN among them
 #pragma unroll
-      for (int e = 0; e < 4; ++e) kinds[e] |= pm[j] == pm[j] ? seen_kinds(pa[j][e]) : 0u;  // (the last split again: no matter)
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) kinds[e] |= pm[j] == pm[j] ? seen_kinds(pa[j][e]) : 0u;
     }
   }
   T* o = static_cast<T*>(a.out) + row * D + d;

@@ -138,3 +138,25 @@ def test_infinities_in_v_beside_scores_that_are_not_finite(dt):
             one = _call(q[:, :, n - 1:n], k, v, [n] * B, True, **m)
             a = got[:, :, n - 1:n]
             assert ((one == a) | (one.isnan() & a.isnan())).all(), n
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("T", [16, 1])
+def test_short_sequences_in_a_wide_table(dt, T):
+    """Tables that hold far more than the sequences, and whose entries behind them
+    point anywhere: the bits of a narrow table."""
+    import mlx_batch_invariant_amd as bi
+    B, Hq, Hkv, D, page, used, wide = 4, 8, 2, 64, 16, 40, 4096
+    q, k, v = _case(dt, B * used, Hq, Hkv, page, page, D, 54)
+    q = q[:B, :, :T].contiguous()
+    table = torch.full((B, wide), -7, dtype=I32)
+    table[:, 100:] = 10**9
+    table[:, :used] = torch.randperm(B * used, generator=torch.Generator().manual_seed(1)).view(B, used)
+    lens = torch.tensor([300, 640, 17, 0], dtype=I32, device="cuda")
+    m = dict(softcap=20.0, slopes=torch.full((Hq,), 0.01, device="cuda"))
+    table = table.cuda()
+    docs = (torch.arange(wide * page, device="cuda") // 200).to(I32).repeat(B, 1)
+    for mods in (m, dict(m, doc_ids=docs), dict(prefix_lens=torch.tensor([100, 640, 5, 9], dtype=I32))):
+        f = lambda n: bi.batch_invariant_paged_attention(q, k, v, table[:, :n], lens, mask="causal", **mods)
+        assert torch.equal(f(wide), f(used))
+        assert not f(wide)[3].any()
