@@ -24,8 +24,9 @@ Operators (each the same computation, and bits, as the Python function named):
   prefix_lens)`` and ``scored_paged_attention(q, k_pages, v_pages, block_table,
   kv_lens, scale, causal, softcap, ...)``: the two with capped scores, a distance
   bias, a document mask or a prefix mask;
-* ``residual_rms_norm(x, residual, post_weight, pre_weight, eps, gate, scale)``:
-  both norms (``batch_invariant_residual_rms_norm``); returns (y, h);
+* ``residual_rms_norm(x, residual, post_weight, pre_weight, eps, gate, scale,
+  post_norm=True, pre_norm=True)``: ``batch_invariant_residual_rms_norm``; returns
+  (y, h), h empty without ``pre_norm``;
 * ``paged_slots(kv_lens, new_lens, block_table!, free_pages, cursor, page_size,
   max_new)``: (slots, positions, kv_lens, cursor), the table changed in place;
 * ``rope_paged_cache(q, k, v, cos, sin, positions, slots, k_pages!, v_pages!,
@@ -114,13 +115,16 @@ def _paged_attention_fake(q, k_pages, v_pages, block_table, kv_lens, scale, caus
 
 @torch.library.custom_op(f"{NAMESPACE}::residual_rms_norm", mutates_args=())
 def residual_rms_norm(x: Tensor, residual: Tensor, post_weight: Optional[Tensor], pre_weight: Optional[Tensor],
-                      eps: float, gate: Optional[Tensor], scale: float) -> tuple[Tensor, Tensor]:
-    return _k.batch_invariant_residual_rms_norm(x, residual, post_weight, pre_weight, eps, gate=gate, scale=scale)
+                      eps: float, gate: Optional[Tensor], scale: float, post_norm: bool = True,
+                      pre_norm: bool = True) -> tuple[Tensor, Tensor]:
+    y, h = _k.batch_invariant_residual_rms_norm(x, residual, post_weight, pre_weight, eps, gate=gate, scale=scale,
+                                                post_norm=post_norm, pre_norm=pre_norm)
+    return y, x.new_empty(0) if h is None else h
 
 
 @residual_rms_norm.register_fake
-def _residual_rms_norm_fake(x, residual, post_weight, pre_weight, eps, gate, scale):
-    return x.new_empty(x.shape), x.new_empty(x.shape)
+def _residual_rms_norm_fake(x, residual, post_weight, pre_weight, eps, gate, scale, post_norm=True, pre_norm=True):
+    return x.new_empty(x.shape), x.new_empty(x.shape if pre_norm else 0)
 
 
 @torch.library.custom_op(f"{NAMESPACE}::paged_slots", mutates_args=("block_table",))
