@@ -10,6 +10,8 @@
 // The sums follow rms_norm's order (bi_rmsnorm.hip): thread t of 256 owns the
 // 8-element chunks t, t + 256, ..., a wave folds by the xor butterfly, the wave
 // sums are added left to right: D alone fixes it.
+#include <algorithm>
+
 #include "bi_common.h"
 
 namespace bi {
@@ -20,7 +22,7 @@ struct ResNormArgs {
   const void *x, *res, *gate, *w_post, *w_pre;
   void *y, *h;
   int64_t x_row, res_row, gate_row, gate_group;   // gate row r / gate_group
-  int64_t rows;
+  int64_t first, rows;                            // rows first .. rows - 1 (of this launch)
   int D;
   float eps, scale;
 };
@@ -100,7 +102,7 @@ __global__ __launch_bounds__(kResThreads) void res_norm_kernel(ResNormArgs a) {
   __shared__ float wave_sums[kResThreads / kWave];
   constexpr int kRowThreads = WPR * kWave;
   const int t = threadIdx.x % kRowThreads;
-  const int64_t row0 = (int64_t)blockIdx.x * (kResThreads / kRowThreads) + threadIdx.x / kRowThreads;
+  const int64_t row0 = a.first + (int64_t)blockIdx.x * (kResThreads / kRowThreads) + threadIdx.x / kRowThreads;
   const bool live = row0 < a.rows;
   const int64_t row = live ? row0 : a.rows - 1;        // (a workgroup's spare rows repeat the last and store nothing)
   const T* x = static_cast<const T*>(a.x) + row * a.x_row;
@@ -176,7 +178,7 @@ __global__ __launch_bounds__(kResThreads) void res_norm_kernel(ResNormArgs a) {
 template <typename T, bool POST, bool PRE>
 __global__ __launch_bounds__(kResThreads) void res_norm_kernel_long(ResNormArgs a) {
   __shared__ float wave_sums[kResThreads / kWave];
-  const int64_t row = blockIdx.x;
+  const int64_t row = a.first + blockIdx.x;
   const T* x = static_cast<const T*>(a.x) + row * a.x_row;
   const T* res = static_cast<const T*>(a.res) + row * a.res_row;
   const T* gate = a.gate ? static_cast<const T*>(a.gate) + row / a.gate_group * a.gate_row : nullptr;
@@ -235,7 +237,8 @@ __global__ __launch_bounds__(kResThreads) void res_norm_kernel_long(ResNormArgs 
 }
 
 template <typename T, bool POST, bool PRE>
-static void launch_res_norm(const ResNormArgs& a, int64_t rows, bool vec, hipStream_t st) {
+static void launch_res_norm(const ResNormArgs& a, bool vec, hipStream_t st) {
+  const int64_t rows = a.rows - a.first;
   const int nchunks = (a.D + 7) / 8;
 #define BI_RES(NC, WPR)                                                                                 \
   do {                                                                                                  \
@@ -257,10 +260,16 @@ static void launch_res_norm(const ResNormArgs& a, int64_t rows, bool vec, hipStr
 }
 
 template <typename T>
-static void launch_res_norm_t(const ResNormArgs& a, int64_t rows, bool post, bool pre, bool vec, hipStream_t st) {
-  if (post && pre) launch_res_norm<T, true, true>(a, rows, vec, st);
-  else if (post) launch_res_norm<T, true, false>(a, rows, vec, st);
-  else launch_res_norm<T, false, true>(a, rows, vec, st);
+static void launch_res_norm_t(ResNormArgs a, bool post, bool pre, bool vec, hipStream_t st) {
+  // A launch holds fewer than 2^32 threads: more rows take several.
+  constexpr int64_t kMost = (int64_t)1 << 23;
+  const int64_t rows = a.rows;
+  for (; a.first < rows; a.first += kMost) {
+    a.rows = std::min(rows, a.first + kMost);
+    if (post && pre) launch_res_norm<T, true, true>(a, vec, st);
+    else if (post) launch_res_norm<T, true, false>(a, vec, st);
+    else launch_res_norm<T, false, true>(a, vec, st);
+  }
 }
 
 }  // namespace bi
@@ -274,7 +283,7 @@ extern "C" int bi_residual_rms_norm(const void* x, int64_t x_row_stride, const v
   if (rows < 0 || D <= 0 || D > (int64_t)1 << 30)
     return fail(BI_E_INVALID_ARG, "%s: bad shape rows=%lld D=%lld", what, (long long)rows, (long long)D);
   if (rows > 0x7fffffffLL)
-    return fail(BI_E_UNSUPPORTED, "%s: rows=%lld exceeds the grid limit", what, (long long)rows);
+    return fail(BI_E_UNSUPPORTED, "%s: rows=%lld (fewer than 2^31)", what, (long long)rows);
   if (dtype != BI_BF16 && dtype != BI_F16 && dtype != BI_F32)
     return fail(BI_E_UNSUPPORTED, "%s: unknown dtype %d", what, dtype);
   if (!post && !pre) return fail(BI_E_INVALID_ARG, "%s: neither norm asked for", what);
@@ -285,12 +294,12 @@ extern "C" int bi_residual_rms_norm(const void* x, int64_t x_row_stride, const v
                 what, (long long)x_row_stride, (long long)res_row_stride, (long long)D, (long long)gate_row_stride,
                 (long long)gate_group);
   bi::ResNormArgs a{x, res, gate, post ? w_post : nullptr, pre ? w_pre : nullptr, y, h, x_row_stride, res_row_stride,
-                    gate ? gate_row_stride : 0, gate ? gate_group : 1, rows, (int)D, eps, scale};
+                    gate ? gate_row_stride : 0, gate ? gate_group : 1, 0, rows, (int)D, eps, scale};
   bool vec = D % 8 == 0 && a.x_row % 8 == 0 && a.res_row % 8 == 0 && a.gate_row % 8 == 0;
   for (const void* p : {x, res, gate, a.w_post, a.w_pre, (const void*)y, (const void*)h}) vec = vec && aligned16(p);
   hipStream_t st = static_cast<hipStream_t>(stream);
-  if (dtype == BI_BF16) bi::launch_res_norm_t<bi::bf16>(a, rows, post, pre, vec, st);
-  else if (dtype == BI_F16) bi::launch_res_norm_t<bi::f16>(a, rows, post, pre, vec, st);
-  else bi::launch_res_norm_t<float>(a, rows, post, pre, vec, st);
+  if (dtype == BI_BF16) bi::launch_res_norm_t<bi::bf16>(a, post, pre, vec, st);
+  else if (dtype == BI_F16) bi::launch_res_norm_t<bi::f16>(a, post, pre, vec, st);
+  else bi::launch_res_norm_t<float>(a, post, pre, vec, st);
   return launch_status(what);
 }
