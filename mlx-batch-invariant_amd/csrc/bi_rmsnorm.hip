@@ -16,6 +16,8 @@
 //
 // Nothing in that sequence depends on how many rows the launch holds, so a
 // row's bits are the same alone or in a batch of thousands.
+#include <algorithm>
+
 #include "bi_common.h"
 
 namespace bi {
@@ -161,20 +163,24 @@ static int launch_rms(const void* x, int64_t xs, const void* w, void* out, int64
   T* op = static_cast<T*>(out);
   const bool vec = (D % kNormVec == 0) && (xs % kNormVec == 0) && bi_host::aligned16(x) &&
                    bi_host::aligned16(out) && (w == nullptr || bi_host::aligned16(w));
-  dim3 grid((unsigned)rows), block(kNormThreads);
   const int Di = (int)D;
   const int nchunks = (int)((D + kNormVec - 1) / kNormVec);
-  if (nchunks <= kNormThreads) {
-    if (vec) rms_norm_kernel<T, 1, true><<<grid, block, 0, st>>>(xp, xs, wp, op, Di, eps);
-    else rms_norm_kernel<T, 1, false><<<grid, block, 0, st>>>(xp, xs, wp, op, Di, eps);
-  } else if (nchunks <= 2 * kNormThreads) {
-    if (vec) rms_norm_kernel<T, 2, true><<<grid, block, 0, st>>>(xp, xs, wp, op, Di, eps);
-    else rms_norm_kernel<T, 2, false><<<grid, block, 0, st>>>(xp, xs, wp, op, Di, eps);
-  } else if (nchunks <= 4 * kNormThreads) {
-    if (vec) rms_norm_kernel<T, 4, true><<<grid, block, 0, st>>>(xp, xs, wp, op, Di, eps);
-    else rms_norm_kernel<T, 4, false><<<grid, block, 0, st>>>(xp, xs, wp, op, Di, eps);
-  } else {
-    rms_norm_kernel_long<T><<<grid, block, 0, st>>>(xp, xs, wp, op, Di, eps);
+  // A launch holds fewer than 2^32 threads: more rows take several.
+  constexpr int64_t kMost = (int64_t)1 << 23;
+  for (int64_t r = 0; r < rows; r += kMost, xp += kMost * xs, op += kMost * D) {
+    const dim3 grid((unsigned)std::min(kMost, rows - r)), block(kNormThreads);
+    if (nchunks <= kNormThreads) {
+      if (vec) rms_norm_kernel<T, 1, true><<<grid, block, 0, st>>>(xp, xs, wp, op, Di, eps);
+      else rms_norm_kernel<T, 1, false><<<grid, block, 0, st>>>(xp, xs, wp, op, Di, eps);
+    } else if (nchunks <= 2 * kNormThreads) {
+      if (vec) rms_norm_kernel<T, 2, true><<<grid, block, 0, st>>>(xp, xs, wp, op, Di, eps);
+      else rms_norm_kernel<T, 2, false><<<grid, block, 0, st>>>(xp, xs, wp, op, Di, eps);
+    } else if (nchunks <= 4 * kNormThreads) {
+      if (vec) rms_norm_kernel<T, 4, true><<<grid, block, 0, st>>>(xp, xs, wp, op, Di, eps);
+      else rms_norm_kernel<T, 4, false><<<grid, block, 0, st>>>(xp, xs, wp, op, Di, eps);
+    } else {
+      rms_norm_kernel_long<T><<<grid, block, 0, st>>>(xp, xs, wp, op, Di, eps);
+    }
   }
   return bi_host::launch_status("bi_rms_norm");
 }
@@ -188,7 +194,7 @@ extern "C" int bi_rms_norm(const void* x, int64_t x_row_stride, const void* w, v
     return fail(BI_E_INVALID_ARG, "bi_rms_norm: bad shape rows=%lld D=%lld", (long long)rows,
                 (long long)D);
   if (rows > 0x7fffffffLL)
-    return fail(BI_E_UNSUPPORTED, "bi_rms_norm: rows=%lld exceeds the grid limit",
+    return fail(BI_E_UNSUPPORTED, "bi_rms_norm: rows=%lld (fewer than 2^31)",
                 (long long)rows);
   if (rows == 0) return BI_OK;
   if (!x || !out) return fail(BI_E_INVALID_ARG, "bi_rms_norm: null x or out");

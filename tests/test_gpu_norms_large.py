@@ -37,3 +37,12 @@ def test_residual_norm():
     y, h = bi.batch_invariant_residual_rms_norm(x, x, w, w, 1e-5, gate=w)
     _same_as_alone(y, lambda a: f(a)[:, :D], n, x)
     _same_as_alone(h, lambda a: f(a)[:, D:], n, x)
+
+
+def test_rms_norm():
+    import mlx_batch_invariant_amd as bi
+    D, n = 8, 2**24 + 300
+    x = _rows(n, D, 2)
+    w = torch.linspace(0.5, 2.0, D, device="cuda").to(torch.bfloat16)
+    f = lambda a: bi.batch_invariant_rms_norm(a, w, 1e-5)
+    _same_as_alone(f(x), f, n, x)
