@@ -20,6 +20,8 @@
 //     are skipped when the tensor is absent; one round-to-nearest-even store.
 //
 // Nothing in that sequence depends on how many rows the launch holds.
+#include <algorithm>
+
 #include "bi_common.h"
 
 namespace bi {
@@ -196,20 +198,24 @@ static int launch_ln(const void* x, int64_t xs, const void* w, const void* b, vo
   T* op = static_cast<T*>(out);
   const bool vec = (D % kLnVec == 0) && (xs % kLnVec == 0) && bi_host::aligned16(x) && bi_host::aligned16(out) &&
                    (w == nullptr || bi_host::aligned16(w)) && (b == nullptr || bi_host::aligned16(b));
-  const dim3 grid((unsigned)rows), block(kLnThreads);
   const int Di = (int)D;
   const int nchunks = (int)((D + kLnVec - 1) / kLnVec);
-  if (nchunks <= kLnThreads) {
-    if (vec) layer_norm_kernel<T, 1, true><<<grid, block, 0, st>>>(xp, xs, wp, bp, op, Di, eps);
-    else layer_norm_kernel<T, 1, false><<<grid, block, 0, st>>>(xp, xs, wp, bp, op, Di, eps);
-  } else if (nchunks <= 2 * kLnThreads) {
-    if (vec) layer_norm_kernel<T, 2, true><<<grid, block, 0, st>>>(xp, xs, wp, bp, op, Di, eps);
-    else layer_norm_kernel<T, 2, false><<<grid, block, 0, st>>>(xp, xs, wp, bp, op, Di, eps);
-  } else if (nchunks <= 4 * kLnThreads) {
-    if (vec) layer_norm_kernel<T, 4, true><<<grid, block, 0, st>>>(xp, xs, wp, bp, op, Di, eps);
-    else layer_norm_kernel<T, 4, false><<<grid, block, 0, st>>>(xp, xs, wp, bp, op, Di, eps);
-  } else {
-    layer_norm_kernel_long<T><<<grid, block, 0, st>>>(xp, xs, wp, bp, op, Di, eps);
+  // A launch holds fewer than 2^32 threads: more rows take several.
+  constexpr int64_t kMost = (int64_t)1 << 23;
+  for (int64_t r = 0; r < rows; r += kMost, xp += kMost * xs, op += kMost * D) {
+    const dim3 grid((unsigned)std::min(kMost, rows - r)), block(kLnThreads);
+    if (nchunks <= kLnThreads) {
+      if (vec) layer_norm_kernel<T, 1, true><<<grid, block, 0, st>>>(xp, xs, wp, bp, op, Di, eps);
+      else layer_norm_kernel<T, 1, false><<<grid, block, 0, st>>>(xp, xs, wp, bp, op, Di, eps);
+    } else if (nchunks <= 2 * kLnThreads) {
+      if (vec) layer_norm_kernel<T, 2, true><<<grid, block, 0, st>>>(xp, xs, wp, bp, op, Di, eps);
+      else layer_norm_kernel<T, 2, false><<<grid, block, 0, st>>>(xp, xs, wp, bp, op, Di, eps);
+    } else if (nchunks <= 4 * kLnThreads) {
+      if (vec) layer_norm_kernel<T, 4, true><<<grid, block, 0, st>>>(xp, xs, wp, bp, op, Di, eps);
+      else layer_norm_kernel<T, 4, false><<<grid, block, 0, st>>>(xp, xs, wp, bp, op, Di, eps);
+    } else {
+      layer_norm_kernel_long<T><<<grid, block, 0, st>>>(xp, xs, wp, bp, op, Di, eps);
+    }
   }
   return bi_host::launch_status("bi_layer_norm");
 }
@@ -222,7 +228,7 @@ extern "C" int bi_layer_norm(const void* x, int64_t x_row_stride, const void* w,
   if (rows < 0 || D <= 0 || D > (int64_t)1 << 30)
     return fail(BI_E_INVALID_ARG, "bi_layer_norm: bad shape rows=%lld D=%lld", (long long)rows, (long long)D);
   if (rows > 0x7fffffffLL)
-    return fail(BI_E_UNSUPPORTED, "bi_layer_norm: rows=%lld exceeds the grid limit", (long long)rows);
+    return fail(BI_E_UNSUPPORTED, "bi_layer_norm: rows=%lld (fewer than 2^31)", (long long)rows);
   if (rows == 0) return BI_OK;
   if (!x || !out) return fail(BI_E_INVALID_ARG, "bi_layer_norm: null x or out");
   if (x_row_stride < D)

@@ -46,3 +46,12 @@ def test_rms_norm():
     w = torch.linspace(0.5, 2.0, D, device="cuda").to(torch.bfloat16)
     f = lambda a: bi.batch_invariant_rms_norm(a, w, 1e-5)
     _same_as_alone(f(x), f, n, x)
+
+
+def test_layer_norm():
+    import mlx_batch_invariant_amd as bi
+    D, n = 8, 2**24 + 300
+    x = _rows(n, D, 3)
+    w = torch.linspace(0.5, 2.0, D, device="cuda").to(torch.bfloat16)
+    f = lambda a: bi.batch_invariant_layer_norm(a, w, w, 1e-5)
+    _same_as_alone(f(x), f, n, x)
