@@ -181,8 +181,10 @@ int decode_impl(const char* what, const void* q, const void* k, const void* v, c
   a.pl = a.pm + up;
   a.pacc = a.pl + up;
   a.ctr = reinterpret_cast<unsigned*>(a.pacc + bh * D);
-  if ((int64_t)a.Hkv * a.nchunk > 65535 || a.nsplit > 0x7fffffff ||
-      (per_key && bh / a.GU > ((int64_t)1 << 27)))  // per-key: 32 threads per unit, < 2^32 threads
+  // (a launch holds fewer than 2^32 threads: the merge has one per output element,
+  // the per-key kernel 32 per unit)
+  if ((int64_t)a.Hkv * a.nchunk > 65535 || a.nsplit > 0x7fffffff || (per_key && bh / a.GU >= ((int64_t)1 << 27)) ||
+      (!(mod && a.nsplit == 1) && B * Hq * D > ((int64_t)1 << 32) - 256))
     return fail(BI_E_UNSUPPORTED, "%s: grid too large", what);
   hipStream_t st = static_cast<hipStream_t>(stream);
   if (mod) {
@@ -254,10 +256,11 @@ int prefill_impl(const char* what, const void* q, const void* k, const void* v, 
                 (long long)strides[5], (long long)strides[8]);
   const int64_t wgs = (Tq * (Hq / Hkv) + 63) / 64;
   // The matrix-core kernel runs one 1-D grid over every (b, kv head, 64-pair
-  // workgroup) item, padded to a multiple of 8.
+  // workgroup) item, padded to a multiple of 8, of 256 threads each and fewer than
+  // 2^32 in all; the per-key kernel 32 threads per unit.
   if (wgs > 0x7fffffffLL || Tq * (Hq / Hkv) > 0x7fffffffLL - 64 ||
-      (!per_key && wgs * Hkv * B > 0x7fffffffLL - 8) ||
-      (per_key && B * Hq * ((Tq + bi::pk_prefill_qb(D) - 1) / bi::pk_prefill_qb(D)) > ((int64_t)1 << 27)))
+      (!per_key && wgs * Hkv * B > ((int64_t)1 << 24) - 8) ||
+      (per_key && B * Hq * ((Tq + bi::pk_prefill_qb(D) - 1) / bi::pk_prefill_qb(D)) >= ((int64_t)1 << 27)))
     return fail(BI_E_UNSUPPORTED, "%s: grid too large", what);
   bi::ModRowsArgs a;
   a.q = q; a.k = k; a.v = v; a.kv_lens = kv_lens; a.out = out;
@@ -447,7 +450,7 @@ extern "C" int bi_attn_scored(const void* q, const void* k, const void* v, const
     if (!ws || ws_bytes < need || !bi_host::aligned16(ws))
       return bi_host::fail(BI_E_WORKSPACE, "%s: 16-byte aligned workspace of %zu bytes required, got %zu", what, need,
                            ws ? ws_bytes : (size_t)0);
-    if (B * ((L + bi::kSplit - 1) / bi::kSplit) > 0x7fffffffLL)
+    if (B * ((L + bi::kSplit - 1) / bi::kSplit) >= (int64_t)1 << 26)  // (64 threads a split find its documents)
       return bi_host::fail(BI_E_UNSUPPORTED, "%s: grid too large", what);
     if (bi::few_rows(B, Hq, Hkv, Tq, L, D, causal, dtype)) partials = static_cast<float*>(ws);
     else mod.ranges = static_cast<const int2*>(ws);
