@@ -5,8 +5,9 @@ which of the two runs)."""
 import pytest
 import torch
 
-from helpers import DT
-from test_gpu_scored_attention import _call, _case, _check
+import paged_ref as ref
+from helpers import DT, bits
+from test_gpu_scored_attention import _call, _case, _check, _mods
 
 pytestmark = pytest.mark.gpu
 I32 = torch.int32
@@ -160,3 +161,93 @@ def test_short_sequences_in_a_wide_table(dt, T):
         f = lambda n: bi.batch_invariant_paged_attention(q, k, v, table[:, :n], lens, mask="causal", **mods)
         assert torch.equal(f(wide), f(used))
         assert not f(wide)[3].any()
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("D", [32, 64, 96, 128, 192, 256])
+@pytest.mark.parametrize("page", [0, 4, 16, 64])
+@pytest.mark.parametrize("which", ["d", "c", "s", "csdp"])
+def test_every_head_dim_walked(dt, D, page, which):
+    """Every head dim and type over two splits, the last one partial, against the
+    formula and against the sequences alone, which take a workgroup per split."""
+    B, Hq, Hkv, T, L = 8, 32 if dt == "f32" and D == 256 else 16, 8, 96, 400
+    assert _walks(dt, B, Hq, Hkv, T, L, D) and not _walks(dt, 1, Hq, Hkv, T, L, D)
+    q, k, v = _case(dt, B, Hq, Hkv, T, L, D, D + page)
+    m = _mods(which, B, Hq, L, D)
+    lens = [400, 257, 399, 256, 300, 97, 50, 0]
+    got = _call(q, k, v, lens, True, page, token_major=page == 16, **m)
+    for b in (0, 1, 6):
+        s = slice(b, b + 1)
+        _check(got[s], q[s], k[s], v[s], lens[s], True, **_one(m, b))
+    for b in range(B):
+        s = slice(b, b + 1)
+        assert bits(_call(q[s], k[s], v[s], lens[s], True, page, **_one(m, b))) == bits(got[s]), b
+
+
+@pytest.mark.parametrize("D", [64, 96, 256])
+def test_wider_cap_and_no_mask_walked(D):
+    """Caps above 128 (the closer tanh, in the kernel with both score terms) and no
+    causal mask, with a bias and without."""
+    B, Hq, Hkv, T, L = 8, 16, 8, 96, 400
+    for dt in ("bf16", "f16"):
+        assert _walks(dt, B, Hq, Hkv, T, L, D, causal=False)
+        q, k, v = _case(dt, B, Hq, Hkv, T, L, D, 55)
+        lens = [400, 257, 399, 256, 300, 97, 50, 0]
+        for m in (dict(softcap=200.0), dict(softcap=200.0, slopes=torch.linspace(0.0, 0.1, Hq))):
+            for causal in (True, False):
+                got = _call(q, k, v, lens, causal, 0, **m)
+                for b in (1, 5):
+                    s = slice(b, b + 1)
+                    # past a cap of 128 the error is 12 2^-24 of the score, not of the cap
+                    c = [x[s].cpu() for x in (q, k, v)]
+                    want, absv, dot, bias = ref.attention(*c, D ** -0.5, lens[s], causal, **m)
+                    allow = ref.attention_allowance(want, absv, 13 * dot, bias, DT[dt], D, 2, 0.0)
+                    assert ((got[s].double().cpu() - want).abs() <= allow).all()
+
+
+@pytest.mark.parametrize("page", [0, 16, 4])
+def test_documents_that_begin_anywhere_walked_fp32(page):
+    """fp32 rows enough for the kernel that walks: documents that begin in each 64 keys
+    of a split, some shorter than 64."""
+    L, D, at = 700, 64, [0, 70, 130, 200, 256, 330, 450, 465, 480, 515, 640]
+    assert _walks("f32", 4, 8, 1, L, L, D)
+    q, k, v = _case("f32", 4, 8, 1, L, L, D, 56)
+    doc = torch.zeros(4, L, dtype=I32)
+    for i, b in enumerate(at):
+        doc[0::2, b:], doc[1::2, b:] = i, len(at) - i
+    lens = [L, 690, 300, 1]
+    got = _call(q, k, v, lens, True, page, doc_ids=doc)
+    for b in range(2):
+        s = slice(b, b + 1)
+        _check(got[s], q[s], k[s], v[s], lens[s], True, doc_ids=doc[s])
+    for b in range(4):
+        s = slice(b, b + 1)
+        assert bits(_call(q[s], k[s], v[s], lens[s], True, page, doc_ids=doc[s])) == bits(got[s])
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("page", [0, 4, 16, 64])
+def test_hidden_infinities_and_nan_walked(dt, page):
+    """Rows of K and V that a query does not see hold infinities and NaN, in the kernel
+    that walks: what it gets is what it got with zeros there."""
+    B, Hq, Hkv, T, L, D = 8, 16, 8, 150, 420, 64
+    assert _walks(dt, B, Hq, Hkv, T, L, D)
+    q, k, v = _case(dt, B, Hq, Hkv, T, L, D, 57)
+    docs = torch.arange(L).div(130, rounding_mode="floor").repeat(B, 1).to(I32)
+    docs[1::2, 200:] = torch.arange(220) % 3
+    lens = [L, L - 30] * 4
+    bad = [(0, 3, "nan"), (0, 135, "inf"), (0, 300, "-inf"), (0, 419, "nan"), (1, 10, "inf"), (1, 310, "nan"),
+           (3, 395, "nan"), (3, 389, "-inf"), (5, 400, "nan"), (5, 419, "inf")]
+    clean, dirty = [k.clone(), v.clone()], [k.clone(), v.clone()]
+    for b, j, x in bad:
+        for i in range(2):
+            clean[i][b, :, j, 5:40], dirty[i][b, :, j, 5:40] = 0.0, float(x)
+    for m in (dict(doc_ids=docs), dict(softcap=4.0), dict(slopes=torch.full((Hq,), 0.1), doc_ids=docs)):
+        see = _visible(lens, T, L, True, **m)
+        sees = torch.zeros(B, T, dtype=torch.bool)
+        for b, j, _ in bad:
+            sees[b] |= see[b, :, j]
+        got, base = _call(q, *dirty, lens, True, page, **m), _call(q, *clean, lens, True, page, **m)
+        blind = ~sees[:, None, :, None].expand(got.shape).cuda()
+        assert torch.equal(got[blind], base[blind]) and base.isfinite().all()
+        assert got[~blind].isnan().any()
