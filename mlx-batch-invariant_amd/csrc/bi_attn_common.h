@@ -155,23 +155,26 @@ __device__ __forceinline__ float mod_score(float dot, const Args& a, float slope
 // An infinity or NaN that a query sees in V comes out in its dim as it is, whatever
 // the key's weight: inf, -inf, or NaN for both or a NaN. (The ordinary product
 // would be NaN where the weight, its low half or a later merge's factor is 0, so it
-// would depend on the weights' rounding.) A kernel whose sums are not finite
-// weighs again without such elements; a split's partial of a dim in which a row
-// sees one is then this NaN, whose low bits say what was seen (1: inf, 2: -inf, 4:
-// NaN), and the merge collects them. Ordinary NaN (of the scores) have other bits.
+// would depend on the weights' rounding.) The kernels look for them where sums are
+// not finite. Kinds: 1 inf, 2 -inf, 4 NaN; 0 a finite number.
+__device__ __forceinline__ uint32_t v_kind(float x) {
+  return fabsf(x) < INFINITY ? 0u : x != x ? 4u : x > 0.0f ? 1u : 2u;
+}
+// The output of a row that saw `kinds` (not 0), l its weight sum: 0 if no key had a
+// score above -inf, NaN if one's score was NaN.
+__device__ __forceinline__ float seen_value(uint32_t kinds, float l) {
+  return l == 0.0f ? 0.0f : l != l ? l : kinds == 1u ? INFINITY : kinds == 2u ? -INFINITY : NAN;
+}
+// Chunks of few rows: a split's partial of a dim in which a row sees one is this NaN
+// with the kinds in its low bits, which the merge collects (ordinary NaN, of the
+// scores, have other bits).
 constexpr uint32_t kSeenTag = 0x7fc5a500u;
-__device__ __forceinline__ uint32_t v_kind(float x) { return x != x ? 4u : x > 0.0f ? 1u : 2u; }
 __device__ __forceinline__ uint32_t seen_kinds(float acc) {
   const uint32_t u = __builtin_bit_cast(uint32_t, acc);
   return (u & ~7u) == kSeenTag ? u & 7u : 0u;
 }
 __device__ __forceinline__ float note_seen(float acc, float x) {
   return __builtin_bit_cast(float, kSeenTag | seen_kinds(acc) | v_kind(x));
-}
-// The output of a row that saw `kinds` (not 0), l its weight sum: 0 if no key had a
-// score above -inf, NaN if one's score was NaN.
-__device__ __forceinline__ float seen_value(uint32_t kinds, float l) {
-  return l == 0.0f ? 0.0f : l != l ? l : kinds == 1u ? INFINITY : kinds == 2u ? -INFINITY : NAN;
 }
 // The output of a row's only split: the merge's fma(0, 0, acc) / l, which is no -0.
 __device__ __forceinline__ float only_split(float acc, float l) {

@@ -178,7 +178,8 @@ constexpr int decode_v_slices() {
 // bf16, capped: 220 us and 9 of merging (plain: 196 and 8). A document mask hides a key from every head of the item, so
 // its V row is cleared in LDS and its weight 0 meets no infinity or NaN; a split
 // without a key of the query's document writes an empty partial (l = 0). Infinities
-// and NaN that the query sees in V: kSeenTag.
+// and NaN that the query sees in V leave sums that are not finite, which the merge
+// looks into (seen_value).
 template <typename T, int D, int GU, bool DYN, int MODE, int MOD = 0>
 __global__ __launch_bounds__(256) void attn_decode_mfma(DecodeArgsOf<MOD> a) {
   constexpr bool ROWPAGED = MODE == kKvRowPaged;
@@ -481,60 +482,20 @@ __global__ __launch_bounds__(256) void attn_decode_mfma(DecodeArgsOf<MOD> a) {
         const int row = 4 * qq + i;
         if constexpr (MOD != 0) {
           if (direct) {                                 // (the merge's fma(0, 0, acc): no -0)
-            if (row < GU)
-              static_cast<T*>(a.out)[(pbase + row) * D + vp * DV + 16 * dt + r] =
-                  to_store<T>(lsum[i] != 0.0f ? (acc[j][i] + 0.0f) / lsum[i] : 0.0f);
+            float x = lsum[i] != 0.0f ? (acc[j][i] + 0.0f) / lsum[i] : 0.0f;
+            if (lsum[i] > 0.0f && !(fabsf(x) < INFINITY)) {  // (hidden keys' rows are zero here)
+              constexpr int kPer = 16 / (int)sizeof(T);
+              const int dim = 16 * dt + r;
+              uint32_t kinds = 0;
+              for (int key = 0; key < n_act; ++key)
+                kinds |= v_kind(to_f32(reinterpret_cast<const T*>(Vs + KV::template off<true>(key, dim / kPer))[dim % kPer]));
+              if (kinds) x = seen_value(kinds, lsum[i]);
+            }
+            if (row < GU) static_cast<T*>(a.out)[(pbase + row) * D + vp * DV + 16 * dt + r] = to_store<T>(x);
             continue;
           }
         }
         if (row < GU) a.pacc[(pbase + (int64_t)row * a.nsplit) * D + vp * DV + 16 * dt + r] = acc[j][i];
-      }
-    }
-    if constexpr (MOD != 0) {
-      bool finite = true;
-#pragma unroll
-      for (int j = 0; j < (NDTV + 3) / 4; ++j)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) finite = finite && (wave + 4 * j >= NDTV || fabsf(acc[j][i]) < INFINITY);
-      // Not finite: weighed again without infinities and NaN, those it sees noted, and
-      // stored again (behind the first stores, which the others need not wait for).
-      if (__ballot(!finite)) {
-#pragma unroll
-        for (int j = 0; j < (NDTV + 3) / 4; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 1
-        for (int ks = 0; ks < kSplit / 32; ++ks) {
-          float p8[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) p8[e] = r < GU ? Ps[r][32 * ks + 16 * (e / 4) + 4 * qq + e % 4] : 0.0f;
-          const PFrag<T> pf = make_pfrag<T>(p8);
-#pragma unroll
-          for (int j = 0; j < (NDTV + 3) / 4; ++j) {
-            const int dt = wave + 4 * j;
-            if (dt < NDTV) acc[j] = pv_step<T>(pf, finite_frag(KV::vfrag(Vs, 32 * ks, dt, lane)), acc[j]);
-          }
-        }
-        for (int key = 0; key < n_act; ++key) {         // (hidden keys' rows are zero here)
-#pragma unroll
-          for (int j = 0; j < (NDTV + 3) / 4; ++j) {
-            if (wave + 4 * j >= NDTV) continue;
-            const int dim = 16 * (wave + 4 * j) + r;
-            constexpr int kPer = 16 / (int)sizeof(T);
-            const float x = to_f32(reinterpret_cast<const T*>(Vs + KV::template off<true>(key, dim / kPer))[dim % kPer]);
-            if (fabsf(x) < INFINITY) continue;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) acc[j][i] = note_seen(acc[j][i], x);
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < (NDTV + 3) / 4; ++j)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int row = 4 * qq + i, dt = wave + 4 * j;
-            if (row >= GU || dt >= NDTV) continue;
-            const int64_t at = (pbase + (int64_t)row * a.nsplit) * D + vp * DV + 16 * dt + r;
-            if (direct) static_cast<T*>(a.out)[at] = to_store<T>(only_split(acc[j][i], lsum[i]));
-            else a.pacc[at] = acc[j][i];
-          }
       }
     }
   }

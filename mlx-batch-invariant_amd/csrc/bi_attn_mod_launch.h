@@ -11,10 +11,10 @@ namespace bi {
 
 // attn_combine_kernel, but a split without a visible key (l = 0 at m = -inf) is
 // not merged: its m would make the factors NaN; one at m = NaN has no acc. (A split
-// whose scores are all NaN has l = NaN and is merged.) Infinities and NaN that the
-// row saw in V: kSeenTag.
+// whose scores are all NaN has l = NaN and is merged.) A sum that is not finite has
+// its thread look through the V column for infinities and NaN that the query sees.
 template <typename T, int D>
-__global__ __launch_bounds__(256) void attn_combine_mod_kernel(DecodeArgs a) {
+__global__ __launch_bounds__(256) void attn_combine_mod_kernel(ModDecodeArgs a) {
   const int64_t gid0 = (int64_t)blockIdx.x * 256 + threadIdx.x;
   const bool live = gid0 < (int64_t)a.B * a.Hq * D;
   const int64_t gid = live ? gid0 : 0;
@@ -23,7 +23,7 @@ __global__ __launch_bounds__(256) void attn_combine_mod_kernel(DecodeArgs a) {
   const int len = a.kv_lens ? min(max(a.kv_lens[b], 0), a.L) : a.L;
   const int ns = (len + kSplit - 1) / kSplit;
   float M = -INFINITY, Ls = 0.0f, A = 0.0f;
-  uint32_t kinds = 0;
+  bool look = false;                                    // a split passed over has an acc that is not finite
   auto merge = [&](float m, float l, float acc) {
     // (merge_split's operations, without a branch: a split passed over multiplies
     // by 1 and adds -0; its acc may be unwritten)
@@ -35,6 +35,7 @@ __global__ __launch_bounds__(256) void attn_combine_mod_kernel(DecodeArgs a) {
     A = __builtin_fmaf(A, c_old, sees ? acc * c_new : -0.0f);
     M = top;
   };
+  auto passed_over = [](float m, float l, float acc) { return m == -INFINITY && l == 0.0f && v_kind(acc) != 0u; };
   int i = 0;
   for (; i + 8 <= ns; i += 8) {                         // partials loaded eight splits ahead, merged in order
     float pm[8], pl[8], pa[8];
@@ -48,18 +49,29 @@ __global__ __launch_bounds__(256) void attn_combine_mod_kernel(DecodeArgs a) {
 #pragma unroll
     for (int j = 0; j < 8; ++j) merge(pm[j], pl[j], pa[j]);
     const float any = ((pa[0] + pa[1]) + (pa[2] + pa[3])) + ((pa[4] + pa[5]) + (pa[6] + pa[7]));
-    if (any != any) {                                   // (a NaN among them)
+    if (!(fabsf(any) < INFINITY)) {
 #pragma unroll
-      for (int j = 0; j < 8; ++j) kinds |= pm[j] == pm[j] ? seen_kinds(pa[j]) : 0u;
+      for (int j = 0; j < 8; ++j) look = look || passed_over(pm[j], pl[j], pa[j]);
     }
   }
   for (; i < ns; ++i) {
     const int64_t po = bh * a.nsplit + i;
-    const float m = a.pm[po], acc = a.pacc[po * D + d];
-    merge(m, a.pl[po], acc);
-    kinds |= m == m ? seen_kinds(acc) : 0u;
+    const float m = a.pm[po], l = a.pl[po], acc = a.pacc[po * D + d];
+    merge(m, l, acc);
+    look = look || passed_over(m, l, acc);
   }
-  if (live) static_cast<T*>(a.out)[bh * D + d] = to_store<T>(kinds ? seen_value(kinds, Ls) : Ls != 0.0f ? A / Ls : 0.0f);
+  float x = Ls != 0.0f ? A / Ls : 0.0f;
+  if (live && Ls > 0.0f && (look || !(fabsf(x) < INFINITY))) {  // (l NaN: NaN, whatever V holds)
+    const int32_t* docs = a.mod.docs ? a.mod.docs + (int64_t)b * a.mod.docs_sb : nullptr;
+    const int hk = (int)(bh % a.Hq) / (a.Hq / a.Hkv);
+    const T* v = static_cast<const T*>(a.v) + d;
+    uint32_t kinds = 0;
+    for (int key = 0; key < len; ++key)
+      if (!docs || docs[key] == docs[len - 1])
+        kinds |= v_kind(to_f32(v[kv_row_off(a, a.v_sb, a.v_sh, a.v_sl, b, hk, key)]));
+    if (kinds) x = seen_value(kinds, Ls);
+  }
+  if (live) static_cast<T*>(a.out)[bh * D + d] = to_store<T>(x);
 }
 
 // One instantiation for both item orders, chosen as for the plain kernel: with at
