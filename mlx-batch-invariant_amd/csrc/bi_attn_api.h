@@ -59,7 +59,8 @@ inline int64_t rows_partial_bytes(int64_t B, int64_t Hq, int64_t Tq, int64_t L, 
 // heads of 64: R = 216, N = 7: 32 / 31; R = 335, N = 18: 80 / 86. fp32, whose walk has
 // no pipeline, 8 / 8 heads of 128: R = 426, N = 3: 102 / 79; R = 569, N = 18: 615 /
 // 454; 32 / 8: R = 623, N = 4: 124 / 131; heads of 32 to 192 turn alike (192: R = 460,
-// N = 3: 114 / 108; R = 623: 184 / 189), of 256, where the walk spills, later: R = 885,
+// N = 3: 114 / 108; R = 623: 184 / 189), of 256, where the walk spills 554 registers
+// and more, later: R = 885,
 // N = 5: 841 / 529. The partials stay below 256 MB. N is what the cache can hold (the
 // host does not know the lengths): a workgroup without keys costs 1.1 ns, so 300 keys
 // in a table of 32768 take 39 us where walking takes 21 (R = 128), and 32768 keys 380

@@ -175,8 +175,10 @@ constexpr int decode_v_slices() {
 
 // MOD (kModAny, ScoreMod): the score terms are chosen at run time, since decode
 // waits for memory: 64 ragged sequences to 8192 keys, 32 / 8 heads of 128, pages of 16,
-// bf16, capped: 220 us and 9 of merging (plain: 196 and 8). A document mask hides a key from every head of the item, so
-// its V row is cleared in LDS and its weight 0 meets no infinity or NaN; a split
+// bf16, capped: 222 us and 9 of merging (plain: 196 and 8); fp32, 32 x 4096 keys,
+// contiguous, heads of 128 310 us (275), of 192 505 (537), of 256 569 (526; its
+// row-paged form spills 190 to 213 registers, the plain one 165 to 179). A document
+// mask hides a key from every head of the item, so its V row is cleared in LDS and its weight 0 meets no infinity or NaN; a split
 // without a key of the query's document writes an empty partial (l = 0). Infinities
 // and NaN that the query sees in V leave sums that are not finite, which the merge
 // looks into (seen_value).

@@ -3,10 +3,17 @@
 // bi_attn_common.h). Layouts, tiles and the order of every sum are those of
 // attn_prefill_mfma (bi_attn_mfma.h): with nothing to change a score or a mask
 // the results are its bits, and a token's are those of the decode kernel. It is
-// a text of its own so that the plain kernel's registers stay as they are. Bound by
-// the issue of vector instructions (19 a score, 59% of the cycles; MFMA 29%): 4 x 2048
-// tokens, causal, 32 / 8 heads of 128, bf16, capped: 293 us, 470 TFLOP/s (the plain
-// kernel 250).
+// a text of its own so that the plain kernel's registers stay as they are. 4 x 2048
+// tokens, causal, 32 / 8 heads of 128, bf16, capped: 300 us, 457 TFLOP/s (the plain
+// kernel 257); vector instructions, some 20 a score, issue in 60% of the SIMDs'
+// cycles, the MFMAs are busy in 31%.
+//
+// Registers: D = 128 takes all 256 in 16 bits, and spills 6 or 7 with a distance bias
+// or with a cap above 128 (which runs there: 395 us where smaller caps take 300).
+// fp32 spills 36 to 77 at D = 192 (4 x 1024 tokens, 32 / 8 heads, capped 790 us; the
+// plain kernel, which spills none, 795) and 554 to 609 at D = 256 (16 / 8 heads: 1294 us;
+// the plain kernel, which spills 80 to 103, 740). 16 bits at D = 256, one workgroup a
+// CU: 4 x 2048 tokens, 16 / 8 heads, capped 354 us, 389 TFLOP/s (plain 281).
 //
 //   scores     s = cap tanh(dot scale / cap) - slope |pos_q - key| in log2 units
 //              (mod_score). Compiled in, since a branch at every score would

@@ -95,7 +95,8 @@ __device__ __forceinline__ float row_sum(float ss, float* wave_sums) {
 // Rows of up to NC * 512 * WPR elements, kept in registers between the sums, WPR
 // waves each: 4 / WPR rows in a workgroup. Bound by HBM: one read of x, residual and
 // gate, one write of y and h. 16384 rows of 4096 with a gate, bf16: 105 us, 5.1 TB/s;
-// rows of 4097 (kAnywhere) 177 us, 425 element by element.
+// rows of 4097 (kAnywhere; a third chunk, in which one thread has work) 177 us, 425
+// element by element.
 template <typename T, int NC, RowForm FORM, bool POST, bool PRE, int WPR>
 __global__ __launch_bounds__(kResThreads) void res_norm_kernel(ResNormArgs a) {
   static_assert(WPR == 4 || NC == 1, "res_norm_kernel: a row's chunks are its threads'");
@@ -174,7 +175,9 @@ __global__ __launch_bounds__(kResThreads) void res_norm_kernel(ResNormArgs a) {
   }
 }
 
-// Longer rows: the same order, x, res and gate read again for each pass.
+// Longer rows: the same order, x, res and gate read again for each pass, element by
+// element: 4096 rows of 9000 / 16384 with a gate for each, bf16: 376 / 687 us, 1.0 TB/s
+// of one pass's bytes (rows of 8192, kept in registers: 77 us, 4.4).
 template <typename T, bool POST, bool PRE>
 __global__ __launch_bounds__(kResThreads) void res_norm_kernel_long(ResNormArgs a) {
   __shared__ float wave_sums[kResThreads / kWave];

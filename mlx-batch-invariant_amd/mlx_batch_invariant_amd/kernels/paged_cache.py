@@ -74,7 +74,8 @@ def paged_slots(kv_lens, new_lens, block_table: torch.Tensor, free_pages, *, pag
     more than T new tokens, is refused: no page, slots -1, its length stays
     (``plan.kv_lens[b] < kv_lens[b] + new_lens[b]`` tells). Behind a request that
     the free list cannot serve only those that need no page are served. Negative
-    counts are 0, lengths past the table's reach are cut to it.
+    counts are 0, lengths past the table's reach are cut to it. (Wider whole numbers
+    are taken modulo 2^32.)
     """
     what = "paged_slots"
     _page_size(what, page_size)
@@ -157,7 +158,8 @@ def rope_paged_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos: tor
     (R a multiple of 8, at most D / 2). ``positions`` ``[B, T]``, or ``[A, B, T]``
     for tokens placed along up to four axes (time, height, width), with
     ``sections`` the A numbers of pairs that turn with each axis, in order
-    (their sum is R). A position outside the tables is clamped into them. Each
+    (their sum is R). A position outside the tables is clamped into them (int32;
+    wider numbers are taken modulo 2^32). Each
     product and sum is in fp32, the result rounded once.
     """
     what = "rope_paged_cache"

@@ -2,8 +2,8 @@
 
 ``y = residual + norm(x) * w_post * gate * scale`` and ``h = norm(y) * w_pre``:
 what a block's output adds to the residual stream, and the next block's input.
-Both sums run in ``rms_norm``'s order (one workgroup per row, fixed by D alone),
-everything else per element in fp32; y and h are rounded once each, h from the
+Both sums run in ``rms_norm``'s order (D alone fixes it, and how many waves a row
+has), everything else per element in fp32; y and h are rounded once each, h from the
 unrounded y. The reference norms only (mlx_batch_invariant/kernels/rmsnorm.py:1-79).
 """
 
