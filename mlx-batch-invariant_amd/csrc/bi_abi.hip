@@ -28,8 +28,20 @@ int fail(int code, const char* fmt, ...) {
   return code;
 }
 
+static thread_local bool g_grid_too_large = false;
+
+bool grid_fits(int64_t blocks, int threads) {
+  if (blocks * threads < ((int64_t)1 << 32)) return true;
+  g_grid_too_large = true;
+  return false;
+}
+
 int launch_status(const char* what) {
   hipError_t e = hipGetLastError();
+  if (g_grid_too_large) {
+    g_grid_too_large = false;
+    return fail(BI_E_UNSUPPORTED, "%s: grid too large", what);
+  }
   if (e != hipSuccess) {
     set_error("%s: launch failed: %s", what, hipGetErrorString(e));
     return (int)e;

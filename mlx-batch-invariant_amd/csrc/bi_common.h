@@ -236,6 +236,9 @@ namespace bi_host {
 void set_error(const char* fmt, ...);
 int fail(int code, const char* fmt, ...);
 int launch_status(const char* what);
+// Whether a 1-D launch holds fewer than 2^32 threads (more wrap without an error).
+// If not, the thread's next launch_status reports it: the caller launches nothing.
+bool grid_fits(int64_t blocks, int threads);
 inline bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
 inline size_t dtype_size(int dt) { return dt == BI_F32 ? 4 : 2; }
 }  // namespace bi_host

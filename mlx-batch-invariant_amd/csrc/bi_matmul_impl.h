@@ -1146,6 +1146,7 @@ template <typename T, class BSrc, int W>
 static void launch_wg(const T* a, int64_t lda, const BSrc& bsrc, T* out, int M, int N, int K, int G,
                       hipStream_t st) {
   dim3 grid(ceil_div(N, 16), 1, 1);
+  if (!bi_host::grid_fits(grid.x, kWave * W)) return;   // (2^27 columns and more at 8 waves)
   const int mt = M <= 16 ? 1 : 2;
   const size_t part_bytes = (size_t)G * mt * kWave * sizeof(f32x4);
   const size_t a_bytes = (size_t)M * (K + 8) * sizeof(T);
