@@ -332,8 +332,9 @@ int bi_attn_prefill_paged(const void* q, const void* k_pages, const void* v_page
  * every key of its sequence); slopes need L <= 2^24. strides[0..8] as for
  * bi_attn_prefill (strides[2] unused at Tq == 1). Same order of operations as
  * bi_attn_decode / bi_attn_prefill, so the same invariances hold, and where no
- * score or mask is changed (slopes 0, one document, no prefix) and V is finite the
- * same bits (infinities in V: those give what the products do, mostly NaN).
+ * score or mask is changed (slopes 0, one document, no prefix) and q, K and V are
+ * finite the same bits (with infinities in V those give what the products do, mostly
+ * NaN; a row with a NaN score, here NaN, is zeros there).
  * Workspace: bi_attn_scored_workspace_bytes; calls that overlap must not share it.
  * Replaces: nothing in the reference (its masks are none and causal,
  * kernels/attention.py:299-310). */

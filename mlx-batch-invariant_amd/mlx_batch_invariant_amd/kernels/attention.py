@@ -54,8 +54,9 @@ the scores and the mask in the matrix-core order: with query t at position
 Hidden keys take no part whatever their rows hold; a query that sees none (one
 in front of a padded prompt, p < 0) gets zeros. An infinity or NaN that a query
 sees in V comes out in its dim, as inf, -inf or (a NaN, or both) NaN, however small
-the key's weight. The invariances above hold, and where nothing is changed (slopes
-of 0, one document, no prefix) and V is finite the bits of the plain call.
+the key's weight; one with a NaN score gets NaN. The invariances above hold, and where
+nothing is changed (slopes of 0, one document, no prefix) and q, K and V are finite the
+bits of the plain call.
 """
 
 from __future__ import annotations
