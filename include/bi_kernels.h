@@ -443,6 +443,70 @@ int bi_rope_paged_cache(const void* q, int64_t q_row, const void* k, int64_t k_r
                         void* q_out, void* k_pages, void* v_pages, int64_t num_pages, int64_t page_size, int64_t B,
                         int64_t T, int64_t Hq, int64_t Hkv, int64_t D, const int64_t* strides, int dtype, void* stream);
 
+/* ---- A paged K/V cache in 8 or 4 bits -----------------------------------------
+ * A row of D values is held as D codes of `bits` bits (4: two to a byte, the low
+ * half first) and one (scale, bias) pair of the operands' type for each
+ * group_size (32, 64 or 128) values, the MLX-affine format; code c stands for
+ * T(fma(c, scale, bias)). Pools: codes [num_pages, Hkv, page_size, D * bits / 8]
+ * bytes, groups [num_pages, Hkv, page_size, D / group_size, 2] of dtype, 16-byte
+ * aligned. strides (host, int64[12]): (page, head, row) of k_codes in bytes,
+ * multiples of 16; of k_groups in elements, even; then of v_codes and v_groups.
+ *
+ * bi_rope_quantized_cache: bi_rope_paged_cache with such pools. The rows that it
+ * would write are quantized by group: bias = min, scale = T((max - min) / (2^bits -
+ * 1)) or 1 where that is 0, code = round((y - bias) / scale) to even, clamped (and
+ * kept below a code whose value would overflow). A group with an infinity or a NaN
+ * reads back as NaN. Of several tokens with one slot, each 16 values of the row
+ * keep some one's codes, and each group some one's pair.
+ * Replaces: nothing in the reference (its weights alone are quantized,
+ * kernels/quantized.py:33-67). */
+int bi_rope_quantized_cache(const void* q, int64_t q_row, const void* k, int64_t k_row, const void* v, int64_t v_row,
+                            const void* cos, const void* sin, int64_t table_rows, int table_dtype,
+                            const int32_t* positions, const int64_t* sections, int64_t axes, const int64_t* slots,
+                            void* q_out, void* k_codes, void* k_groups, void* v_codes, void* v_groups,
+                            int64_t num_pages, int64_t page_size, int64_t B, int64_t T, int64_t Hq, int64_t Hkv,
+                            int64_t D, int bits, int64_t group_size, const int64_t* strides, int dtype, void* stream);
+
+/* Whole sequences out of such pools: k_out, v_out contiguous [B, Hkv, L, D] of
+ * dtype, 16-byte aligned. Row p of sequence b comes from row p % page_size of page
+ * block_table[b * table_stride + p / page_size] (clamped into the pool); rows from
+ * kv_lens[b] (device int32 [B], clamped to [0, L]; null: L) on are zeros if fill,
+ * else left as they are. */
+int bi_read_quantized_cache(const void* k_codes, const void* k_groups, const void* v_codes, const void* v_groups,
+                            const int64_t* strides, const int32_t* block_table, int64_t table_stride,
+                            int64_t page_size, int64_t num_pages, const int32_t* kv_lens, void* k_out, void* v_out,
+                            int64_t B, int64_t Hkv, int64_t L, int64_t D, int bits, int64_t group_size, int fill,
+                            int dtype, void* stream);
+
+/* ---- Attention over quantized pages, and behind shared prefixes ---------------
+ * bi_attn_decode_paged / bi_attn_prefill_paged for any Tq >= 1 (causal applies to
+ * Tq == 1 too, where it hides nothing), with two things more.
+ * bits 4 or 8: k, v are codes and k_groups, v_groups their pairs (above; group_size
+ * divides D); bits 0: rows of dtype, k_groups and v_groups null. strides (host,
+ * int64[15]): q (sequence, head, token), k (page, head, row), v; with bits codes in
+ * bytes, and behind them the pairs of k and v.
+ * groups > 0: sequences shared_starts[n] .. shared_starts[n + 1] - 1 (device int32
+ * [groups + 1], rising; null for one group of all) begin with the same shared_lens[n]
+ * keys (device int32 [groups]; null: shared_len for one group). Their whole 256-key
+ * splits that the first sequence holds are read from its pages, once for all of the
+ * group; a sequence in no group, or alone in one, shares nothing.
+ * The results are the bits of the plain calls on the same keys (codes: on the rows
+ * read back) where q, K and V are finite. Hidden keys take no part whatever their
+ * rows hold; a query that sees no key gets zeros; infinities and NaN that a query
+ * sees in V come out as bi_attn_scored's do.
+ * Workspace (16-byte aligned): bi_attn_pages_workspace_bytes; calls that overlap must
+ * not share it.
+ * Replaces: nothing in the reference (kernels/attention.py:87-254 reads one
+ * contiguous cache of plain rows for each sequence). */
+size_t bi_attn_pages_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t Tq, int64_t L, int64_t D,
+                                     int64_t groups, int bits, int causal, int dtype);
+int bi_attn_pages(const void* q, const void* k, const void* k_groups, const void* v, const void* v_groups, int bits,
+                  int64_t group_size, const int32_t* block_table, int64_t table_stride, int64_t page_size,
+                  int64_t num_pages, const int32_t* kv_lens, const int32_t* shared_starts, const int32_t* shared_lens,
+                  int64_t shared_len, int64_t groups, void* out, int64_t B, int64_t Hq, int64_t Hkv, int64_t Tq,
+                  int64_t L, int64_t D, const int64_t* strides, int causal, float scale, int dtype, void* ws,
+                  size_t ws_bytes, void* stream);
+
 /* ---- The norms around a block ------------------------------------------------
  * u = x * inv(x) * w_post (post == 0: u = x), y = res + u * gate * scale,
  * h = y * inv(y) * w_pre (pre == 0: no h), inv(z) = 1 / sqrt(ss(z) / D + eps)

@@ -1,7 +1,8 @@
 /* bi_pycall.c — a CPython binding of the most frequently called C-ABI entry
  * points (bi_quantized_matmul, bi_matmul, bi_rms_norm, and the operators of a
- * paged serving step: bi_paged_slots, bi_rope_paged_cache, bi_attn_scored,
- * bi_residual_rms_norm) for eager callers.
+ * paged serving step: bi_paged_slots, bi_rope_paged_cache, bi_rope_quantized_cache,
+ * bi_read_quantized_cache, bi_attn_scored, bi_attn_pages, bi_residual_rms_norm) for
+ * eager callers.
  *
  * ctypes converts every argument through its argtypes on each call (about
  * 3 us for the 15 arguments of bi_quantized_matmul); here the arguments are
@@ -38,6 +39,9 @@ static __typeof__(&bi_paged_slots) g_slots;
 static __typeof__(&bi_rope_paged_cache) g_rope;
 static __typeof__(&bi_attn_scored) g_scored;
 static __typeof__(&bi_residual_rms_norm) g_resnorm;
+static __typeof__(&bi_rope_quantized_cache) g_ropeq;
+static __typeof__(&bi_read_quantized_cache) g_readq;
+static __typeof__(&bi_attn_pages) g_pages;
 
 #define PTR(v) ((void*)(intptr_t)(v))
 
@@ -61,10 +65,11 @@ static int read_i64(PyObject* const* args, Py_ssize_t n, Py_ssize_t want, Py_ssi
 }
 
 static PyObject* py_bind(PyObject* self, PyObject* args) {
-  unsigned long long a[7];
+  unsigned long long a[10];
   (void)self;
-  if (!PyArg_ParseTuple(args, "KKKKKKK", &a[0], &a[1], &a[2], &a[3], &a[4], &a[5], &a[6])) return NULL;
-  for (int i = 0; i < 7; ++i) {
+  if (!PyArg_ParseTuple(args, "KKKKKKKKKK", &a[0], &a[1], &a[2], &a[3], &a[4], &a[5], &a[6], &a[7], &a[8], &a[9]))
+    return NULL;
+  for (int i = 0; i < 10; ++i) {
     if (!a[i]) {
       PyErr_SetString(PyExc_ValueError, "bind: null entry point");
       return NULL;
@@ -77,6 +82,9 @@ static PyObject* py_bind(PyObject* self, PyObject* args) {
   g_rope = (__typeof__(g_rope))(uintptr_t)a[4];
   g_scored = (__typeof__(g_scored))(uintptr_t)a[5];
   g_resnorm = (__typeof__(g_resnorm))(uintptr_t)a[6];
+  g_ropeq = (__typeof__(g_ropeq))(uintptr_t)a[7];
+  g_readq = (__typeof__(g_readq))(uintptr_t)a[8];
+  g_pages = (__typeof__(g_pages))(uintptr_t)a[9];
   Py_RETURN_NONE;
 }
 
@@ -217,6 +225,52 @@ static PyObject* py_residual_rms_norm(PyObject* self, PyObject* const* args, Py_
   return PyLong_FromLong(rc);
 }
 
+/* ... positions, axes, its 4 sections, slots, ... D, bits, group size, the 12 strides, dtype, stream */
+static PyObject* py_rope_quantized_cache(PyObject* self, PyObject* const* args, Py_ssize_t n) {
+  int64_t v[45];
+  int rc;
+  (void)self;
+  NEED(g_ropeq, "rope_quantized_cache")
+  if (read_mixed(args, n, "iiiiiiiiiiiiiiiiiiiiiiiiiiiiiiiiiiiiiiiiiiiii", v, NULL, "rope_quantized_cache")) return NULL;
+  Py_BEGIN_ALLOW_THREADS
+  rc = g_ropeq(PTR(v[0]), v[1], PTR(v[2]), v[3], PTR(v[4]), v[5], PTR(v[6]), PTR(v[7]), v[8], (int)v[9], PTR(v[10]),
+               &v[12], v[11], PTR(v[16]), PTR(v[17]), PTR(v[18]), PTR(v[19]), PTR(v[20]), PTR(v[21]), v[22], v[23],
+               v[24], v[25], v[26], v[27], v[28], (int)v[29], v[30], &v[31], (int)v[43], PTR(v[44]));
+  Py_END_ALLOW_THREADS
+  return PyLong_FromLong(rc);
+}
+
+/* the 4 pools, the 12 strides, block_table, ... */
+static PyObject* py_read_quantized_cache(PyObject* self, PyObject* const* args, Py_ssize_t n) {
+  int64_t v[32];
+  int rc;
+  (void)self;
+  NEED(g_readq, "read_quantized_cache")
+  if (read_mixed(args, n, "iiiiiiiiiiiiiiiiiiiiiiiiiiiiiiii", v, NULL, "read_quantized_cache")) return NULL;
+  Py_BEGIN_ALLOW_THREADS
+  rc = g_readq(PTR(v[0]), PTR(v[1]), PTR(v[2]), PTR(v[3]), &v[4], PTR(v[16]), v[17], v[18], v[19], PTR(v[20]),
+               PTR(v[21]), PTR(v[22]), v[23], v[24], v[25], v[26], (int)v[27], v[28], (int)v[29], (int)v[30],
+               PTR(v[31]));
+  Py_END_ALLOW_THREADS
+  return PyLong_FromLong(rc);
+}
+
+/* ... L, D, the 15 strides, causal, scale, dtype, ... */
+static PyObject* py_attn_pages(PyObject* self, PyObject* const* args, Py_ssize_t n) {
+  int64_t v[44];
+  double d[44];
+  int rc;
+  (void)self;
+  NEED(g_pages, "attn_pages")
+  if (read_mixed(args, n, "iiiiiiiiiiiiiiiiiiiiiiiiiiiiiiiiiiiiiiifiiii", v, d, "attn_pages")) return NULL;
+  Py_BEGIN_ALLOW_THREADS
+  rc = g_pages(PTR(v[0]), PTR(v[1]), PTR(v[2]), PTR(v[3]), PTR(v[4]), (int)v[5], v[6], PTR(v[7]), v[8], v[9], v[10],
+               PTR(v[11]), PTR(v[12]), PTR(v[13]), v[14], v[15], PTR(v[16]), v[17], v[18], v[19], v[20], v[21], v[22],
+               &v[23], (int)v[38], (float)d[39], (int)v[40], PTR(v[41]), (size_t)v[42], PTR(v[43]));
+  Py_END_ALLOW_THREADS
+  return PyLong_FromLong(rc);
+}
+
 static PyMethodDef methods[] = {
     {"bind", py_bind, METH_VARARGS, "bind(...): addresses of the C-ABI entry points, in the order below"},
     {"quantized_matmul", (PyCFunction)(void (*)(void))py_quantized_matmul, METH_FASTCALL,
@@ -231,6 +285,12 @@ static PyMethodDef methods[] = {
      "bi_attn_scored: the 9 strides and the 5 fields of bi_score_mod one by one"},
     {"residual_rms_norm", (PyCFunction)(void (*)(void))py_residual_rms_norm, METH_FASTCALL,
      "bi_residual_rms_norm with the C ABI's arguments"},
+    {"rope_quantized_cache", (PyCFunction)(void (*)(void))py_rope_quantized_cache, METH_FASTCALL,
+     "bi_rope_quantized_cache: axes before its 4 sections, and the 12 strides, one by one"},
+    {"read_quantized_cache", (PyCFunction)(void (*)(void))py_read_quantized_cache, METH_FASTCALL,
+     "bi_read_quantized_cache: the 12 strides one by one"},
+    {"attn_pages", (PyCFunction)(void (*)(void))py_attn_pages, METH_FASTCALL,
+     "bi_attn_pages: the 15 strides one by one"},
     {NULL, NULL, 0, NULL}};
 
 static struct PyModuleDef module = {PyModuleDef_HEAD_INIT, "_bi_pycall", NULL, -1, methods, NULL, NULL, NULL, NULL};

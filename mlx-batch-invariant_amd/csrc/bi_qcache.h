@@ -1,0 +1,115 @@
+// bi_qcache.h — rows of a cache held in 8 or 4 bits. A row of D values is D codes
+// (8 bits: a byte each; 4 bits: two to a byte, the low half first) and one (scale,
+// bias) pair of type T for each group of 32, 64 or 128 values; code c stands for
+// T(fma(c, scale, bias)), as in the quantized matmul.
+#pragma once
+
+#include "bi_common.h"
+
+namespace bi {
+
+template <typename T> struct Pair { float s, b; };        // a group's scale and bias
+
+template <typename T>
+__device__ __forceinline__ Pair<T> load_pair(const T* p) {
+  Pair<T> g;
+  if constexpr (sizeof(T) == 2) {
+    const uint32_t u = *reinterpret_cast<const uint32_t*>(p);
+    g.s = to_f32(__builtin_bit_cast(T, (uint16_t)u));
+    g.b = to_f32(__builtin_bit_cast(T, (uint16_t)(u >> 16)));
+  } else {
+    const u32x2 u = *reinterpret_cast<const u32x2*>(p);
+    g.s = __builtin_bit_cast(float, (uint32_t)u[0]);
+    g.b = __builtin_bit_cast(float, (uint32_t)u[1]);
+  }
+  return g;
+}
+
+// Eight and sixteen consecutive codes.
+template <int BITS> struct Codes8;
+template <> struct Codes8<8> { uint32_t w[2]; };
+template <> struct Codes8<4> { uint32_t w[1]; };
+template <int BITS> struct Codes16 {
+  uint32_t w[BITS / 2];
+  __device__ __forceinline__ Codes8<BITS> half(int h) const {
+    Codes8<BITS> c;
+#pragma unroll
+    for (int i = 0; i < BITS / 4; ++i) c.w[i] = w[h * (BITS / 4) + i];
+    return c;
+  }
+};
+
+template <int BITS>
+__device__ __forceinline__ Codes8<BITS> load_codes8(const char* p) {
+  Codes8<BITS> c;
+  if constexpr (BITS == 8) {
+    const u32x2 u = *reinterpret_cast<const u32x2*>(p);
+    c.w[0] = u[0];
+    c.w[1] = u[1];
+  } else {
+    c.w[0] = *reinterpret_cast<const uint32_t*>(p);
+  }
+  return c;
+}
+
+template <int BITS>
+__device__ __forceinline__ Codes16<BITS> load_codes16(const char* p) {
+  Codes16<BITS> c;
+  if constexpr (BITS == 8) {
+    const u32x4 u = *reinterpret_cast<const u32x4*>(p);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c.w[i] = u[i];
+  } else {
+    const u32x2 u = *reinterpret_cast<const u32x2*>(p);
+    c.w[0] = u[0];
+    c.w[1] = u[1];
+  }
+  return c;
+}
+
+// The values of 8 codes, as floats that hold T's before the rounding.
+template <int BITS>
+__device__ __forceinline__ void code_floats(Codes8<BITS> c, float (&x)[8]) {
+  if constexpr (BITS == 8) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = (float)(c.w[e / 4] >> (8 * (e % 4)) & 255u);
+  } else {
+    const uint32_t even = c.w[0] & 0x0f0f0f0fu, odd = c.w[0] >> 4 & 0x0f0f0f0fu;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = (float)((e & 1 ? odd : even) >> (8 * (e / 2)) & 255u);
+  }
+}
+
+// T(fma(code, scale, bias)) of 8 codes of one group. The fma's result is kept in a
+// register of its own: folded into the conversion (v_fma_mixlo_f16) it would round
+// once where the quantized matmul rounds twice.
+template <typename T, int BITS>
+__device__ __forceinline__ typename Frag<T>::type dequant_frag(Codes8<BITS> c, Pair<T> g) {
+  typedef float f32x2v __attribute__((ext_vector_type(2)));
+  typedef T tx2 __attribute__((ext_vector_type(2)));
+  float x[8];
+  code_floats<BITS>(c, x);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    x[e] = __builtin_fmaf(x[e], g.s, g.b);
+    if constexpr (sizeof(T) == 2) asm("" : "+v"(x[e]));
+  }
+  typename Frag<T>::type f;
+  if constexpr (sizeof(T) == 2) {
+#pragma unroll
+    for (int e = 0; e < 8; e += 2) {
+      const tx2 y = __builtin_convertvector(f32x2v{x[e], x[e + 1]}, tx2);
+      f[e] = y[0];
+      f[e + 1] = y[1];
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      f.lo[e] = x[e];
+      f.hi[e] = x[4 + e];
+    }
+  }
+  return f;
+}
+
+}  // namespace bi

@@ -22,9 +22,15 @@ from .kernels import (
     batch_invariant_quantized_matmul,
     batch_invariant_residual_rms_norm,
     batch_invariant_rms_norm,
+    batch_invariant_quantized_paged_attention,
+    batch_invariant_shared_prefix_attention,
     PagedSlots,
+    QuantizedPages,
     paged_slots,
+    quantized_pages,
+    read_quantized_cache,
     rope_paged_cache,
+    rope_quantized_cache,
 )
 from .kernels.quantized import (quantize, dequantize, pack, unpack, cache_dequantized, drop_dequantized,
                                 cache_packed, drop_packed)
@@ -49,6 +55,12 @@ __all__ = [
     "PagedSlots",
     "paged_slots",
     "rope_paged_cache",
+    "QuantizedPages",
+    "quantized_pages",
+    "rope_quantized_cache",
+    "read_quantized_cache",
+    "batch_invariant_quantized_paged_attention",
+    "batch_invariant_shared_prefix_attention",
     "quantize",
     "dequantize",
     "cache_dequantized",

@@ -96,6 +96,19 @@ _SIGNATURES = {
                                            _vp, ctypes.POINTER(_c_i64), _c_i64, _vp, _vp, _vp, _vp, _c_i64, _c_i64,
                                            _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, ctypes.POINTER(_c_i64),
                                            ctypes.c_int, _vp]),
+    "bi_rope_quantized_cache": (ctypes.c_int, [_vp, _c_i64, _vp, _c_i64, _vp, _c_i64, _vp, _vp, _c_i64, ctypes.c_int,
+                                               _vp, ctypes.POINTER(_c_i64), _c_i64, _vp, _vp, _vp, _vp, _vp, _vp,
+                                               _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, ctypes.c_int,
+                                               _c_i64, ctypes.POINTER(_c_i64), ctypes.c_int, _vp]),
+    "bi_read_quantized_cache": (ctypes.c_int, [_vp, _vp, _vp, _vp, ctypes.POINTER(_c_i64), _vp, _c_i64, _c_i64, _c_i64,
+                                               _vp, _vp, _vp, _c_i64, _c_i64, _c_i64, _c_i64, ctypes.c_int, _c_i64,
+                                               ctypes.c_int, ctypes.c_int, _vp]),
+    "bi_attn_pages_workspace_bytes": (ctypes.c_size_t, [_c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64,
+                                                        ctypes.c_int, ctypes.c_int, ctypes.c_int]),
+    "bi_attn_pages": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, ctypes.c_int, _c_i64, _vp, _c_i64, _c_i64, _c_i64, _vp,
+                                     _vp, _vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64,
+                                     ctypes.POINTER(_c_i64), ctypes.c_int, ctypes.c_float, ctypes.c_int, _vp,
+                                     ctypes.c_size_t, _vp]),
     "bi_residual_rms_norm": (ctypes.c_int, [_vp, _c_i64, _vp, _c_i64, _vp, _c_i64, _c_i64, _vp, _vp, _vp, _vp,
                                             _c_i64, _c_i64, ctypes.c_float, ctypes.c_float, ctypes.c_int,
                                             ctypes.c_int, ctypes.c_int, _vp]),
@@ -163,10 +176,14 @@ slots_call = None
 rope_paged_call = None
 scored_call = None
 residual_norm_call = None
+rope_quantized_call = None
+read_quantized_call = None
+pages_call = None
 
 
 def _bind_fast(lib) -> None:
     global qmm_call, matmul_call, rms_norm_call, slots_call, rope_paged_call, scored_call, residual_norm_call
+    global rope_quantized_call, read_quantized_call, pages_call
     qmm_call, matmul_call, rms_norm_call = lib.bi_quantized_matmul, lib.bi_matmul, lib.bi_rms_norm
     slots_call, residual_norm_call = lib.bi_paged_slots, lib.bi_residual_rms_norm
 
@@ -177,17 +194,30 @@ def _bind_fast(lib) -> None:
     def scored_call(*a):
         return lib.bi_attn_scored(*a[:15], (_c_i64 * 9)(*a[15:24]), a[24], a[25], ScoreMod(*a[26:31]), *a[31:])
 
+    def rope_quantized_call(*a):
+        return lib.bi_rope_quantized_cache(*a[:11], (_c_i64 * 4)(*a[12:16]), a[11], *a[16:31], (_c_i64 * 12)(*a[31:43]),
+                                           *a[43:])
+
+    def read_quantized_call(*a):
+        return lib.bi_read_quantized_cache(*a[:4], (_c_i64 * 12)(*a[4:16]), *a[16:])
+
+    def pages_call(*a):
+        return lib.bi_attn_pages(*a[:23], (_c_i64 * 15)(*a[23:38]), *a[38:])
+
     try:
         from . import _bi_pycall as fast
     except ImportError:
         return
     addr = [ctypes.cast(getattr(lib, n), ctypes.c_void_p).value
             for n in ("bi_quantized_matmul", "bi_matmul", "bi_rms_norm", "bi_paged_slots", "bi_rope_paged_cache",
-                      "bi_attn_scored", "bi_residual_rms_norm")]
+                      "bi_attn_scored", "bi_residual_rms_norm", "bi_rope_quantized_cache", "bi_read_quantized_cache",
+                      "bi_attn_pages")]
     fast.bind(*addr)
     qmm_call, matmul_call, rms_norm_call = fast.quantized_matmul, fast.matmul, fast.rms_norm
     slots_call, rope_paged_call = fast.paged_slots, fast.rope_paged_cache
     scored_call, residual_norm_call = fast.attn_scored, fast.residual_rms_norm
+    rope_quantized_call, read_quantized_call = fast.rope_quantized_cache, fast.read_quantized_cache
+    pages_call = fast.attn_pages
 
 
 def exported_symbols() -> list[str]:

@@ -25,6 +25,14 @@ from .layernorm import batch_invariant_layer_norm
 from .quantized import batch_invariant_quantized_matmul
 from .residual_norm import batch_invariant_residual_rms_norm
 from .paged_cache import PagedSlots, paged_slots, rope_paged_cache
+from .quantized_cache import (
+    QuantizedPages,
+    batch_invariant_quantized_paged_attention,
+    batch_invariant_shared_prefix_attention,
+    quantized_pages,
+    read_quantized_cache,
+    rope_quantized_cache,
+)
 from .attention import (
     batch_invariant_attention,
     batch_invariant_decode_attention,
@@ -46,4 +54,10 @@ __all__ = [
     "PagedSlots",
     "paged_slots",
     "rope_paged_cache",
+    "QuantizedPages",
+    "quantized_pages",
+    "rope_quantized_cache",
+    "read_quantized_cache",
+    "batch_invariant_quantized_paged_attention",
+    "batch_invariant_shared_prefix_attention",
 ]

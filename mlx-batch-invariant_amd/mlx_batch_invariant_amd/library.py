@@ -32,6 +32,15 @@ Operators (each the same computation, and bits, as the Python function named):
 * ``rope_paged_cache(q, k, v, cos, sin, positions, slots, k_pages!, v_pages!,
   sections)``: the rotated queries, the pools changed in place.
 
+* ``rope_quantized_cache(q, k, v, cos, sin, positions, slots, k_codes!, k_groups!,
+  v_codes!, v_groups!, bits, group_size, sections)``, ``read_quantized_cache(k_codes,
+  k_groups, v_codes, v_groups, block_table, kv_lens, bits, group_size)`` and
+  ``quantized_paged_attention(q, k_codes, k_groups, v_codes, v_groups, block_table,
+  kv_lens, bits, group_size, scale, causal, shared_starts, shared_lens)``: the pools of
+  a quantized paged cache, tensor by tensor;
+* ``shared_prefix_attention(q, k_pages, v_pages, block_table, kv_lens, scale, causal,
+  shared_starts, shared_lens)``: ``batch_invariant_shared_prefix_attention``.
+
 The ops have no autograd formula (inference kernels, as in the reference).
 """
 
@@ -179,4 +188,67 @@ def scored_paged_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_ta
 @scored_paged_attention.register_fake
 def _scored_paged_attention_fake(q, k_pages, v_pages, block_table, kv_lens, scale, causal, softcap, slopes, doc_ids,
                                  prefix_lens):
+    return q.new_empty(q.shape)
+
+
+@torch.library.custom_op(f"{NAMESPACE}::rope_quantized_cache", mutates_args=("k_codes", "k_groups", "v_codes", "v_groups"))
+def rope_quantized_cache(q: Tensor, k: Tensor, v: Tensor, cos: Tensor, sin: Tensor, positions: Tensor, slots: Tensor,
+                         k_codes: Tensor, k_groups: Tensor, v_codes: Tensor, v_groups: Tensor, bits: int,
+                         group_size: int, sections: Optional[list[int]]) -> Tensor:
+    return _k.rope_quantized_cache(q, k, v, cos, sin, positions, slots,
+                                   _k.QuantizedPages(k_codes, k_groups, bits, group_size),
+                                   _k.QuantizedPages(v_codes, v_groups, bits, group_size), sections=sections)
+
+
+@rope_quantized_cache.register_fake
+def _rope_quantized_cache_fake(q, k, v, cos, sin, positions, slots, k_codes, k_groups, v_codes, v_groups, bits,
+                               group_size, sections):
+    B, T, H, D = q.shape
+    return q.new_empty((B, H, T, D))
+
+
+@torch.library.custom_op(f"{NAMESPACE}::read_quantized_cache", mutates_args=())
+def read_quantized_cache(k_codes: Tensor, k_groups: Tensor, v_codes: Tensor, v_groups: Tensor, block_table: Tensor,
+                         kv_lens: Optional[Tensor], bits: int, group_size: int) -> Tensor:
+    """Keys and values as one tensor [2, B, Hkv, L, D] (an operator's outputs share no memory)."""
+    k, v = _k.read_quantized_cache(_k.QuantizedPages(k_codes, k_groups, bits, group_size),
+                                   _k.QuantizedPages(v_codes, v_groups, bits, group_size), block_table, kv_lens)
+    return k._base if k._base is not None else torch.stack([k, v])
+
+
+@read_quantized_cache.register_fake
+def _read_quantized_cache_fake(k_codes, k_groups, v_codes, v_groups, block_table, kv_lens, bits, group_size):
+    _, H, page, W = k_codes.shape
+    B, cols = block_table.shape
+    return k_groups.new_empty((2, B, H, cols * page, W * 8 // bits))
+
+
+@torch.library.custom_op(f"{NAMESPACE}::quantized_paged_attention", mutates_args=())
+def quantized_paged_attention(q: Tensor, k_codes: Tensor, k_groups: Tensor, v_codes: Tensor, v_groups: Tensor,
+                              block_table: Tensor, kv_lens: Optional[Tensor], bits: int, group_size: int,
+                              scale: float, causal: bool, shared_starts: Optional[Tensor],
+                              shared_lens: Optional[Tensor]) -> Tensor:
+    return _k.batch_invariant_quantized_paged_attention(
+        q, _k.QuantizedPages(k_codes, k_groups, bits, group_size), _k.QuantizedPages(v_codes, v_groups, bits, group_size),
+        block_table, kv_lens, scale=scale, mask="causal" if causal else None, shared_starts=shared_starts,
+        shared_lens=shared_lens)
+
+
+@quantized_paged_attention.register_fake
+def _quantized_paged_attention_fake(q, k_codes, k_groups, v_codes, v_groups, block_table, kv_lens, bits, group_size, scale,
+                                    causal, shared_starts, shared_lens):
+    return q.new_empty(q.shape)
+
+
+@torch.library.custom_op(f"{NAMESPACE}::shared_prefix_attention", mutates_args=())
+def shared_prefix_attention(q: Tensor, k_pages: Tensor, v_pages: Tensor, block_table: Tensor, kv_lens: Optional[Tensor],
+                            scale: float, causal: bool, shared_starts: Optional[Tensor],
+                            shared_lens: Tensor) -> Tensor:
+    return _k.batch_invariant_shared_prefix_attention(q, k_pages, v_pages, block_table, kv_lens, scale=scale,
+                                                      mask="causal" if causal else None, shared_starts=shared_starts,
+                                                      shared_lens=shared_lens)
+
+
+@shared_prefix_attention.register_fake
+def _shared_prefix_attention_fake(q, k_pages, v_pages, block_table, kv_lens, scale, causal, shared_starts, shared_lens):
     return q.new_empty(q.shape)

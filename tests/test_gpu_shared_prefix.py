@@ -1,0 +1,241 @@
+"""Attention of sequences that share prefixes: the bits of the plain paged attention,
+whatever the groups; the others' table entries of shared splits are not read."""
+
+import pytest
+import torch
+
+import paged_ref as ref
+from helpers import DT, gen, randn
+from test_gpu_quantized_cache import random_pool
+
+pytestmark = pytest.mark.gpu
+I32 = torch.int32
+
+
+def _bi():
+    import mlx_batch_invariant_amd as bi
+    return bi
+
+
+def _case(sizes, shared, own, page, g, lead=0, tail=0):
+    """A table of groups of `sizes` sequences whose first shared[n] keys (rounded down to whole
+    pages) are the same pages, `lead` and `tail` sequences in no group around them; `own`: each
+    sequence's further keys. Returns table, lens, starts, pages."""
+    B, rows, at = lead + sum(sizes) + tail, [], 0
+    cols = (max(shared, default=0) + max(own)) // page + 2
+    group = [-1] * lead + [n for n, s in enumerate(sizes) for _ in range(s)] + [-1] * tail
+    first = {}
+    lens = []
+    for b in range(B):
+        n = group[b]
+        keep = shared[n] // page if n >= 0 else 0
+        row = list(range(at, at + cols))
+        at += cols
+        if n >= 0:
+            row[:keep] = first.setdefault(n, row)[:keep]
+        rows.append(row)
+        lens.append(keep * page + own[b % len(own)])
+    order = torch.randperm(at, generator=g)
+    starts = [lead]
+    for s in sizes:
+        starts.append(starts[-1] + s)
+    whole = [s // page * page for s in shared]
+    return order[torch.tensor(rows)].to(I32), torch.tensor(lens, dtype=I32), starts, whole, at
+
+
+def _pools(n, Hkv, page, D, dt, g, nbits):
+    if nbits:
+        return [random_pool(n, Hkv, page, D, nbits, 32, dt, g) for _ in range(2)]
+    return [randn((n, Hkv, page, D), DT[dt], g) for _ in range(2)]
+
+
+def _calls(nbits, q, kp, vp, table, lens, mask, **shared):
+    bi = _bi()
+    if nbits:
+        call = bi.batch_invariant_quantized_paged_attention
+        return call(q, kp, vp, table, lens, mask=mask, **shared), call(q, kp, vp, table, lens, mask=mask)
+    return (bi.batch_invariant_shared_prefix_attention(q, kp, vp, table, lens, mask=mask, **shared),
+            bi.batch_invariant_paged_attention(q, kp, vp, table, lens, mask=mask))
+
+
+dev = lambda x: torch.tensor(x, dtype=I32, device="cuda")
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("nbits", [0, 8, 4])
+@pytest.mark.parametrize("T", [1, 4])
+@pytest.mark.parametrize("sizes,shared,lead,tail", [([9], [1024], 0, 0), ([2, 1, 5], [600, 900, 256], 1, 2), ([3, 0, 4], [255, 70, 1300], 0, 1),
+                                                    ([40], [512], 3, 0)])
+def test_bits(dt, nbits, T, sizes, shared, lead, tail):
+    g = gen(sum(sizes) + T)
+    page, D = 16, 64
+    table, lens, starts, whole, n = _case(sizes, shared, [5, 300, 17, 256, 4], page, g, lead, tail)
+    kp, vp = _pools(n, 2, page, D, dt, g, nbits)
+    q = randn((len(lens), 6, T, D), DT[dt], g, 2.0)
+    got, want = _calls(nbits, q, kp, vp, table.cuda(), lens.cuda(), "causal", shared_starts=dev(starts), shared_lens=dev(whole))
+    assert torch.equal(got, want)
+    got, want = _calls(nbits, q, kp, vp, table.cuda(), lens.cuda(), None, shared_starts=dev(starts), shared_lens=dev(whole))
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("D", [32, 96, 128, 192, 256])
+@pytest.mark.parametrize("Hq,Hkv,page", [(4, 1, 64), (3, 3, 1), (34, 2, 256)])
+def test_head_dims(dt, D, Hq, Hkv, page):
+    g = gen(D + Hq)
+    table, lens, starts, whole, n = _case([5], [768], [40, 1], page, g)
+    kp, vp = _pools(n, Hkv, page, D, dt, g, 0)
+    q = randn((5, Hq, 1, D), DT[dt], g)
+    got, want = _calls(0, q, kp, vp, table.cuda(), lens.cuda(), None, shared_lens=whole[0])
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("nbits", [0, 8])
+def test_pages_of_others_are_not_read(nbits):
+    """Only the group's first sequence needs the shared splits' table entries."""
+    g = gen(77)
+    page, D = 16, 64
+    table, lens, starts, whole, n = _case([6], [700], [30, 200], page, g)
+    kp, vp = _pools(n, 2, page, D, "bf16", g, nbits)
+    q = randn((6, 8, 2, D), torch.bfloat16, g)
+    _, want = _calls(nbits, q, kp, vp, table.cuda(), lens.cuda(), "causal", shared_lens=whole[0])
+    table[1:, :512 // page] = -1
+    got, _ = _calls(nbits, q, kp, vp, table.cuda(), lens.cuda(), "causal", shared_lens=dev([whole[0]]))
+    assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("starts,shared", [([0, 4, 2, 8], [512, 512, 512]), ([-5, 3, 99], [1 << 30, -4]), ([7, 7, 7], [512, 512]),
+                                           ([3, 1], [512]), ([0, 8], [100000])])
+def test_odd_groups(starts, shared):
+    """Starts that fall, repeat or lie outside the batch, lengths past the keys: with tables that
+    are the same everywhere, the plain bits."""
+    g = gen(5)
+    page, D = 16, 64
+    table, lens, _, _, n = _case([8], [1024], [9, 100, 500], page, g)
+    lens[2], lens[5] = 0, 300
+    kp, vp = _pools(n, 2, page, D, "f16", g, 0)
+    q = randn((8, 4, 3, D), torch.float16, g)
+    got, want = _calls(0, q, kp, vp, table.cuda(), lens.cuda(), "causal", shared_starts=dev(starts), shared_lens=dev(shared))
+    assert torch.equal(got, want)
+
+
+def test_first_sequence_holds_less():
+    """A first sequence shorter than the shared length: what it lacks comes from each one's own pages."""
+    g = gen(6)
+    page, D = 16, 64
+    table, lens, _, whole, n = _case([4], [1024], [9, 100], page, g)
+    lens[0] = 300
+    kp, vp = _pools(n, 2, page, D, "bf16", g, 0)
+    q = randn((4, 4, 1, D), torch.bfloat16, g)
+    got, want = _calls(0, q, kp, vp, table.cuda(), lens.cuda(), None, shared_lens=1024)
+    assert torch.equal(got, want)
+
+
+def test_many_groups():
+    """More groups and sequences than the plan's workgroup has threads."""
+    g = gen(7)
+    sizes = [1 + i % 3 for i in range(1300)]
+    table, lens, starts, whole, n = _case(sizes, [256] * 1300, [3, 40], 256, g)
+    table = table[:, :3].contiguous()
+    kp, vp = _pools(n, 1, 256, 32, "bf16", g, 4)
+    q = randn((len(lens), 2, 1, 32), torch.bfloat16, g)
+    got, want = _calls(4, q, kp, vp, table.cuda(), lens.cuda(), None, shared_starts=dev(starts), shared_lens=dev(whole))
+    assert torch.equal(got, want)
+
+
+def test_many_rows():
+    """Chunks of many rows: the kernels that walk, the same bits."""
+    for nbits in (0, 8):
+        g = gen(8)
+        table, lens, starts, whole, n = _case([6], [1024], [500, 300], 16, g)
+        kp, vp = _pools(n, 2, 16, 64, "bf16", g, nbits)
+        q = randn((6, 8, 200, 64), torch.bfloat16, g)
+        got, want = _calls(nbits, q, kp, vp, table.cuda(), lens.cuda(), "causal", shared_lens=whole[0])
+        assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+def test_values(dt):
+    g = gen(9)
+    table, lens, starts, whole, n = _case([5], [512], [9, 100], 16, g)
+    kp, vp = _pools(n, 2, 16, 64, dt, g, 0)
+    q = randn((5, 4, 2, 64), DT[dt], g)
+    got, _ = _calls(0, q, kp, vp, table.cuda(), lens.cuda(), "causal", shared_lens=whole[0])
+    k, v = (p.cpu()[table.long()].transpose(1, 2).reshape(5, 2, -1, 64) for p in (kp, vp))
+    want, absv, dot, bias = ref.attention(q.cpu(), k, v, 64 ** -0.5, lens, True)
+    assert ((got.cpu().double() - want).abs() <= ref.attention_allowance(want, absv, dot, bias, DT[dt], 64, 3)).all()
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("D", [64, 256])
+def test_not_finite(dt, D):
+    """Infinities and NaN behind sequences and in hidden keys take no part; seen ones come out in their dim."""
+    bi, g = _bi(), gen(10)
+    page, inf = 16, float("inf")
+    table, lens, _, whole, n = _case([3], [512], [40, 60], page, g)
+    kp, vp = _pools(n, 1, page, D, dt, g, 0)
+    q = randn((3, 2, 4, D), DT[dt], g)
+    call = lambda: bi.batch_invariant_shared_prefix_attention(q, kp, vp, table.cuda(), lens.cuda(), mask="causal", shared_lens=512)
+    clean = call()
+    for b in range(3):
+        for p in range(int(lens[b]), table.shape[1] * page):
+            kp[table[b, p // page], :, p % page] = float("nan")
+            vp[table[b, p // page], :, p % page] = inf
+    assert torch.equal(call(), clean)
+    want = clean.clone()
+    p = int(lens[1]) - 2                                  # seen by the last two of sequence 1's tokens
+    vp[table[1, p // page], 0, p % page, 3] = -inf
+    want[1, :, 2:, 3] = -inf
+    p = int(lens[2]) - 1
+    vp[table[2, p // page], 0, p % page, 5] = inf
+    vp[table[2, 0], 0, 7, 5] = -inf                        # a shared key: every row sees it
+    want[:, :, :, 5] = -inf
+    want[2, :, 3, 5] = float("nan")
+    got = call()
+    assert torch.equal(torch.isnan(got), torch.isnan(want))
+    assert torch.equal(torch.nan_to_num(got.float(), 0, 9, -9), torch.nan_to_num(want.float(), 0, 9, -9))
+    q[0, 0, 1, 0] = float("nan")
+    got = call()
+    assert torch.isnan(got[0, 0, 1]).all() and not torch.isnan(got[0, 1]).any()
+
+
+def test_graph_with_changing_groups():
+    """One captured call serves other groups, lengths and tables; every replay has the eager bits."""
+    bi, g = _bi(), gen(11)
+    page, D, B = 16, 64, 8
+    kp, vp = _pools(900, 2, page, D, "bf16", g, 0)
+    qp = _pools(900, 2, page, D, "bf16", g, 8)
+    q = randn((B, 8, 1, D), torch.bfloat16, g)
+    cases = []
+    for sizes, shared in (([8], [1024]), ([3, 5], [512, 768]), ([2, 2], [256, 1024])):
+        table, lens, starts, whole, _ = _case(sizes, shared, [9, 100], page, g, tail=B - sum(sizes))
+        starts, whole = (starts + [starts[-1]] * 2)[:3], (whole + [0])[:2]
+        full = torch.zeros(B, 72, dtype=I32)
+        full[:, :table.shape[1]] = table
+        cases.append([full.cuda(), lens.cuda(), dev(starts), dev(whole)])
+    held = [t.clone() for t in cases[0]]
+
+    def step():
+        more = dict(shared_starts=held[2], shared_lens=held[3])
+        return (bi.batch_invariant_shared_prefix_attention(q, kp, vp, *held[:2], **more),
+                bi.batch_invariant_quantized_paged_attention(q, *qp, *held[:2], **more),
+                bi.batch_invariant_quantized_paged_attention(q, *qp, *held[:2]))
+
+    step()
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        step()
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for case in cases + cases[:2]:
+        for h, c in zip(held, case):
+            h.copy_(c)
+        graph.replay()
+        torch.cuda.synchronize()
+        for x, y in zip(out, step()):
+            assert torch.equal(x, y)
+        want = bi.batch_invariant_paged_attention(q, kp, vp, *held[:2])
+        assert torch.equal(out[0], want) and torch.equal(out[1], out[2])
