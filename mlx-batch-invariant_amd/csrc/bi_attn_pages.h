@@ -21,6 +21,37 @@ __device__ __forceinline__ int pages_len(const PagesArgs& a, int b) {
   return a.kv_lens ? min(max(a.kv_lens[b], 0), a.L) : a.L;
 }
 
+// The same of a wave-uniform sequence, by a scalar load: waiting for it does not wait
+// for the vector loads in flight, which return in order.
+__device__ __forceinline__ int pages_len_uniform(const PagesArgs& a, int b) {
+  if (!a.kv_lens) return a.L;
+  return min(max(load_uniform_i32(a.kv_lens + __builtin_amdgcn_readfirstlane(b)), 0), a.L);
+}
+
+// The operands of a P.V step in LDS, the two halves of a lane 64 lanes apart.
+template <typename T>
+__device__ __forceinline__ void store_pfrag(u32x4* p, const PFrag<T>& pf) {
+  if constexpr (sizeof(T) == 2) {
+    p[0] = __builtin_bit_cast(u32x4, pf.hi);
+    p[kWave] = __builtin_bit_cast(u32x4, pf.lo);
+  } else {
+    p[0] = __builtin_bit_cast(u32x4, pf.f.lo);
+    p[kWave] = __builtin_bit_cast(u32x4, pf.f.hi);
+  }
+}
+template <typename T>
+__device__ __forceinline__ PFrag<T> load_pfrag(const u32x4* p) {
+  PFrag<T> pf;
+  if constexpr (sizeof(T) == 2) {
+    pf.hi = __builtin_bit_cast(typename Frag<T>::type, p[0]);
+    pf.lo = __builtin_bit_cast(typename Frag<T>::type, p[kWave]);
+  } else {
+    pf.f.lo = __builtin_bit_cast(f32x4, p[0]);
+    pf.f.hi = __builtin_bit_cast(f32x4, p[kWave]);
+  }
+  return pf;
+}
+
 // ---------------------------------------------------------------------------
 // The plan of a call with shared prefixes: segments (groups, then sequences) with
 // the first item of each, and how many 16-row chunks an item takes. One workgroup.
@@ -152,16 +183,14 @@ static __global__ __launch_bounds__(kPlanThreads) void pages_plan_kernel(PagesAr
 // of the split (K in registers, dequantized there), the maxima are exchanged
 // through LDS, each wave leaves its keys' weights there as the operands of the
 // P.V steps, and wave w computes the dims 16 dt, dt = NJ w .. NJ w + NJ - 1, from
-// the split's V in LDS. BITS 0: rows of T; 8 or 4: codes. MULTI: items of several
-// chunks, from the plan; else one chunk of at most 16 rows a sequence, and each
-// workgroup finds its items from the lengths.
+// the split's V in LDS. BITS 0: rows of T; 8 or 4: codes.
 // ---------------------------------------------------------------------------
 template <typename T, int D>
 constexpr int pages_v_slices() {
   return (kSplit * D * (int)sizeof(T) + (128 << 10) - 1) >> 17;
 }
 
-template <typename T, int D, int BITS, bool MULTI>
+template <typename T, int D, int BITS>
 __global__ __launch_bounds__(256) void attn_pages(PagesArgs a) {
   typedef typename Frag<T>::type F;
   constexpr int NVP = pages_v_slices<T, D>();
@@ -187,69 +216,33 @@ __global__ __launch_bounds__(256) void attn_pages(PagesArgs a) {
   // chunks of one split, and the heads of one page, share its cache.
   const int w0 = (int)(blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8);
 
-  int per = 1, items = 0;
-  int c64 = -1, lo = 0, hi = 0, incl = 0;                 // MULTI: segments 64 c64 .., else sequences
-  const int nseg = MULTI ? a.groups + a.B : a.B;
-  if constexpr (MULTI) {
-    items = a.plan[0];
-    per = a.plan[1];
-  }
-  for (int item = w0;; item += (int)gridDim.x) {
-    int seq0, nseq, split, hk, chunk0;
-    if constexpr (MULTI) {
-      if (item >= items) break;
-      // the last segment that starts at or before the item (ones without items share a start with the next)
-      const int32_t* seg = a.plan + 2;
-      int at = 0;
-      for (int step = 1 << (31 - __builtin_clz(nseg)); step > 0; step >>= 1)
-        if (at + step < nseg && seg[(int64_t)(at + step) * kPlanWords] <= item) at += step;
-      at = __builtin_amdgcn_readfirstlane(at);
-      const int32_t* s = seg + (int64_t)at * kPlanWords;
-      seq0 = s[1];
-      nseq = s[2];
-      const int runs = (int)(((int64_t)nseq * rows1 + 16 * per - 1) / (16 * per));
-      int local = item - s[0];
-      const int x = local / runs;
-      chunk0 = (local - x * runs) * per;
-      hk = x % a.Hkv;
-      split = s[3] + x / a.Hkv;
-    } else {
-      while (item >= hi && 64 * (c64 + 1) < nseg) {
-        ++c64;
-        const int b = 64 * c64 + lane;
-        incl = b < nseg ? (direct ? 1 : (pages_len(a, b) + kSplit - 1) / kSplit) * a.Hkv : 0;
-#pragma unroll
-        for (int off = 1; off < kWave; off <<= 1) {
-          const int up = __shfl_up(incl, off, kWave);
-          if (lane >= off) incl += up;
-        }
-        lo = hi;
-        hi = lo + __builtin_amdgcn_readlane(incl, 63);
-      }
-      if (item >= hi) break;
-      const int i = __popcll(__ballot(lo + incl <= item));
-      seq0 = 64 * c64 + i;
-      nseq = 1;
-      chunk0 = 0;
-      const int local = item - lo - (i ? __builtin_amdgcn_readlane(incl, max(i - 1, 0)) : 0);
-      hk = local % a.Hkv;
-      split = local / a.Hkv;
-    }
+  const int items = a.plan[0], per = a.plan[1], nseg = a.groups + a.B;
+  const int32_t* seg = a.plan + 2;
+  for (int item = w0; item < items; item += (int)gridDim.x) {
+    // the last segment that starts at or before the item (ones without items share a start with the next)
+    int at = 0;
+    for (int step = 1 << (31 - __builtin_clz(nseg)); step > 0; step >>= 1)
+      if (at + step < nseg && seg[(int64_t)(at + step) * kPlanWords] <= item) at += step;
+    at = __builtin_amdgcn_readfirstlane(at);
+    const int32_t* sg = seg + (int64_t)at * kPlanWords;
+    int seq0 = sg[1];
+    const int nseq = sg[2];
+    const int runs = (int)(((int64_t)nseq * rows1 + 16 * per - 1) / (16 * per));
+    const int local = item - sg[0], x = local / runs;
+    const int chunk0 = (local - x * runs) * per;
+    int hk = x % a.Hkv, split = sg[3] + x / a.Hkv;
     seq0 = __builtin_amdgcn_readfirstlane(seq0);
     hk = __builtin_amdgcn_readfirstlane(hk);
     split = __builtin_amdgcn_readfirstlane(split);
     const int nrows = nseq * rows1;                       // of the segment
     const int j0 = split * kSplit;
-    const int len0 = __builtin_amdgcn_readfirstlane(pages_len(a, seq0));
+    const int len0 = pages_len_uniform(a, seq0);
     const int n_act = min(kSplit, len0 - j0);
     // Row p of the segment: its index among the outputs, the keys of the split that it may see.
     auto row_of = [&](int p, int& b, int& h, int& t) {
-      b = seq0;
-      if (MULTI) {
-        const int x = p / rows1;
-        b += x;
-        p -= x * rows1;
-      }
+      const int x = p / rows1;
+      b = seq0 + x;
+      p -= x * rows1;
       t = p / G;
       h = hk * G + p - t * G;
     };
@@ -332,7 +325,7 @@ __global__ __launch_bounds__(256) void attn_pages(PagesArgs a) {
     };
     if constexpr (NVP == 1) copy_v(0);
 
-    const int chunks = MULTI ? min(per, (nrows - 16 * chunk0 + 15) / 16) : 1;
+    const int chunks = min(per, (nrows - 16 * chunk0 + 15) / 16);
     for (int c = 0; c < chunks; ++c) {
       const int chunk = chunk0 + c;
       // This lane's row of the scores.
@@ -342,14 +335,14 @@ __global__ __launch_bounds__(256) void attn_pages(PagesArgs a) {
         if (p < nrows) {
           int b, h, t;
           row_of(p, b, h, t);
-          const int len = MULTI ? pages_len(a, b) : len0;
+          const int len = pages_len(a, b);
           lim = (a.causal ? len - a.Tq + t + 1 : len) - j0;
           row = (b * a.Hq + h) * a.Tq + t;
         }
       }
       const bool any = __ballot(lim > 0) != 0;            // (the same in every wave)
       if (!any && !direct) {
-        if (MULTI && c + 1 < chunks) q_frags(chunk + 1, qf);
+        if (c + 1 < chunks) q_frags(chunk + 1, qf);
         continue;
       }
       float s[KT][4];
@@ -365,7 +358,7 @@ __global__ __launch_bounds__(256) void attn_pages(PagesArgs a) {
           m = fmaxf(m, s[t][i]);
         }
       }
-      if (MULTI && c + 1 < chunks) q_frags(chunk + 1, qf);
+      if (c + 1 < chunks) q_frags(chunk + 1, qf);
       m = quarter_max(m);
       if (qq == 0) mx[wave][r] = m;
       __syncthreads();
@@ -377,13 +370,7 @@ __global__ __launch_bounds__(256) void attn_pages(PagesArgs a) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) p8[e] = __builtin_amdgcn_exp2f(s[2 * h + e / 4][e % 4] - msub);
         const PFrag<T> pf = make_pfrag<T>(p8);
-        if constexpr (sizeof(T) == 2) {
-          Ps[2 * wave + h][0][lane] = __builtin_bit_cast(u32x4, pf.hi);
-          Ps[2 * wave + h][1][lane] = __builtin_bit_cast(u32x4, pf.lo);
-        } else {
-          Ps[2 * wave + h][0][lane] = __builtin_bit_cast(u32x4, pf.f.lo);
-          Ps[2 * wave + h][1][lane] = __builtin_bit_cast(u32x4, pf.f.hi);
-        }
+        store_pfrag<T>(&Ps[2 * wave + h][0][lane], pf);
       }
       if (!direct && wave == 0 && qq == 0 && lim > 0) a.pm[(int64_t)row * a.nsplit + split] = m;
       int arow[4], alim[4];                               // the rows of the accumulators, 4 qq + i
@@ -392,18 +379,6 @@ __global__ __launch_bounds__(256) void attn_pages(PagesArgs a) {
         arow[i] = __shfl(row, 4 * qq + i, kWave);
         alim[i] = __shfl(lim, 4 * qq + i, kWave);
       }
-      auto p_frag = [&](int ks) {
-        PFrag<T> pf;
-        const u32x4 x0 = Ps[ks][0][lane], x1 = Ps[ks][1][lane];
-        if constexpr (sizeof(T) == 2) {
-          pf.hi = __builtin_bit_cast(F, x0);
-          pf.lo = __builtin_bit_cast(F, x1);
-        } else {
-          pf.f.lo = __builtin_bit_cast(f32x4, x0);
-          pf.f.hi = __builtin_bit_cast(f32x4, x1);
-        }
-        return pf;
-      };
       const int sum_wave = c & 3;                         // which wave adds up the weights
       f32x4 lsum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -420,7 +395,7 @@ __global__ __launch_bounds__(256) void attn_pages(PagesArgs a) {
           for (int j = 0; j < NJ; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll 2
           for (int ks = 0; ks < kSplit / 32; ++ks) {
-            const PFrag<T> pf = p_frag(ks);
+            const PFrag<T> pf = load_pfrag<T>(&Ps[ks][0][lane]);
 #pragma unroll
             for (int j = 0; j < NJ; ++j) {
               if (NJ * wave + j >= NDTV) continue;
@@ -476,6 +451,440 @@ __global__ __launch_bounds__(256) void attn_pages(PagesArgs a) {
       }
     }
     __syncthreads();                                      // every wave is done with Vs, pg before the next item's
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Codes, at most 16 rows a sequence and kv head (a decode step, a few draft tokens):
+// the codes of V stay codes in LDS. One 256-thread workgroup per item (sequence,
+// split, kv head), neighbouring items on one XCD. Wave w's keys are 64 w .. 64 w + 63
+// of the split, lane l's page that of key 64 w + l (read an item ahead), so that a
+// wave finds all its rows by lane exchanges; it scores them with K dequantized in
+// registers. For P.V wave w takes the dims 16 dt, dt = NJ w .. NJ w + NJ - 1: a
+// transposing LDS read gives a lane the codes of 8 keys (4 bits: 16) of one dim, and
+// each is dequantized once, with its key's pair from LDS.
+// ---------------------------------------------------------------------------
+// The tile of V's codes: row r, 16-byte chunk c in slot c ^ key(r) where a row holds a
+// power of two of them, so that the rows of a transposing read (32 keys, one chunk)
+// fall in distinct banks.
+template <int D, int BITS>
+struct CodeTile {
+  static constexpr int kRowBytes = D * BITS / 8;
+  static constexpr int kCPR = kRowBytes / 16;
+  static constexpr bool kSwz = (kCPR & (kCPR - 1)) == 0;
+  static __device__ __forceinline__ int key(int r) {
+    const int x = (r & 7) | (r >> 4 & 1) << 3;
+    return !kSwz ? 0 : kCPR == 16 ? x : kCPR == 8 ? x >> 1 : kCPR == 4 ? x >> 2 : kCPR == 2 ? x >> 3 : 0;
+  }
+  static __device__ __forceinline__ int off(int r, int c) { return r * kRowBytes + ((c ^ key(r)) << 4); }
+};
+
+typedef int i32x2_t __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) i32x2_t lds_i32x2;
+// (restrict: see lds_read_tr16)
+__device__ __forceinline__ i32x2_t lds_read_tr8(lds_i32x2* __restrict p) { return __builtin_amdgcn_ds_read_tr8_b64_v2i32(p); }
+__device__ __forceinline__ i32x2_t lds_read_tr4(lds_i32x2* __restrict p) { return __builtin_amdgcn_ds_read_tr4_b64_v2i32(p); }
+
+// The codes of K row r that lane (r, qq) needs as score operands, dims 32 st + 8 qq .. + 7
+// of every step st, are pieces of 8 or 4 bytes. A lane reads longer ones instead, the
+// steps four at a time (lane qq those of step qq whole) or two (half a step), and the
+// four lanes of a row hand each other their pieces by swaps of 16-lane rows.
+__device__ __forceinline__ void swap32(uint32_t& x, uint32_t& y) {   // x's upper 32 lanes for y's lower 32
+  const auto p = __builtin_amdgcn_permlane32_swap(x, y, false, false);
+  x = p[0];
+  y = p[1];
+}
+__device__ __forceinline__ void swap16(uint32_t& x, uint32_t& y) {   // x's odd rows for y's even rows
+  const auto p = __builtin_amdgcn_permlane16_swap(x, y, false, false);
+  x = p[0];
+  y = p[1];
+}
+template <int KS, int BITS>
+struct KRow {
+  static constexpr int kW = BITS / 4;                     // words of a piece
+  uint32_t w[KS][kW];
+  __device__ __forceinline__ void load(const char* row, int qq) {
+    int st = 0;
+#pragma unroll
+    for (; st + 4 <= KS; st += 4) {                       // 4 pieces: 16 or 32 bytes
+#pragma unroll
+      for (int h = 0; h < kW; ++h) {
+        const u32x4 x = *reinterpret_cast<const u32x4*>(row + 4 * BITS * st + 4 * BITS * qq + 16 * h);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[st + (4 * h + i) / kW][(4 * h + i) % kW] = x[i];
+      }
+    }
+    if constexpr (KS % 4 >= 2) {                          // 2 pieces: 8 or 16 bytes
+      const char* p = row + 4 * BITS * st + 2 * BITS * qq;
+      if constexpr (BITS == 8) {
+        const u32x4 x = *reinterpret_cast<const u32x4*>(p);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) w[st + i / 2][i % 2] = x[i];
+      } else {
+        const u32x2 x = *reinterpret_cast<const u32x2*>(p);
+        w[st][0] = x[0];
+        w[st + 1][0] = x[1];
+      }
+      st += 2;
+    }
+    if constexpr (KS % 2 == 1) {
+      const Codes8<BITS> c = load_codes8<BITS>(row + 4 * BITS * st + BITS * qq);
+#pragma unroll
+      for (int i = 0; i < kW; ++i) w[st][i] = c.w[i];
+    }
+  }
+  __device__ __forceinline__ void arrange() {
+    int st = 0;
+#pragma unroll
+    for (; st + 4 <= KS; st += 4)
+#pragma unroll
+      for (int i = 0; i < kW; ++i) {
+        swap32(w[st][i], w[st + 2][i]);
+        swap32(w[st + 1][i], w[st + 3][i]);
+        swap16(w[st][i], w[st + 1][i]);
+        swap16(w[st + 2][i], w[st + 3][i]);
+      }
+    if constexpr (KS % 4 >= 2)
+#pragma unroll
+      for (int i = 0; i < kW; ++i) {
+        swap16(w[st][i], w[st + 1][i]);
+        swap32(w[st][i], w[st + 1][i]);
+      }
+  }
+  __device__ __forceinline__ Codes8<BITS> codes(int st) const {
+    Codes8<BITS> c;
+#pragma unroll
+    for (int i = 0; i < kW; ++i) c.w[i] = w[st][i];
+    return c;
+  }
+};
+
+// N words of memory that is 4-byte aligned.
+template <int N>
+__device__ __forceinline__ void load_words(const void* p, uint32_t* w) {
+  typedef uint32_t v4 __attribute__((ext_vector_type(4), aligned(4)));
+  typedef uint32_t v2 __attribute__((ext_vector_type(2), aligned(4)));
+  int i = 0;
+#pragma unroll
+  for (; i + 4 <= N; i += 4) {
+    const v4 x = *reinterpret_cast<const v4*>(static_cast<const char*>(p) + 4 * i);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) w[i + e] = x[e];
+  }
+  if constexpr (N % 4 >= 2) {
+    const v2 x = *reinterpret_cast<const v2*>(static_cast<const char*>(p) + 4 * i);
+    w[i] = x[0];
+    w[i + 1] = x[1];
+    i += 2;
+  }
+  if constexpr (N % 2 == 1) w[i] = *reinterpret_cast<const uint32_t*>(static_cast<const char*>(p) + 4 * i);
+}
+
+// Workgroups per CU that the registers are held to.
+template <typename T, int D>
+constexpr int codes_min_blocks() {
+  return sizeof(T) == 2 && D <= 128 ? 3 : 1;
+}
+
+template <typename T, int D, int BITS, int GS>
+__global__ __launch_bounds__(256, (codes_min_blocks<T, D>())) void attn_codes(PagesArgs a) {
+  typedef typename Frag<T>::type F;
+  typedef CodeTile<D, BITS> CT;
+  constexpr int KT = 4, KS = D / 32, NDT = D / 16, NJ = (NDT + 3) / 4;
+  constexpr int NCOPY = kSplit * CT::kCPR / 64 / 4;       // V copy instructions of a wave
+  constexpr int PW = sizeof(T) == 2 ? 1 : 2;              // words of a pair
+  constexpr int NG = D / GS;                              // groups of a row
+  // Pairs that a wave's dim tiles need: one where they share a group (two tiles from
+  // an even one on, four of 64 dims), else one for each or for two of them.
+  constexpr int NS = NJ == 3 ? 3 : NJ == 4 && GS == 32 ? 2 : 1;
+  __shared__ __attribute__((aligned(1024))) char Vs[kSplit * CT::kRowBytes];
+  __shared__ u32x4 Ps[8][2][kWave];
+  __shared__ float mx[4][16];
+  __shared__ __attribute__((aligned(16))) float vsc[NG][kSplit], vbi[NG][kSplit];   // V's scales and biases
+
+  const int tid = threadIdx.x;
+  const int lane = tid % kWave;
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int r = lane % 16, qq = lane / 16;
+  const int G = a.Hq / a.Hkv, rows1 = a.Tq * G;
+  // Row p of the sequence is column 4 (p % 4) + p / 4 of the scores, so that up to four
+  // rows are the first register of the accumulators' four lane rows.
+  const int my_p = r / 4 + r % 4 * 4;
+  const int ni = (rows1 + 3) / 4;                         // registers that hold rows
+  const bool direct = a.nsplit == 1;
+  const int page_mask = (1 << a.page_shift) - 1;
+  const int w0 = (int)(blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8);
+
+  // Item -> (sequence, split, kv head), found from the lengths 64 sequences at a time;
+  // a workgroup's items rise.
+  int c64 = -1, lo = 0, hi = 0, incl = 0;
+  struct Item { int b, split, hk, n_act; };               // n_act < 0: no more items
+  auto locate = [&](int item) -> Item {
+    while (item >= hi && 64 * (c64 + 1) < a.B) {
+      ++c64;
+      const int b = 64 * c64 + lane;
+      incl = b < a.B ? (direct ? 1 : (pages_len(a, b) + kSplit - 1) / kSplit) * a.Hkv : 0;
+#pragma unroll
+      for (int off = 1; off < kWave; off <<= 1) {
+        const int up = __shfl_up(incl, off, kWave);
+        if (lane >= off) incl += up;
+      }
+      lo = hi;
+      hi = lo + __builtin_amdgcn_readlane(incl, 63);
+    }
+    if (item >= hi) return Item{0, 0, 0, -1};
+    const int i = __popcll(__ballot(lo + incl <= item));
+    const int local = item - lo - (i ? __builtin_amdgcn_readlane(incl, max(i - 1, 0)) : 0);
+    Item it;
+    it.b = 64 * c64 + i;
+    it.split = local / a.Hkv;
+    it.hk = local - it.split * a.Hkv;
+    it.n_act = min(kSplit, pages_len_uniform(a, it.b) - it.split * kSplit);
+    return it;
+  };
+  auto page_of = [&](const Item& it) {
+    if (it.n_act <= 0) return 0;
+    const int pos = it.split * kSplit + min(tid, it.n_act - 1);
+    return a.table[(int64_t)it.b * a.table_stride + (pos >> a.page_shift)];
+  };
+
+  Item it = locate(w0);
+  int page = page_of(it);
+  for (int item = w0; it.n_act >= 0; item += (int)gridDim.x) {
+    const int b = it.b, hk = it.hk, j0 = it.split * kSplit, n_act = it.n_act, split = it.split;
+    const int my_page = clamp_page(page, a.num_pages);
+    // (token, head) p of the sequence, heads inside tokens.
+    auto out_row = [&](int p) { return (b * a.Hq + hk * G + p % G) * a.Tq + p / G; };
+    if (n_act == 0) {                                     // (direct, an empty sequence) no keys: zeros
+      for (int i = tid; i < rows1 * D; i += 256) static_cast<T*>(a.out)[(int64_t)out_row(i / D) * D + i % D] = (T)0.0f;
+      it = locate(item + (int)gridDim.x);
+      page = page_of(it);
+      continue;
+    }
+    const int total = pages_len_uniform(a, b);
+
+    // Memory requests: pairs of this lane's key, Q^T, K, V. A lane finds its own key's
+    // rows; the others' come by lane exchanges.
+    const uint32_t my_row = (j0 + min(tid, n_act - 1)) & page_mask;
+    auto row_off = [&](int64_t sp, int64_t sl) { return (uint64_t)(uint32_t)my_page * (uint32_t)sp + (uint64_t)my_row * (uint32_t)sl; };
+    const uint64_t k_off = row_off(a.k_sp, a.k_sl), v_off = row_off(a.v_sp, a.v_sl);
+    auto off_of = [&](uint64_t off, int l) {
+      return (uint64_t)(uint32_t)__shfl((int)(uint32_t)off, l, kWave) | (uint64_t)(uint32_t)__shfl((int)(uint32_t)(off >> 32), l, kWave) << 32;
+    };
+    uint32_t kp[NG][PW], vp[NG][PW];
+    {
+      const T* kg = static_cast<const T*>(a.kg) + hk * a.kg_sh + row_off(a.kg_sp, a.kg_sl);
+      const T* vg = static_cast<const T*>(a.vg) + hk * a.vg_sh + row_off(a.vg_sp, a.vg_sl);
+      load_words<NG * PW>(kg, &kp[0][0]);
+      load_words<NG * PW>(vg, &vp[0][0]);
+    }
+    F qf[KS];
+    {
+      const int p = min(my_p, rows1 - 1);
+      const T* qrow = static_cast<const T*>(a.q) + (int64_t)b * a.q_sb + (int64_t)(hk * G + p % G) * a.q_sh + (int64_t)(p / G) * a.q_st;
+#pragma unroll
+      for (int st = 0; st < KS; ++st) qf[st] = my_p < rows1 ? frag_load(qrow + 32 * st + 8 * qq) : frag_zero<F>();
+    }
+    KRow<KS, BITS> kc[KT];
+#pragma unroll
+    for (int t = 0; t < KT; ++t) kc[t].load(static_cast<const char*>(a.k) + hk * a.k_sh + off_of(k_off, 16 * t + r), qq);
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int c = 0; c < NCOPY; ++c) {
+      const int f = 64 * c + lane, row = f / CT::kCPR, slot = f - row * CT::kCPR;
+      const char* vr = static_cast<const char*>(a.v) + hk * a.v_sh + off_of(v_off, row);
+      copy_to_lds16(vr + ((slot ^ CT::key(64 * wave + row)) << 4), Vs + 1024 * (wave * NCOPY + c));
+    }
+    it = locate(item + (int)gridDim.x);                   // the next item's pages
+    page = page_of(it);
+
+    // V's pairs to LDS.
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      const Pair<T> x = unpack_pair<T>(vp[g]);
+      vsc[g][tid] = x.s;
+      vbi[g][tid] = x.b;
+    }
+    int lim = 0, row = -1;
+    if (my_p < rows1) {
+      lim = (a.causal ? total - a.Tq + my_p / G + 1 : total) - j0;
+      row = out_row(my_p);
+    }
+    float s[KT][4];
+    float m = -INFINITY;
+#pragma unroll
+    for (int t = 0; t < KT; ++t) {
+      f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+      Pair<T> g[NG];
+#pragma unroll
+      for (int i = 0; i < NG; ++i) {
+        uint32_t u[PW];
+#pragma unroll
+        for (int w = 0; w < PW; ++w) u[w] = (uint32_t)__shfl((int)kp[i][w], 16 * t + r, kWave);
+        g[i] = unpack_pair<T>(u);
+      }
+      kc[t].arrange();
+#pragma unroll
+      for (int st = 0; st < KS; ++st) acc = mfma_step(dequant_frag<T, BITS>(kc[t].codes(st), g[32 * st / GS]), qf[st], acc);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        s[t][i] = 64 * wave + 16 * t + 4 * qq + i < lim ? acc[i] * a.scale_log2 : -INFINITY;
+        m = fmaxf(m, s[t][i]);
+      }
+    }
+    m = quarter_max(m);
+    if (qq == 0) mx[wave][r] = m;
+    stage_barrier<63>();                                  // (V's copies may still be in flight)
+    m = fmaxf(fmaxf(mx[0][r], mx[1][r]), fmaxf(mx[2][r], mx[3][r]));
+    const float msub = m == -INFINITY ? 0.0f : m;         // no visible key: weights 0, not NaN
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      float p8[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) p8[e] = __builtin_amdgcn_exp2f(s[2 * h + e / 4][e % 4] - msub);
+      store_pfrag<T>(&Ps[2 * wave + h][0][lane], make_pfrag<T>(p8));
+    }
+    if (!direct && wave == 0 && qq == 0 && lim > 0) a.pm[(int64_t)row * a.nsplit + split] = m;
+    int arow[4], alim[4];                                 // the rows of the accumulators, 4 qq + i
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      arow[i] = -1;
+      alim[i] = 0;
+      if (i < ni) {
+        arow[i] = __shfl(row, 4 * qq + i, kWave);
+        alim[i] = __shfl(lim, 4 * qq + i, kWave);
+      }
+    }
+    stage_barrier<0>();                                   // V landed, weights and pairs visible
+
+    f32x4 acc[NJ], lsum = {0.f, 0.f, 0.f, 0.f};
+    // P.V of this wave's dim tiles; `clean` takes infinities and NaN of V as 0.
+    // The reads of a step are requested a step ahead, codes two steps.
+    struct Step {
+      PFrag<T> pf;
+      float s[NS][8], b[NS][8];
+    };
+    auto read_step = [&](Step& x, int ks) __attribute__((always_inline)) {
+      x.pf = load_pfrag<T>(&Ps[ks][0][lane]);
+#pragma unroll
+      for (int i = 0; i < NS; ++i) {
+        const int g = min((NJ * wave + (NJ == 3 ? 1 : 2) * i) * 16 / GS, NG - 1);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const f32x4 sx = *reinterpret_cast<const f32x4*>(&vsc[g][32 * ks + 16 * h + 4 * qq]);
+          const f32x4 bx = *reinterpret_cast<const f32x4*>(&vbi[g][32 * ks + 16 * h + 4 * qq]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            x.s[i][4 * h + e] = sx[e];
+            x.b[i][4 * h + e] = bx[e];
+          }
+        }
+      }
+    };
+    auto read_codes = [&](Codes8<BITS> (&c)[2][NJ], int k2) __attribute__((always_inline)) {
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const int dt = min(NJ * wave + j, NDT - 1);
+        if constexpr (BITS == 8) {
+          const int u = r >> 1, key = 64 * k2 + 4 * qq + (u & 3) + (u & 4) * 4;
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const i32x2_t w = lds_read_tr8((lds_i32x2*)(Vs + CT::off(key + 32 * h, dt) + 8 * (r & 1)));
+            c[h][j].w[0] = (uint32_t)w[0];
+            c[h][j].w[BITS / 4 - 1] = (uint32_t)w[1];
+          }
+        } else {
+          const int key = 64 * k2 + 32 * (r >> 3) + 4 * qq + (r & 3) + (r & 4) * 4;
+          const i32x2_t w = lds_read_tr4((lds_i32x2*)(Vs + CT::off(key, dt >> 1) + 8 * (dt & 1)));
+          c[0][j].w[0] = (uint32_t)w[0];
+          c[1][j].w[0] = (uint32_t)w[1];
+        }
+      }
+    };
+    auto step_of = [&](const Step& x, const Codes8<BITS> (&c)[NJ], bool clean) __attribute__((always_inline)) {
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
+        const int i = NS == 1 ? 0 : j / (NJ == 3 ? 1 : 2);
+        F v = dequant_frag8<T, BITS>(c[j], x.s[i], x.b[i]);
+        if (clean) v = finite_frag(v);
+        acc[j] = pv_step<T>(x.pf, v, acc[j]);             // (a wave without a tile computes the last one, unused)
+      }
+    };
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    {
+      Step st[2];
+      Codes8<BITS> vc[2][2][NJ];
+      read_codes(vc[0], 0);
+      read_step(st[0], 0);
+#pragma unroll
+      for (int ks = 0; ks < kSplit / 32; ++ks) {
+        if (ks % 2 == 0 && ks + 2 < kSplit / 32) read_codes(vc[(ks / 2 + 1) % 2], ks / 2 + 1);
+        if (ks + 1 < kSplit / 32) read_step(st[(ks + 1) % 2], ks + 1);
+        step_of(st[ks % 2], vc[ks / 2 % 2][ks % 2], false);
+      }
+    }
+    const int sum_wave = NDT < 4 * NJ ? 3 : 0;            // (the wave with the fewest dims adds up the weights)
+    if (wave == sum_wave || direct) {
+#pragma unroll
+      for (int ks = 0; ks < kSplit / 32; ++ks) lsum = pv_step<T>(load_pfrag<T>(&Ps[ks][0][lane]), ones_frag<T>(), lsum);
+    }
+    // A hidden key's weight 0 times an infinity or NaN of its V row is NaN: such a
+    // wave weighs again without them and notes the ones its rows see (kSeenTag).
+    bool finite = true;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) finite = finite && (NJ * wave + j >= NDT || fabsf(acc[j][i]) < INFINITY);
+    if (__ballot(!finite)) {
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+      for (int k2 = 0; k2 < kSplit / 64; ++k2) {
+        Codes8<BITS> vc[2][NJ];
+        Step x;
+        read_codes(vc, k2);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          read_step(x, 2 * k2 + h);
+          step_of(x, vc[h], true);
+        }
+      }
+      for (int key = 0; key < n_act; ++key) {
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+          if (NJ * wave + j >= NDT) continue;
+          const int dim = 16 * (NJ * wave + j) + r, byte = dim * BITS / 8;
+          const uint32_t c = (uint8_t)Vs[CT::off(key, byte >> 4) + (byte & 15)];
+          const float code = (float)(BITS == 8 ? c : c >> 4 * (dim & 1) & 15u);
+          const float x = to_f32(to_store<T>(__builtin_fmaf(code, vsc[dim / GS][key], vbi[dim / GS][key])));
+          if (fabsf(x) < INFINITY) continue;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (key < alim[i]) acc[j][i] = note_seen(acc[j][i], x);
+        }
+      }
+    }
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+      if (NJ * wave + j >= NDT) continue;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (i >= ni) continue;
+        const int d = 16 * (NJ * wave + j) + r;
+        if (direct) {
+          if (arow[i] >= 0) static_cast<T*>(a.out)[(int64_t)arow[i] * D + d] = to_store<T>(only_split(acc[j][i], lsum[i]));
+        } else if (alim[i] > 0) {
+          a.pacc[((int64_t)arow[i] * a.nsplit + split) * D + d] = acc[j][i];
+        }
+      }
+    }
+    if (!direct && wave == sum_wave && r == 0) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (i < ni && alim[i] > 0) a.pl[(int64_t)arow[i] * a.nsplit + split] = lsum[i];
+    }
+    stage_barrier<63>();                                  // every wave is done with Vs, Ps and the pairs
   }
 }
 

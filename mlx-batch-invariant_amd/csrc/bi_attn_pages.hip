@@ -148,6 +148,10 @@ extern "C" int bi_attn_pages(const void* q, const void* k, const void* k_groups,
     a.vg_sp = strides[12]; a.vg_sh = strides[13]; a.vg_sl = strides[14];
     a.gshift = group_size == 32 ? 5 : group_size == 64 ? 6 : 7;
   }
+  // (a lane finds its rows by 32-bit strides)
+  for (int i = 3; i < 15; ++i)
+    if (bits && i % 3 != 1 && strides[i] > 0xffffffffLL)
+      return fail(BI_E_UNSUPPORTED, "%s: page or row stride %lld of codes (below 2^32)", what, (long long)strides[i]);
   a.table_stride = table_stride;
   a.B = (int)B; a.Hq = (int)Hq; a.Hkv = (int)Hkv; a.Tq = (int)Tq; a.L = (int)L; a.nsplit = (int)nsplit;
   a.causal = causal ? 1 : 0; a.groups = (int)groups;

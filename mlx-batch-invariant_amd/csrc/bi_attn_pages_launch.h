@@ -1,5 +1,6 @@
 // bi_attn_pages_launch.h — host launcher of the kernels of bi_attn_pages.h, included by
-// bi_attn_pages_{bf16,f16,f32}.hip, which instantiate it for every head dim.
+// bi_attn_pages_{bf16,f16,f32}.hip (head dims to 128) and bi_attn_pages_wide_{...}.hip
+// (192 and 256, whose registers go by other rules: see build.py).
 #pragma once
 
 #include "bi_attn_launch.h"
@@ -7,15 +8,14 @@
 
 namespace bi {
 
-template <typename T, int D, int BITS, bool MULTI>
-static int launch_pages_as(const PagesArgs& a, hipStream_t st) {
-  static int cache[kMaxDev] = {};
-  int grid = resident_grid(attn_pages<T, D, BITS, MULTI>, cache);
-  if (grid <= 0) return bi_host::fail(BI_E_UNSUPPORTED, "bi_attn_pages: device occupancy query failed");
-  if constexpr (MULTI) pages_plan_kernel<<<1, kPlanThreads, 0, st>>>(a, grid);
-  const int64_t most = (int64_t)a.B * a.nsplit * a.Hkv * ((a.Tq * (a.Hq / a.Hkv) + 15) / 16);   // no segment has more
-  grid = (int)((std::min<int64_t>(grid, most) + 7) / 8 * 8);
-  attn_pages<T, D, BITS, MULTI><<<grid, 256, 0, st>>>(a);
+// Workgroups of a kernel that the device holds at once, a multiple of 8 (one share for each XCD), and no more than there can be items.
+template <typename K>
+static int pages_grid(K kern, int (&cache)[kMaxDev], int64_t most) {
+  return (int)((std::min<int64_t>(resident_grid(kern, cache), most) + 7) / 8 * 8);
+}
+
+template <typename T, int D>
+static int merge_pages(const PagesArgs& a, hipStream_t st) {
   if (a.nsplit > 1) {
     const int64_t n = (int64_t)a.B * a.Hq * a.Tq * (D / 4);
     attn_pages_merge<T, D><<<(unsigned)((n + 255) / 256), 256, 0, st>>>(a);
@@ -23,20 +23,44 @@ static int launch_pages_as(const PagesArgs& a, hipStream_t st) {
   return bi_host::launch_status("bi_attn_pages");
 }
 
-template <typename T, int D>
-int launch_pages(const PagesArgs& a, int bits, hipStream_t st) {
-  const bool multi = a.groups > 0 || a.Tq * (a.Hq / a.Hkv) > 16;
-  if (bits == 0) return launch_pages_as<T, D, 0, true>(a, st);
-  if (bits == 8) return multi ? launch_pages_as<T, D, 8, true>(a, st) : launch_pages_as<T, D, 8, false>(a, st);
-  return multi ? launch_pages_as<T, D, 4, true>(a, st) : launch_pages_as<T, D, 4, false>(a, st);
+constexpr const char* kNoOccupancy = "bi_attn_pages: device occupancy query failed";
+
+template <typename T, int D, int BITS>
+static int launch_planned(const PagesArgs& a, hipStream_t st) {
+  static int cache[kMaxDev] = {};
+  const int64_t most = (int64_t)a.B * a.nsplit * a.Hkv * ((a.Tq * (a.Hq / a.Hkv) + 15) / 16);   // no segment has more
+  const int slots = pages_grid(attn_pages<T, D, BITS>, cache, (int64_t)1 << 30);
+  if (slots <= 0) return bi_host::fail(BI_E_UNSUPPORTED, kNoOccupancy);
+  pages_plan_kernel<<<1, kPlanThreads, 0, st>>>(a, slots);
+  attn_pages<T, D, BITS><<<pages_grid(attn_pages<T, D, BITS>, cache, most), 256, 0, st>>>(a);
+  return merge_pages<T, D>(a, st);
 }
 
-#define BI_PAGES_INSTANTIATE(T)                                                   \
-  template int launch_pages<T, 32>(const PagesArgs&, int, hipStream_t);           \
-  template int launch_pages<T, 64>(const PagesArgs&, int, hipStream_t);           \
-  template int launch_pages<T, 96>(const PagesArgs&, int, hipStream_t);           \
-  template int launch_pages<T, 128>(const PagesArgs&, int, hipStream_t);          \
-  template int launch_pages<T, 192>(const PagesArgs&, int, hipStream_t);          \
-  template int launch_pages<T, 256>(const PagesArgs&, int, hipStream_t);
+template <typename T, int D, int BITS, int GS>
+static int launch_codes_as(const PagesArgs& a, hipStream_t st) {
+  static int cache[kMaxDev] = {};
+  const int grid = pages_grid(attn_codes<T, D, BITS, GS>, cache, (int64_t)a.B * a.nsplit * a.Hkv);
+  if (grid <= 0) return bi_host::fail(BI_E_UNSUPPORTED, kNoOccupancy);
+  attn_codes<T, D, BITS, GS><<<grid, 256, 0, st>>>(a);
+  return merge_pages<T, D>(a, st);
+}
+template <typename T, int D, int BITS>
+static int launch_codes(const PagesArgs& a, hipStream_t st) {
+  if constexpr (D % 64 == 0)
+    if (a.gshift == 6) return launch_codes_as<T, D, BITS, 64>(a, st);
+  if constexpr (D % 128 == 0)
+    if (a.gshift == 7) return launch_codes_as<T, D, BITS, 128>(a, st);
+  return launch_codes_as<T, D, BITS, 32>(a, st);
+}
+
+template <typename T, int D>
+int launch_pages(const PagesArgs& a, int bits, hipStream_t st) {
+  if (bits == 0) return launch_planned<T, D, 0>(a, st);
+  if (a.groups == 0 && a.Tq * (a.Hq / a.Hkv) <= 16)
+    return bits == 8 ? launch_codes<T, D, 8>(a, st) : launch_codes<T, D, 4>(a, st);
+  return bits == 8 ? launch_planned<T, D, 8>(a, st) : launch_planned<T, D, 4>(a, st);
+}
+
+#define BI_PAGES_INSTANTIATE(T, D) template int launch_pages<T, D>(const PagesArgs&, int, hipStream_t);
 
 }  // namespace bi

@@ -11,18 +11,27 @@ namespace bi {
 template <typename T> struct Pair { float s, b; };        // a group's scale and bias
 
 template <typename T>
-__device__ __forceinline__ Pair<T> load_pair(const T* p) {
+__device__ __forceinline__ Pair<T> unpack_pair(const uint32_t* u) {
   Pair<T> g;
   if constexpr (sizeof(T) == 2) {
-    const uint32_t u = *reinterpret_cast<const uint32_t*>(p);
-    g.s = to_f32(__builtin_bit_cast(T, (uint16_t)u));
-    g.b = to_f32(__builtin_bit_cast(T, (uint16_t)(u >> 16)));
+    g.s = to_f32(__builtin_bit_cast(T, (uint16_t)u[0]));
+    g.b = to_f32(__builtin_bit_cast(T, (uint16_t)(u[0] >> 16)));
   } else {
-    const u32x2 u = *reinterpret_cast<const u32x2*>(p);
-    g.s = __builtin_bit_cast(float, (uint32_t)u[0]);
-    g.b = __builtin_bit_cast(float, (uint32_t)u[1]);
+    g.s = __builtin_bit_cast(float, u[0]);
+    g.b = __builtin_bit_cast(float, u[1]);
   }
   return g;
+}
+template <typename T>
+__device__ __forceinline__ Pair<T> load_pair(const T* p) {
+  if constexpr (sizeof(T) == 2) {
+    const uint32_t u = *reinterpret_cast<const uint32_t*>(p);
+    return unpack_pair<T>(&u);
+  } else {
+    const u32x2 v = *reinterpret_cast<const u32x2*>(p);
+    const uint32_t u[2] = {v[0], v[1]};
+    return unpack_pair<T>(u);
+  }
 }
 
 // Eight and sixteen consecutive codes.
@@ -80,18 +89,18 @@ __device__ __forceinline__ void code_floats(Codes8<BITS> c, float (&x)[8]) {
   }
 }
 
-// T(fma(code, scale, bias)) of 8 codes of one group. The fma's result is kept in a
-// register of its own: folded into the conversion (v_fma_mixlo_f16) it would round
-// once where the quantized matmul rounds twice.
+// T(fma(code, scale, bias)) of 8 codes, each with a pair of its own or all of one
+// group. The fma's result is kept in a register of its own: folded into the conversion
+// (v_fma_mixlo_f16) it would round once where the quantized matmul rounds twice.
 template <typename T, int BITS>
-__device__ __forceinline__ typename Frag<T>::type dequant_frag(Codes8<BITS> c, Pair<T> g) {
+__device__ __forceinline__ typename Frag<T>::type dequant_frag8(Codes8<BITS> c, const float (&s)[8], const float (&b)[8]) {
   typedef float f32x2v __attribute__((ext_vector_type(2)));
   typedef T tx2 __attribute__((ext_vector_type(2)));
   float x[8];
   code_floats<BITS>(c, x);
 #pragma unroll
   for (int e = 0; e < 8; ++e) {
-    x[e] = __builtin_fmaf(x[e], g.s, g.b);
+    x[e] = __builtin_fmaf(x[e], s[e], b[e]);
     if constexpr (sizeof(T) == 2) asm("" : "+v"(x[e]));
   }
   typename Frag<T>::type f;
@@ -110,6 +119,11 @@ __device__ __forceinline__ typename Frag<T>::type dequant_frag(Codes8<BITS> c, P
     }
   }
   return f;
+}
+template <typename T, int BITS>
+__device__ __forceinline__ typename Frag<T>::type dequant_frag(Codes8<BITS> c, Pair<T> g) {
+  const float s[8] = {g.s, g.s, g.s, g.s, g.s, g.s, g.s, g.s}, b[8] = {g.b, g.b, g.b, g.b, g.b, g.b, g.b, g.b};
+  return dequant_frag8<T, BITS>(c, s, b);
 }
 
 }  // namespace bi
