@@ -238,6 +238,15 @@ __device__ __forceinline__ void load_uniform4_i32(const int32_t* p0, const int32
       : "memory");
 }
 
+// A wave-uniform pointer held in scalar registers, whatever the compiler can prove.
+template <typename P>
+__device__ __forceinline__ const P* uniform_ptr(const P* p) {
+  const uint64_t u = reinterpret_cast<uint64_t>(p);
+  const uint64_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)u);
+  const uint64_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(u >> 32));
+  return reinterpret_cast<const P*>(hi << 32 | lo);
+}
+
 // min(max(x, 0), most) of a wave-uniform x, kept in a scalar register: the
 // compiler clamps with v_med3_i32 otherwise, and a buffer resource whose size
 // is a vector register costs a readfirstlane loop around every copy.

@@ -69,15 +69,6 @@ constexpr int mod_min_blocks() {
   return sizeof(T) != 2 || D > 128 || MODE == kKvRowPaged ? 1 : 2;
 }
 
-// A wave-uniform pointer held in scalar registers, whatever the compiler can prove.
-template <typename P>
-__device__ __forceinline__ const P* uniform_ptr(const P* p) {
-  const uint64_t u = reinterpret_cast<uint64_t>(p);
-  const uint64_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)u);
-  const uint64_t hi = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(u >> 32));
-  return reinterpret_cast<const P*>(hi << 32 | lo);
-}
-
 template <typename T, int D, int MODE, int MOD>
 __global__ __launch_bounds__(256, (mod_min_blocks<T, D, MODE>())) void attn_prefill_mod(ModPrefillArgs a) {
   constexpr bool ROWPAGED = MODE == kKvRowPaged, TILED = MODE == kKvTilePaged;

@@ -503,19 +503,19 @@ template <int KS, int BITS>
 struct KRow {
   static constexpr int kW = BITS / 4;                     // words of a piece
   uint32_t w[KS][kW];
-  __device__ __forceinline__ void load(const char* row, int qq) {
+  __device__ __forceinline__ void load(const char* base, uint32_t off, int qq) {   // (a wave-uniform base takes the offset as it is)
     int st = 0;
 #pragma unroll
     for (; st + 4 <= KS; st += 4) {                       // 4 pieces: 16 or 32 bytes
 #pragma unroll
       for (int h = 0; h < kW; ++h) {
-        const u32x4 x = *reinterpret_cast<const u32x4*>(row + 4 * BITS * st + 4 * BITS * qq + 16 * h);
+        const u32x4 x = *reinterpret_cast<const u32x4*>(base + (off + (uint32_t)(4 * BITS * qq)) + (4 * BITS * st + 16 * h));
 #pragma unroll
         for (int i = 0; i < 4; ++i) w[st + (4 * h + i) / kW][(4 * h + i) % kW] = x[i];
       }
     }
     if constexpr (KS % 4 >= 2) {                          // 2 pieces: 8 or 16 bytes
-      const char* p = row + 4 * BITS * st + 2 * BITS * qq;
+      const char* p = base + (off + (uint32_t)(2 * BITS * qq)) + 4 * BITS * st;
       if constexpr (BITS == 8) {
         const u32x4 x = *reinterpret_cast<const u32x4*>(p);
 #pragma unroll
@@ -528,7 +528,7 @@ struct KRow {
       st += 2;
     }
     if constexpr (KS % 2 == 1) {
-      const Codes8<BITS> c = load_codes8<BITS>(row + 4 * BITS * st + BITS * qq);
+      const Codes8<BITS> c = load_codes8<BITS>(base + (off + (uint32_t)(BITS * qq)) + 4 * BITS * st);
 #pragma unroll
       for (int i = 0; i < kW; ++i) w[st][i] = c.w[i];
     }
@@ -581,13 +581,13 @@ __device__ __forceinline__ void load_words(const void* p, uint32_t* w) {
 }
 
 // Workgroups per CU that the registers are held to.
-template <typename T, int D>
+template <typename T, int D, int BITS>
 constexpr int codes_min_blocks() {
-  return sizeof(T) == 2 && D <= 128 ? 3 : 1;
+  return sizeof(T) == 2 && D <= 128 ? (BITS == 4 ? 4 : 3) : 1;
 }
 
 template <typename T, int D, int BITS, int GS>
-__global__ __launch_bounds__(256, (codes_min_blocks<T, D>())) void attn_codes(PagesArgs a) {
+__global__ __launch_bounds__(256, (codes_min_blocks<T, D, BITS>())) void attn_codes(PagesArgs a) {
   typedef typename Frag<T>::type F;
   typedef CodeTile<D, BITS> CT;
   constexpr int KT = 4, KS = D / 32, NDT = D / 16, NJ = (NDT + 3) / 4;
@@ -637,8 +637,12 @@ __global__ __launch_bounds__(256, (codes_min_blocks<T, D>())) void attn_codes(Pa
     const int local = item - lo - (i ? __builtin_amdgcn_readlane(incl, max(i - 1, 0)) : 0);
     Item it;
     it.b = 64 * c64 + i;
-    it.split = local / a.Hkv;
+    it.split = (int)__umulhi((unsigned)local, a.hkv_inv);  // local / Hkv, or one less
     it.hk = local - it.split * a.Hkv;
+    if (it.hk >= a.Hkv) {
+      it.hk -= a.Hkv;
+      ++it.split;
+    }
     it.n_act = min(kSplit, pages_len_uniform(a, it.b) - it.split * kSplit);
     return it;
   };
@@ -648,15 +652,15 @@ __global__ __launch_bounds__(256, (codes_min_blocks<T, D>())) void attn_codes(Pa
     return a.table[(int64_t)it.b * a.table_stride + (pos >> a.page_shift)];
   };
 
+  // (token, head) p of sequence b, heads inside tokens.
+  auto out_row = [&](int b, int hk, int p) { return (b * a.Hq + hk * G + p % G) * a.Tq + p / G; };
   Item it = locate(w0);
   int page = page_of(it);
   for (int item = w0; it.n_act >= 0; item += (int)gridDim.x) {
     const int b = it.b, hk = it.hk, j0 = it.split * kSplit, n_act = it.n_act, split = it.split;
-    const int my_page = clamp_page(page, a.num_pages);
-    // (token, head) p of the sequence, heads inside tokens.
-    auto out_row = [&](int p) { return (b * a.Hq + hk * G + p % G) * a.Tq + p / G; };
     if (n_act == 0) {                                     // (direct, an empty sequence) no keys: zeros
-      for (int i = tid; i < rows1 * D; i += 256) static_cast<T*>(a.out)[(int64_t)out_row(i / D) * D + i % D] = (T)0.0f;
+      for (int i = tid; i < rows1 * D; i += 256)
+        static_cast<T*>(a.out)[(int64_t)out_row(b, hk, i / D) * D + i % D] = (T)0.0f;
       it = locate(item + (int)gridDim.x);
       page = page_of(it);
       continue;
@@ -665,19 +669,12 @@ __global__ __launch_bounds__(256, (codes_min_blocks<T, D>())) void attn_codes(Pa
 
     // Memory requests: pairs of this lane's key, Q^T, K, V. A lane finds its own key's
     // rows; the others' come by lane exchanges.
+    const uint32_t my_page = (uint32_t)clamp_page(page, a.num_pages);
     const uint32_t my_row = (j0 + min(tid, n_act - 1)) & page_mask;
-    auto row_off = [&](int64_t sp, int64_t sl) { return (uint64_t)(uint32_t)my_page * (uint32_t)sp + (uint64_t)my_row * (uint32_t)sl; };
-    const uint64_t k_off = row_off(a.k_sp, a.k_sl), v_off = row_off(a.v_sp, a.v_sl);
-    auto off_of = [&](uint64_t off, int l) {
-      return (uint64_t)(uint32_t)__shfl((int)(uint32_t)off, l, kWave) | (uint64_t)(uint32_t)__shfl((int)(uint32_t)(off >> 32), l, kWave) << 32;
-    };
+    auto row_off = [&](int64_t sp, int64_t sl) { return (uint64_t)my_page * (uint32_t)sp + (uint64_t)my_row * (uint32_t)sl; };
     uint32_t kp[NG][PW], vp[NG][PW];
-    {
-      const T* kg = static_cast<const T*>(a.kg) + hk * a.kg_sh + row_off(a.kg_sp, a.kg_sl);
-      const T* vg = static_cast<const T*>(a.vg) + hk * a.vg_sh + row_off(a.vg_sp, a.vg_sl);
-      load_words<NG * PW>(kg, &kp[0][0]);
-      load_words<NG * PW>(vg, &vp[0][0]);
-    }
+    load_words<NG * PW>(static_cast<const T*>(a.kg) + hk * a.kg_sh + row_off(a.kg_sp, a.kg_sl), &kp[0][0]);
+    load_words<NG * PW>(static_cast<const T*>(a.vg) + hk * a.vg_sh + row_off(a.vg_sp, a.vg_sl), &vp[0][0]);
     F qf[KS];
     {
       const int p = min(my_p, rows1 - 1);
@@ -686,15 +683,51 @@ __global__ __launch_bounds__(256, (codes_min_blocks<T, D>())) void attn_codes(Pa
       for (int st = 0; st < KS; ++st) qf[st] = my_p < rows1 ? frag_load(qrow + 32 * st + 8 * qq) : frag_zero<F>();
     }
     KRow<KS, BITS> kc[KT];
+    const char* kb = uniform_ptr(static_cast<const char*>(a.k) + hk * a.k_sh);
+    const char* vb = uniform_ptr(static_cast<const char*>(a.v) + hk * a.v_sh);
+    // (offsets within tiles are taken from the lane anew for every item: kept over the
+    // items they hold registers)
+    int l = lane;
+    asm volatile("" : "+v"(l));
+    auto v_piece = [&](int c, int& row) {                 // of the wave's copy c: its row and 16-byte piece
+      if constexpr (CT::kSwz) {                           // (the wave's first row is a multiple of 64, so the keys agree)
+        constexpr int kRPC = 64 / CT::kCPR;               // rows of a copy
+        row = l / CT::kCPR + kRPC * c;
+        return (l % CT::kCPR) ^ CT::key(l / CT::kCPR) ^ (kRPC >= 32 ? 0 : CT::key(kRPC * c & (kRPC >= 8 ? 16 : 23)));
+      } else {
+        row = (64 * c + l) / CT::kCPR;
+        return 64 * c + l - row * CT::kCPR;
+      }
+    };
+    if (a.near) {                                         // pools below 4 GiB: 32-bit offsets
+      const uint32_t k_off = my_page * (uint32_t)a.k_sp + my_row * (uint32_t)a.k_sl;
+      const uint32_t v_off = my_page * (uint32_t)a.v_sp + my_row * (uint32_t)a.v_sl;
 #pragma unroll
-    for (int t = 0; t < KT; ++t) kc[t].load(static_cast<const char*>(a.k) + hk * a.k_sh + off_of(k_off, 16 * t + r), qq);
-    asm volatile("" ::: "memory");
+      for (int t = 0; t < KT; ++t) kc[t].load(kb, (uint32_t)__shfl((int)k_off, 16 * t + r, kWave), qq);
+      asm volatile("" ::: "memory");
 #pragma unroll
-    for (int c = 0; c < NCOPY; ++c) {
-      const int f = 64 * c + lane, row = f / CT::kCPR, slot = f - row * CT::kCPR;
-      const char* vr = static_cast<const char*>(a.v) + hk * a.v_sh + off_of(v_off, row);
-      copy_to_lds16(vr + ((slot ^ CT::key(64 * wave + row)) << 4), Vs + 1024 * (wave * NCOPY + c));
+      for (int c = 0; c < NCOPY; ++c) {
+        int row;
+        const int piece = v_piece(c, row);
+        copy_to_lds16(vb + ((uint32_t)__shfl((int)v_off, row, kWave) + (uint32_t)(piece << 4)), Vs + 1024 * (wave * NCOPY + c));
+      }
+    } else {
+      const uint64_t k_off = row_off(a.k_sp, a.k_sl), v_off = row_off(a.v_sp, a.v_sl);
+      auto off_of = [&](uint64_t off, int l) {
+        return (uint64_t)(uint32_t)__shfl((int)(uint32_t)off, l, kWave) |
+               (uint64_t)(uint32_t)__shfl((int)(uint32_t)(off >> 32), l, kWave) << 32;
+      };
+#pragma unroll
+      for (int t = 0; t < KT; ++t) kc[t].load(kb + off_of(k_off, 16 * t + r), 0u, qq);
+      asm volatile("" ::: "memory");
+#pragma unroll
+      for (int c = 0; c < NCOPY; ++c) {
+        int row;
+        const int piece = v_piece(c, row);
+        copy_to_lds16(vb + off_of(v_off, row) + (piece << 4), Vs + 1024 * (wave * NCOPY + c));
+      }
     }
+    asm volatile("" ::: "memory");
     it = locate(item + (int)gridDim.x);                   // the next item's pages
     page = page_of(it);
 
@@ -708,30 +741,37 @@ __global__ __launch_bounds__(256, (codes_min_blocks<T, D>())) void attn_codes(Pa
     int lim = 0, row = -1;
     if (my_p < rows1) {
       lim = (a.causal ? total - a.Tq + my_p / G + 1 : total) - j0;
-      row = out_row(my_p);
+      row = out_row(b, hk, my_p);
     }
     float s[KT][4];
     float m = -INFINITY;
+    auto scores = [&](auto masked) __attribute__((always_inline)) {
 #pragma unroll
-    for (int t = 0; t < KT; ++t) {
-      f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-      Pair<T> g[NG];
+      for (int t = 0; t < KT; ++t) {
+        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+        Pair<T> g[NG];
 #pragma unroll
-      for (int i = 0; i < NG; ++i) {
-        uint32_t u[PW];
+        for (int i = 0; i < NG; ++i) {
+          uint32_t u[PW];
 #pragma unroll
-        for (int w = 0; w < PW; ++w) u[w] = (uint32_t)__shfl((int)kp[i][w], 16 * t + r, kWave);
-        g[i] = unpack_pair<T>(u);
+          for (int w = 0; w < PW; ++w) u[w] = (uint32_t)__shfl((int)kp[i][w], 16 * t + r, kWave);
+          g[i] = unpack_pair<T>(u);
+        }
+        kc[t].arrange();
+#pragma unroll
+        for (int st = 0; st < KS; ++st) acc = mfma_step(dequant_frag<T, BITS>(kc[t].codes(st), g[32 * st / GS]), qf[st], acc);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const bool seen = !decltype(masked)::value || 64 * wave + 16 * t + 4 * qq + i < lim;
+          s[t][i] = seen ? acc[i] * a.scale_log2 : -INFINITY;
+          m = fmaxf(m, s[t][i]);
+        }
+        __builtin_amdgcn_sched_barrier(0);
       }
-      kc[t].arrange();
-#pragma unroll
-      for (int st = 0; st < KS; ++st) acc = mfma_step(dequant_frag<T, BITS>(kc[t].codes(st), g[32 * st / GS]), qf[st], acc);
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        s[t][i] = 64 * wave + 16 * t + 4 * qq + i < lim ? acc[i] * a.scale_log2 : -INFINITY;
-        m = fmaxf(m, s[t][i]);
-      }
-    }
+    };
+    // (columns without a row may hold anything)
+    if (__ballot(my_p < rows1 && lim < kSplit)) scores(std::true_type());
+    else scores(std::false_type());
     m = quarter_max(m);
     if (qq == 0) mx[wave][r] = m;
     stage_barrier<63>();                                  // (V's copies may still be in flight)
@@ -781,21 +821,30 @@ __global__ __launch_bounds__(256, (codes_min_blocks<T, D>())) void attn_codes(Pa
         }
       }
     };
-    auto read_codes = [&](Codes8<BITS> (&c)[2][NJ], int k2) __attribute__((always_inline)) {
+    // Byte of this lane's part of the first keys' codes of each dim tile; 32 (64) keys
+    // further the key repeats.
+    int at[NJ];
+    {
+      int lr = l % 16;
+      const int key = BITS == 8 ? 4 * qq + (lr >> 1 & 3) + (lr >> 1 & 4) * 4 : 32 * (lr >> 3) + 4 * qq + (lr & 3) + (lr & 4) * 4;
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
         const int dt = min(NJ * wave + j, NDT - 1);
+        at[j] = BITS == 8 ? CT::off(key, dt) + 8 * (lr & 1) : CT::off(key, dt >> 1) + 8 * (dt & 1);
+      }
+    }
+    auto read_codes = [&](Codes8<BITS> (&c)[2][NJ], int k2) __attribute__((always_inline)) {
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) {
         if constexpr (BITS == 8) {
-          const int u = r >> 1, key = 64 * k2 + 4 * qq + (u & 3) + (u & 4) * 4;
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const i32x2_t w = lds_read_tr8((lds_i32x2*)(Vs + CT::off(key + 32 * h, dt) + 8 * (r & 1)));
+            const i32x2_t w = lds_read_tr8((lds_i32x2*)(Vs + at[j] + (64 * k2 + 32 * h) * CT::kRowBytes));
             c[h][j].w[0] = (uint32_t)w[0];
             c[h][j].w[BITS / 4 - 1] = (uint32_t)w[1];
           }
         } else {
-          const int key = 64 * k2 + 32 * (r >> 3) + 4 * qq + (r & 3) + (r & 4) * 4;
-          const i32x2_t w = lds_read_tr4((lds_i32x2*)(Vs + CT::off(key, dt >> 1) + 8 * (dt & 1)));
+          const i32x2_t w = lds_read_tr4((lds_i32x2*)(Vs + at[j] + 64 * k2 * CT::kRowBytes));
           c[0][j].w[0] = (uint32_t)w[0];
           c[1][j].w[0] = (uint32_t)w[1];
         }
@@ -822,6 +871,7 @@ __global__ __launch_bounds__(256, (codes_min_blocks<T, D>())) void attn_codes(Pa
         if (ks % 2 == 0 && ks + 2 < kSplit / 32) read_codes(vc[(ks / 2 + 1) % 2], ks / 2 + 1);
         if (ks + 1 < kSplit / 32) read_step(st[(ks + 1) % 2], ks + 1);
         step_of(st[ks % 2], vc[ks / 2 % 2][ks % 2], false);
+        __builtin_amdgcn_sched_barrier(0);                // (or every step's reads are gathered in front, and spill)
       }
     }
     const int sum_wave = NDT < 4 * NJ ? 3 : 0;            // (the wave with the fewest dims adds up the weights)

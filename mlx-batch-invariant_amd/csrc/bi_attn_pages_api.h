@@ -15,6 +15,8 @@ struct PagesArgs {
   int64_t q_sb, q_sh, q_st, k_sp, k_sh, k_sl, v_sp, v_sh, v_sl;  // codes: bytes
   int64_t kg_sp, kg_sh, kg_sl, vg_sp, vg_sh, vg_sl, table_stride;
   int B, Hq, Hkv, Tq, L, nsplit, causal, groups, shared_len, page_shift, num_pages, gshift;
+  int near;                              // codes: every byte of the pools lies below 2^32 from their start
+  unsigned hkv_inv;                      // 2^32 / Hkv, rounded down (2^32 - 1 for 1)
   float scale_log2;
 };
 

@@ -83,7 +83,10 @@ __device__ __forceinline__ void code_floats(Codes8<BITS> c, float (&x)[8]) {
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = (float)(c.w[e / 4] >> (8 * (e % 4)) & 255u);
   } else {
-    const uint32_t even = c.w[0] & 0x0f0f0f0fu, odd = c.w[0] >> 4 & 0x0f0f0f0fu;
+    uint32_t even = c.w[0] & 0x0f0f0f0fu, odd = c.w[0] >> 4 & 0x0f0f0f0fu;
+    // (three instructions for eight codes, which are converted from bytes then; seen
+    // through, each code costs one of its own)
+    asm("" : "+v"(even), "+v"(odd));
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] = (float)((e & 1 ? odd : even) >> (8 * (e / 2)) & 255u);
   }
