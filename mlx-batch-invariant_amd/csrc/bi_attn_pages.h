@@ -486,9 +486,9 @@ __device__ __forceinline__ i32x2_t lds_read_tr8(lds_i32x2* __restrict p) { retur
 __device__ __forceinline__ i32x2_t lds_read_tr4(lds_i32x2* __restrict p) { return __builtin_amdgcn_ds_read_tr4_b64_v2i32(p); }
 
 // The codes of K row r that lane (r, qq) needs as score operands, dims 32 st + 8 qq .. + 7
-// of every step st, are pieces of 8 or 4 bytes. A lane reads longer ones instead, the
-// steps four at a time (lane qq those of step qq whole) or two (half a step), and the
-// four lanes of a row hand each other their pieces by swaps of 16-lane rows.
+// of every step st, are pieces of 8 or 4 bytes. A lane reads 16 bytes instead, the
+// row's four lanes 64 in a run: two steps of 8 bits (lane qq half of step qq / 2) or four
+// of 4 (lane qq step qq), and they hand each other their pieces by swaps of 16-lane rows.
 __device__ __forceinline__ void swap32(uint32_t& x, uint32_t& y) {   // x's upper 32 lanes for y's lower 32
   const auto p = __builtin_amdgcn_permlane32_swap(x, y, false, false);
   x = p[0];
@@ -502,49 +502,49 @@ __device__ __forceinline__ void swap16(uint32_t& x, uint32_t& y) {   // x's odd 
 template <int KS, int BITS>
 struct KRow {
   static constexpr int kW = BITS / 4;                     // words of a piece
+  static constexpr int kFour = BITS == 4 ? KS / 4 * 4 : 0;   // steps read four at a time; the others in twos, the last alone
   uint32_t w[KS][kW];
   __device__ __forceinline__ void load(const char* base, uint32_t off, int qq) {   // (a wave-uniform base takes the offset as it is)
-    int st = 0;
+    if constexpr (kFour > 0) {
+      const char* p = base + (off + (uint32_t)(16 * qq));
 #pragma unroll
-    for (; st + 4 <= KS; st += 4) {                       // 4 pieces: 16 or 32 bytes
+      for (int st = 0; st < kFour; st += 4) {
+        const u32x4 x = *reinterpret_cast<const u32x4*>(p + 4 * BITS * st);
 #pragma unroll
-      for (int h = 0; h < kW; ++h) {
-        const u32x4 x = *reinterpret_cast<const u32x4*>(base + (off + (uint32_t)(4 * BITS * qq)) + (4 * BITS * st + 16 * h));
-#pragma unroll
-        for (int i = 0; i < 4; ++i) w[st + (4 * h + i) / kW][(4 * h + i) % kW] = x[i];
+        for (int i = 0; i < 4; ++i) w[st + i][0] = x[i];
       }
     }
-    if constexpr (KS % 4 >= 2) {                          // 2 pieces: 8 or 16 bytes
-      const char* p = base + (off + (uint32_t)(2 * BITS * qq)) + 4 * BITS * st;
-      if constexpr (BITS == 8) {
-        const u32x4 x = *reinterpret_cast<const u32x4*>(p);
+    if constexpr (KS - kFour >= 2) {
+      const char* p = base + (off + (uint32_t)(2 * BITS * qq));
 #pragma unroll
-        for (int i = 0; i < 4; ++i) w[st + i / 2][i % 2] = x[i];
-      } else {
-        const u32x2 x = *reinterpret_cast<const u32x2*>(p);
-        w[st][0] = x[0];
-        w[st + 1][0] = x[1];
+      for (int st = kFour; st + 2 <= KS; st += 2) {
+        if constexpr (BITS == 8) {
+          const u32x4 x = *reinterpret_cast<const u32x4*>(p + 4 * BITS * st);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) w[st + i / 2][i % 2] = x[i];
+        } else {
+          const u32x2 x = *reinterpret_cast<const u32x2*>(p + 4 * BITS * st);
+          w[st][0] = x[0];
+          w[st + 1][0] = x[1];
+        }
       }
-      st += 2;
     }
     if constexpr (KS % 2 == 1) {
-      const Codes8<BITS> c = load_codes8<BITS>(base + (off + (uint32_t)(BITS * qq)) + 4 * BITS * st);
+      const Codes8<BITS> c = load_codes8<BITS>(base + (off + (uint32_t)(BITS * qq)) + 4 * BITS * (KS - 1));
 #pragma unroll
-      for (int i = 0; i < kW; ++i) w[st][i] = c.w[i];
+      for (int i = 0; i < kW; ++i) w[KS - 1][i] = c.w[i];
     }
   }
   __device__ __forceinline__ void arrange() {
-    int st = 0;
 #pragma unroll
-    for (; st + 4 <= KS; st += 4)
+    for (int st = 0; st < kFour; st += 4) {
+      swap32(w[st][0], w[st + 2][0]);
+      swap32(w[st + 1][0], w[st + 3][0]);
+      swap16(w[st][0], w[st + 1][0]);
+      swap16(w[st + 2][0], w[st + 3][0]);
+    }
 #pragma unroll
-      for (int i = 0; i < kW; ++i) {
-        swap32(w[st][i], w[st + 2][i]);
-        swap32(w[st + 1][i], w[st + 3][i]);
-        swap16(w[st][i], w[st + 1][i]);
-        swap16(w[st + 2][i], w[st + 3][i]);
-      }
-    if constexpr (KS % 4 >= 2)
+    for (int st = kFour; st + 2 <= KS; st += 2)
 #pragma unroll
       for (int i = 0; i < kW; ++i) {
         swap16(w[st][i], w[st + 1][i]);
@@ -938,51 +938,54 @@ __global__ __launch_bounds__(256, (codes_min_blocks<T, D, BITS>())) void attn_co
   }
 }
 
-// Merges the splits of every row, left to right, and divides: one thread per four
-// dims of a row. A split in which the row sees no score above -inf (l = 0 at m =
-// -inf) is passed over.
+// Merges the splits of every row, left to right, and divides: one thread per two dims
+// of a row, the partials of 16 splits requested together (decode has few rows: a
+// thread's time is its round trips). A split in which the row sees no score above -inf
+// (l = 0 at m = -inf) is passed over.
 template <typename T, int D>
 __global__ __launch_bounds__(256) void attn_pages_merge(PagesArgs a) {
+  typedef float f32x2m __attribute__((ext_vector_type(2)));
+  constexpr int kDeep = 16;
   const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t row = id / (D / 4);                       // (b, head, token), the output's order
+  const int64_t row = id / (D / 2);                       // (b, head, token), the output's order
   if (row >= (int64_t)a.B * a.Hq * a.Tq) return;
-  const int d = (int)(id % (D / 4)) * 4;
+  const int d = (int)(id % (D / 2)) * 2;
   const int t = (int)(row % a.Tq), b = (int)(row / a.Tq / a.Hq);
   const int len = pages_len(a, b);
   const int seen = a.causal ? len - a.Tq + t + 1 : len;
   const int ns = seen > 0 ? (seen + kSplit - 1) / kSplit : 0;
-  float M = -INFINITY, Ls = 0.0f, A[4] = {0.f, 0.f, 0.f, 0.f};
-  uint32_t kinds[4] = {0, 0, 0, 0};
+  float M = -INFINITY, Ls = 0.0f, A[2] = {0.f, 0.f};
+  uint32_t kinds[2] = {0, 0};
   const int64_t p0 = row * a.nsplit;
-  for (int i0 = 0; i0 < ns; i0 += 4) {                    // four splits' partials requested together
-    float pm[4], pl[4];
-    f32x4 pa[4];
+  for (int i0 = 0; i0 < ns; i0 += kDeep) {
+    float pm[kDeep], pl[kDeep];
+    f32x2m pa[kDeep];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < kDeep; ++j) {
       const int64_t p = p0 + min(i0 + j, ns - 1);
       pm[j] = a.pm[p];
       pl[j] = a.pl[p];
-      pa[j] = *reinterpret_cast<const f32x4*>(a.pacc + p * D + d);
+      pa[j] = *reinterpret_cast<const f32x2m*>(a.pacc + p * D + d);
     }
+    float odd = 0.0f;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < kDeep; ++j) {
       if (i0 + j < ns && (pm[j] > -INFINITY || pl[j] != 0.0f)) {
-        const float acc[4] = {pa[j][0], pa[j][1], pa[j][2], pa[j][3]};
-        merge_split<4>(M, Ls, A, pm[j], pl[j], acc);
+        const float acc[2] = {pa[j][0], pa[j][1]};
+        merge_split<2>(M, Ls, A, pm[j], pl[j], acc);
       }
+      odd += pa[j][0] + pa[j][1];                         // (the last split several times: no matter)
     }
-    const f32x4 any = (pa[0] + pa[1]) + (pa[2] + pa[3]);  // (the last split several times: no matter)
-    const float odd = (any[0] + any[1]) + (any[2] + any[3]);
     if (odd != odd) {                                     // a NaN among them
 #pragma unroll
-      for (int j = 0; j < 4; ++j)
+      for (int j = 0; j < kDeep; ++j)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) kinds[e] |= seen_kinds(pa[j][e]);
+        for (int e = 0; e < 2; ++e) kinds[e] |= seen_kinds(pa[j][e]);
     }
   }
   T* o = static_cast<T*>(a.out) + row * D + d;
 #pragma unroll
-  for (int e = 0; e < 4; ++e)
+  for (int e = 0; e < 2; ++e)
     o[e] = to_store<T>(kinds[e] ? seen_value(kinds[e], Ls) : Ls != 0.0f ? A[e] / Ls : 0.0f);
 }
 
