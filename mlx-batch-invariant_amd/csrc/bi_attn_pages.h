@@ -21,33 +21,39 @@ __device__ __forceinline__ int pages_len(const PagesArgs& a, int b) {
   return a.kv_lens ? min(max(a.kv_lens[b], 0), a.L) : a.L;
 }
 
-// The same of a wave-uniform sequence, by a scalar load: waiting for it does not wait
+// x / d for x >= 0 from inv = inverse(d).
+__device__ __forceinline__ int quotient(int x, int d, unsigned inv) {
+  const int q = (int)__umulhi((unsigned)x, inv);          // or one less
+  return x - q * d >= d ? q + 1 : q;
+}
+
+// The length of a wave-uniform sequence, by a scalar load: waiting for it does not wait
 // for the vector loads in flight, which return in order.
 __device__ __forceinline__ int pages_len_uniform(const PagesArgs& a, int b) {
   if (!a.kv_lens) return a.L;
   return min(max(load_uniform_i32(a.kv_lens + __builtin_amdgcn_readfirstlane(b)), 0), a.L);
 }
 
-// The operands of a P.V step in LDS, the two halves of a lane 64 lanes apart.
+// The operands of a P.V step in LDS, the two halves of a lane `half` pieces apart.
 template <typename T>
-__device__ __forceinline__ void store_pfrag(u32x4* p, const PFrag<T>& pf) {
+__device__ __forceinline__ void store_pfrag(u32x4* p, int half, const PFrag<T>& pf) {
   if constexpr (sizeof(T) == 2) {
     p[0] = __builtin_bit_cast(u32x4, pf.hi);
-    p[kWave] = __builtin_bit_cast(u32x4, pf.lo);
+    p[half] = __builtin_bit_cast(u32x4, pf.lo);
   } else {
     p[0] = __builtin_bit_cast(u32x4, pf.f.lo);
-    p[kWave] = __builtin_bit_cast(u32x4, pf.f.hi);
+    p[half] = __builtin_bit_cast(u32x4, pf.f.hi);
   }
 }
 template <typename T>
-__device__ __forceinline__ PFrag<T> load_pfrag(const u32x4* p) {
+__device__ __forceinline__ PFrag<T> load_pfrag(const u32x4* p, int half) {
   PFrag<T> pf;
   if constexpr (sizeof(T) == 2) {
     pf.hi = __builtin_bit_cast(typename Frag<T>::type, p[0]);
-    pf.lo = __builtin_bit_cast(typename Frag<T>::type, p[kWave]);
+    pf.lo = __builtin_bit_cast(typename Frag<T>::type, p[half]);
   } else {
     pf.f.lo = __builtin_bit_cast(f32x4, p[0]);
-    pf.f.hi = __builtin_bit_cast(f32x4, p[kWave]);
+    pf.f.hi = __builtin_bit_cast(f32x4, p[half]);
   }
   return pf;
 }
@@ -62,8 +68,9 @@ __device__ __forceinline__ PFrag<T> load_pfrag(const u32x4* p) {
 // shared splits are whole and lie within the first sequence's own keys.
 // ---------------------------------------------------------------------------
 constexpr int kPlanThreads = 1024;
-constexpr int kPlanRounds = 4;           // items a workgroup of the resident grid gets, at least, where chunks allow
+constexpr int kPlanRounds = 1;           // items a workgroup of the resident grid gets, at least, where chunks allow
 constexpr int kPlanMostChunks = 32;
+constexpr int kPlanCached = 2048;        // segments whose first items a workgroup keeps in LDS
 
 __device__ __forceinline__ int plan_start(const PagesArgs& a, int n) {
   return a.starts ? min(max(a.starts[n], 0), a.B) : n ? a.B : 0;
@@ -177,314 +184,6 @@ static __global__ __launch_bounds__(kPlanThreads) void pages_plan_kernel(PagesAr
   }
 }
 
-// ---------------------------------------------------------------------------
-// One 256-thread workgroup per item (segment, split, kv head, run of 16-row
-// chunks), a resident grid over all items. Wave w scores keys 64 w .. 64 w + 63
-// of the split (K in registers, dequantized there), the maxima are exchanged
-// through LDS, each wave leaves its keys' weights there as the operands of the
-// P.V steps, and wave w computes the dims 16 dt, dt = NJ w .. NJ w + NJ - 1, from
-// the split's V in LDS. BITS 0: rows of T; 8 or 4: codes.
-// ---------------------------------------------------------------------------
-template <typename T, int D>
-constexpr int pages_v_slices() {
-  return (kSplit * D * (int)sizeof(T) + (128 << 10) - 1) >> 17;
-}
-
-template <typename T, int D, int BITS>
-__global__ __launch_bounds__(256) void attn_pages(PagesArgs a) {
-  typedef typename Frag<T>::type F;
-  constexpr int NVP = pages_v_slices<T, D>();
-  constexpr int DV = D / NVP;
-  typedef KVTile<T, DV> KV;
-  constexpr int KT = 4, KS = D / 32;
-  constexpr int NDTV = DV / 16, NJ = (NDTV + 3) / 4;
-  constexpr int CPW = KV::copies(kSplit) / 4;
-  static_assert(DV % 32 == 0 && CPW >= 1, "attn_pages: V slice tiling");
-  __shared__ __attribute__((aligned(1024))) char Vs[kSplit * KV::kRowBytes];
-  __shared__ u32x4 Ps[8][2][kWave];                       // P.V operands of every 32-key step
-  __shared__ float mx[4][16];
-  __shared__ int pg[kSplit];                              // page of each key of the split
-
-  const int tid = threadIdx.x;
-  const int lane = tid % kWave;
-  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
-  const int r = lane % 16, qq = lane / 16;
-  const int G = a.Hq / a.Hkv, rows1 = a.Tq * G;
-  const bool direct = a.nsplit == 1;
-  const int page_mask = (1 << a.page_shift) - 1;
-  // Neighbouring items on one XCD (workgroups reach the 8 of them in turn): the
-  // chunks of one split, and the heads of one page, share its cache.
-  const int w0 = (int)(blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8);
-
-  const int items = a.plan[0], per = a.plan[1], nseg = a.groups + a.B;
-  const int32_t* seg = a.plan + 2;
-  for (int item = w0; item < items; item += (int)gridDim.x) {
-    // the last segment that starts at or before the item (ones without items share a start with the next)
-    int at = 0;
-    for (int step = 1 << (31 - __builtin_clz(nseg)); step > 0; step >>= 1)
-      if (at + step < nseg && seg[(int64_t)(at + step) * kPlanWords] <= item) at += step;
-    at = __builtin_amdgcn_readfirstlane(at);
-    const int32_t* sg = seg + (int64_t)at * kPlanWords;
-    int seq0 = sg[1];
-    const int nseq = sg[2];
-    const int runs = (int)(((int64_t)nseq * rows1 + 16 * per - 1) / (16 * per));
-    const int local = item - sg[0], x = local / runs;
-    const int chunk0 = (local - x * runs) * per;
-    int hk = x % a.Hkv, split = sg[3] + x / a.Hkv;
-    seq0 = __builtin_amdgcn_readfirstlane(seq0);
-    hk = __builtin_amdgcn_readfirstlane(hk);
-    split = __builtin_amdgcn_readfirstlane(split);
-    const int nrows = nseq * rows1;                       // of the segment
-    const int j0 = split * kSplit;
-    const int len0 = pages_len_uniform(a, seq0);
-    const int n_act = min(kSplit, len0 - j0);
-    // Row p of the segment: its index among the outputs, the keys of the split that it may see.
-    auto row_of = [&](int p, int& b, int& h, int& t) {
-      const int x = p / rows1;
-      b = seq0 + x;
-      p -= x * rows1;
-      t = p / G;
-      h = hk * G + p - t * G;
-    };
-    if (n_act <= 0) {                                     // (direct, an empty sequence) no keys: zeros
-      for (int i = tid; i < nrows * D; i += 256) {
-        int b, h, t;
-        row_of(i / D, b, h, t);
-        static_cast<T*>(a.out)[(((int64_t)b * a.Hq + h) * a.Tq + t) * D + i % D] = (T)0.0f;
-      }
-      continue;
-    }
-
-    {                                                     // pages of the split's keys
-      const int pos = j0 + min(tid, n_act - 1);
-      pg[tid] = clamp_page(a.table[(int64_t)seq0 * a.table_stride + (pos >> a.page_shift)], a.num_pages);
-    }
-    __syncthreads();
-
-    auto q_frags = [&](int chunk, F (&qf)[KS]) {
-      const int p = 16 * chunk + r;
-      int b, h, t;
-      row_of(min(p, nrows - 1), b, h, t);
-      const T* qrow = static_cast<const T*>(a.q) + (int64_t)b * a.q_sb + (int64_t)h * a.q_sh + (int64_t)t * a.q_st;
-#pragma unroll
-      for (int st = 0; st < KS; ++st) qf[st] = p < nrows ? frag_load(qrow + 32 * st + 8 * qq) : frag_zero<F>();
-    };
-    F qf[KS];
-    q_frags(chunk0, qf);
-    F kf[KT][KS];
-#pragma unroll
-    for (int t = 0; t < KT; ++t) {
-      const int key = min(64 * wave + 16 * t + r, n_act - 1);
-      const int64_t page = pg[key];
-      const int row = (j0 + key) & page_mask;
-      if constexpr (BITS == 0) {
-        const T* kr = static_cast<const T*>(a.k) + page * a.k_sp + hk * a.k_sh + row * a.k_sl + 8 * qq;
-#pragma unroll
-        for (int st = 0; st < KS; ++st) kf[t][st] = frag_load(kr + 32 * st);
-      } else {
-        const char* kr = static_cast<const char*>(a.k) + page * a.k_sp + hk * a.k_sh + row * a.k_sl + qq * BITS;
-        const T* kg = static_cast<const T*>(a.kg) + page * a.kg_sp + hk * a.kg_sh + row * a.kg_sl;
-#pragma unroll
-        for (int st = 0; st < KS; ++st)
-          kf[t][st] = dequant_frag<T, BITS>(load_codes8<BITS>(kr + 4 * BITS * st), load_pair(kg + 2 * (32 * st >> a.gshift)));
-      }
-    }
-    auto copy_v = [&](int vp) __attribute__((always_inline)) {
-      if constexpr (BITS == 0) {
-        auto vrow = [&](int key) {
-          return static_cast<const T*>(a.v) + (int64_t)pg[key] * a.v_sp + hk * a.v_sh +
-                 (int64_t)((j0 + key) & page_mask) * a.v_sl + vp * DV;
-        };
-#pragma unroll
-        for (int c = 0; c < CPW; ++c) KV::template copy<true>(Vs, wave * CPW + c, vrow, n_act, lane);
-      } else {
-        constexpr int PPR = DV / 16;                      // pieces of 16 codes per row
-#pragma unroll
-        for (int i = 0; i < PPR; ++i) {
-          const int f = tid + 256 * i, key = f / PPR, d = (f - key * PPR) * 16 + vp * DV;
-          const int at = min(key, n_act - 1);
-          const int64_t page = pg[at];
-          const int row = (j0 + at) & page_mask;
-          const char* vr = static_cast<const char*>(a.v) + page * a.v_sp + hk * a.v_sh + row * a.v_sl + d / 8 * BITS;
-          const T* vg = static_cast<const T*>(a.vg) + page * a.vg_sp + hk * a.vg_sh + row * a.vg_sl;
-          const Codes16<BITS> c = load_codes16<BITS>(vr);
-          const Pair<T> g = load_pair(vg + 2 * (d >> a.gshift));
-          const int dv = d - vp * DV;
-#pragma unroll
-          for (int h = 0; h < 2; ++h) {
-            const F x = dequant_frag<T, BITS>(c.half(h), g);
-            if constexpr (sizeof(T) == 2) {
-              *reinterpret_cast<u32x4*>(Vs + KV::template off<true>(key, dv / 8 + h)) = __builtin_bit_cast(u32x4, x);
-            } else {
-              *reinterpret_cast<f32x4*>(Vs + KV::template off<true>(key, dv / 4 + 2 * h)) = x.lo;
-              *reinterpret_cast<f32x4*>(Vs + KV::template off<true>(key, dv / 4 + 2 * h + 1)) = x.hi;
-            }
-          }
-        }
-      }
-    };
-    if constexpr (NVP == 1) copy_v(0);
-
-    const int chunks = min(per, (nrows - 16 * chunk0 + 15) / 16);
-    for (int c = 0; c < chunks; ++c) {
-      const int chunk = chunk0 + c;
-      // This lane's row of the scores.
-      int lim = 0, row = -1;
-      {
-        const int p = 16 * chunk + r;
-        if (p < nrows) {
-          int b, h, t;
-          row_of(p, b, h, t);
-          const int len = pages_len(a, b);
-          lim = (a.causal ? len - a.Tq + t + 1 : len) - j0;
-          row = (b * a.Hq + h) * a.Tq + t;
-        }
-      }
-      const bool any = __ballot(lim > 0) != 0;            // (the same in every wave)
-      if (!any && !direct) {
-        if (c + 1 < chunks) q_frags(chunk + 1, qf);
-        continue;
-      }
-      float s[KT][4];
-      float m = -INFINITY;
-#pragma unroll
-      for (int t = 0; t < KT; ++t) {
-        f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int st = 0; st < KS; ++st) acc = mfma_step(kf[t][st], qf[st], acc);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          s[t][i] = 64 * wave + 16 * t + 4 * qq + i < lim ? acc[i] * a.scale_log2 : -INFINITY;
-          m = fmaxf(m, s[t][i]);
-        }
-      }
-      if (c + 1 < chunks) q_frags(chunk + 1, qf);
-      m = quarter_max(m);
-      if (qq == 0) mx[wave][r] = m;
-      __syncthreads();
-      m = fmaxf(fmaxf(mx[0][r], mx[1][r]), fmaxf(mx[2][r], mx[3][r]));
-      const float msub = m == -INFINITY ? 0.0f : m;       // no visible key: weights 0, not NaN
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        float p8[8];
-#pragma unroll
-        for (int e = 0; e < 8; ++e) p8[e] = __builtin_amdgcn_exp2f(s[2 * h + e / 4][e % 4] - msub);
-        const PFrag<T> pf = make_pfrag<T>(p8);
-        store_pfrag<T>(&Ps[2 * wave + h][0][lane], pf);
-      }
-      if (!direct && wave == 0 && qq == 0 && lim > 0) a.pm[(int64_t)row * a.nsplit + split] = m;
-      int arow[4], alim[4];                               // the rows of the accumulators, 4 qq + i
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        arow[i] = __shfl(row, 4 * qq + i, kWave);
-        alim[i] = __shfl(lim, 4 * qq + i, kWave);
-      }
-      const int sum_wave = c & 3;                         // which wave adds up the weights
-      f32x4 lsum = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int vp = 0; vp < NVP; ++vp) {
-        if constexpr (NVP > 1) {
-          __syncthreads();                                // every wave is done with the last slice
-          copy_v(vp);
-        }
-        stage_barrier<0>();                               // V landed, weights visible
-        f32x4 acc[NJ];
-        // P.V of this wave's dim tiles; `clean` takes infinities and NaN of V as 0.
-        auto weigh = [&](bool clean, bool sum) __attribute__((always_inline)) {
-#pragma unroll
-          for (int j = 0; j < NJ; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 2
-          for (int ks = 0; ks < kSplit / 32; ++ks) {
-            const PFrag<T> pf = load_pfrag<T>(&Ps[ks][0][lane]);
-#pragma unroll
-            for (int j = 0; j < NJ; ++j) {
-              if (NJ * wave + j >= NDTV) continue;
-              F v = KV::vfrag(Vs, 32 * ks, NJ * wave + j, lane);
-              if (clean) v = finite_frag(v);
-              acc[j] = pv_step<T>(pf, v, acc[j]);
-            }
-            if (sum) lsum = pv_step<T>(pf, ones_frag<T>(), lsum);
-          }
-        };
-        weigh(false, vp == 0 && (wave == sum_wave || direct));
-        // A hidden key's weight 0 times an infinity or NaN of its V row is NaN: such a
-        // wave weighs again without them and notes the ones its rows see (kSeenTag).
-        bool finite = true;
-#pragma unroll
-        for (int j = 0; j < NJ; ++j)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) finite = finite && (NJ * wave + j >= NDTV || fabsf(acc[j][i]) < INFINITY);
-        if (__ballot(!finite)) {
-          weigh(true, false);
-          for (int key = 0; key < n_act; ++key) {
-#pragma unroll
-            for (int j = 0; j < NJ; ++j) {
-              if (NJ * wave + j >= NDTV) continue;
-              const int dim = 16 * (NJ * wave + j) + r;
-              constexpr int kPer = 16 / (int)sizeof(T);
-              const float x = to_f32(reinterpret_cast<const T*>(Vs + KV::template off<true>(key, dim / kPer))[dim % kPer]);
-              if (fabsf(x) < INFINITY) continue;
-#pragma unroll
-              for (int i = 0; i < 4; ++i)
-                if (key < alim[i]) acc[j][i] = note_seen(acc[j][i], x);
-            }
-          }
-        }
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-          if (NJ * wave + j >= NDTV) continue;
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int d = vp * DV + 16 * (NJ * wave + j) + r;
-            if (direct) {
-              if (arow[i] >= 0) static_cast<T*>(a.out)[(int64_t)arow[i] * D + d] = to_store<T>(only_split(acc[j][i], lsum[i]));
-            } else if (alim[i] > 0) {
-              a.pacc[((int64_t)arow[i] * a.nsplit + split) * D + d] = acc[j][i];
-            }
-          }
-        }
-      }
-      if (!direct && wave == sum_wave && r == 0) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (alim[i] > 0) a.pl[(int64_t)arow[i] * a.nsplit + split] = lsum[i];
-      }
-    }
-    __syncthreads();                                      // every wave is done with Vs, pg before the next item's
-  }
-}
-
-// ---------------------------------------------------------------------------
-// Codes, at most 16 rows a sequence and kv head (a decode step, a few draft tokens):
-// the codes of V stay codes in LDS. One 256-thread workgroup per item (sequence,
-// split, kv head), neighbouring items on one XCD. Wave w's keys are 64 w .. 64 w + 63
-// of the split, lane l's page that of key 64 w + l (read an item ahead), so that a
-// wave finds all its rows by lane exchanges; it scores them with K dequantized in
-// registers. For P.V wave w takes the dims 16 dt, dt = NJ w .. NJ w + NJ - 1: a
-// transposing LDS read gives a lane the codes of 8 keys (4 bits: 16) of one dim, and
-// each is dequantized once, with its key's pair from LDS.
-// ---------------------------------------------------------------------------
-// The tile of V's codes: row r, 16-byte chunk c in slot c ^ key(r) where a row holds a
-// power of two of them, so that the rows of a transposing read (32 keys, one chunk)
-// fall in distinct banks.
-template <int D, int BITS>
-struct CodeTile {
-  static constexpr int kRowBytes = D * BITS / 8;
-  static constexpr int kCPR = kRowBytes / 16;
-  static constexpr bool kSwz = (kCPR & (kCPR - 1)) == 0;
-  static __device__ __forceinline__ int key(int r) {
-    const int x = (r & 7) | (r >> 4 & 1) << 3;
-    return !kSwz ? 0 : kCPR == 16 ? x : kCPR == 8 ? x >> 1 : kCPR == 4 ? x >> 2 : kCPR == 2 ? x >> 3 : 0;
-  }
-  static __device__ __forceinline__ int off(int r, int c) { return r * kRowBytes + ((c ^ key(r)) << 4); }
-};
-
-typedef int i32x2_t __attribute__((ext_vector_type(2)));
-typedef __attribute__((address_space(3))) i32x2_t lds_i32x2;
-// (restrict: see lds_read_tr16)
-__device__ __forceinline__ i32x2_t lds_read_tr8(lds_i32x2* __restrict p) { return __builtin_amdgcn_ds_read_tr8_b64_v2i32(p); }
-__device__ __forceinline__ i32x2_t lds_read_tr4(lds_i32x2* __restrict p) { return __builtin_amdgcn_ds_read_tr4_b64_v2i32(p); }
-
 // The codes of K row r that lane (r, qq) needs as score operands, dims 32 st + 8 qq .. + 7
 // of every step st, are pieces of 8 or 4 bytes. A lane reads 16 bytes instead, the
 // row's four lanes 64 in a run: two steps of 8 bits (lane qq half of step qq / 2) or four
@@ -559,6 +258,394 @@ struct KRow {
   }
 };
 
+// ---------------------------------------------------------------------------
+// One 256-thread workgroup per item (segment, split, kv head, run of 16-row
+// chunks), a resident grid over all items. Wave w's keys are 64 w .. 64 w + 63 of the
+// split, lane l's page that of key 64 w + l. K of those keys stays in the wave's
+// registers and V of the split in LDS (codes: dequantized once), so that a chunk of
+// rows costs its Q^T, its products and the exchange of maxima and weights. Wave w takes
+// the dims 16 dt, dt = NJ w .. NJ w + NJ - 1, of P.V. (fp32 rows of more than 128 dims: V
+// in two slices, copied for every chunk.) BITS 0: rows of T; 8 or 4: codes.
+// ---------------------------------------------------------------------------
+template <typename T, int D>
+constexpr int pages_v_slices() {
+  return (kSplit * D * (int)sizeof(T) + (128 << 10) - 1) >> 17;
+}
+// Workgroups per CU that the registers are held to: two where LDS has room for both.
+template <typename T, int D>
+constexpr int pages_min_blocks() {
+  return sizeof(T) == 2 && D <= 128 ? 2 : 1;
+}
+
+template <typename T, int D, int BITS>
+__global__ __launch_bounds__(256, (pages_min_blocks<T, D>())) void attn_pages(PagesArgs a) {
+  typedef typename Frag<T>::type F;
+  constexpr int NVP = pages_v_slices<T, D>();
+  constexpr int DV = D / NVP;
+  typedef KVTile<T, DV> KV;
+  constexpr int KT = 4, KS = D / 32;
+  constexpr int NDTV = DV / 16, NJ = (NDTV + 3) / 4;
+  constexpr int CPW = KV::copies(kSplit) / 4;
+  constexpr int kPBytes = 8 * 2 * kWave * 16;             // P.V operands of every 32-key step
+  constexpr int kVBytes = kSplit * KV::kRowBytes;
+  // Rows of 256 bytes: V fills 64 KB, and with the weights behind it two workgroups
+  // would not fit a CU. Its last two steps go to registers and the weights over them.
+  constexpr int KEEP = NVP == 1 && kVBytes == (64 << 10) ? 2 : 0;
+  constexpr int kPAt = kVBytes - KEEP * 32 * KV::kRowBytes;
+  static_assert(DV % 32 == 0 && CPW >= 1 && kPBytes >= KEEP * 32 * KV::kRowBytes, "attn_pages: V slice tiling");
+  __shared__ __attribute__((aligned(1024))) char Vs[kPAt + kPBytes];
+  __shared__ float mx[4][16];
+  extern __shared__ int first_s[];                        // first items of the segments, if they fit
+  u32x4* const Ps = reinterpret_cast<u32x4*>(Vs + kPAt);
+
+  const int tid = threadIdx.x;
+  const int lane = tid % kWave;
+  const int wave = __builtin_amdgcn_readfirstlane(tid / kWave);
+  const int r = lane % 16, qq = lane / 16;
+  const int G = a.Hq / a.Hkv, rows1 = a.Tq * G;
+  const bool direct = a.nsplit == 1;
+  const int page_mask = (1 << a.page_shift) - 1;
+  // Neighbouring items on one XCD (workgroups reach the 8 of them in turn): the
+  // chunks of one split, and the heads of one page, share its cache.
+  const int w0 = (int)(blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8);
+  const int dt0 = min(NJ * wave, NDTV - NJ < 0 ? 0 : NDTV - 1);   // this wave's first dim tile (a wave without one repeats the last)
+
+  const int items = a.plan[0], per = a.plan[1], nseg = a.groups + a.B;
+  const int32_t* seg = a.plan + 2;
+  struct Item { int seq0, nseq, split, hk, chunk0, n_act; };   // n_act < 0: no more items
+  auto locate = [&](int item) -> Item {
+    if (item >= items) return Item{0, 0, 0, 0, 0, -1};
+    // the last segment that starts at or before the item (ones without items share a start with the next)
+    int at = 0;
+    if (nseg <= kPlanCached) {
+      for (int i = lane; i < nseg; i += kWave) at += __popcll(__ballot(first_s[i] <= item));   // (starts rise)
+      at = __builtin_amdgcn_readfirstlane(at) - 1;
+    } else {
+      for (int step = 1 << (31 - __builtin_clz(nseg)); step > 0; step >>= 1)
+        if (at + step < nseg && load_uniform_i32(uniform_ptr(seg + (int64_t)(at + step) * kPlanWords)) <= item) at += step;
+    }
+    const int32_t* sg = uniform_ptr(seg + (int64_t)at * kPlanWords);
+    int w[4];
+    load_uniform4_i32(sg, sg + 1, sg + 2, sg + 3, w);
+    Item it;
+    it.seq0 = w[1];
+    it.nseq = w[2];
+    const int runs = (int)(((int64_t)it.nseq * rows1 + 16 * per - 1) / (16 * per));
+    const int local = item - w[0], x = local / runs, y = quotient(x, a.Hkv, a.hkv_inv);
+    it.chunk0 = (local - x * runs) * per;
+    it.hk = x - y * a.Hkv;
+    it.split = w[3] + y;
+    it.n_act = min(kSplit, pages_len_uniform(a, it.seq0) - it.split * kSplit);
+    return it;
+  };
+  auto page_of = [&](const Item& it) {
+    if (it.n_act <= 0) return 0;
+    const int pos = it.split * kSplit + min(tid, it.n_act - 1);
+    return a.table[(int64_t)it.seq0 * a.table_stride + (pos >> a.page_shift)];
+  };
+
+  if (nseg <= kPlanCached) {
+    for (int i = tid; i < nseg; i += 256) first_s[i] = seg[(int64_t)i * kPlanWords];
+    __syncthreads();
+  }
+  Item it = locate(w0);
+  int page = page_of(it);
+  for (int item = w0; it.n_act >= 0; item += (int)gridDim.x) {
+    const int seq0 = it.seq0, hk = it.hk, split = it.split, chunk0 = it.chunk0, n_act = it.n_act;
+    const int nrows = it.nseq * rows1, j0 = split * kSplit;   // rows of the segment
+    // Row p of the segment: (sequence, head, token).
+    auto row_of = [&](int p, int& b, int& h, int& t) {
+      const int x = quotient(p, rows1, a.rows1_inv);
+      b = seq0 + x;
+      p -= x * rows1;
+      t = quotient(p, G, a.g_inv);
+      h = hk * G + p - t * G;
+    };
+    if (n_act == 0) {                                     // (direct, an empty sequence) no keys: zeros
+      for (int i = tid; i < nrows * D; i += 256) {
+        int b, h, t;
+        row_of(i / D, b, h, t);
+        static_cast<T*>(a.out)[(((int64_t)b * a.Hq + h) * a.Tq + t) * D + i % D] = (T)0.0f;
+      }
+      it = locate(item + (int)gridDim.x);
+      page = page_of(it);
+      continue;
+    }
+
+    // A chunk's rows: this lane's Q^T, its index among the outputs (-1: none), and how
+    // many keys of the split it may see.
+    struct Rows { F qf[KS]; int row, lim; };
+    auto request_rows = [&](int chunk, Rows& x) __attribute__((always_inline)) {
+      const int p = 16 * chunk + r;
+      int b, h, t;
+      row_of(min(p, nrows - 1), b, h, t);
+      const T* qrow = static_cast<const T*>(a.q) + (int64_t)b * a.q_sb + (int64_t)h * a.q_sh + (int64_t)t * a.q_st;
+#pragma unroll
+      for (int st = 0; st < KS; ++st) x.qf[st] = frag_load(qrow + 32 * st + 8 * qq);   // (columns without a row are never stored)
+      const int len = pages_len(a, b);
+      x.row = p < nrows ? (b * a.Hq + h) * a.Tq + t : -1;
+      x.lim = p < nrows ? (a.causal ? len - a.Tq + t + 1 : len) - j0 : 0;
+    };
+    // This lane's key; the others' offsets come by lane exchanges.
+    const int64_t my_page = clamp_page(page, a.num_pages);
+    const int64_t my_row = (j0 + min(tid, n_act - 1)) & page_mask;
+    const int64_t k_off = my_page * a.k_sp + my_row * a.k_sl, v_off = my_page * a.v_sp + my_row * a.v_sl;
+    auto off_of = [&](int64_t off, int l) {
+      return (int64_t)((uint64_t)(uint32_t)__shfl((int)(uint32_t)off, l, kWave) |
+                       (uint64_t)(uint32_t)__shfl((int)(uint32_t)((uint64_t)off >> 32), l, kWave) << 32);
+    };
+    const char* kb = uniform_ptr(static_cast<const char*>(a.k) + hk * a.k_sh * (BITS ? 1 : (int)sizeof(T)));
+    const char* vb = uniform_ptr(static_cast<const char*>(a.v) + hk * a.v_sh * (BITS ? 1 : (int)sizeof(T)));
+    // V of the wave's 64 keys to LDS, codes as the values they stand for.
+    auto copy_v = [&](int vp) __attribute__((always_inline)) {
+      int l = lane;
+      asm volatile("" : "+v"(l));                         // (offsets within tiles are not kept over the items)
+      if constexpr (BITS == 0) {
+#pragma unroll
+        for (int c = 0; c < CPW; ++c) {
+          const int f = 64 * c + l, row = f / KV::kCPR, slot = f - row * KV::kCPR;   // of the wave's rows
+          const T* vr = reinterpret_cast<const T*>(vb) + off_of(v_off, row) + vp * DV;
+          copy_to_lds16(vr + (slot ^ KV::template key<true>(64 * wave + row)) * (16 / (int)sizeof(T)), Vs + 1024 * (wave * CPW + c));
+          if (c % 4 == 3) __builtin_amdgcn_sched_barrier(0);   // (a few addresses at a time)
+        }
+      } else {
+        constexpr int PPR = DV / 16;                      // pieces of 16 codes per row
+        const int64_t vg_off = my_page * a.vg_sp + my_row * a.vg_sl;
+#pragma unroll
+        for (int i = 0; i < PPR; ++i) {
+          const int f = l + 64 * i, row = f / PPR, dv = (f - row * PPR) * 16, d = dv + vp * DV;
+          const Codes16<BITS> c = load_codes16<BITS>(vb + off_of(v_off, row) + d / 8 * BITS);
+          const Pair<T> g = load_pair(static_cast<const T*>(a.vg) + hk * a.vg_sh + off_of(vg_off, row) + 2 * (d >> a.gshift));
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const F x = dequant_frag<T, BITS>(c.half(h), g);
+            if constexpr (sizeof(T) == 2) {
+              *reinterpret_cast<u32x4*>(Vs + KV::template off<true>(64 * wave + row, dv / 8 + h)) = __builtin_bit_cast(u32x4, x);
+            } else {
+              *reinterpret_cast<f32x4*>(Vs + KV::template off<true>(64 * wave + row, dv / 4 + 2 * h)) = x.lo;
+              *reinterpret_cast<f32x4*>(Vs + KV::template off<true>(64 * wave + row, dv / 4 + 2 * h + 1)) = x.hi;
+            }
+          }
+        }
+      }
+    };
+    F vf[KEEP ? KEEP : 1][NJ];
+    if constexpr (NVP == 1) copy_v(0);
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+    Rows rows;
+    request_rows(chunk0, rows);
+    F kf[KT][KS];
+    if constexpr (BITS == 0) {
+#pragma unroll
+      for (int t = 0; t < KT; ++t) {
+        const T* kr = reinterpret_cast<const T*>(kb) + off_of(k_off, 16 * t + r) + 8 * qq;
+#pragma unroll
+        for (int st = 0; st < KS; ++st) kf[t][st] = frag_load(kr + 32 * st);
+      }
+    } else {
+      const int64_t kg_off = my_page * a.kg_sp + my_row * a.kg_sl;
+      KRow<KS, BITS> kc[KT];
+      Pair<T> g[KT][KS];
+#pragma unroll
+      for (int t = 0; t < KT; ++t) {
+        kc[t].load(kb + off_of(k_off, 16 * t + r), 0u, qq);
+        const T* kg = static_cast<const T*>(a.kg) + hk * a.kg_sh + off_of(kg_off, 16 * t + r);
+#pragma unroll
+        for (int st = 0; st < KS; ++st) g[t][st] = load_pair(kg + 2 * (32 * st >> a.gshift));
+      }
+#pragma unroll
+      for (int t = 0; t < KT; ++t) {
+        kc[t].arrange();
+#pragma unroll
+        for (int st = 0; st < KS; ++st) kf[t][st] = dequant_frag<T, BITS>(kc[t].codes(st), g[t][st]);
+      }
+    }
+    asm volatile("" ::: "memory");
+
+    it = locate(item + (int)gridDim.x);                   // the next item's pages
+    page = page_of(it);
+    if constexpr (KEEP > 0) {
+      stage_barrier<0>();                                 // V landed
+#pragma unroll
+      for (int k = 0; k < KEEP; ++k)
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) vf[k][j] = KV::vfrag(Vs, 32 * (8 - KEEP + k), min(dt0 + j, NDTV - 1), lane);
+      stage_barrier<63>();                                // read by everyone
+    }
+
+    const int chunks = min(per, (nrows - 16 * chunk0 + 15) / 16);
+    bool landed = false;
+    for (int c = 0; c < chunks; ++c) {
+      const int row = rows.row, lim = rows.lim;
+      if (!direct && !__ballot(lim > 0)) {                // no partials: the merge reads none (the same in every wave)
+        if (c + 1 < chunks) request_rows(chunk0 + c + 1, rows);
+        continue;
+      }
+      float s[KT][4];
+      float m = -INFINITY;
+      auto scores = [&](auto masked) __attribute__((always_inline)) {
+#pragma unroll
+        for (int t = 0; t < KT; ++t) {
+          f32x4 acc = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int st = 0; st < KS; ++st) acc = mfma_step(kf[t][st], rows.qf[st], acc);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const bool seen = !decltype(masked)::value || 64 * wave + 16 * t + 4 * qq + i < lim;
+            s[t][i] = seen ? acc[i] * a.scale_log2 : -INFINITY;
+            m = fmaxf(m, s[t][i]);
+          }
+        }
+      };
+      if (__ballot(row >= 0 && lim < kSplit)) scores(std::true_type());
+      else scores(std::false_type());
+      if (c + 1 < chunks) request_rows(chunk0 + c + 1, rows);
+      m = quarter_max(m);
+      if (qq == 0) mx[wave][r] = m;
+      stage_barrier<63>();
+      m = fmaxf(fmaxf(mx[0][r], mx[1][r]), fmaxf(mx[2][r], mx[3][r]));
+      const float msub = m == -INFINITY ? 0.0f : m;       // no visible key: weights 0, not NaN
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        float p8[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) p8[e] = __builtin_amdgcn_exp2f(s[2 * h + e / 4][e % 4] - msub);
+        store_pfrag<T>(Ps + (2 * wave + h) * 2 * kWave + lane, kWave, make_pfrag<T>(p8));
+      }
+      if (!direct && wave == 0 && qq == 0 && lim > 0) a.pm[(int64_t)row * a.nsplit + split] = m;
+      int arow[4], alim[4];                               // the rows of the accumulators, 4 qq + i
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        arow[i] = __shfl(row, 4 * qq + i, kWave);
+        alim[i] = __shfl(lim, 4 * qq + i, kWave);
+      }
+      const int sum_wave = c & 3;                         // which wave adds up the weights
+      f32x4 lsum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int vp = 0; vp < NVP; ++vp) {
+        if constexpr (NVP > 1) {
+          __syncthreads();                                // every wave is done with the last slice
+          copy_v(vp);
+          stage_barrier<0>();
+        } else if (KEEP == 0 && !landed) {
+          landed = true;
+          stage_barrier<0>();                             // weights visible, V landed
+        } else {
+          stage_barrier<63>();
+        }
+        f32x4 acc[NJ];
+        int vl = lane;
+        asm volatile("" : "+v"(vl));
+        // P.V of this wave's dim tiles; `clean` takes infinities and NaN of V as 0.
+        // One wave also adds up the weights, a chain beside the others'.
+        auto weigh = [&](bool clean, auto sum) __attribute__((always_inline)) {
+#pragma unroll
+          for (int j = 0; j < NJ; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int ks = 0; ks < kSplit / 32; ++ks) {
+            const PFrag<T> pf = load_pfrag<T>(Ps + ks * 2 * kWave + lane, kWave);
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+              F v = ks < 8 - KEEP ? KV::vfrag(Vs, 32 * ks, min(dt0 + j, NDTV - 1), vl) : vf[ks < 8 - KEEP ? 0 : ks - 8 + KEEP][j];
+              if (clean) v = finite_frag(v);
+              acc[j] = pv_step<T>(pf, v, acc[j]);
+            }
+            if constexpr (decltype(sum)::value) lsum = pv_step<T>(pf, ones_frag<T>(), lsum);
+            if (ks % 4 == 3) __builtin_amdgcn_sched_barrier(0);   // (or every step's reads are gathered in front, and spill)
+          }
+        };
+        if (vp == 0 && (wave == sum_wave || direct)) weigh(false, std::true_type());
+        else weigh(false, std::false_type());
+        // A hidden key's weight 0 times an infinity or NaN of its V row is NaN: such a
+        // wave weighs again without them and notes the ones its rows see (kSeenTag), which
+        // it looks for in the pages.
+        bool finite = true;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) finite = finite && (NJ * wave + j >= NDTV || fabsf(acc[j][i]) < INFINITY);
+        if (__ballot(!finite)) {
+          weigh(true, std::false_type());
+          int dim0 = vp * DV + 16 * dt0 + r;
+          asm volatile("" : "+v"(dim0));
+          for (int key = 0; key < n_act; ++key) {
+            const int pos = j0 + key;
+            const int64_t pg = clamp_page(a.table[(int64_t)seq0 * a.table_stride + (pos >> a.page_shift)], a.num_pages);
+            const int64_t prow = pos & page_mask;
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) {
+              const int dim = min(dim0 + 16 * j, D - 16 + r);
+              float x;
+              if constexpr (BITS == 0) {
+                x = to_f32(reinterpret_cast<const T*>(vb)[pg * a.v_sp + prow * a.v_sl + dim]);
+              } else {
+                const uint32_t code = (uint8_t)vb[pg * a.v_sp + prow * a.v_sl + dim * BITS / 8];
+                const Pair<T> g = load_pair(static_cast<const T*>(a.vg) + hk * a.vg_sh + pg * a.vg_sp + prow * a.vg_sl + 2 * (dim >> a.gshift));
+                x = to_f32(to_store<T>(__builtin_fmaf((float)(BITS == 8 ? code : code >> 4 * (dim & 1) & 15u), g.s, g.b)));
+              }
+              if (fabsf(x) < INFINITY) continue;
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (key < alim[i]) acc[j][i] = note_seen(acc[j][i], x);
+            }
+          }
+        }
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+          if (NJ * wave + j >= NDTV) continue;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int d = vp * DV + 16 * (NJ * wave + j) + r;
+            if (direct) {
+              if (arow[i] >= 0) static_cast<T*>(a.out)[(int64_t)arow[i] * D + d] = to_store<T>(only_split(acc[j][i], lsum[i]));
+            } else if (alim[i] > 0) {
+              a.pacc[((int64_t)arow[i] * a.nsplit + split) * D + d] = acc[j][i];
+            }
+          }
+        }
+      }
+      if (!direct && wave == sum_wave && r == 0) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (alim[i] > 0) a.pl[(int64_t)arow[i] * a.nsplit + split] = lsum[i];
+      }
+    }
+    stage_barrier<63>();                                  // every wave is done with LDS
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Codes, at most 16 rows a sequence and kv head (a decode step, a few draft tokens):
+// the codes of V stay codes in LDS. One 256-thread workgroup per item (sequence,
+// split, kv head), neighbouring items on one XCD. Wave w's keys are 64 w .. 64 w + 63
+// of the split, lane l's page that of key 64 w + l (read an item ahead), so that a
+// wave finds all its rows by lane exchanges; it scores them with K dequantized in
+// registers. For P.V wave w takes the dims 16 dt, dt = NJ w .. NJ w + NJ - 1: a
+// transposing LDS read gives a lane the codes of 8 keys (4 bits: 16) of one dim, and
+// each is dequantized once, with its key's pair from LDS.
+// ---------------------------------------------------------------------------
+// The tile of V's codes: row r, 16-byte chunk c in slot c ^ key(r) where a row holds a
+// power of two of them, so that the rows of a transposing read (32 keys, one chunk)
+// fall in distinct banks.
+template <int D, int BITS>
+struct CodeTile {
+  static constexpr int kRowBytes = D * BITS / 8;
+  static constexpr int kCPR = kRowBytes / 16;
+  static constexpr bool kSwz = (kCPR & (kCPR - 1)) == 0;
+  static __device__ __forceinline__ int key(int r) {
+    const int x = (r & 7) | (r >> 4 & 1) << 3;
+    return !kSwz ? 0 : kCPR == 16 ? x : kCPR == 8 ? x >> 1 : kCPR == 4 ? x >> 2 : kCPR == 2 ? x >> 3 : 0;
+  }
+  static __device__ __forceinline__ int off(int r, int c) { return r * kRowBytes + ((c ^ key(r)) << 4); }
+};
+
+typedef int i32x2_t __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) i32x2_t lds_i32x2;
+// (restrict: see lds_read_tr16)
+__device__ __forceinline__ i32x2_t lds_read_tr8(lds_i32x2* __restrict p) { return __builtin_amdgcn_ds_read_tr8_b64_v2i32(p); }
+__device__ __forceinline__ i32x2_t lds_read_tr4(lds_i32x2* __restrict p) { return __builtin_amdgcn_ds_read_tr4_b64_v2i32(p); }
+
 // N words of memory that is 4-byte aligned.
 template <int N>
 __device__ __forceinline__ void load_words(const void* p, uint32_t* w) {
@@ -580,6 +667,9 @@ __device__ __forceinline__ void load_words(const void* p, uint32_t* w) {
   if constexpr (N % 2 == 1) w[i] = *reinterpret_cast<const uint32_t*>(static_cast<const char*>(p) + 4 * i);
 }
 
+// Rows whose weights a workgroup keeps in LDS (4, 8 or 16).
+__host__ __device__ inline int codes_rows(int rows1) { return rows1 <= 4 ? 4 : rows1 <= 8 ? 8 : 16; }
+
 // Workgroups per CU that the registers are held to.
 template <typename T, int D, int BITS>
 constexpr int codes_min_blocks() {
@@ -596,11 +686,11 @@ __global__ __launch_bounds__(256, (codes_min_blocks<T, D, BITS>())) void attn_co
   constexpr int NG = D / GS;                              // groups of a row
   // Pairs that a wave's dim tiles need: one where they share a group (two tiles from
   // an even one on, four of 64 dims), else one for each or for two of them.
-  constexpr int NS = NJ == 3 ? 3 : NJ == 4 && GS == 32 ? 2 : 1;
+  constexpr int NS = NJ == 3 ? 3 : NJ == 4 && GS == 32 ? 4 : 1;
   __shared__ __attribute__((aligned(1024))) char Vs[kSplit * CT::kRowBytes];
-  __shared__ u32x4 Ps[8][2][kWave];
-  __shared__ float mx[4][16];
   __shared__ __attribute__((aligned(16))) float vsc[NG][kSplit], vbi[NG][kSplit];   // V's scales and biases
+  __shared__ float mx[4][16];
+  extern __shared__ u32x4 Ps[];                           // [step][half][lane row][row of the sequence]
 
   const int tid = threadIdx.x;
   const int lane = tid % kWave;
@@ -611,6 +701,8 @@ __global__ __launch_bounds__(256, (codes_min_blocks<T, D, BITS>())) void attn_co
   // rows are the first register of the accumulators' four lane rows.
   const int my_p = r / 4 + r % 4 * 4;
   const int ni = (rows1 + 3) / 4;                         // registers that hold rows
+  const int rc = codes_rows(rows1);                       // rows that Ps holds; lanes without one read another's
+  const int ps = qq * rc + (my_p & (rc - 1));
   const bool direct = a.nsplit == 1;
   const int page_mask = (1 << a.page_shift) - 1;
   const int w0 = (int)(blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8);
@@ -637,12 +729,8 @@ __global__ __launch_bounds__(256, (codes_min_blocks<T, D, BITS>())) void attn_co
     const int local = item - lo - (i ? __builtin_amdgcn_readlane(incl, max(i - 1, 0)) : 0);
     Item it;
     it.b = 64 * c64 + i;
-    it.split = (int)__umulhi((unsigned)local, a.hkv_inv);  // local / Hkv, or one less
+    it.split = quotient(local, a.Hkv, a.hkv_inv);
     it.hk = local - it.split * a.Hkv;
-    if (it.hk >= a.Hkv) {
-      it.hk -= a.Hkv;
-      ++it.split;
-    }
     it.n_act = min(kSplit, pages_len_uniform(a, it.b) - it.split * kSplit);
     return it;
   };
@@ -654,6 +742,10 @@ __global__ __launch_bounds__(256, (codes_min_blocks<T, D, BITS>())) void attn_co
 
   // (token, head) p of sequence b, heads inside tokens.
   auto out_row = [&](int b, int hk, int p) { return (b * a.Hq + hk * G + p % G) * a.Tq + p / G; };
+  auto off_of = [&](uint64_t off, int l) {
+    return (uint64_t)(uint32_t)__shfl((int)(uint32_t)off, l, kWave) |
+           (uint64_t)(uint32_t)__shfl((int)(uint32_t)(off >> 32), l, kWave) << 32;
+  };
   Item it = locate(w0);
   int page = page_of(it);
   for (int item = w0; it.n_act >= 0; item += (int)gridDim.x) {
@@ -713,10 +805,6 @@ __global__ __launch_bounds__(256, (codes_min_blocks<T, D, BITS>())) void attn_co
       }
     } else {
       const uint64_t k_off = row_off(a.k_sp, a.k_sl), v_off = row_off(a.v_sp, a.v_sl);
-      auto off_of = [&](uint64_t off, int l) {
-        return (uint64_t)(uint32_t)__shfl((int)(uint32_t)off, l, kWave) |
-               (uint64_t)(uint32_t)__shfl((int)(uint32_t)(off >> 32), l, kWave) << 32;
-      };
 #pragma unroll
       for (int t = 0; t < KT; ++t) kc[t].load(kb + off_of(k_off, 16 * t + r), 0u, qq);
       asm volatile("" ::: "memory");
@@ -782,7 +870,7 @@ __global__ __launch_bounds__(256, (codes_min_blocks<T, D, BITS>())) void attn_co
       float p8[8];
 #pragma unroll
       for (int e = 0; e < 8; ++e) p8[e] = __builtin_amdgcn_exp2f(s[2 * h + e / 4][e % 4] - msub);
-      store_pfrag<T>(&Ps[2 * wave + h][0][lane], make_pfrag<T>(p8));
+      if (my_p < rc) store_pfrag<T>(Ps + (2 * wave + h) * 8 * rc + ps, 4 * rc, make_pfrag<T>(p8));
     }
     if (!direct && wave == 0 && qq == 0 && lim > 0) a.pm[(int64_t)row * a.nsplit + split] = m;
     int arow[4], alim[4];                                 // the rows of the accumulators, 4 qq + i
@@ -805,18 +893,18 @@ __global__ __launch_bounds__(256, (codes_min_blocks<T, D, BITS>())) void attn_co
       float s[NS][8], b[NS][8];
     };
     auto read_step = [&](Step& x, int ks) __attribute__((always_inline)) {
-      x.pf = load_pfrag<T>(&Ps[ks][0][lane]);
+      x.pf = load_pfrag<T>(Ps + ks * 8 * rc + ps, 4 * rc);
 #pragma unroll
       for (int i = 0; i < NS; ++i) {
         const int g = min((NJ * wave + (NJ == 3 ? 1 : 2) * i) * 16 / GS, NG - 1);
 #pragma unroll
         for (int h = 0; h < 2; ++h) {
-          const f32x4 sx = *reinterpret_cast<const f32x4*>(&vsc[g][32 * ks + 16 * h + 4 * qq]);
-          const f32x4 bx = *reinterpret_cast<const f32x4*>(&vbi[g][32 * ks + 16 * h + 4 * qq]);
+          const f32x4 s4 = *reinterpret_cast<const f32x4*>(&vsc[g][32 * ks + 16 * h + 4 * qq]);
+          const f32x4 b4 = *reinterpret_cast<const f32x4*>(&vbi[g][32 * ks + 16 * h + 4 * qq]);
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            x.s[i][4 * h + e] = sx[e];
-            x.b[i][4 * h + e] = bx[e];
+            x.s[i][4 * h + e] = s4[e];
+            x.b[i][4 * h + e] = b4[e];
           }
         }
       }
@@ -825,7 +913,8 @@ __global__ __launch_bounds__(256, (codes_min_blocks<T, D, BITS>())) void attn_co
     // further the key repeats.
     int at[NJ];
     {
-      int lr = l % 16;
+      int lr = r;
+      asm volatile("" : "+v"(lr));                     // (not kept over the items)
       const int key = BITS == 8 ? 4 * qq + (lr >> 1 & 3) + (lr >> 1 & 4) * 4 : 32 * (lr >> 3) + 4 * qq + (lr & 3) + (lr & 4) * 4;
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
@@ -877,7 +966,7 @@ __global__ __launch_bounds__(256, (codes_min_blocks<T, D, BITS>())) void attn_co
     const int sum_wave = NDT < 4 * NJ ? 3 : 0;            // (the wave with the fewest dims adds up the weights)
     if (wave == sum_wave || direct) {
 #pragma unroll
-      for (int ks = 0; ks < kSplit / 32; ++ks) lsum = pv_step<T>(load_pfrag<T>(&Ps[ks][0][lane]), ones_frag<T>(), lsum);
+      for (int ks = 0; ks < kSplit / 32; ++ks) lsum = pv_step<T>(load_pfrag<T>(Ps + ks * 8 * rc + ps, 4 * rc), ones_frag<T>(), lsum);
     }
     // A hidden key's weight 0 times an infinity or NaN of its V row is NaN: such a
     // wave weighs again without them and notes the ones its rows see (kSeenTag).

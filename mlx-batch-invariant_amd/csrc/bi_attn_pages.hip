@@ -154,7 +154,9 @@ extern "C" int bi_attn_pages(const void* q, const void* k, const void* k_groups,
       return fail(BI_E_UNSUPPORTED, "%s: page or row stride %lld of codes (below 2^32)", what, (long long)strides[i]);
   auto reach = [&](int i) { return (num_pages - 1) * strides[i] + (Hkv - 1) * strides[i + 1] + (page_size - 1) * strides[i + 2] + D; };
   a.near = bits && reach(3) < ((int64_t)1 << 32) && reach(6) < ((int64_t)1 << 32);
-  a.hkv_inv = Hkv == 1 ? 0xffffffffu : (unsigned)(((int64_t)1 << 32) / Hkv);
+  a.hkv_inv = bi::inverse(Hkv);
+  a.rows1_inv = bi::inverse(rows1);
+  a.g_inv = bi::inverse(Hq / Hkv);
   a.table_stride = table_stride;
   a.B = (int)B; a.Hq = (int)Hq; a.Hkv = (int)Hkv; a.Tq = (int)Tq; a.L = (int)L; a.nsplit = (int)nsplit;
   a.causal = causal ? 1 : 0; a.groups = (int)groups;

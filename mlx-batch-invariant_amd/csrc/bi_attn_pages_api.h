@@ -16,9 +16,12 @@ struct PagesArgs {
   int64_t kg_sp, kg_sh, kg_sl, vg_sp, vg_sh, vg_sl, table_stride;
   int B, Hq, Hkv, Tq, L, nsplit, causal, groups, shared_len, page_shift, num_pages, gshift;
   int near;                              // codes: every byte of the pools lies below 2^32 from their start
-  unsigned hkv_inv;                      // 2^32 / Hkv, rounded down (2^32 - 1 for 1)
+  unsigned hkv_inv, rows1_inv, g_inv;    // inverse() of Hkv, of Tq G (rows of a sequence and kv head) and of G
   float scale_log2;
 };
+
+// 2^32 / d, rounded down (2^32 - 1 for 1): quotients by one product and a correction.
+inline unsigned inverse(int64_t d) { return d == 1 ? 0xffffffffu : (unsigned)(((int64_t)1 << 32) / d); }
 
 constexpr int kPlanWords = 5;            // of a segment in the plan
 

@@ -8,10 +8,20 @@
 
 namespace bi {
 
-// Workgroups of a kernel that the device holds at once, a multiple of 8 (one share for each XCD), and no more than there can be items.
+// Workgroups of a kernel with `lds` bytes of dynamic LDS that the device holds at once,
+// a multiple of 8 (one share for each XCD), and no more than there can be items.
 template <typename K>
-static int pages_grid(K kern, int (&cache)[kMaxDev], int64_t most) {
-  return (int)((std::min<int64_t>(resident_grid(kern, cache), most) + 7) / 8 * 8);
+static int pages_grid(K kern, size_t lds, int (&cache)[kMaxDev], int64_t most) {
+  int dev = 0;
+  if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= kMaxDev) return 0;
+  if (cache[dev] <= 0) {                                  // (every writer stores the same value)
+    int cus = 0, per_cu = 0;
+    if (hipDeviceGetAttribute(&cus, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess ||
+        hipOccupancyMaxActiveBlocksPerMultiprocessor(&per_cu, kern, 256, lds) != hipSuccess || cus <= 0 || per_cu <= 0)
+      return 0;
+    cache[dev] = cus * per_cu;
+  }
+  return (int)((std::min<int64_t>(cache[dev], most) + 7) / 8 * 8);
 }
 
 template <typename T, int D>
@@ -27,21 +37,26 @@ constexpr const char* kNoOccupancy = "bi_attn_pages: device occupancy query fail
 
 template <typename T, int D, int BITS>
 static int launch_planned(const PagesArgs& a, hipStream_t st) {
-  static int cache[kMaxDev] = {};
+  static int cache[2][kMaxDev] = {};
   const int64_t most = (int64_t)a.B * a.nsplit * a.Hkv * ((a.Tq * (a.Hq / a.Hkv) + 15) / 16);   // no segment has more
-  const int slots = pages_grid(attn_pages<T, D, BITS>, cache, (int64_t)1 << 30);
+  // (first items of many segments take their full share of LDS, of few 1 KB)
+  const int many = a.groups + a.B > 256;
+  const size_t lds = (many ? kPlanCached : 256) * sizeof(int);
+  const int slots = pages_grid(attn_pages<T, D, BITS>, lds, cache[many], (int64_t)1 << 30);
   if (slots <= 0) return bi_host::fail(BI_E_UNSUPPORTED, kNoOccupancy);
   pages_plan_kernel<<<1, kPlanThreads, 0, st>>>(a, slots);
-  attn_pages<T, D, BITS><<<pages_grid(attn_pages<T, D, BITS>, cache, most), 256, 0, st>>>(a);
+  attn_pages<T, D, BITS><<<pages_grid(attn_pages<T, D, BITS>, lds, cache[many], most), 256, lds, st>>>(a);
   return merge_pages<T, D>(a, st);
 }
 
 template <typename T, int D, int BITS, int GS>
 static int launch_codes_as(const PagesArgs& a, hipStream_t st) {
-  static int cache[kMaxDev] = {};
-  const int grid = pages_grid(attn_codes<T, D, BITS, GS>, cache, (int64_t)a.B * a.nsplit * a.Hkv);
+  static int cache[3][kMaxDev] = {};
+  const int rc = codes_rows(a.Tq * (a.Hq / a.Hkv));
+  const size_t lds = (size_t)rc * 4 * 2 * (kSplit / 32) * sizeof(u32x4);
+  const int grid = pages_grid(attn_codes<T, D, BITS, GS>, lds, cache[rc / 8], (int64_t)a.B * a.nsplit * a.Hkv);
   if (grid <= 0) return bi_host::fail(BI_E_UNSUPPORTED, kNoOccupancy);
-  attn_codes<T, D, BITS, GS><<<grid, 256, 0, st>>>(a);
+  attn_codes<T, D, BITS, GS><<<grid, 256, lds, st>>>(a);
   return merge_pages<T, D>(a, st);
 }
 template <typename T, int D, int BITS>
