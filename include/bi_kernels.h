@@ -484,7 +484,9 @@ int bi_read_quantized_cache(const void* k_codes, const void* k_groups, const voi
  * bits 4 or 8: k, v are codes and k_groups, v_groups their pairs (above; group_size
  * divides D); bits 0: rows of dtype, k_groups and v_groups null. strides (host,
  * int64[15]): q (sequence, head, token), k (page, head, row), v; with bits codes in
- * bytes, and behind them the pairs of k and v.
+ * bytes, and behind them the pairs of k and v; with bits pages and rows, and for calls
+ * of few rows (Tq == 1, and up to 64 rows a sequence and kv head) q, lie less than
+ * 2^32 of these units apart.
  * groups > 0: sequences shared_starts[n] .. shared_starts[n + 1] - 1 (device int32
  * [groups + 1], rising; null for one group of all) begin with the same shared_lens[n]
  * keys (device int32 [groups]; null: shared_len for one group). Their whole 256-key

@@ -34,6 +34,8 @@ __device__ __forceinline__ int pages_len_uniform(const PagesArgs& a, int b) {
   return min(max(load_uniform_i32(a.kv_lens + __builtin_amdgcn_readfirstlane(b)), 0), a.L);
 }
 
+typedef int i32x4_t __attribute__((ext_vector_type(4)));
+
 // The operands of a P.V step in LDS, the two halves of a lane `half` pieces apart.
 template <typename T>
 __device__ __forceinline__ void store_pfrag(u32x4* p, int half, const PFrag<T>& pf) {
@@ -294,7 +296,8 @@ __global__ __launch_bounds__(256, (pages_min_blocks<T, D>())) void attn_pages(Pa
   constexpr int kPAt = kVBytes - KEEP * 32 * KV::kRowBytes;
   static_assert(DV % 32 == 0 && CPW >= 1 && kPBytes >= KEEP * 32 * KV::kRowBytes, "attn_pages: V slice tiling");
   __shared__ __attribute__((aligned(1024))) char Vs[kPAt + kPBytes];
-  __shared__ float mx[4][16];
+  __shared__ __attribute__((aligned(16))) float mx[16][4];   // a row's maximum in each wave's keys
+  __shared__ __attribute__((aligned(16))) int row_s[16], lim_s[16];
   extern __shared__ int first_s[];                        // first items of the segments, if they fit
   u32x4* const Ps = reinterpret_cast<u32x4*>(Vs + kPAt);
 
@@ -379,7 +382,9 @@ __global__ __launch_bounds__(256, (pages_min_blocks<T, D>())) void attn_pages(Pa
       const int p = 16 * chunk + r;
       int b, h, t;
       row_of(min(p, nrows - 1), b, h, t);
-      const T* qrow = static_cast<const T*>(a.q) + (int64_t)b * a.q_sb + (int64_t)h * a.q_sh + (int64_t)t * a.q_st;
+      // (strides of Q below 2^32: one product each)
+      const T* qrow = static_cast<const T*>(a.q) + ((uint64_t)(uint32_t)b * (uint32_t)a.q_sb + (uint64_t)(uint32_t)h * (uint32_t)a.q_sh +
+                                                    (uint64_t)(uint32_t)t * (uint32_t)a.q_st);
 #pragma unroll
       for (int st = 0; st < KS; ++st) x.qf[st] = frag_load(qrow + 32 * st + 8 * qq);   // (columns without a row are never stored)
       const int len = pages_len(a, b);
@@ -502,9 +507,16 @@ __global__ __launch_bounds__(256, (pages_min_blocks<T, D>())) void attn_pages(Pa
       else scores(std::false_type());
       if (c + 1 < chunks) request_rows(chunk0 + c + 1, rows);
       m = quarter_max(m);
-      if (qq == 0) mx[wave][r] = m;
+      if (qq == 0) mx[r][wave] = m;
+      if (tid < 16) {
+        row_s[tid] = row;
+        lim_s[tid] = lim;
+      }
       stage_barrier<63>();
-      m = fmaxf(fmaxf(mx[0][r], mx[1][r]), fmaxf(mx[2][r], mx[3][r]));
+      const f32x4 m4 = *reinterpret_cast<const f32x4*>(mx[r]);
+      const i32x4_t arow = *reinterpret_cast<const i32x4_t*>(row_s + 4 * qq);   // the rows of the accumulators, 4 qq + i
+      const i32x4_t alim = *reinterpret_cast<const i32x4_t*>(lim_s + 4 * qq);
+      m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
       const float msub = m == -INFINITY ? 0.0f : m;       // no visible key: weights 0, not NaN
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -514,12 +526,6 @@ __global__ __launch_bounds__(256, (pages_min_blocks<T, D>())) void attn_pages(Pa
         store_pfrag<T>(Ps + (2 * wave + h) * 2 * kWave + lane, kWave, make_pfrag<T>(p8));
       }
       if (!direct && wave == 0 && qq == 0 && lim > 0) a.pm[(int64_t)row * a.nsplit + split] = m;
-      int arow[4], alim[4];                               // the rows of the accumulators, 4 qq + i
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        arow[i] = __shfl(row, 4 * qq + i, kWave);
-        alim[i] = __shfl(lim, 4 * qq + i, kWave);
-      }
       const int sum_wave = c & 3;                         // which wave adds up the weights
       f32x4 lsum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
@@ -560,12 +566,12 @@ __global__ __launch_bounds__(256, (pages_min_blocks<T, D>())) void attn_pages(Pa
         // A hidden key's weight 0 times an infinity or NaN of its V row is NaN: such a
         // wave weighs again without them and notes the ones its rows see (kSeenTag), which
         // it looks for in the pages.
-        bool finite = true;
+        float size = 0.0f;                                // (an infinite sum of finite ones costs time only)
 #pragma unroll
         for (int j = 0; j < NJ; ++j)
 #pragma unroll
-          for (int i = 0; i < 4; ++i) finite = finite && (NJ * wave + j >= NDTV || fabsf(acc[j][i]) < INFINITY);
-        if (__ballot(!finite)) {
+          for (int i = 0; i < 4; ++i) size += fabsf(acc[j][i]);
+        if (__ballot(!(size < INFINITY))) {
           weigh(true, std::false_type());
           int dim0 = vp * DV + 16 * dt0 + r;
           asm volatile("" : "+v"(dim0));
@@ -591,17 +597,25 @@ __global__ __launch_bounds__(256, (pages_min_blocks<T, D>())) void attn_pages(Pa
             }
           }
         }
-#pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-          if (NJ * wave + j >= NDTV) continue;
+        const uint32_t dim = (uint32_t)(vp * DV + 16 * NJ * wave + r);
+        if (direct) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            const int d = vp * DV + 16 * (NJ * wave + j) + r;
-            if (direct) {
-              if (arow[i] >= 0) static_cast<T*>(a.out)[(int64_t)arow[i] * D + d] = to_store<T>(only_split(acc[j][i], lsum[i]));
-            } else if (alim[i] > 0) {
-              a.pacc[((int64_t)arow[i] * a.nsplit + split) * D + d] = acc[j][i];
-            }
+            T* o = static_cast<T*>(a.out) + ((uint64_t)(uint32_t)arow[i] * (uint32_t)D + dim);
+            if (arow[i] >= 0)
+#pragma unroll
+              for (int j = 0; j < NJ; ++j)
+                if (NDTV % 4 == 0 || NJ * wave + j < NDTV) o[16 * j] = to_store<T>(only_split(acc[j][i], lsum[i]));
+          }
+        } else {                                          // (a row's partials: fewer than 2^32 elements)
+          const uint32_t row_n = (uint32_t)a.nsplit * (uint32_t)D, at = (uint32_t)split * (uint32_t)D + dim;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float* o = a.pacc + ((uint64_t)(uint32_t)arow[i] * row_n + at);
+            if (alim[i] > 0)
+#pragma unroll
+              for (int j = 0; j < NJ; ++j)
+                if (NDTV % 4 == 0 || NJ * wave + j < NDTV) o[16 * j] = acc[j][i];
           }
         }
       }

@@ -99,13 +99,18 @@ extern "C" int bi_attn_pages(const void* q, const void* k, const void* k_groups,
     const int rc = check_quant(what, D, bits, group_size, pools, 4, qs, dtype);
     if (rc) return rc;
   }
+  // (a lane finds its rows by 32-bit strides)
+  const bool few = bi::pages_few_rows(B, Hq, Hkv, Tq, L, D, groups, bits, causal, dtype);
+  for (int i = 0; i < 15; ++i)
+    if ((i < 3 ? few : bits && i % 3 != 1) && strides[i] > 0xffffffffLL)
+      return fail(BI_E_UNSUPPORTED, "%s: stride %d (%lld) must be below 2^32", what, i, (long long)strides[i]);
   const size_t need = bi_attn_pages_workspace_bytes(B, Hq, Hkv, Tq, L, D, groups, bits, causal, dtype);
   if (need > 0 && (!ws || ws_bytes < need || !aligned16(ws)))
     return fail(BI_E_WORKSPACE, "%s: 16-byte aligned workspace of %zu bytes required, got %zu", what, need,
                 ws ? ws_bytes : (size_t)0);
   hipStream_t st = static_cast<hipStream_t>(stream);
 
-  if (!bi::pages_few_rows(B, Hq, Hkv, Tq, L, D, groups, bits, causal, dtype)) {
+  if (!few) {
     const bi_score_mod none = {0.0f, nullptr, nullptr, 0, nullptr};
     if (!bits)
       return bi_attn_scored(q, k, v, block_table, table_stride, page_size, num_pages, kv_lens, out, B, Hq, Hkv, Tq, L, D,
@@ -148,10 +153,6 @@ extern "C" int bi_attn_pages(const void* q, const void* k, const void* k_groups,
     a.vg_sp = strides[12]; a.vg_sh = strides[13]; a.vg_sl = strides[14];
     a.gshift = group_size == 32 ? 5 : group_size == 64 ? 6 : 7;
   }
-  // (a lane finds its rows by 32-bit strides)
-  for (int i = 3; i < 15; ++i)
-    if (bits && i % 3 != 1 && strides[i] > 0xffffffffLL)
-      return fail(BI_E_UNSUPPORTED, "%s: page or row stride %lld of codes (below 2^32)", what, (long long)strides[i]);
   auto reach = [&](int i) { return (num_pages - 1) * strides[i] + (Hkv - 1) * strides[i + 1] + (page_size - 1) * strides[i + 2] + D; };
   a.near = bits && reach(3) < ((int64_t)1 << 32) && reach(6) < ((int64_t)1 << 32);
   a.hkv_inv = bi::inverse(Hkv);

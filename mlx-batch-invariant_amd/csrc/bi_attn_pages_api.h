@@ -28,11 +28,25 @@ constexpr int kPlanWords = 5;            // of a segment in the plan
 template <typename T, int D>
 int launch_pages(const PagesArgs& a, int bits, hipStream_t st);
 
-// Whether attn_pages takes a call (a workgroup per split, partials merged by a second
-// launch), or the kernels of bi_attn_scored.
+// Whether a call goes to the kernels of few rows (a workgroup per split, partials merged
+// by a last launch), or to those of bi_attn_scored, which score a sequence's rows 64
+// at a time over all keys and know neither codes nor shared prefixes. Besides single
+// tokens and what few_rows splits anyway (32/8 heads of 128, 2648 keys, 2048 of them
+// shared in 4 groups, us here and there):
+//  - codes of up to 64 rows a sequence and kv head, as reading them back costs more:
+//    32 sequences of 1, 2, 4 chunks of 16 rows 65 / 199, 125 / 196, 191 / 189, 4 sequences
+//    24 / 45, 45 / 50, 55 / 62; of 8 chunks 300 / 210 and 78 / 84;
+//  - one chunk of 16-bit rows, where the prefix is read four times less often and
+//    sequences are not so few that the others would split their keys too: 32 sequences
+//    67 / 91, 16 in 4 groups 47 / 53, 8 in 2 groups 41 / 37; of 2 chunks 101 / 90.
+//    (fp32: 158 / 147.)
 inline bool pages_few_rows(int64_t B, int64_t Hq, int64_t Hkv, int64_t Tq, int64_t L, int64_t D, int64_t groups, int bits,
                            int causal, int dtype) {
-  return Tq == 1 || few_rows(B, Hq, Hkv, Tq, L, D, causal, dtype);
+  if (Tq == 1 || few_rows(B, Hq, Hkv, Tq, L, D, causal, dtype)) return true;
+  const int64_t G = Hq / Hkv;
+  if (Tq > 64 || Tq * G > 64 || rows_partial_bytes(B, Hq, Tq, L, D) > ((int64_t)2 << 30)) return false;
+  if (bits) return true;
+  return groups > 0 && dtype != BI_F32 && Tq * G <= 16 && B >= 4 * groups && B * Hkv >= 128;
 }
 
 }  // namespace bi

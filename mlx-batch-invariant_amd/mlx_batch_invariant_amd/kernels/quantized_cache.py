@@ -252,7 +252,7 @@ def _attend(what, q, k, v, kg, vg, bits, gs, num_pages, Hkv, page_size, kv_strid
         return out
     if L == 0 or num_pages == 0:
         return out.zero_()
-    if not _aligned(q):
+    if not _aligned(q) or max(q.stride()) >> 32:
         q = q.clone(memory_format=torch.contiguous_format)
     dt = _lib.DTYPE_CODE[q.dtype]
     n = _lib.ws_bytes("bi_attn_pages_workspace_bytes", B, Hq, Hkv, Tq, L, D, groups, bits, int(causal), dt)
