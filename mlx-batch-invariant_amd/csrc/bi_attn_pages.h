@@ -61,16 +61,16 @@ __device__ __forceinline__ PFrag<T> load_pfrag(const u32x4* p, int half) {
 }
 
 // ---------------------------------------------------------------------------
-// The plan of a call with shared prefixes: segments (groups, then sequences) with
-// the first item of each, and how many 16-row chunks an item takes. One workgroup.
-// plan: [0] items in all, [1] chunks of 16 rows an item, [2 ...] for each segment
-// (first item, first sequence, sequences, first split, splits).
+// The plan of a call: segments (groups, then sequences) with the first item of each,
+// and how many 16-row chunks an item takes. Of each segment kPlanWords words: first
+// item, first sequence, sequences, first split, splits.
 // Groups are the runs starts[n] .. starts[n + 1] of sequences (clamped, each from
 // the last one's end on); one of fewer than two sequences shares nothing. The
 // shared splits are whole and lie within the first sequence's own keys.
+// Every workgroup of attn_pages plans a call of up to kPlanFused segments for itself, in
+// LDS (a launch of its own takes 7 us); of more, one workgroup does it in front of them.
 // ---------------------------------------------------------------------------
 constexpr int kPlanThreads = 1024;
-constexpr int kPlanRounds = 1;           // items a workgroup of the resident grid gets, at least, where chunks allow
 constexpr int kPlanMostChunks = 32;
 constexpr int kPlanCached = 2048;        // segments whose first items a workgroup keeps in LDS
 
@@ -78,29 +78,30 @@ __device__ __forceinline__ int plan_start(const PagesArgs& a, int n) {
   return a.starts ? min(max(a.starts[n], 0), a.B) : n ? a.B : 0;
 }
 
-static __global__ __launch_bounds__(kPlanThreads) void pages_plan_kernel(PagesArgs a, int slots) {
-  __shared__ int64_t part[kPlanThreads / kWave];
-  __shared__ int64_t total_s;
-  __shared__ int carry_s;
+// By a workgroup of NT threads; `seg` in LDS or in memory, `part` in LDS. (All counts
+// stay below 2^31: the caller's items at one chunk each do.)
+template <int NT>
+__device__ __forceinline__ void plan_segments(const PagesArgs& a, int32_t* seg, int* part, int& items, int& per) {
   const int tid = threadIdx.x, lane = tid % kWave, wave = tid / kWave;
-  int32_t* seg = a.plan + 2;
   const int rows1 = a.Tq * (a.Hq / a.Hkv);                // rows of one sequence and kv head
-  // Sequences: all splits their own to begin with.
-  for (int b = tid; b < a.B; b += kPlanThreads) {
+  // Sequences: all splits their own to begin with (the first word: the length).
+  for (int b = tid; b < a.B; b += NT) {
     int32_t* s = seg + (int64_t)(a.groups + b) * kPlanWords;
+    const int len = pages_len(a, b);
+    s[0] = len;
     s[1] = b;
     s[2] = 1;
     s[3] = 0;
-    s[4] = max((pages_len(a, b) + kSplit - 1) / kSplit, a.nsplit == 1 ? 1 : 0);   // (one split: its items write the results)
+    s[4] = max((len + kSplit - 1) / kSplit, a.nsplit == 1 ? 1 : 0);   // (one split: its items write the results)
   }
-  if (tid == 0) carry_s = 0;
-  __syncthreads();
-  // Groups, 1024 at a time; ends of earlier ones bound a start from below.
-  for (int n0 = 0; n0 < a.groups; n0 += kPlanThreads) {
+  // Groups, NT at a time; ends of earlier ones bound a start from below.
+  int ends = 0;
+  for (int n0 = 0; n0 == 0 || n0 < a.groups; n0 += NT) {
     const int n = n0 + tid;
-    int lo = n < a.groups ? plan_start(a, n) : 0, hi = n < a.groups ? plan_start(a, n + 1) : 0;
-    // running maximum of every start up to this one's end
-    int run = max(lo, hi);
+    int lo = n < a.groups ? plan_start(a, n) : 0;
+    const int hi = n < a.groups ? plan_start(a, n + 1) : 0;
+    const int want = n < a.groups && a.slens ? min(max(a.slens[n], 0), a.L) : a.shared_len;
+    int run = max(lo, hi);                                // the running maximum of all starts
 #pragma unroll
     for (int off = 1; off < kWave; off <<= 1) {
       const int up = __shfl_up(run, off, kWave);
@@ -108,29 +109,25 @@ static __global__ __launch_bounds__(kPlanThreads) void pages_plan_kernel(PagesAr
     }
     if (lane == kWave - 1) part[wave] = run;
     __syncthreads();
-    int before = carry_s;
-    for (int w = 0; w < wave; ++w) before = max(before, (int)part[w]);
+    int before = ends;
+    for (int w = 0; w < NT / kWave; ++w) {
+      if (w < wave) before = max(before, part[w]);
+      ends = max(ends, part[w]);
+    }
     const int up = __shfl_up(run, 1, kWave);
     if (lane > 0) before = max(before, up);
-    lo = max(lo, before);                                 // (before: all ends of the groups in front)
-    __syncthreads();
-    if (tid == kPlanThreads - 1) carry_s = max(before, run);
+    lo = max(lo, before);
     if (n < a.groups) {
-      int splits = 0;
-      if (hi - lo > 1 && a.nsplit > 1) {
-        const int want = a.slens ? min(max(a.slens[n], 0), a.L) : a.shared_len;
-        splits = min(want, pages_len(a, lo)) / kSplit;
-      }
       int32_t* s = seg + (int64_t)n * kPlanWords;
       s[1] = lo;
       s[2] = max(hi - lo, 0);
       s[3] = 0;
-      s[4] = splits;
+      s[4] = hi - lo > 1 && a.nsplit > 1 ? min(want, (int)seg[(int64_t)(a.groups + lo) * kPlanWords]) / kSplit : 0;
     }
     __syncthreads();
   }
   // Their sequences' own splits begin behind the shared ones.
-  for (int n = wave; n < a.groups; n += kPlanThreads / kWave) {
+  for (int n = wave; n < a.groups; n += NT / kWave) {
     const int32_t* s = seg + (int64_t)n * kPlanWords;
     const int lo = s[1], size = s[2], splits = s[4];
     if (splits == 0) continue;
@@ -142,46 +139,51 @@ static __global__ __launch_bounds__(kPlanThreads) void pages_plan_kernel(PagesAr
   }
   __syncthreads();
   const int nseg = a.groups + a.B;
-  auto chunks_of = [&](const int32_t* s) { return (int64_t)(((int64_t)s[2] * rows1 + 15) / 16); };
-  auto sum = [&](int64_t x) -> int64_t {                  // over the workgroup
-#pragma unroll
-    for (int off = 32; off >= 1; off >>= 1) x += __shfl_xor((long long)x, off, kWave);
-    __syncthreads();
-    if (lane == 0) part[wave] = x;
-    __syncthreads();
-    x = 0;
-    for (int w = 0; w < kPlanThreads / kWave; ++w) x += part[w];
-    return x;
-  };
-  int64_t units = 0;
-  for (int i = tid; i < nseg; i += kPlanThreads) {
+  auto chunks_of = [&](const int32_t* s) { return (s[2] * rows1 + 15) / 16; };
+  int units = 0;
+  for (int i = tid; i < nseg; i += NT) {
     const int32_t* s = seg + (int64_t)i * kPlanWords;
     units += s[4] * chunks_of(s);
   }
-  units = sum(units) * a.Hkv;
-  const int per = (int)min(max(units / ((int64_t)slots * kPlanRounds), (int64_t)1), (int64_t)kPlanMostChunks);
-  // First items: an exclusive scan, 1024 segments at a time.
-  int64_t base = 0;
-  for (int i0 = 0; i0 < nseg; i0 += kPlanThreads) {
+#pragma unroll
+  for (int off = 32; off >= 1; off >>= 1) units += __shfl_xor(units, off, kWave);
+  if (lane == 0) part[wave] = units;
+  __syncthreads();
+  units = 0;
+  for (int w = 0; w < NT / kWave; ++w) units += part[w];
+  per = min(max(units * a.Hkv / a.slots, 1), kPlanMostChunks);
+  // First items: an exclusive scan.
+  items = 0;
+  for (int i0 = 0; i0 < nseg; i0 += NT) {
     const int i = i0 + tid;
     int32_t* s = seg + (int64_t)min(i, nseg - 1) * kPlanWords;
-    const int64_t items = i < nseg ? s[4] * ((chunks_of(s) + per - 1) / per) * a.Hkv : 0;
-    int64_t incl = items;
+    const int own = i < nseg ? s[4] * ((chunks_of(s) + per - 1) / per) * a.Hkv : 0;
+    int incl = own;
 #pragma unroll
     for (int off = 1; off < kWave; off <<= 1) {
-      const int64_t up = __shfl_up((long long)incl, off, kWave);
+      const int up = __shfl_up(incl, off, kWave);
       if (lane >= off) incl += up;
     }
     __syncthreads();
     if (lane == kWave - 1) part[wave] = incl;
     __syncthreads();
-    int64_t first = base;
-    for (int w = 0; w < wave; ++w) first += part[w];
-    if (i < nseg) s[0] = (int32_t)(first + incl - items);
-    for (int w = 0; w < kPlanThreads / kWave; ++w) base += part[w];
+    int first = items + incl - own;
+    for (int w = 0; w < NT / kWave; ++w) {
+      if (w < wave) first += part[w];
+      items += part[w];
+    }
+    if (i < nseg) s[0] = first;
   }
-  if (tid == 0) {
-    a.plan[0] = (int32_t)base;
+  __syncthreads();
+}
+
+// plan: [0] items in all, [1] chunks an item, [2 ...] the segments.
+static __global__ __launch_bounds__(kPlanThreads) void pages_plan_kernel(PagesArgs a) {
+  __shared__ int part[kPlanThreads / kWave];
+  int items, per;
+  plan_segments<kPlanThreads>(a, a.plan + 2, part, items, per);
+  if (threadIdx.x == 0) {
+    a.plan[0] = items;
     a.plan[1] = per;
   }
 }
@@ -298,7 +300,7 @@ __global__ __launch_bounds__(256, (pages_min_blocks<T, D>())) void attn_pages(Pa
   __shared__ __attribute__((aligned(1024))) char Vs[kPAt + kPBytes];
   __shared__ __attribute__((aligned(16))) float mx[16][4];   // a row's maximum in each wave's keys
   __shared__ __attribute__((aligned(16))) int row_s[16], lim_s[16];
-  extern __shared__ int first_s[];                        // first items of the segments, if they fit
+  extern __shared__ int seg_s[];                          // the plan's segments, or their first items
   u32x4* const Ps = reinterpret_cast<u32x4*>(Vs + kPAt);
 
   const int tid = threadIdx.x;
@@ -313,23 +315,43 @@ __global__ __launch_bounds__(256, (pages_min_blocks<T, D>())) void attn_pages(Pa
   const int w0 = (int)(blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8);
   const int dt0 = min(NJ * wave, NDTV - NJ < 0 ? 0 : NDTV - 1);   // this wave's first dim tile (a wave without one repeats the last)
 
-  const int items = a.plan[0], per = a.plan[1], nseg = a.groups + a.B;
+  const int nseg = a.groups + a.B;
+  const bool fused = nseg <= kPlanFused;
   const int32_t* seg = a.plan + 2;
+  int items, per;
+  if (fused) {
+    plan_segments<256>(a, seg_s, row_s, items, per);
+    items = __builtin_amdgcn_readfirstlane(items);
+    per = __builtin_amdgcn_readfirstlane(per);
+  } else {
+    items = a.plan[0];
+    per = a.plan[1];
+    if (nseg <= kPlanCached) {
+      for (int i = tid; i < nseg; i += 256) seg_s[i] = seg[(int64_t)i * kPlanWords];
+      __syncthreads();
+    }
+  }
   struct Item { int seq0, nseq, split, hk, chunk0, n_act; };   // n_act < 0: no more items
   auto locate = [&](int item) -> Item {
     if (item >= items) return Item{0, 0, 0, 0, 0, -1};
     // the last segment that starts at or before the item (ones without items share a start with the next)
     int at = 0;
     if (nseg <= kPlanCached) {
-      for (int i = lane; i < nseg; i += kWave) at += __popcll(__ballot(first_s[i] <= item));   // (starts rise)
+      const int words = fused ? kPlanWords : 1;
+      for (int i = lane; i < nseg; i += kWave) at += __popcll(__ballot(seg_s[i * words] <= item));   // (starts rise)
       at = __builtin_amdgcn_readfirstlane(at) - 1;
     } else {
       for (int step = 1 << (31 - __builtin_clz(nseg)); step > 0; step >>= 1)
         if (at + step < nseg && load_uniform_i32(uniform_ptr(seg + (int64_t)(at + step) * kPlanWords)) <= item) at += step;
     }
-    const int32_t* sg = uniform_ptr(seg + (int64_t)at * kPlanWords);
     int w[4];
-    load_uniform4_i32(sg, sg + 1, sg + 2, sg + 3, w);
+    if (fused) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) w[i] = __builtin_amdgcn_readfirstlane(seg_s[at * kPlanWords + i]);
+    } else {
+      const int32_t* sg = uniform_ptr(seg + (int64_t)at * kPlanWords);
+      load_uniform4_i32(sg, sg + 1, sg + 2, sg + 3, w);
+    }
     Item it;
     it.seq0 = w[1];
     it.nseq = w[2];
@@ -347,10 +369,6 @@ __global__ __launch_bounds__(256, (pages_min_blocks<T, D>())) void attn_pages(Pa
     return a.table[(int64_t)it.seq0 * a.table_stride + (pos >> a.page_shift)];
   };
 
-  if (nseg <= kPlanCached) {
-    for (int i = tid; i < nseg; i += 256) first_s[i] = seg[(int64_t)i * kPlanWords];
-    __syncthreads();
-  }
   Item it = locate(w0);
   int page = page_of(it);
   for (int item = w0; it.n_act >= 0; item += (int)gridDim.x) {

@@ -15,6 +15,7 @@ struct PagesArgs {
   int64_t q_sb, q_sh, q_st, k_sp, k_sh, k_sl, v_sp, v_sh, v_sl;  // codes: bytes
   int64_t kg_sp, kg_sh, kg_sl, vg_sp, vg_sh, vg_sl, table_stride;
   int B, Hq, Hkv, Tq, L, nsplit, causal, groups, shared_len, page_shift, num_pages, gshift;
+  int slots;                             // workgroups of attn_pages that the device holds at once
   int near;                              // codes: every byte of the pools lies below 2^32 from their start
   unsigned hkv_inv, rows1_inv, g_inv;    // inverse() of Hkv, of Tq G (rows of a sequence and kv head) and of G
   float scale_log2;
@@ -24,6 +25,7 @@ struct PagesArgs {
 inline unsigned inverse(int64_t d) { return d == 1 ? 0xffffffffu : (unsigned)(((int64_t)1 << 32) / d); }
 
 constexpr int kPlanWords = 5;            // of a segment in the plan
+constexpr int kPlanFused = 256;          // segments of a plan that every workgroup makes for itself
 
 template <typename T, int D>
 int launch_pages(const PagesArgs& a, int bits, hipStream_t st);

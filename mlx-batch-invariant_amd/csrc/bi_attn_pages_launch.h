@@ -36,15 +36,14 @@ static int merge_pages(const PagesArgs& a, hipStream_t st) {
 constexpr const char* kNoOccupancy = "bi_attn_pages: device occupancy query failed";
 
 template <typename T, int D, int BITS>
-static int launch_planned(const PagesArgs& a, hipStream_t st) {
+static int launch_planned(PagesArgs a, hipStream_t st) {
   static int cache[2][kMaxDev] = {};
   const int64_t most = (int64_t)a.B * a.nsplit * a.Hkv * ((a.Tq * (a.Hq / a.Hkv) + 15) / 16);   // no segment has more
-  // (first items of many segments take their full share of LDS, of few 1 KB)
-  const int many = a.groups + a.B > 256;
-  const size_t lds = (many ? kPlanCached : 256) * sizeof(int);
-  const int slots = pages_grid(attn_pages<T, D, BITS>, lds, cache[many], (int64_t)1 << 30);
-  if (slots <= 0) return bi_host::fail(BI_E_UNSUPPORTED, kNoOccupancy);
-  pages_plan_kernel<<<1, kPlanThreads, 0, st>>>(a, slots);
+  const int many = a.groups + a.B > kPlanFused;
+  const size_t lds = (many ? kPlanCached : kPlanFused * kPlanWords) * sizeof(int);
+  a.slots = pages_grid(attn_pages<T, D, BITS>, lds, cache[many], (int64_t)1 << 30);
+  if (a.slots <= 0) return bi_host::fail(BI_E_UNSUPPORTED, kNoOccupancy);
+  if (many) pages_plan_kernel<<<1, kPlanThreads, 0, st>>>(a);
   attn_pages<T, D, BITS><<<pages_grid(attn_pages<T, D, BITS>, lds, cache[many], most), 256, lds, st>>>(a);
   return merge_pages<T, D>(a, st);
 }
