@@ -1059,54 +1059,102 @@ __global__ __launch_bounds__(256, (codes_min_blocks<T, D, BITS>())) void attn_co
   }
 }
 
-// Merges the splits of every row, left to right, and divides: one thread per two dims
-// of a row, the partials of 16 splits requested together (decode has few rows: a
-// thread's time is its round trips). A split in which the row sees no score above -inf
-// (l = 0 at m = -inf) is passed over.
+// Merges the splits of every row, left to right, and divides. A row's lanes are whole
+// 16-lane rows of one wave, kE dims a lane; the partials of 16 splits are requested
+// together (decode has few rows: a row's time is its round trips). Lane j of each 16 takes
+// split j's maximum and sum: running maxima are a scan, so every split's two factors
+// come from all lanes at once, and each one's turn is a product and an fma a dim.
+// A split in which the row sees no score above -inf (l = 0 at m = -inf) is passed over.
+template <int D>
+struct MergeRow {
+  static constexpr int kE = D > 128 ? 4 : 2;
+  static constexpr int kLanes = D / kE <= 16 ? 16 : D / kE <= 32 ? 32 : 64;
+};
+// x of lane J of the lane's row of 16.
+template <int J>
+__device__ __forceinline__ float row_lane(float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), 0x150 + J, 0xf, 0xf, false));
+}
+template <int N, int J = 0, class F>
+__device__ __forceinline__ void in_turn(const F& f) {
+  if constexpr (J < N) {
+    f(std::integral_constant<int, J>());
+    in_turn<N, J + 1>(f);
+  }
+}
+// The maximum of lanes 0 .. j of the row of 16, in lane j.
+__device__ __forceinline__ float row_scan_max(float x) {
+  auto up = [](float x, auto by) {                        // (-inf from before the row)
+    return fmaxf(x, __builtin_bit_cast(float, __builtin_amdgcn_update_dpp((int)0xff800000, __builtin_bit_cast(int, x),
+                                                                           0x110 + decltype(by)::value, 0xf, 0xf, false)));
+  };
+  x = up(x, std::integral_constant<int, 1>());
+  x = up(x, std::integral_constant<int, 2>());
+  x = up(x, std::integral_constant<int, 4>());
+  return up(x, std::integral_constant<int, 8>());
+}
+
 template <typename T, int D>
 __global__ __launch_bounds__(256) void attn_pages_merge(PagesArgs a) {
-  typedef float f32x2m __attribute__((ext_vector_type(2)));
-  constexpr int kDeep = 16;
-  const int64_t id = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int64_t row = id / (D / 2);                       // (b, head, token), the output's order
-  if (row >= (int64_t)a.B * a.Hq * a.Tq) return;
-  const int d = (int)(id % (D / 2)) * 2;
-  const int t = (int)(row % a.Tq), b = (int)(row / a.Tq / a.Hq);
-  const int len = pages_len(a, b);
+  constexpr int kE = MergeRow<D>::kE, kLanes = MergeRow<D>::kLanes, kDeep = 16;
+  typedef float fE __attribute__((ext_vector_type(kE)));
+  const int row0 = (int)(blockIdx.x * (256 / kLanes) + threadIdx.x / kLanes), rows = a.B * a.Hq * a.Tq;   // (b, head, token), the output's order
+  int row = min(row0, rows - 1);                          // (lanes without work follow the last)
+  if (kLanes == kWave) row = __builtin_amdgcn_readfirstlane(row);
+  const int d0 = threadIdx.x % kLanes * kE, d = min(d0, D - kE), j16 = threadIdx.x % 16;
+  const int bh = row / a.Tq, t = row - bh * a.Tq;
+  const int len = pages_len(a, bh / a.Hq);
   const int seen = a.causal ? len - a.Tq + t + 1 : len;
-  const int ns = seen > 0 ? (seen + kSplit - 1) / kSplit : 0;
-  float M = -INFINITY, Ls = 0.0f, A[2] = {0.f, 0.f};
-  uint32_t kinds[2] = {0, 0};
-  const int64_t p0 = row * a.nsplit;
-  for (int i0 = 0; i0 < ns; i0 += kDeep) {
-    float pm[kDeep], pl[kDeep];
-    f32x2m pa[kDeep];
+  int ns = seen > 0 ? (seen + kSplit - 1) / kSplit : 0;
+  if (kLanes == kWave) ns = __builtin_amdgcn_readfirstlane(ns);
+  float M = -INFINITY, Ls = 0.0f, A[kE];
+  uint32_t kinds[kE];
 #pragma unroll
-    for (int j = 0; j < kDeep; ++j) {
-      const int64_t p = p0 + min(i0 + j, ns - 1);
-      pm[j] = a.pm[p];
-      pl[j] = a.pl[p];
-      pa[j] = *reinterpret_cast<const f32x2m*>(a.pacc + p * D + d);
-    }
+  for (int e = 0; e < kE; ++e) A[e] = 0.0f, kinds[e] = 0;
+  const float *pm = a.pm + (int64_t)row * a.nsplit, *pl = a.pl + (int64_t)row * a.nsplit;
+  const float* pacc = a.pacc + (int64_t)row * a.nsplit * D + d;
+  auto batch = [&](int i0, auto all) __attribute__((always_inline)) {
+    const int i = min(i0 + j16, ns - 1);
+    const float m = pm[i], l = pl[i];
+    fE pa[kDeep];
+#pragma unroll
+    for (int j = 0; j < kDeep; ++j)
+      pa[j] = *reinterpret_cast<const fE*>(pacc + (int64_t)(decltype(all)::value ? i0 + j : min(i0 + j, ns - 1)) * D);
+    const bool live = i0 + j16 < ns && (m > -INFINITY || l != 0.0f);
+    const float Mi = fmaxf(M, row_scan_max(live ? m : -INFINITY));            // after split i
+    const float Mb = __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(__builtin_bit_cast(int, M), __builtin_bit_cast(int, Mi), 0x111, 0xf, 0xf, false));   // before it
+    const float c_old = live ? __builtin_amdgcn_exp2f(Mb - Mi) : 1.0f, c_new = __builtin_amdgcn_exp2f(m - Mi);
+    const float lc = live ? l * c_new : -0.0f;            // (x 1 + -0 is x)
+    const float on = live ? 1.0f : 0.0f;
+    M = row_lane<15>(Mi);
     float odd = 0.0f;
+    auto turn = [&](auto jc, auto every) __attribute__((always_inline)) {
+      constexpr int j = decltype(jc)::value;
+      const float co = row_lane<j>(c_old), cn = row_lane<j>(c_new);
+      const bool in = decltype(every)::value || row_lane<j>(on) != 0.0f;
+      Ls = __builtin_fmaf(Ls, co, row_lane<j>(lc));
 #pragma unroll
-    for (int j = 0; j < kDeep; ++j) {
-      if (i0 + j < ns && (pm[j] > -INFINITY || pl[j] != 0.0f)) {
-        const float acc[2] = {pa[j][0], pa[j][1]};
-        merge_split<2>(M, Ls, A, pm[j], pl[j], acc);
+      for (int e = 0; e < kE; ++e) {
+        A[e] = __builtin_fmaf(A[e], co, in ? pa[j][e] * cn : -0.0f);
+        odd += pa[j][e];                                  // (the last split several times: no matter)
       }
-      odd += pa[j][0] + pa[j][1];                         // (the last split several times: no matter)
-    }
+    };
+    if (decltype(all)::value && !__ballot(!live)) in_turn<kDeep>([&](auto j) __attribute__((always_inline)) { turn(j, std::true_type()); });
+    else in_turn<kDeep>([&](auto j) __attribute__((always_inline)) { turn(j, std::false_type()); });
     if (odd != odd) {                                     // a NaN among them
 #pragma unroll
       for (int j = 0; j < kDeep; ++j)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) kinds[e] |= seen_kinds(pa[j][e]);
+        for (int e = 0; e < kE; ++e) kinds[e] |= seen_kinds(pa[j][e]);
     }
-  }
-  T* o = static_cast<T*>(a.out) + row * D + d;
+  };
+  int i0 = 0;
+  for (; i0 + kDeep <= ns; i0 += kDeep) batch(i0, std::true_type());
+  if (i0 < ns) batch(i0, std::false_type());
+  if (row0 >= rows || d0 >= D) return;
+  T* o = static_cast<T*>(a.out) + (int64_t)row * D + d;
 #pragma unroll
-  for (int e = 0; e < 2; ++e)
+  for (int e = 0; e < kE; ++e)
     o[e] = to_store<T>(kinds[e] ? seen_value(kinds[e], Ls) : Ls != 0.0f ? A[e] / Ls : 0.0f);
 }
 

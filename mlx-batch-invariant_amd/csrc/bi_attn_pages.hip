@@ -138,7 +138,7 @@ extern "C" int bi_attn_pages(const void* q, const void* k, const void* k_groups,
   // (items, rows and the merge's threads in 32 bits)
   if (B * Hq * Tq > 0x7fffffffLL || rows1 > 0x7fffffffLL - 16 || B * rows1 > 0x7fffffffLL - 1024 ||
       (double)nsplit * Hkv * ((double)B * ((rows1 + 15) / 16) + groups) > 2e9 || n > ((int64_t)1 << 36) ||
-      B * Hq * Tq * (D / 2) > ((int64_t)1 << 32) - 256)
+      B * Hq * Tq * 64 > ((int64_t)1 << 32) - 256)
     return fail(BI_E_UNSUPPORTED, "%s: grid too large", what);
   bi::PagesArgs a;
   a.q = q; a.k = k; a.v = v; a.kg = k_groups; a.vg = v_groups;

@@ -27,7 +27,7 @@ static int pages_grid(K kern, size_t lds, int (&cache)[kMaxDev], int64_t most) {
 template <typename T, int D>
 static int merge_pages(const PagesArgs& a, hipStream_t st) {
   if (a.nsplit > 1) {
-    const int64_t n = (int64_t)a.B * a.Hq * a.Tq * (D / 2);
+    const int64_t n = (int64_t)a.B * a.Hq * a.Tq * MergeRow<D>::kLanes;
     attn_pages_merge<T, D><<<(unsigned)((n + 255) / 256), 256, 0, st>>>(a);
   }
   return bi_host::launch_status("bi_attn_pages");
