@@ -17,11 +17,14 @@ namespace bi {
 // in fp32 with IEEE quotients: the framework's quantizer on the rows that
 // bi_rope_paged_cache writes. A group with an infinity or a NaN gets NaN for both.
 //
-// Bound by HBM bytes for prompts and by the launch for a decode step. One thread
+// Bound by HBM bytes for prompts and by the launch for a decode step: 8192 tokens of 32 / 8
+// heads of 128 in bf16 to 8 bits move 184 MB in 40 us, 4.6 TB/s (50 us with a division
+// for each value and index, and a thread for one head of Q). One thread
 // takes 16 values of a row; a key's thread also reads the pairs that its values turn
 // with (the row is in the cache then), so that it holds 16 neighbours and a group is
 // 2, 4 or 8 neighbouring lanes. Rows are whole numbers of groups, so no group
-// straddles a wave. Threads of queries take two runs of 8 that turn together.
+// straddles a wave. Threads of queries take two runs of 8 that turn together, of two
+// heads, which turn alike.
 // ---------------------------------------------------------------------------
 struct RopeQuantArgs {
   const void *q, *k, *v, *cos, *sin;
@@ -35,9 +38,16 @@ struct RopeQuantArgs {
   int64_t vc_sp, vc_sh, vc_sl, vg_sp, vg_sh, vg_sl;
   int64_t num_slots;
   int B, T, Hq, Hkv, D, half, table_rows, axes, shift, gshift;
+  unsigned cph, cph_inv, t_inv, hq_inv, hkv_inv;       // pieces of 16 dims per head; 2^32 / cph, T, heads (pairs of q's) and 2 Hkv
   unsigned q_blocks;                                   // workgroups of queries; the others take keys and values
   int end[4];                                          // pairs of dims up to each axis's end
 };
+
+// x / d from inv = 2^32 / d rounded down (2^32 - 1 for 1).
+__device__ __forceinline__ unsigned quotient(unsigned x, unsigned d, unsigned inv) {
+  const unsigned q = __umulhi(x, inv);                 // or one less
+  return x - q * d >= d ? q + 1 : q;
+}
 
 // cos and sin of pairs d .. d + 7 of token bt.
 template <typename TAB>
@@ -68,41 +78,50 @@ __device__ __forceinline__ void table8(const RopeQuantArgs& a, unsigned bt, int 
 
 template <typename T, typename TAB, int BITS>
 __global__ __launch_bounds__(256) void rope_quant_kernel(RopeQuantArgs a) {
-  const unsigned cph = (unsigned)a.D / 16;
+  const unsigned cph = a.cph;
   if (blockIdx.x < a.q_blocks) {
-    const unsigned id = blockIdx.x * 256u + threadIdx.x;
-    const unsigned c = id % cph, rest = id / cph;
-    const unsigned t = rest % (unsigned)a.T, rest2 = rest / (unsigned)a.T;
-    const unsigned h = rest2 % (unsigned)a.Hq, b = rest2 / (unsigned)a.Hq;
+    const unsigned id = blockIdx.x * 256u + threadIdx.x, hn = ((unsigned)a.Hq + 1) / 2;
+    const unsigned rest = quotient(id, cph, a.cph_inv), c = id - rest * cph;
+    const unsigned rest2 = quotient(rest, (unsigned)a.T, a.t_inv), t = rest - rest2 * (unsigned)a.T;
+    const unsigned b = quotient(rest2, hn, a.hq_inv), h0 = 2 * (rest2 - b * hn);
     if (b >= (unsigned)a.B) return;
+    const int heads = min(2, a.Hq - (int)h0);
     const unsigned bt = b * (unsigned)a.T + t;
     const int rc = a.half / 8;
     const bool turn = (int)c < rc;
     const int d1 = turn ? 8 * (int)c : 2 * a.half + 16 * ((int)c - rc);
     const int d2 = turn ? a.half + 8 * (int)c : d1 + 8;
-    const T* src = static_cast<const T*>(a.q) + (int64_t)bt * a.q_row + (int64_t)h * a.D;
-    float x1[8], x2[8], co[8], si[8];
-    load8<T>(src + d1, x1);
-    load8<T>(src + d2, x2);
-    if (turn) {
-      table8<TAB>(a, bt, d1, co, si);
+    const T* src = static_cast<const T*>(a.q) + (int64_t)bt * a.q_row + (int64_t)h0 * a.D;
+    float x1[2][8], x2[2][8], co[8], si[8];
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float y1 = __builtin_fmaf(x1[e], co[e], -(x2[e] * si[e]));
-        const float y2 = __builtin_fmaf(x2[e], co[e], x1[e] * si[e]);
-        x1[e] = y1;
-        x2[e] = y2;
-      }
+    for (int h = 0; h < 2; ++h) {
+      if (h >= heads) continue;
+      load8<T>(src + h * a.D + d1, x1[h]);
+      load8<T>(src + h * a.D + d2, x2[h]);
     }
-    T* dst = static_cast<T*>(a.qo) + (((int64_t)b * a.Hq + h) * a.T + t) * a.D;
-    store8<T>(dst + d1, x1);
-    store8<T>(dst + d2, x2);
+    if (turn) table8<TAB>(a, bt, d1, co, si);
+    T* dst = static_cast<T*>(a.qo) + (((int64_t)b * a.Hq + h0) * a.T + t) * a.D;
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      if (h >= heads) continue;
+      if (turn) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const float y1 = __builtin_fmaf(x1[h][e], co[e], -(x2[h][e] * si[e]));
+          const float y2 = __builtin_fmaf(x2[h][e], co[e], x1[h][e] * si[e]);
+          x1[h][e] = y1;
+          x2[h][e] = y2;
+        }
+      }
+      store8<T>(dst + (int64_t)h * a.T * a.D + d1, x1[h]);
+      store8<T>(dst + (int64_t)h * a.T * a.D + d2, x2[h]);
+    }
     return;
   }
   const unsigned id = (blockIdx.x - a.q_blocks) * 256u + threadIdx.x;
-  const unsigned c = id % cph, rest = id / cph;
-  const unsigned t = rest % (unsigned)a.T, rest2 = rest / (unsigned)a.T;
-  const unsigned hv = rest2 % (2u * a.Hkv), b = rest2 / (2u * a.Hkv);
+  const unsigned rest = quotient(id, cph, a.cph_inv), c = id - rest * cph;
+  const unsigned rest2 = quotient(rest, (unsigned)a.T, a.t_inv), t = rest - rest2 * (unsigned)a.T;
+  const unsigned b = quotient(rest2, 2u * a.Hkv, a.hkv_inv), hv = rest2 - b * (2u * a.Hkv);
   // (Threads past the end and of padding rows stay for the lanes that share their wave.)
   const bool live = b < (unsigned)a.B;
   const bool key = hv < (unsigned)a.Hkv;
@@ -164,17 +183,37 @@ __global__ __launch_bounds__(256) void rope_quant_kernel(RopeQuantArgs a) {
   T* pairs = key ? static_cast<T*>(a.kg) + page * a.kg_sp + h * a.kg_sh + row * a.kg_sl
                  : static_cast<T*>(a.vg) + page * a.vg_sp + h * a.vg_sh + row * a.vg_sl;
   uint32_t w[BITS / 2];
+  auto encode = [&](auto divide) __attribute__((always_inline)) {
 #pragma unroll
-  for (int i = 0; i < BITS / 2; ++i) w[i] = 0;
+    for (int i = 0; i < BITS / 2; ++i) w[i] = 0;
 #pragma unroll
-  for (int i = 0; i < 2; ++i)
+    for (int i = 0; i < 2; ++i)
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float y = __builtin_rintf((x[i][e] - lo) / scale);
-      const uint32_t code = (uint32_t)fminf(fmaxf(y, 0.0f), most);
-      const int at = (8 * i + e) * BITS;
-      w[at / 32] |= code << (at % 32);
-    }
+      for (int e = 0; e < 8; ++e) {
+        const float y = __builtin_rintf(divide(x[i][e] - lo));
+        const uint32_t code = (uint32_t)fminf(fmaxf(y, 0.0f), most);
+        const int at = (8 * i + e) * BITS;
+        w[at / 32] |= code << (at % 32);
+      }
+  };
+  // The IEEE quotient of n by the group's scale s without a division each: from r, the
+  // rounded 1 / s, q = n r is off by less than 2 units in its last place, n - q s is exact,
+  // and q + r (n - q s) lies within 2^-23 units of n / s before it is rounded. A
+  // quotient by a scale of 11 bits or fewer is 2^-13 units at least from where its rounding
+  // turns; by one of 24 bits that step gives a neighbour of n / s, and from such a q a second
+  // one the rounded quotient (Markstein 1990). Of a q below 1/4, code 0 in any case, the
+  // remainder may be no normal number; scales from 2^-80 on keep it exact above.
+  if (scale >= 0x1p-80f && range < INFINITY) {
+    const float r = 1.0f / scale;
+    encode([&](float n) {
+      float q = n * r;
+#pragma unroll
+      for (int i = 0; i < (sizeof(T) == 2 ? 1 : 2); ++i) q = __builtin_fmaf(__builtin_fmaf(-q, scale, n), r, q);
+      return q;
+    });
+  } else {
+    encode([&](float n) { return n / scale; });
+  }
   if constexpr (BITS == 8) *reinterpret_cast<u32x4*>(codes + 16 * c) = u32x4{w[0], w[1], w[2], w[3]};
   else *reinterpret_cast<u32x2*>(codes + 8 * c) = u32x2{w[0], w[1]};
   if (c % (unsigned)lanes == 0) {
@@ -303,7 +342,7 @@ extern "C" int bi_rope_quantized_cache(const void* q, int64_t q_row, const void*
     return fail(BI_E_UNSUPPORTED, "%s: dtype %d with tables of dtype %d (the same, or fp32)", what, dtype, table_dtype);
   if (B > 0x7fffffffLL || T > 0x7fffffffLL || Hq > 65536 || Hkv > 65536 || D > 65536 || table_rows > 0x7fffffffLL ||
       num_pages > 0x7fffffffLL || B * T > ((int64_t)1 << 31) - 1 ||
-      B * T * (Hq + 2 * Hkv) * (D / 16) > ((int64_t)1 << 32) - 1024)  // threads
+      B * T * (Hq + 1 + 2 * Hkv) * (D / 16) > ((int64_t)1 << 32) - 1024)  // threads
     return fail(BI_E_UNSUPPORTED, "%s: shape too large", what);
   bi::RopeQuantArgs a;
   int64_t half = 0;
@@ -338,7 +377,13 @@ extern "C" int bi_rope_quantized_cache(const void* q, int64_t q_row, const void*
   a.B = (int)B; a.T = (int)T; a.Hq = (int)Hq; a.Hkv = (int)Hkv; a.D = (int)D; a.half = (int)half;
   a.table_rows = (int)table_rows; a.axes = (int)axes; a.shift = shift; a.gshift = shift_of(group_size);
   const int64_t per_head = B * T * (D / 16);
-  a.q_blocks = (unsigned)((per_head * Hq + 255) / 256);
+  auto inverse = [](int64_t d) { return d == 1 ? 0xffffffffu : (unsigned)(((int64_t)1 << 32) / d); };
+  a.cph = (unsigned)(D / 16);
+  a.cph_inv = inverse(D / 16);
+  a.t_inv = inverse(T);
+  a.hq_inv = inverse((Hq + 1) / 2);
+  a.hkv_inv = inverse(2 * Hkv);
+  a.q_blocks = (unsigned)((per_head * ((Hq + 1) / 2) + 255) / 256);
   const unsigned grid = a.q_blocks + (unsigned)((per_head * 2 * Hkv + 255) / 256);
   hipStream_t st = static_cast<hipStream_t>(stream);
   auto launch = [&](auto t, auto tab) {
