@@ -92,8 +92,8 @@ def _pools(what: str, k_pages: QuantizedPages, v_pages: QuantizedPages, dtype=No
     strides = []
     for p in (k_pages, v_pages):
         c, g = p.codes.stride(), p.groups.stride()
-        if (c[3] != 1 or any(s % 16 for s in c[:3]) or p.codes.data_ptr() % 16 or g[4] != 1
-                or (groups.shape[3] > 1 and g[3] != 2) or any(s % 2 for s in g[:3]) or p.groups.data_ptr() % 16):
+        if (c[3] != 1 or (c[0] | c[1] | c[2] | p.codes.data_ptr() | p.groups.data_ptr()) & 15 or g[4] != 1
+                or (groups.shape[3] > 1 and g[3] != 2) or (g[0] | g[1] | g[2]) & 1):
             raise ValueError(f"{what}: pool rows must be contiguous and 16-byte aligned; got strides {c} of codes, "
                              f"{g} of groups")
         strides += [*c[:3], *g[:3]]
