@@ -68,8 +68,31 @@ def _format(what: str, bits, group_size, head_dim: int) -> None:
         raise ValueError(f"{what}: head dim {head_dim} is no whole number of groups of {group_size}")
 
 
+_layouts: dict = {}
+
+
 def _pools(what: str, k_pages: QuantizedPages, v_pages: QuantizedPages, dtype=None):
-    """Checks a pair of pools; (num_pages, Hkv, page_size, D, the 12 strides)."""
+    """Checks a pair of pools; (num_pages, Hkv, page_size, D, the 12 strides). Shapes, strides and types
+    that passed once are remembered (a lookup is cheaper than the checks on every step)."""
+    if type(k_pages) is QuantizedPages is type(v_pages):
+        kc, kg, bits, gs = k_pages
+        vc, vg, v_bits, v_gs = v_pages
+        key = (kc.shape, kc.stride(), kg.shape, kg.stride(), vc.shape, vc.stride(), vg.shape, vg.stride(), kc.dtype, kg.dtype,
+               vc.dtype, vg.dtype, bits, gs, v_bits, v_gs, dtype)
+        seen = _layouts.get(key)
+        if seen is not None and not (kc.data_ptr() | kg.data_ptr() | vc.data_ptr() | vg.data_ptr()) & 15:
+            return seen
+    else:
+        key = None
+    seen = _check_pools(what, k_pages, v_pages, dtype)
+    if key is not None:
+        if len(_layouts) > 1024:
+            _layouts.clear()
+        _layouts[key] = seen
+    return seen
+
+
+def _check_pools(what: str, k_pages: QuantizedPages, v_pages: QuantizedPages, dtype):
     for p in (k_pages, v_pages):
         if not isinstance(p, QuantizedPages):
             raise ValueError(f"{what}: pools must be QuantizedPages; got {type(p).__name__}")
