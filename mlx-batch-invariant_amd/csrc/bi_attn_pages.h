@@ -270,6 +270,14 @@ struct KRow {
 // rows costs its Q^T, its products and the exchange of maxima and weights. Wave w takes
 // the dims 16 dt, dt = NJ w .. NJ w + NJ - 1, of P.V. (fp32 rows of more than 128 dims: V
 // in two slices, copied for every chunk.) BITS 0: rows of T; 8 or 4: codes.
+// Bound by instructions where many rows share a prefix: a chunk takes a CU about 1.3 us,
+// 48 products a wave (as long as 0.35 us) among some 330 vector instructions and
+// two exchanges; by latency and bytes where they share little. 64 sequences of 32 / 8
+// heads of 128 in bf16 behind 8192 keys: 60 us, 67 in all with the merge, where
+// every sequence reading its own keys takes 322; without the shared keys 24 in all.
+// Of a second half of the grid that takes its items from the last on, loads beside the
+// others' products, nothing came (57 -> 59 us), nor of waiting for the next rows in front
+// of the stores.
 // ---------------------------------------------------------------------------
 template <typename T, int D>
 constexpr int pages_v_slices() {
@@ -656,6 +664,12 @@ __global__ __launch_bounds__(256, (pages_min_blocks<T, D>())) void attn_pages(Pa
 // registers. For P.V wave w takes the dims 16 dt, dt = NJ w .. NJ w + NJ - 1: a
 // transposing LDS read gives a lane the codes of 8 keys (4 bits: 16) of one dim, and
 // each is dequantized once, with its key's pair from LDS.
+// Bound by bytes at 8 bits and by the vector instructions at 4, of which dequantizing
+// takes two thirds (a conversion, an fma and half a rounding pair for every value): 64
+// sequences of up to 8192 keys, 32 / 8 heads of 128: 141 to 165 us on different cards for
+// 8 bits in bf16 (572 MB; a copy takes 112), 100 to 110 for 4 bits in fp16 (302 MB, 59).
+// Codes converted before they go to LDS took 500 and 459, the next item's codes
+// requested an item ahead, with two workgroups a CU for the registers, 176 and 136.
 // ---------------------------------------------------------------------------
 // The tile of V's codes: row r, 16-byte chunk c in slot c ^ key(r) where a row holds a
 // power of two of them, so that the rows of a transposing read (32 keys, one chunk)
@@ -1064,6 +1078,8 @@ __global__ __launch_bounds__(256, (codes_min_blocks<T, D, BITS>())) void attn_co
 // together (decode has few rows: a row's time is its round trips). Lane j of each 16 takes
 // split j's maximum and sum: running maxima are a scan, so every split's two factors
 // come from all lanes at once, and each one's turn is a product and an fma a dim.
+// Bound by round trips: 2048 rows of 34 splits of 128 dims, 35 MB, 8.8 us (13.0 with the
+// factors worked out by every lane).
 // A split in which the row sees no score above -inf (l = 0 at m = -inf) is passed over.
 template <int D>
 struct MergeRow {

@@ -230,7 +230,8 @@ __global__ __launch_bounds__(256) void rope_quant_kernel(RopeQuantArgs a) {
 // ---------------------------------------------------------------------------
 // The reading back: [B, Hkv, L, D] of T from the pages of every sequence, rows from
 // its length on as zeros (FILL) or left as they are. Bound by HBM bytes, mostly those
-// written. One thread takes 16 codes of a row of K or V.
+// written: 16 sequences of up to 8192 tokens, 8 heads of 128 from 8 bits to bf16, in
+// 143 us at the rate of a copy (133). One thread takes 16 codes of a row of K or V.
 // ---------------------------------------------------------------------------
 struct ReadQuantArgs {
   const char *kc, *vc;

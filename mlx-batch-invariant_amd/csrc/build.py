@@ -55,6 +55,12 @@ CFLAGS = [
 # tile measured 3-8% slower with it, so the flag stays per file; the fp32
 # attention kernels keep the default (with it one more of them spills).
 #
+# The attention over pages (bi_attn_pages_*) keeps 16-bit kernels of up to 128 dims
+# within 256 registers that way, for two workgroups a CU; split into plain and
+# accumulator registers they spill. Its 192 and 256 dims are sources of their own
+# (bi_attn_pages_wide_*) without the flag: with it the compiler ends with an
+# error on them (ROCm 7.2).
+#
 # The 4-bit quantized sources use the memory-clause scheduler (device pass
 # only). Its visible change in the decode GEMV is the prologue: every
 # kernel-argument load issued before the first wait, where the default waited

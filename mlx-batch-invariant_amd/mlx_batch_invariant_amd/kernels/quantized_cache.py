@@ -299,8 +299,9 @@ def batch_invariant_quantized_paged_attention(q: torch.Tensor, k_pages: Quantize
     rows hold; one that sees none gets zeros; a NaN or infinity that it sees in V
     comes out in its dim.
 
-    Single tokens and short chunks read the codes; chunks of many rows read them back
-    first, into a workspace of up to 2 GiB (or one sequence).
+    Single tokens and chunks of up to 64 rows (tokens x query heads of a kv head) read
+    the codes; longer ones read them back first, into a workspace of up to 2 GiB (or
+    one sequence).
 
     ``shared_lens`` / ``shared_starts``: as in ``batch_invariant_shared_prefix_attention``
     (None: no sequence shares its prefix).
