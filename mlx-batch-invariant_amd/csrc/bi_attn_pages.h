@@ -664,8 +664,8 @@ __global__ __launch_bounds__(256, (pages_min_blocks<T, D>())) void attn_pages(Pa
 // registers. For P.V wave w takes the dims 16 dt, dt = NJ w .. NJ w + NJ - 1: a
 // transposing LDS read gives a lane the codes of 8 keys (4 bits: 16) of one dim, and
 // each is dequantized once, with its key's pair from LDS.
-// Bound by bytes at 8 bits and by the vector instructions at 4, of which dequantizing
-// takes two thirds (a conversion, an fma and half a rounding pair for every value): 64
+// Bound by bytes at 8 bits, by bytes and vector instructions at 4 (an fma, half a
+// rounding pair and some cutting for every value, most of a step's instructions): 64
 // sequences of up to 8192 keys, 32 / 8 heads of 128: 141 to 165 us on different cards for
 // 8 bits in bf16 (572 MB; a copy takes 112), 100 to 110 for 4 bits in fp16 (302 MB, 59).
 // Codes converted before they go to LDS took 500 and 459, the next item's codes
@@ -734,7 +734,10 @@ __global__ __launch_bounds__(256, (codes_min_blocks<T, D, BITS>())) void attn_co
   // an even one on, four of 64 dims), else one for each or for two of them.
   constexpr int NS = NJ == 3 ? 3 : NJ == 4 && GS == 32 ? 4 : 1;
   __shared__ __attribute__((aligned(1024))) char Vs[kSplit * CT::kRowBytes];
-  __shared__ __attribute__((aligned(16))) float vsc[NG][kSplit], vbi[NG][kSplit];   // V's scales and biases
+  __shared__ __attribute__((aligned(16))) float vsc[NG][kSplit], vbi[NG][kSplit];   // V's scales (times the codes' factors) and biases
+  // (a wave's scales may be too large for that: fp16's are finite times 2^24)
+  constexpr bool BIG = BITS == 4 && !std::is_same<T, f16>::value;
+  __shared__ int big_s[4];
   __shared__ float mx[4][16];
   extern __shared__ u32x4 Ps[];                           // [step][half][lane row][row of the sequence]
 
@@ -865,13 +868,25 @@ __global__ __launch_bounds__(256, (codes_min_blocks<T, D, BITS>())) void attn_co
     it = locate(item + (int)gridDim.x);                   // the next item's pages
     page = page_of(it);
 
-    // V's pairs to LDS.
+    // V's pairs to LDS. (A wave that holds a scale of 2^100 or more converts its codes.)
+    bool k_big = false, v_big = false;
+    if constexpr (BIG) {
+      float ks = 0.0f, vs = 0.0f;
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        ks = fmaxf(ks, fabsf(unpack_pair<T>(kp[g]).s));
+        vs = fmaxf(vs, fabsf(unpack_pair<T>(vp[g]).s));
+      }
+      k_big = __ballot(ks >= 0x1p100f) != 0;
+      v_big = __ballot(vs >= 0x1p100f) != 0;
+    }
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       const Pair<T> x = unpack_pair<T>(vp[g]);
-      vsc[g][tid] = x.s;
+      vsc[g][tid] = x.s * (v_big ? 1.0f : code_factor<BITS>(tid));   // (a step's element e is key e of 4 from a multiple of 4 on)
       vbi[g][tid] = x.b;
     }
+    if (BIG && lane == 0) big_s[wave] = v_big;
     int lim = 0, row = -1;
     if (my_p < rows1) {
       lim = (a.causal ? total - a.Tq + my_p / G + 1 : total) - j0;
@@ -879,7 +894,7 @@ __global__ __launch_bounds__(256, (codes_min_blocks<T, D, BITS>())) void attn_co
     }
     float s[KT][4];
     float m = -INFINITY;
-    auto scores = [&](auto masked) __attribute__((always_inline)) {
+    auto scores = [&](auto masked, auto big) __attribute__((always_inline)) {
 #pragma unroll
       for (int t = 0; t < KT; ++t) {
         f32x4 acc = {0.f, 0.f, 0.f, 0.f};
@@ -893,7 +908,22 @@ __global__ __launch_bounds__(256, (codes_min_blocks<T, D, BITS>())) void attn_co
         }
         kc[t].arrange();
 #pragma unroll
-        for (int st = 0; st < KS; ++st) acc = mfma_step(dequant_frag<T, BITS>(kc[t].codes(st), g[32 * st / GS]), qf[st], acc);
+        for (int st = 0; st < KS; ++st) {
+          const Pair<T> p = g[32 * st / GS];
+          F k;
+          if constexpr (decltype(big)::value) {
+            k = dequant_frag<T, BITS>(kc[t].codes(st), p);
+          } else {
+            float sc[8], bi[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              sc[e] = p.s * code_factor<BITS>(e);
+              bi[e] = p.b;
+            }
+            k = dequant_scaled8<T, BITS>(kc[t].codes(st), sc, bi);
+          }
+          acc = mfma_step(k, qf[st], acc);
+        }
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           const bool seen = !decltype(masked)::value || 64 * wave + 16 * t + 4 * qq + i < lim;
@@ -904,8 +934,9 @@ __global__ __launch_bounds__(256, (codes_min_blocks<T, D, BITS>())) void attn_co
       }
     };
     // (columns without a row may hold anything)
-    if (__ballot(my_p < rows1 && lim < kSplit)) scores(std::true_type());
-    else scores(std::false_type());
+    if (k_big) scores(std::true_type(), std::true_type());
+    else if (__ballot(my_p < rows1 && lim < kSplit)) scores(std::true_type(), std::false_type());
+    else scores(std::false_type(), std::false_type());
     m = quarter_max(m);
     if (qq == 0) mx[wave][r] = m;
     stage_barrier<63>();                                  // (V's copies may still be in flight)
@@ -985,18 +1016,43 @@ __global__ __launch_bounds__(256, (codes_min_blocks<T, D, BITS>())) void attn_co
         }
       }
     };
-    auto step_of = [&](const Step& x, const Codes8<BITS> (&c)[NJ], bool clean) __attribute__((always_inline)) {
+    auto step_of = [&](const Step& x, const Codes8<BITS> (&c)[NJ], bool clean, auto big) __attribute__((always_inline)) {
 #pragma unroll
       for (int j = 0; j < NJ; ++j) {
         const int i = NS == 1 ? 0 : j / (NJ == 3 ? 1 : 2);
-        F v = dequant_frag8<T, BITS>(c[j], x.s[i], x.b[i]);
+        F v;
+        if constexpr (decltype(big)::value) v = dequant_frag8<T, BITS>(c[j], x.s[i], x.b[i]);
+        else v = dequant_scaled8<T, BITS>(c[j], x.s[i], x.b[i]);
         if (clean) v = finite_frag(v);
         acc[j] = pv_step<T>(x.pf, v, acc[j]);             // (a wave without a tile computes the last one, unused)
       }
     };
+    // The scale of a key as its pair has it, from LDS.
+    auto plain = [&](float sc, int key) { return BIG && big_s[key / 64] ? sc : sc * (1.0f / code_factor<BITS>(key)); };
+    auto weigh = [&](bool clean) __attribute__((always_inline)) {   // (rare ones, in little code)
+#pragma unroll
+      for (int j = 0; j < NJ; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 1
+      for (int k2 = 0; k2 < kSplit / 64; ++k2) {
+        Codes8<BITS> vc[2][NJ];
+        Step x;
+        read_codes(vc, k2);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          read_step(x, 2 * k2 + h);
+#pragma unroll
+          for (int i = 0; i < NS; ++i)
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x.s[i][e] = plain(x.s[i][e], 64 * k2 + e);
+          step_of(x, vc[h], clean, std::true_type());
+        }
+      }
+    };
 #pragma unroll
     for (int j = 0; j < NJ; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    {
+    if (BIG && __builtin_amdgcn_readfirstlane(big_s[0] | big_s[1] | big_s[2] | big_s[3])) {
+      weigh(false);
+    } else {
       Step st[2];
       Codes8<BITS> vc[2][2][NJ];
       read_codes(vc[0], 0);
@@ -1005,7 +1061,7 @@ __global__ __launch_bounds__(256, (codes_min_blocks<T, D, BITS>())) void attn_co
       for (int ks = 0; ks < kSplit / 32; ++ks) {
         if (ks % 2 == 0 && ks + 2 < kSplit / 32) read_codes(vc[(ks / 2 + 1) % 2], ks / 2 + 1);
         if (ks + 1 < kSplit / 32) read_step(st[(ks + 1) % 2], ks + 1);
-        step_of(st[ks % 2], vc[ks / 2 % 2][ks % 2], false);
+        step_of(st[ks % 2], vc[ks / 2 % 2][ks % 2], false, std::false_type());
         __builtin_amdgcn_sched_barrier(0);                // (or every step's reads are gathered in front, and spill)
       }
     }
@@ -1022,19 +1078,7 @@ __global__ __launch_bounds__(256, (codes_min_blocks<T, D, BITS>())) void attn_co
 #pragma unroll
       for (int i = 0; i < 4; ++i) finite = finite && (NJ * wave + j >= NDT || fabsf(acc[j][i]) < INFINITY);
     if (__ballot(!finite)) {
-#pragma unroll
-      for (int j = 0; j < NJ; ++j) acc[j] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 1
-      for (int k2 = 0; k2 < kSplit / 64; ++k2) {
-        Codes8<BITS> vc[2][NJ];
-        Step x;
-        read_codes(vc, k2);
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          read_step(x, 2 * k2 + h);
-          step_of(x, vc[h], true);
-        }
-      }
+      weigh(true);
       for (int key = 0; key < n_act; ++key) {
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
@@ -1042,7 +1086,7 @@ __global__ __launch_bounds__(256, (codes_min_blocks<T, D, BITS>())) void attn_co
           const int dim = 16 * (NJ * wave + j) + r, byte = dim * BITS / 8;
           const uint32_t c = (uint8_t)Vs[CT::off(key, byte >> 4) + (byte & 15)];
           const float code = (float)(BITS == 8 ? c : c >> 4 * (dim & 1) & 15u);
-          const float x = to_f32(to_store<T>(__builtin_fmaf(code, vsc[dim / GS][key], vbi[dim / GS][key])));
+          const float x = to_f32(to_store<T>(__builtin_fmaf(code, plain(vsc[dim / GS][key], key), vbi[dim / GS][key])));
           if (fabsf(x) < INFINITY) continue;
 #pragma unroll
           for (int i = 0; i < 4; ++i)

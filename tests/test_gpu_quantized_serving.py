@@ -335,3 +335,32 @@ def test_library_ops():
     kd, vd = (values(p).cuda() for p in a)
     want = bi.batch_invariant_shared_prefix_attention(got, kd, vd, table, lens, scale=0.2, shared_starts=dev([0, 2]), shared_lens=dev([256]))
     assert torch.equal(want, ops.shared_prefix_attention(got, kd, vd, table, lens, 0.2, False, dev([0, 2]), dev([256])))
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("nbits,gs,D", [(4, 32, 64), (4, 64, 128), (4, 32, 256), (8, 64, 64)])
+@pytest.mark.parametrize("which", ["k", "v", "kv"])
+def test_scales_of_every_size(dt, nbits, gs, D, which):
+    """Scales at both ends of their type, in a few keys or all of one wave's, beside ordinary ones."""
+    bi, g = _bi(), gen(D + nbits)
+    B, Hq, Hkv, page, L, n = 3, 4, 2, 16, 700, 150
+    table = torch.randperm(n, generator=g)[:B * 44].reshape(B, 44).to(I32).cuda()
+    lens = dev([L, 256, 65])
+    high, low = (1e4, 6e-8) if dt == "f16" else (2.0 ** 118, 2.0 ** -130)
+    for part in range(3):
+        pools = [random_pool(n, Hkv, page, D, nbits, gs, dt, g) for _ in range(2)]
+        for p, name in zip(pools, "kv"):
+            if name not in which:
+                continue
+            pages = table.cpu().long()
+            rows = (pages[0, 5:6], pages[:, 0:4].flatten(), torch.arange(n))[part]   # one page, the first wave of each, all
+            for size, pick in ((high, rows), (low, pages[1, 9:11])):
+                p.groups[pick.cuda(), :, ::3] *= size
+        for t in ("k" in which and part == 2, False):
+            for T in (1, 3):
+                q = randn((B, Hq, T, D), DT[dt], g) * (2.0 / high if t else 1.0 / (1 + (high if "k" in which else 0)))
+                got = bi.batch_invariant_quantized_paged_attention(q, *pools, table, lens, mask="causal")
+                k, v = bi.read_quantized_cache(*pools, table, lens)
+                want = bi.batch_invariant_attention(q, k, v, kv_lens=lens, mask="causal")
+                assert torch.isfinite(want).all()
+                assert torch.equal(got, want), (part, T)
