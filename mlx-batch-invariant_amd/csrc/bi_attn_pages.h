@@ -36,6 +36,15 @@ __device__ __forceinline__ int pages_len_uniform(const PagesArgs& a, int b) {
 
 typedef int i32x4_t __attribute__((ext_vector_type(4)));
 
+// The item that the workgroup takes in a round, of the 8 XCDs (which workgroups reach
+// in turn) each a run of neighbours: the chunks of one split, and the heads of one
+// page, share its cache. The last round is dealt to all XCDs too. -1: none is left.
+__device__ __forceinline__ int dealt(int round, int items) {
+  const int grid = (int)gridDim.x, base = round * grid, n = min(items - base, grid);
+  const int run = (n + 7) / 8, i = (int)(blockIdx.x / 8), at = (int)(blockIdx.x % 8) * run + i;
+  return i < run && at < n ? base + at : -1;
+}
+
 // The operands of a P.V step in LDS, the two halves of a lane `half` pieces apart.
 template <typename T>
 __device__ __forceinline__ void store_pfrag(u32x4* p, int half, const PFrag<T>& pf) {
@@ -318,9 +327,6 @@ __global__ __launch_bounds__(256, (pages_min_blocks<T, D>())) void attn_pages(Pa
   const int G = a.Hq / a.Hkv, rows1 = a.Tq * G;
   const bool direct = a.nsplit == 1;
   const int page_mask = (1 << a.page_shift) - 1;
-  // Neighbouring items on one XCD (workgroups reach the 8 of them in turn): the
-  // chunks of one split, and the heads of one page, share its cache.
-  const int w0 = (int)(blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8);
   const int dt0 = min(NJ * wave, NDTV - NJ < 0 ? 0 : NDTV - 1);   // this wave's first dim tile (a wave without one repeats the last)
 
   const int nseg = a.groups + a.B;
@@ -341,7 +347,7 @@ __global__ __launch_bounds__(256, (pages_min_blocks<T, D>())) void attn_pages(Pa
   }
   struct Item { int seq0, nseq, split, hk, chunk0, n_act; };   // n_act < 0: no more items
   auto locate = [&](int item) -> Item {
-    if (item >= items) return Item{0, 0, 0, 0, 0, -1};
+    if (item < 0) return Item{0, 0, 0, 0, 0, -1};
     // the last segment that starts at or before the item (ones without items share a start with the next)
     int at = 0;
     if (nseg <= kPlanCached) {
@@ -377,9 +383,9 @@ __global__ __launch_bounds__(256, (pages_min_blocks<T, D>())) void attn_pages(Pa
     return a.table[(int64_t)it.seq0 * a.table_stride + (pos >> a.page_shift)];
   };
 
-  Item it = locate(w0);
+  Item it = locate(dealt(0, items));
   int page = page_of(it);
-  for (int item = w0; it.n_act >= 0; item += (int)gridDim.x) {
+  for (int round = 1; it.n_act >= 0; ++round) {
     const int seq0 = it.seq0, hk = it.hk, split = it.split, chunk0 = it.chunk0, n_act = it.n_act;
     const int nrows = it.nseq * rows1, j0 = split * kSplit;   // rows of the segment
     // Row p of the segment: (sequence, head, token).
@@ -396,7 +402,7 @@ __global__ __launch_bounds__(256, (pages_min_blocks<T, D>())) void attn_pages(Pa
         row_of(i / D, b, h, t);
         static_cast<T*>(a.out)[(((int64_t)b * a.Hq + h) * a.Tq + t) * D + i % D] = (T)0.0f;
       }
-      it = locate(item + (int)gridDim.x);
+      it = locate(dealt(round, items));
       page = page_of(it);
       continue;
     }
@@ -494,7 +500,7 @@ __global__ __launch_bounds__(256, (pages_min_blocks<T, D>())) void attn_pages(Pa
     }
     asm volatile("" ::: "memory");
 
-    it = locate(item + (int)gridDim.x);                   // the next item's pages
+    it = locate(dealt(round, items));                   // the next item's pages
     page = page_of(it);
     if constexpr (KEEP > 0) {
       stage_barrier<0>();                                 // V landed
@@ -666,8 +672,10 @@ __global__ __launch_bounds__(256, (pages_min_blocks<T, D>())) void attn_pages(Pa
 // each is dequantized once, with its key's pair from LDS.
 // Bound by bytes at 8 bits, by bytes and vector instructions at 4 (an fma, half a
 // rounding pair and some cutting for every value, most of a step's instructions): 64
-// sequences of up to 8192 keys, 32 / 8 heads of 128: 141 to 165 us on different cards for
-// 8 bits in bf16 (572 MB; a copy takes 112), 100 to 110 for 4 bits in fp16 (302 MB, 59).
+// sequences of up to 8192 keys, 32 / 8 heads of 128: 139 to 160 us on different cards for
+// 8 bits in bf16 (572 MB; a copy takes 112), 85 to 92 for 4 bits in fp16 (303 MB, 59).
+// Nothing that follows from the lane alone is kept over the items: at 128 registers it
+// goes to scratch memory, and reading it back waits for every copy in flight (97 us).
 // Codes converted before they go to LDS took 500 and 459, the next item's codes
 // requested an item ahead, with two workgroups a CU for the registers, 176 and 136.
 // ---------------------------------------------------------------------------
@@ -754,26 +762,41 @@ __global__ __launch_bounds__(256, (codes_min_blocks<T, D, BITS>())) void attn_co
   const int ps = qq * rc + (my_p & (rc - 1));
   const bool direct = a.nsplit == 1;
   const int page_mask = (1 << a.page_shift) - 1;
-  const int w0 = (int)(blockIdx.x % 8 * (gridDim.x / 8) + blockIdx.x / 8);
 
   // Item -> (sequence, split, kv head), found from the lengths 64 sequences at a time;
   // a workgroup's items rise.
   int c64 = -1, lo = 0, hi = 0, incl = 0;
   struct Item { int b, split, hk, n_act; };               // n_act < 0: no more items
-  auto locate = [&](int item) -> Item {
-    while (item >= hi && 64 * (c64 + 1) < a.B) {
-      ++c64;
-      const int b = 64 * c64 + lane;
-      incl = b < a.B ? (direct ? 1 : (pages_len(a, b) + kSplit - 1) / kSplit) * a.Hkv : 0;
+  auto items_of = [&](int b) { return b < a.B ? (direct ? 1 : (pages_len(a, b) + kSplit - 1) / kSplit) * a.Hkv : 0; };
+  auto scan = [&] {
+    int l = lane;
+    asm volatile("" : "+v"(l));                         // (its addresses are not kept over the items)
+    ++c64;
+    incl = items_of(64 * c64 + l);
 #pragma unroll
-      for (int off = 1; off < kWave; off <<= 1) {
-        const int up = __shfl_up(incl, off, kWave);
-        if (lane >= off) incl += up;
-      }
-      lo = hi;
-      hi = lo + __builtin_amdgcn_readlane(incl, 63);
+    for (int off = 1; off < kWave; off <<= 1) {
+      const int up = __shfl_up(incl, off, kWave);
+      if (lane >= off) incl += up;
     }
-    if (item >= hi) return Item{0, 0, 0, -1};
+    lo = hi;
+    hi = lo + __builtin_amdgcn_readlane(incl, 63);
+  };
+  scan();
+  int items = hi;                                         // of all sequences
+  if (a.B > 64) {
+    int sum = 0;
+    for (int b = tid; b < a.B; b += 256) sum += items_of(b);
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) sum += __shfl_xor(sum, off, kWave);
+    int* part = reinterpret_cast<int*>(&mx[0][0]);
+    if (lane == 0) part[wave] = sum;
+    __syncthreads();
+    items = __builtin_amdgcn_readfirstlane(part[0] + part[1] + part[2] + part[3]);
+    __syncthreads();
+  }
+  auto locate = [&](int item) -> Item {
+    while (item >= hi && 64 * (c64 + 1) < a.B) scan();
+    if (item < 0) return Item{0, 0, 0, -1};
     const int i = __popcll(__ballot(lo + incl <= item));
     const int local = item - lo - (i ? __builtin_amdgcn_readlane(incl, max(i - 1, 0)) : 0);
     Item it;
@@ -783,6 +806,9 @@ __global__ __launch_bounds__(256, (codes_min_blocks<T, D, BITS>())) void attn_co
     it.n_act = min(kSplit, pages_len_uniform(a, it.b) - it.split * kSplit);
     return it;
   };
+  const int full = items / (int)gridDim.x * (int)gridDim.x;   // items of the rounds that every workgroup has one of
+  const int last = dealt(items / (int)gridDim.x, items);
+  auto next = [&](int item) { return item + (int)gridDim.x < full ? item + (int)gridDim.x : item < full ? last : -1; };
   auto page_of = [&](const Item& it) {
     if (it.n_act <= 0) return 0;
     const int pos = it.split * kSplit + min(tid, it.n_act - 1);
@@ -790,19 +816,24 @@ __global__ __launch_bounds__(256, (codes_min_blocks<T, D, BITS>())) void attn_co
   };
 
   // (token, head) p of sequence b, heads inside tokens.
-  auto out_row = [&](int b, int hk, int p) { return (b * a.Hq + hk * G + p % G) * a.Tq + p / G; };
+  auto out_row = [&](int b, int hk, int p) {
+    const int x = quotient(p, G, a.g_inv);
+    return (b * a.Hq + hk * G + p - x * G) * a.Tq + x;
+  };
   auto off_of = [&](uint64_t off, int l) {
     return (uint64_t)(uint32_t)__shfl((int)(uint32_t)off, l, kWave) |
            (uint64_t)(uint32_t)__shfl((int)(uint32_t)(off >> 32), l, kWave) << 32;
   };
-  Item it = locate(w0);
+  int item = full ? dealt(0, items) : last;
+  Item it = locate(item);
   int page = page_of(it);
-  for (int item = w0; it.n_act >= 0; item += (int)gridDim.x) {
+  for (; it.n_act >= 0;) {
     const int b = it.b, hk = it.hk, j0 = it.split * kSplit, n_act = it.n_act, split = it.split;
     if (n_act == 0) {                                     // (direct, an empty sequence) no keys: zeros
       for (int i = tid; i < rows1 * D; i += 256)
         static_cast<T*>(a.out)[(int64_t)out_row(b, hk, i / D) * D + i % D] = (T)0.0f;
-      it = locate(item + (int)gridDim.x);
+      item = next(item);
+      it = locate(item);
       page = page_of(it);
       continue;
     }
@@ -818,8 +849,11 @@ __global__ __launch_bounds__(256, (codes_min_blocks<T, D, BITS>())) void attn_co
     load_words<NG * PW>(static_cast<const T*>(a.vg) + hk * a.vg_sh + row_off(a.vg_sp, a.vg_sl), &vp[0][0]);
     F qf[KS];
     {
-      const int p = min(my_p, rows1 - 1);
-      const T* qrow = static_cast<const T*>(a.q) + (int64_t)b * a.q_sb + (int64_t)(hk * G + p % G) * a.q_sh + (int64_t)(p / G) * a.q_st;
+      int p = min(my_p, rows1 - 1);
+      asm volatile("" : "+v"(p));                         // (what follows from lanes alone is not kept over the items: registers)
+      const int x = quotient(p, G, a.g_inv);
+      const T* qrow = static_cast<const T*>(a.q) + ((uint64_t)(uint32_t)b * (uint32_t)a.q_sb + (uint64_t)(uint32_t)(hk * G + p - x * G) * (uint32_t)a.q_sh +
+                                                    (uint64_t)(uint32_t)x * (uint32_t)a.q_st);
 #pragma unroll
       for (int st = 0; st < KS; ++st) qf[st] = my_p < rows1 ? frag_load(qrow + 32 * st + 8 * qq) : frag_zero<F>();
     }
@@ -865,7 +899,8 @@ __global__ __launch_bounds__(256, (codes_min_blocks<T, D, BITS>())) void attn_co
       }
     }
     asm volatile("" ::: "memory");
-    it = locate(item + (int)gridDim.x);                   // the next item's pages
+    item = next(item);
+    it = locate(item);                   // the next item's pages
     page = page_of(it);
 
     // V's pairs to LDS. (A wave that holds a scale of 2^100 or more converts its codes.)
@@ -889,8 +924,10 @@ __global__ __launch_bounds__(256, (codes_min_blocks<T, D, BITS>())) void attn_co
     if (BIG && lane == 0) big_s[wave] = v_big;
     int lim = 0, row = -1;
     if (my_p < rows1) {
-      lim = (a.causal ? total - a.Tq + my_p / G + 1 : total) - j0;
-      row = out_row(b, hk, my_p);
+      int p = my_p;
+      asm volatile("" : "+v"(p));
+      lim = (a.causal ? total - a.Tq + quotient(p, G, a.g_inv) + 1 : total) - j0;
+      row = out_row(b, hk, p);
     }
     float s[KT][4];
     float m = -INFINITY;
@@ -938,9 +975,12 @@ __global__ __launch_bounds__(256, (codes_min_blocks<T, D, BITS>())) void attn_co
     else if (__ballot(my_p < rows1 && lim < kSplit)) scores(std::true_type(), std::false_type());
     else scores(std::false_type(), std::false_type());
     m = quarter_max(m);
-    if (qq == 0) mx[wave][r] = m;
+    // (an address read back from scratch memory here would wait for V's copies)
+    int ln = lane;
+    asm volatile("" : "+v"(ln));
+    if (ln < 16) mx[wave][ln] = m;
     stage_barrier<63>();                                  // (V's copies may still be in flight)
-    m = fmaxf(fmaxf(mx[0][r], mx[1][r]), fmaxf(mx[2][r], mx[3][r]));
+    m = fmaxf(fmaxf(mx[0][ln % 16], mx[1][ln % 16]), fmaxf(mx[2][ln % 16], mx[3][ln % 16]));
     const float msub = m == -INFINITY ? 0.0f : m;         // no visible key: weights 0, not NaN
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
@@ -1094,18 +1134,29 @@ __global__ __launch_bounds__(256, (codes_min_blocks<T, D, BITS>())) void attn_co
         }
       }
     }
-#pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-      if (NJ * wave + j >= NDT) continue;
+    int rr = r;
+    asm volatile("" : "+v"(rr));                          // (addresses are not kept over the items)
+    const uint32_t dim = (uint32_t)(16 * NJ * wave + rr);
+    if (direct) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         if (i >= ni) continue;
-        const int d = 16 * (NJ * wave + j) + r;
-        if (direct) {
-          if (arow[i] >= 0) static_cast<T*>(a.out)[(int64_t)arow[i] * D + d] = to_store<T>(only_split(acc[j][i], lsum[i]));
-        } else if (alim[i] > 0) {
-          a.pacc[((int64_t)arow[i] * a.nsplit + split) * D + d] = acc[j][i];
-        }
+        T* o = static_cast<T*>(a.out) + ((uint64_t)(uint32_t)arow[i] * (uint32_t)D + dim);
+        if (arow[i] >= 0)
+#pragma unroll
+          for (int j = 0; j < NJ; ++j)
+            if (NDT % 4 == 0 || NJ * wave + j < NDT) o[16 * j] = to_store<T>(only_split(acc[j][i], lsum[i]));
+      }
+    } else {                                              // (a row's partials: fewer than 2^32 elements)
+      const uint32_t row_n = (uint32_t)a.nsplit * (uint32_t)D, at = (uint32_t)split * (uint32_t)D + dim;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if (i >= ni) continue;
+        float* o = a.pacc + ((uint64_t)(uint32_t)arow[i] * row_n + at);
+        if (alim[i] > 0)
+#pragma unroll
+          for (int j = 0; j < NJ; ++j)
+            if (NDT % 4 == 0 || NJ * wave + j < NDT) o[16 * j] = acc[j][i];
       }
     }
     if (!direct && wave == sum_wave && r == 0) {
