@@ -345,9 +345,9 @@ __global__ __launch_bounds__(256, (pages_min_blocks<T, D>())) void attn_pages(Pa
       __syncthreads();
     }
   }
-  struct Item { int seq0, nseq, split, hk, chunk0, n_act; };   // n_act < 0: no more items
+  struct Item { int seq0, nseq, split, hk, chunk0, chunks, n_act; };   // n_act < 0: no more items
   auto locate = [&](int item) -> Item {
-    if (item < 0) return Item{0, 0, 0, 0, 0, -1};
+    if (item < 0) return Item{0, 0, 0, 0, 0, 0, -1};
     // the last segment that starts at or before the item (ones without items share a start with the next)
     int at = 0;
     if (nseg <= kPlanCached) {
@@ -369,9 +369,10 @@ __global__ __launch_bounds__(256, (pages_min_blocks<T, D>())) void attn_pages(Pa
     Item it;
     it.seq0 = w[1];
     it.nseq = w[2];
-    const int runs = (int)(((int64_t)it.nseq * rows1 + 16 * per - 1) / (16 * per));
+    const int all = (it.nseq * rows1 + 15) / 16, runs = (all + per - 1) / per, each = (all + runs - 1) / runs;   // (even runs)
     const int local = item - w[0], x = local / runs, y = quotient(x, a.Hkv, a.hkv_inv);
-    it.chunk0 = (local - x * runs) * per;
+    it.chunk0 = (local - x * runs) * each;
+    it.chunks = min(each, all - it.chunk0);
     it.hk = x - y * a.Hkv;
     it.split = w[3] + y;
     it.n_act = min(kSplit, pages_len_uniform(a, it.seq0) - it.split * kSplit);
@@ -386,7 +387,7 @@ __global__ __launch_bounds__(256, (pages_min_blocks<T, D>())) void attn_pages(Pa
   Item it = locate(dealt(0, items));
   int page = page_of(it);
   for (int round = 1; it.n_act >= 0; ++round) {
-    const int seq0 = it.seq0, hk = it.hk, split = it.split, chunk0 = it.chunk0, n_act = it.n_act;
+    const int seq0 = it.seq0, hk = it.hk, split = it.split, chunk0 = it.chunk0, chunks = it.chunks, n_act = it.n_act;
     const int nrows = it.nseq * rows1, j0 = split * kSplit;   // rows of the segment
     // Row p of the segment: (sequence, head, token).
     auto row_of = [&](int p, int& b, int& h, int& t) {
@@ -511,7 +512,6 @@ __global__ __launch_bounds__(256, (pages_min_blocks<T, D>())) void attn_pages(Pa
       stage_barrier<63>();                                // read by everyone
     }
 
-    const int chunks = min(per, (nrows - 16 * chunk0 + 15) / 16);
     bool landed = false;
     for (int c = 0; c < chunks; ++c) {
       const int row = rows.row, lim = rows.lim;
