@@ -282,8 +282,8 @@ struct KRow {
 // Bound by instructions where many rows share a prefix: a chunk takes a CU about 1.3 us,
 // 48 products a wave (as long as 0.35 us) among some 330 vector instructions and
 // two exchanges; by latency and bytes where they share little. 64 sequences of 32 / 8
-// heads of 128 in bf16 behind 8192 keys: 60 us, 67 in all with the merge, where
-// every sequence reading its own keys takes 322; without the shared keys 24 in all.
+// heads of 128 in bf16 behind 8192 keys, 256 of their own: 63 us with the merge, where
+// every sequence reading its own keys takes 323; without the shared keys 24.
 // Of a second half of the grid that takes its items from the last on, loads beside the
 // others' products, nothing came (57 -> 59 us), nor of waiting for the next rows in front
 // of the stores.
@@ -673,7 +673,7 @@ __global__ __launch_bounds__(256, (pages_min_blocks<T, D>())) void attn_pages(Pa
 // Bound by bytes at 8 bits, by bytes and vector instructions at 4 (an fma, half a
 // rounding pair and some cutting for every value, most of a step's instructions): 64
 // sequences of up to 8192 keys, 32 / 8 heads of 128: 139 to 160 us on different cards for
-// 8 bits in bf16 (572 MB; a copy takes 112), 85 to 92 for 4 bits in fp16 (303 MB, 59).
+// 8 bits in bf16 (572 MB; a copy takes 112), 92 to 100 for 4 bits in fp16 (303 MB, 59).
 // Nothing that follows from the lane alone is kept over the items: at 128 registers it
 // goes to scratch memory, and reading it back waits for every copy in flight (97 us).
 // Codes converted before they go to LDS took 500 and 459, the next item's codes

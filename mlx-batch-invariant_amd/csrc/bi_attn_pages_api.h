@@ -46,7 +46,7 @@ inline bool pages_few_rows(int64_t B, int64_t Hq, int64_t Hkv, int64_t Tq, int64
                            int causal, int dtype) {
   if (Tq == 1 || few_rows(B, Hq, Hkv, Tq, L, D, causal, dtype)) return true;
   const int64_t G = Hq / Hkv;
-  if (Tq > 64 || Tq * G > 64 || rows_partial_bytes(B, Hq, Tq, L, D) > ((int64_t)2 << 30)) return false;
+  if (Tq > 64 || Tq * G > 64 || (double)B * Hq > 1e9 || rows_partial_bytes(B, Hq, Tq, L, D) > ((int64_t)2 << 30)) return false;
   if (bits) return true;
   return groups > 0 && dtype != BI_F32 && Tq * G <= 16 && B >= 4 * groups && B * Hkv >= 128;
 }

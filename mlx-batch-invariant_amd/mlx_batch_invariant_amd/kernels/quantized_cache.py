@@ -135,7 +135,8 @@ def rope_quantized_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cos:
     (2^bits - 1)`` rounded to the type (1 where that is 0), ``code = round((y - bias) /
     scale)``, clamped. A code whose value the rounded scale would put past the type's
     largest number is not used. A group with an infinity or a NaN reads back as
-    NaN.
+    NaN. Of several tokens with one slot, each 16 values of the row keep some one's codes
+    and each group some one's pair.
     """
     what = "rope_quantized_cache"
     qs, ks = q.shape, k.shape
