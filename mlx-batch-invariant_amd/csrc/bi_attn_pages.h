@@ -292,10 +292,12 @@ template <typename T, int D>
 constexpr int pages_v_slices() {
   return (kSplit * D * (int)sizeof(T) + (128 << 10) - 1) >> 17;
 }
-// Workgroups per CU that the registers are held to: two where LDS has room for both.
+// Workgroups per CU that the registers are held to: two where LDS has room for them. (64
+// dims fit three anyway, and held to them are slower, 43 instead of 41 us for 64
+// sequences behind 8192 keys; 32 dims gain, 32 instead of 34.5.)
 template <typename T, int D>
 constexpr int pages_min_blocks() {
-  return sizeof(T) == 2 && D <= 128 ? 2 : 1;
+  return sizeof(T) == 4 || D > 128 ? 1 : D > 32 ? 2 : 3;
 }
 
 template <typename T, int D, int BITS>

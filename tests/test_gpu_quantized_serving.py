@@ -244,7 +244,7 @@ def test_rows_to_either_way(dt, Hq, Hkv):
         assert torch.equal(bi.batch_invariant_shared_prefix_attention(q, *plain, table, lens, mask="causal", **share), want)
 
 
-@pytest.mark.parametrize("B,groups", [(200, 55), (200, 56), (200, 57), (2000, 100)])
+@pytest.mark.parametrize("B,groups", [(140, 51), (140, 52), (140, 53), (200, 55), (200, 56), (200, 57), (2000, 100)])
 def test_plans_of_many_segments(B, groups):
     """Plans that every workgroup makes, that one makes, and of more segments than LDS keeps."""
     bi, g = _bi(), gen(B + groups)
