@@ -25,7 +25,7 @@ struct PagesArgs {
 inline unsigned inverse(int64_t d) { return d == 1 ? 0xffffffffu : (unsigned)(((int64_t)1 << 32) / d); }
 
 constexpr int kPlanWords = 5;            // of a segment in the plan
-constexpr int kPlanFused = 192;          // segments of a plan that every workgroup makes for itself (3.75 KB of LDS: with 4 KB three
+constexpr int kPlanFused = 192;          // segments of a plan that every workgroup makes for itself (3.75 KB of LDS: with 5 KB three
                                          // workgroups of 64 dims would not fit a CU, 46 instead of 41 us for 64 sequences behind 8192 keys)
 
 template <typename T, int D>
