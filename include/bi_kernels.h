@@ -496,12 +496,16 @@ int bi_read_quantized_cache(const void* k_codes, const void* k_groups, const voi
  * read back) where q, K and V are finite. Hidden keys take no part whatever their
  * rows hold; a query that sees no key gets zeros; infinities and NaN that a query
  * sees in V come out as bi_attn_scored's do.
- * Workspace (16-byte aligned): bi_attn_pages_workspace_bytes; calls that overlap must
- * not share it.
+ * Workspace (16-byte aligned): bi_attn_pages_workspace_bytes for any page size,
+ * bi_attn_pages_workspace_bytes_paged for one (less where groups > 0, many rows); calls that
+ * overlap must not share it. Groups over plain pages of more than 256 keys need, for many
+ * rows, K and V whose page and row strides have one ratio (BI_E_UNSUPPORTED otherwise).
  * Replaces: nothing in the reference (kernels/attention.py:87-254 reads one
  * contiguous cache of plain rows for each sequence). */
 size_t bi_attn_pages_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t Tq, int64_t L, int64_t D,
                                      int64_t groups, int bits, int causal, int dtype);
+size_t bi_attn_pages_workspace_bytes_paged(int64_t B, int64_t Hq, int64_t Hkv, int64_t Tq, int64_t L, int64_t D,
+                                           int64_t groups, int bits, int causal, int dtype, int64_t page_size);
 int bi_attn_pages(const void* q, const void* k, const void* k_groups, const void* v, const void* v_groups, int bits,
                   int64_t group_size, const int32_t* block_table, int64_t table_stride, int64_t page_size,
                   int64_t num_pages, const int32_t* kv_lens, const int32_t* shared_starts, const int32_t* shared_lens,

@@ -17,10 +17,6 @@
 
 namespace bi {
 
-__device__ __forceinline__ int pages_len(const PagesArgs& a, int b) {
-  return a.kv_lens ? min(max(a.kv_lens[b], 0), a.L) : a.L;
-}
-
 // x / d for x >= 0 from inv = inverse(d).
 __device__ __forceinline__ int quotient(int x, int d, unsigned inv) {
   const int q = (int)__umulhi((unsigned)x, inv);          // or one less
@@ -75,17 +71,14 @@ __device__ __forceinline__ PFrag<T> load_pfrag(const u32x4* p, int half) {
 // item, first sequence, sequences, first split, splits.
 // Groups are the runs starts[n] .. starts[n + 1] of sequences (clamped, each from
 // the last one's end on); one of fewer than two sequences shares nothing. The
-// shared splits are whole and lie within the first sequence's own keys.
+// shared splits are whole and lie within the first sequence's own keys. (shared_source_kernel
+// finds one sequence's group by the same rule.)
 // Every workgroup of attn_pages plans a call of up to kPlanFused segments for itself, in
 // LDS (a launch of its own takes 7 us); of more, one workgroup does it in front of them.
 // ---------------------------------------------------------------------------
 constexpr int kPlanThreads = 1024;
 constexpr int kPlanMostChunks = 32;
 constexpr int kPlanCached = 2048;        // segments whose first items a workgroup keeps in LDS
-
-__device__ __forceinline__ int plan_start(const PagesArgs& a, int n) {
-  return a.starts ? min(max(a.starts[n], 0), a.B) : n ? a.B : 0;
-}
 
 // By a workgroup of NT threads; `seg` in LDS or in memory, `part` in LDS. (All counts
 // stay below 2^31: the caller's items at one chunk each do.)

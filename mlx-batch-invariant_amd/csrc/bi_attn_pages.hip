@@ -1,14 +1,71 @@
 // bi_attn_pages.hip — C ABI of attention over quantized pages and of batches that
 // share prefixes (bi_attn_pages). Kernels of few rows: bi_attn_pages.h. Many rows go
-// through the kernels of bi_attn_scored with nothing changed, quantized pages read
-// back into the workspace first (bi_read_quantized_cache), a slice of the sequences
-// at a time.
+// through the kernels of bi_attn_scored with nothing changed: quantized pages read
+// back into the workspace first, a slice of the sequences at a time, shared prefixes
+// by a block table of their own there.
+#include <numeric>
+
 #include "bi_attn_pages_api.h"
 
 namespace bi_host {
 int check_quant(const char* what, int64_t D, int64_t bits, int64_t group_size, const void* const* pointers, int n,
                 const int64_t* strides, int dtype);
+int read_quantized(const void* k_codes, const void* k_groups, const void* v_codes, const void* v_groups,
+                   const int64_t* strides, const int32_t* block_table, int64_t table_stride, int64_t page_size,
+                   int64_t num_pages, const int32_t* kv_lens, const int32_t* source, const int32_t* all, void* k_out,
+                   void* v_out, int64_t B, int64_t Hkv, int64_t L, int64_t D, int bits, int64_t group_size, int fill,
+                   int dtype, void* stream);
 }
+
+namespace bi {
+
+// Where the first keys of a sequence lie, for the kernels of many rows: a workgroup per
+// sequence. By the plan's rule (bi_attn_pages.h), sequence b is in group n, the first with
+// starts[n + 1] > b, if no start up to starts[n] lies above b; the largest of those is
+// the group's first sequence. cols 0: out [B, 2], that sequence and how many keys come from
+// it. Else out [B, cols] is a block table of pages of `unit` = min(page size, 256) keys:
+// pages as they are, or of a larger page's 256 keys the piece page * per_page + its
+// number * per_split. (Entries behind a sequence's length are not written.)
+__global__ __launch_bounds__(256) void shared_source_kernel(PagesArgs a, int32_t* out, int64_t cols, int per_page, int per_split) {
+  __shared__ int part[2][4];
+  const int b = blockIdx.x, tid = threadIdx.x;
+  auto least = [&](int x, int at) {
+#pragma unroll
+    for (int off = 32; off >= 1; off >>= 1) x = min(x, __shfl_xor(x, off, kWave));
+    if (tid % kWave == 0) part[at][tid / kWave] = x;
+    __syncthreads();
+    return min(min(part[at][0], part[at][1]), min(part[at][2], part[at][3]));
+  };
+  int n = a.groups;
+  for (int i = tid; i < n; i += 256)
+    if (plan_start(a, i + 1) > b) n = i;
+  n = least(n, 0);
+  int lo = 0;
+  for (int i = tid; i <= n && i < a.groups; i += 256) lo = max(lo, plan_start(a, i));
+  lo = -least(-lo, 1);
+  int keys = 0;
+  if (n < a.groups && lo <= b && plan_start(a, n + 1) - lo > 1) {
+    const int want = a.slens ? min(max(a.slens[n], 0), a.L) : a.shared_len;
+    keys = min(want, pages_len(a, lo)) / kSplit * kSplit;
+  }
+  if (cols == 0) {
+    if (tid == 0) {
+      out[2 * b] = lo;
+      out[2 * b + 1] = keys;
+    }
+    return;
+  }
+  const int split_shift = __builtin_ctz(kSplit), shift = min(a.page_shift, split_shift);
+  const int used = (int)(((int64_t)pages_len(a, b) + (1 << shift) - 1) >> shift);
+  for (int c = tid; c < used; c += 256) {
+    const int pos = c << shift, row = pos < keys ? lo : b;
+    const int page = (int)clamp_page(a.table[row * a.table_stride + (pos >> a.page_shift)], a.num_pages);
+    const int piece = (pos & ((1 << a.page_shift) - 1)) >> split_shift;
+    out[b * cols + c] = a.page_shift <= split_shift ? page : page * per_page + piece * per_split;
+  }
+}
+
+}  // namespace bi
 
 namespace {
 
@@ -22,8 +79,40 @@ int64_t dense_slice(int64_t B, int64_t Hkv, int64_t L, int64_t D, int dtype) {
   return std::max<int64_t>(1, std::min(B, kDenseBytes / dense_bytes(Hkv, L, D, dtype)));
 }
 
+// A page of more than a split as pages of one split: a page's and a split's strides in
+// units, the largest one that K and V have in common up to a factor, which is each one's page stride
+// then. False: there is none, or the last one's number is no int32.
+struct Pieces {
+  int64_t per_page, per_split, k, v, count;
+};
+bool pieces_of(int64_t k_sp, int64_t k_sl, int64_t v_sp, int64_t v_sl, int64_t num_pages, int64_t page_size, Pieces* p) {
+  for (int64_t s : {k_sp, k_sl, v_sp, v_sl})
+    if (s > ((int64_t)1 << 50)) return false;
+  if (num_pages == 1) k_sp = v_sp = 0;
+  k_sl *= bi::kSplit;
+  v_sl *= bi::kSplit;
+  p->k = std::gcd(k_sp, k_sl);
+  p->v = std::gcd(v_sp, v_sl);
+  if (p->k && p->v && (k_sp / p->k != v_sp / p->v || k_sl / p->k != v_sl / p->v)) return false;
+  p->per_page = p->k ? k_sp / p->k : p->v ? v_sp / p->v : 0;
+  p->per_split = p->k ? k_sl / p->k : p->v ? v_sl / p->v : 0;
+  const double last = (double)(num_pages - 1) * p->per_page + (double)(page_size / bi::kSplit - 1) * p->per_split;
+  if (last >= 2147483647.0) return false;
+  p->count = (int64_t)last + 1;
+  return true;
+}
+
 size_t partial_bytes(int64_t B, int64_t Hq, int64_t Tq, int64_t L, int64_t D) {
   return ((size_t)bi::rows_partial_bytes(B, Hq, Tq, L, D) + 15) / 16 * 16;
+}
+
+// What shared_source_kernel writes: a table of pages of at most a split, or (codes) two words a sequence.
+int64_t table_cols(int64_t L, int64_t page_size) {
+  const int64_t unit = std::min<int64_t>(page_size, bi::kSplit);
+  return (L + unit - 1) / unit;
+}
+size_t source_bytes(int64_t B, int64_t L, int64_t groups, int bits, int64_t page_size) {
+  return groups == 0 ? 0 : ((size_t)B * (bits ? 2 : table_cols(L, page_size)) * sizeof(int32_t) + 15) / 16 * 16;
 }
 
 bool bad_shape(int64_t B, int64_t Hq, int64_t Hkv, int64_t Tq, int64_t L, int64_t D, int64_t groups) {
@@ -33,16 +122,21 @@ bool bad_shape(int64_t B, int64_t Hq, int64_t Hkv, int64_t Tq, int64_t L, int64_
 
 }  // namespace
 
-extern "C" size_t bi_attn_pages_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t Tq, int64_t L, int64_t D,
-                                                int64_t groups, int bits, int causal, int dtype) {
-  if (bad_shape(B, Hq, Hkv, Tq, L, D, groups)) return 0;
+extern "C" size_t bi_attn_pages_workspace_bytes_paged(int64_t B, int64_t Hq, int64_t Hkv, int64_t Tq, int64_t L, int64_t D,
+                                                      int64_t groups, int bits, int causal, int dtype, int64_t page_size) {
+  if (bad_shape(B, Hq, Hkv, Tq, L, D, groups) || page_size <= 0) return 0;
   if (bi::pages_few_rows(B, Hq, Hkv, Tq, L, D, groups, bits, causal, dtype))
     return partial_bytes(B, Hq, Tq, L, D) + (size_t)(2 + bi::kPlanWords * (groups + B)) * sizeof(int32_t);
   const int64_t nb = bits ? dense_slice(B, Hkv, L, D, dtype) : B;
   size_t n = bi_attn_scored_workspace_bytes(nb, Hq, Hkv, Tq, L, D, causal, 0, dtype);
   if (bits) n = std::max(n, bi_attn_scored_workspace_bytes((B - 1) % nb + 1, Hq, Hkv, Tq, L, D, causal, 0, dtype));
-  n = (n + 15) / 16 * 16;
+  n = (n + 15) / 16 * 16 + source_bytes(B, L, groups, bits, page_size);
   return n + (bits ? (size_t)(nb * dense_bytes(Hkv, L, D, dtype)) : 0);
+}
+
+extern "C" size_t bi_attn_pages_workspace_bytes(int64_t B, int64_t Hq, int64_t Hkv, int64_t Tq, int64_t L, int64_t D,
+                                                int64_t groups, int bits, int causal, int dtype) {
+  return bi_attn_pages_workspace_bytes_paged(B, Hq, Hkv, Tq, L, D, groups, bits, causal, dtype, 1);
 }
 
 extern "C" int bi_attn_pages(const void* q, const void* k, const void* k_groups, const void* v, const void* v_groups,
@@ -104,27 +198,56 @@ extern "C" int bi_attn_pages(const void* q, const void* k, const void* k_groups,
   for (int i = 0; i < 15; ++i)
     if ((i < 3 ? few : bits && i % 3 != 1) && strides[i] > 0xffffffffLL)
       return fail(BI_E_UNSUPPORTED, "%s: stride %d (%lld) must be below 2^32", what, i, (long long)strides[i]);
-  const size_t need = bi_attn_pages_workspace_bytes(B, Hq, Hkv, Tq, L, D, groups, bits, causal, dtype);
+  Pieces pieces = {1, 0, strides[3], strides[6], num_pages};
+  if (!few && !bits && groups > 0 && page_size > bi::kSplit &&
+      !pieces_of(strides[3], strides[5], strides[6], strides[8], num_pages, page_size, &pieces))
+    return fail(BI_E_UNSUPPORTED,
+                "%s: shared prefixes of many rows over pages of %lld keys need K and V of one layout (page strides %lld, "
+                "%lld, row strides %lld, %lld)", what, (long long)page_size, (long long)strides[3], (long long)strides[6],
+                (long long)strides[5], (long long)strides[8]);
+  const size_t need = bi_attn_pages_workspace_bytes_paged(B, Hq, Hkv, Tq, L, D, groups, bits, causal, dtype, page_size);
   if (need > 0 && (!ws || ws_bytes < need || !aligned16(ws)))
     return fail(BI_E_WORKSPACE, "%s: 16-byte aligned workspace of %zu bytes required, got %zu", what, need,
                 ws ? ws_bytes : (size_t)0);
   hipStream_t st = static_cast<hipStream_t>(stream);
 
+  bi::PagesArgs a;
+  a.kv_lens = kv_lens; a.table = block_table; a.starts = shared_starts; a.slens = shared_lens;
+  a.table_stride = table_stride;
+  a.B = (int)B; a.L = (int)L; a.groups = (int)groups;
+  a.shared_len = (int)std::min(std::max<int64_t>(shared_len, 0), L);
+  a.page_shift = shift; a.num_pages = (int)num_pages;
+
   if (!few) {
     const bi_score_mod none = {0.0f, nullptr, nullptr, 0, nullptr};
-    if (!bits)
-      return bi_attn_scored(q, k, v, block_table, table_stride, page_size, num_pages, kv_lens, out, B, Hq, Hkv, Tq, L, D,
-                            strides, causal, scale, &none, dtype, ws, ws_bytes, stream);
+    const size_t source_n = source_bytes(B, L, groups, bits, page_size);
+    int32_t* source = groups ? static_cast<int32_t*>(ws) : nullptr;
+    if (groups) {
+      const int64_t cols = bits ? 0 : table_cols(L, page_size);
+      bi::shared_source_kernel<<<(unsigned)B, 256, 0, st>>>(a, source, cols, (int)pieces.per_page, (int)pieces.per_split);
+      const int rc = launch_status(what);
+      if (rc) return rc;
+    }
+    char* after = static_cast<char*>(ws) + source_n;
+    ws_bytes -= source_n;
+    if (!bits) {
+      if (!groups)
+        return bi_attn_scored(q, k, v, block_table, table_stride, page_size, num_pages, kv_lens, out, B, Hq, Hkv, Tq, L, D,
+                              strides, causal, scale, &none, dtype, ws, ws_bytes, stream);
+      const int64_t st9[9] = {strides[0], strides[1], strides[2], pieces.k, strides[4], strides[5], pieces.v, strides[7], strides[8]};
+      return bi_attn_scored(q, k, v, source, table_cols(L, page_size), std::min<int64_t>(page_size, bi::kSplit), pieces.count,
+                            kv_lens, out, B, Hq, Hkv, Tq, L, D, st9, causal, scale, &none, dtype, after, ws_bytes, stream);
+    }
     const int64_t nb = dense_slice(B, Hkv, L, D, dtype), one = Hkv * L * D;
     const int64_t dense_st[9] = {strides[0], strides[1], strides[2], one, L * D, D, one, L * D, D};
-    char* kd = static_cast<char*>(ws);
+    char* kd = after;
     char* vd = kd + nb * one * es;
     char* rest = vd + nb * one * es;                      // (a multiple of 16 bytes: D is one of 32)
     for (int64_t b0 = 0; b0 < B; b0 += nb) {
       const int64_t n = std::min(nb, B - b0);
-      int rc = bi_read_quantized_cache(k, k_groups, v, v_groups, qs, block_table + b0 * table_stride, table_stride,
-                                       page_size, num_pages, kv_lens ? kv_lens + b0 : nullptr, kd, vd, n, Hkv, L, D, bits,
-                                       group_size, 0, dtype, stream);
+      int rc = read_quantized(k, k_groups, v, v_groups, qs, block_table + b0 * table_stride, table_stride, page_size,
+                              num_pages, kv_lens ? kv_lens + b0 : nullptr, source ? source + 2 * b0 : nullptr, block_table,
+                              kd, vd, n, Hkv, L, D, bits, group_size, 0, dtype, stream);
       if (rc) return rc;
       rc = bi_attn_scored(static_cast<const char*>(q) + b0 * strides[0] * es, kd, vd, nullptr, 0, 0, 0,
                           kv_lens ? kv_lens + b0 : nullptr, static_cast<char*>(out) + b0 * Hq * Tq * D * es, n, Hq, Hkv, Tq,
@@ -140,9 +263,8 @@ extern "C" int bi_attn_pages(const void* q, const void* k, const void* k_groups,
       (double)nsplit * Hkv * ((double)B * ((rows1 + 15) / 16) + groups) > 2e9 || n > ((int64_t)1 << 36) ||
       B * Hq * Tq * 64 > ((int64_t)1 << 32) - 256)
     return fail(BI_E_UNSUPPORTED, "%s: grid too large", what);
-  bi::PagesArgs a;
   a.q = q; a.k = k; a.v = v; a.kg = k_groups; a.vg = v_groups;
-  a.kv_lens = kv_lens; a.table = block_table; a.starts = shared_starts; a.slens = shared_lens; a.out = out;
+  a.out = out;
   a.q_sb = strides[0]; a.q_sh = strides[1]; a.q_st = strides[2];
   a.k_sp = strides[3]; a.k_sh = strides[4]; a.k_sl = strides[5];
   a.v_sp = strides[6]; a.v_sh = strides[7]; a.v_sl = strides[8];
@@ -158,11 +280,8 @@ extern "C" int bi_attn_pages(const void* q, const void* k, const void* k_groups,
   a.hkv_inv = bi::inverse(Hkv);
   a.rows1_inv = bi::inverse(rows1);
   a.g_inv = bi::inverse(Hq / Hkv);
-  a.table_stride = table_stride;
-  a.B = (int)B; a.Hq = (int)Hq; a.Hkv = (int)Hkv; a.Tq = (int)Tq; a.L = (int)L; a.nsplit = (int)nsplit;
-  a.causal = causal ? 1 : 0; a.groups = (int)groups;
-  a.shared_len = (int)std::min(std::max<int64_t>(shared_len, 0), L);
-  a.page_shift = shift; a.num_pages = (int)num_pages;
+  a.Hq = (int)Hq; a.Hkv = (int)Hkv; a.Tq = (int)Tq; a.nsplit = (int)nsplit;
+  a.causal = causal ? 1 : 0;
   a.scale_log2 = scale * bi::kLog2e;
   const int64_t up = (n + 3) / 4 * 4;
   a.pm = static_cast<float*>(ws);

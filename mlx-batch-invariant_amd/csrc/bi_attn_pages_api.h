@@ -21,6 +21,14 @@ struct PagesArgs {
   float scale_log2;
 };
 
+__device__ __forceinline__ int pages_len(const PagesArgs& a, int b) {
+  return a.kv_lens ? min(max(a.kv_lens[b], 0), a.L) : a.L;
+}
+
+__device__ __forceinline__ int plan_start(const PagesArgs& a, int n) {
+  return a.starts ? min(max(a.starts[n], 0), a.B) : n ? a.B : 0;
+}
+
 // 2^32 / d, rounded down (2^32 - 1 for 1): quotients by one product and a correction.
 inline unsigned inverse(int64_t d) { return d == 1 ? 0xffffffffu : (unsigned)(((int64_t)1 << 32) / d); }
 
@@ -33,7 +41,8 @@ int launch_pages(const PagesArgs& a, int bits, hipStream_t st);
 
 // Whether a call goes to the kernels of few rows (a workgroup per split, partials merged
 // by a last launch), or to those of bi_attn_scored, which score a sequence's rows 64
-// at a time over all keys and know neither codes nor shared prefixes. Besides single
+// at a time over all keys and know neither codes nor shared prefixes (bi_attn_pages
+// reads codes back and finds the shared pages for them). Besides single
 // tokens and what few_rows splits anyway (32/8 heads of 128, 2648 keys, 2048 of them
 // shared in 4 groups, us here and there):
 //  - codes of up to 64 rows a sequence and kv head, as reading them back costs more:

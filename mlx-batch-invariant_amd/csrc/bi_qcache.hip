@@ -232,11 +232,13 @@ __global__ __launch_bounds__(256) void rope_quant_kernel(RopeQuantArgs a) {
 // its length on as zeros (FILL) or left as they are. Bound by HBM bytes, mostly those
 // written: 16 sequences of up to 8192 tokens, 8 heads of 128 from 8 bits to bf16, in
 // 143 us at the rate of a copy (133). One thread takes 16 codes of a row of K or V.
+// `source` (null: none): of each sequence the one in whose pages its first keys lie
+// (a row of `all`) and how many do.
 // ---------------------------------------------------------------------------
 struct ReadQuantArgs {
   const char *kc, *vc;
   const void *kg, *vg;
-  const int32_t *table, *kv_lens;
+  const int32_t *table, *kv_lens, *source, *all;
   void *ko, *vo;
   int64_t kc_sp, kc_sh, kc_sl, kg_sp, kg_sh, kg_sl, vc_sp, vc_sh, vc_sl, vg_sp, vg_sh, vg_sl, table_stride;
   int Hkv, L, D, shift, gshift, num_pages, fill;
@@ -255,7 +257,9 @@ __global__ __launch_bounds__(256) void read_quant_kernel(ReadQuantArgs a) {
   T* dst = static_cast<T*>(key ? a.ko : a.vo) + (((int64_t)b * a.Hkv + h) * a.L + pos) * a.D + 16 * c;
   typename Frag<T>::type y[2];
   if ((int)pos < len) {
-    const int64_t page = min(max(a.table[(int64_t)b * a.table_stride + (pos >> a.shift)], 0), a.num_pages - 1);
+    const bool shared = a.source && (int)pos < a.source[2 * b + 1];
+    const int32_t* of = shared ? a.all + a.source[2 * b] * a.table_stride : a.table + b * a.table_stride;
+    const int64_t page = min(max(of[pos >> a.shift], 0), a.num_pages - 1);
     const int64_t row = pos & ((1u << a.shift) - 1);
     const char* codes = key ? a.kc + page * a.kc_sp + h * a.kc_sh + row * a.kc_sl : a.vc + page * a.vc_sp + h * a.vc_sh + row * a.vc_sl;
     const T* pairs = key ? static_cast<const T*>(a.kg) + page * a.kg_sp + h * a.kg_sh + row * a.kg_sl
@@ -400,13 +404,14 @@ extern "C" int bi_rope_quantized_cache(const void* q, int64_t q_row, const void*
   return launch_status(what);
 }
 
-extern "C" int bi_read_quantized_cache(const void* k_codes, const void* k_groups, const void* v_codes,
-                                       const void* v_groups, const int64_t* strides, const int32_t* block_table,
-                                       int64_t table_stride, int64_t page_size, int64_t num_pages,
-                                       const int32_t* kv_lens, void* k_out, void* v_out, int64_t B, int64_t Hkv,
-                                       int64_t L, int64_t D, int bits, int64_t group_size, int fill, int dtype,
-                                       void* stream) {
-  using namespace bi_host;
+namespace bi_host {
+
+// bi_read_quantized_cache with ReadQuantArgs' source.
+int read_quantized(const void* k_codes, const void* k_groups, const void* v_codes, const void* v_groups,
+                   const int64_t* strides, const int32_t* block_table, int64_t table_stride, int64_t page_size,
+                   int64_t num_pages, const int32_t* kv_lens, const int32_t* source, const int32_t* all, void* k_out,
+                   void* v_out, int64_t B, int64_t Hkv, int64_t L, int64_t D, int bits, int64_t group_size, int fill,
+                   int dtype, void* stream) {
   const char* what = "bi_read_quantized_cache";
   const int shift = shift_of(page_size);
   if (shift < 0)
@@ -429,7 +434,7 @@ extern "C" int bi_read_quantized_cache(const void* k_codes, const void* k_groups
     return fail(BI_E_UNSUPPORTED, "%s: shape too large", what);
   bi::ReadQuantArgs a;
   a.kc = static_cast<const char*>(k_codes); a.vc = static_cast<const char*>(v_codes); a.kg = k_groups; a.vg = v_groups;
-  a.table = block_table; a.kv_lens = kv_lens; a.ko = k_out; a.vo = v_out; a.table_stride = table_stride;
+  a.table = block_table; a.kv_lens = kv_lens; a.source = source; a.all = all; a.ko = k_out; a.vo = v_out; a.table_stride = table_stride;
   a.kc_sp = strides[0]; a.kc_sh = strides[1]; a.kc_sl = strides[2];
   a.kg_sp = strides[3]; a.kg_sh = strides[4]; a.kg_sl = strides[5];
   a.vc_sp = strides[6]; a.vc_sh = strides[7]; a.vc_sl = strides[8];
@@ -447,4 +452,17 @@ extern "C" int bi_read_quantized_cache(const void* k_codes, const void* k_groups
   else if (dtype == BI_F16) launch(bi::f16());
   else launch(float());
   return launch_status(what);
+}
+
+}  // namespace bi_host
+
+extern "C" int bi_read_quantized_cache(const void* k_codes, const void* k_groups, const void* v_codes,
+                                       const void* v_groups, const int64_t* strides, const int32_t* block_table,
+                                       int64_t table_stride, int64_t page_size, int64_t num_pages,
+                                       const int32_t* kv_lens, void* k_out, void* v_out, int64_t B, int64_t Hkv,
+                                       int64_t L, int64_t D, int bits, int64_t group_size, int fill, int dtype,
+                                       void* stream) {
+  return bi_host::read_quantized(k_codes, k_groups, v_codes, v_groups, strides, block_table, table_stride, page_size,
+                                 num_pages, kv_lens, nullptr, nullptr, k_out, v_out, B, Hkv, L, D, bits, group_size, fill,
+                                 dtype, stream);
 }

@@ -105,6 +105,8 @@ _SIGNATURES = {
                                                ctypes.c_int, ctypes.c_int, _vp]),
     "bi_attn_pages_workspace_bytes": (ctypes.c_size_t, [_c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64,
                                                         ctypes.c_int, ctypes.c_int, ctypes.c_int]),
+    "bi_attn_pages_workspace_bytes_paged": (ctypes.c_size_t, [_c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64,
+                                                              ctypes.c_int, ctypes.c_int, ctypes.c_int, _c_i64]),
     "bi_attn_pages": (ctypes.c_int, [_vp, _vp, _vp, _vp, _vp, ctypes.c_int, _c_i64, _vp, _c_i64, _c_i64, _c_i64, _vp,
                                      _vp, _vp, _c_i64, _c_i64, _vp, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64, _c_i64,
                                      ctypes.POINTER(_c_i64), ctypes.c_int, ctypes.c_float, ctypes.c_int, _vp,

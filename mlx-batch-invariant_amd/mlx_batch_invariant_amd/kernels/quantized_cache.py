@@ -279,7 +279,7 @@ def _attend(what, q, k, v, kg, vg, bits, gs, num_pages, Hkv, page_size, kv_strid
     if not _aligned(q) or max(q.stride()) >> 32:
         q = q.clone(memory_format=torch.contiguous_format)
     dt = _lib.DTYPE_CODE[q.dtype]
-    n = _lib.ws_bytes("bi_attn_pages_workspace_bytes", B, Hq, Hkv, Tq, L, D, groups, bits, int(causal), dt)
+    n = _lib.ws_bytes("bi_attn_pages_workspace_bytes_paged", B, Hq, Hkv, Tq, L, D, groups, bits, int(causal), dt, page_size)
     ws = _lib.workspace(n, dev)
     rc = _lib.launch(index, _lib.pages_call, q.data_ptr(), k.data_ptr(), _lib.ptr(kg), v.data_ptr(), _lib.ptr(vg), bits, gs,
                      table.data_ptr(), table.shape[1], page_size, num_pages, _lib.ptr(kl), _lib.ptr(starts),

@@ -239,3 +239,93 @@ def test_graph_with_changing_groups():
             assert torch.equal(x, y)
         want = bi.batch_invariant_paged_attention(q, kp, vp, *held[:2])
         assert torch.equal(out[0], want) and torch.equal(out[1], out[2])
+
+
+# ---- whose pages are read --------------------------------------------------------------
+
+def _rows_of(nbits, kp, vp, table):
+    """K and V of every sequence through its own table row, [B, Hkv, L, D]."""
+    if nbits:
+        return _bi().read_quantized_cache(kp, vp, table)
+    return [p[table.long()].transpose(1, 2).flatten(2, 3).contiguous() for p in (kp, vp)]
+
+
+def _check_sources(dt, nbits, Hq, Hkv, D, T, page, sizes, shared, lens, mask, seed, lead=0, tail=0, layout="page"):
+    """Sequences with pages all of their own: the shared splits' keys are those of the group's first
+    sequence, the others' table entries of whole pages there are not read."""
+    bi, g = _bi(), gen(seed)
+    B = lead + sum(sizes) + tail
+    L = max(max(lens), 1)
+    cols = -(-L // page)
+    lens = torch.tensor([lens[b % len(lens)] for b in range(B)], dtype=I32)
+    n = B * cols
+    table = torch.randperm(n, generator=g).reshape(B, cols).to(I32).cuda()
+    kp, vp = _pools(n, Hkv, page, D, dt, g, nbits)
+    if layout == "row":                                  # heads inside rows in memory
+        kp, vp = (p.transpose(1, 2).contiguous().transpose(1, 2) for p in (kp, vp))
+    q = randn((B, Hq, T, D), DT[dt], g, 2.0)
+    k, v = _rows_of(nbits, kp, vp, table)
+    starts = [lead]
+    given = table.clone()
+    for s, keys in zip(sizes, shared):
+        lo = starts[-1]
+        starts.append(lo + s)
+        keys = min(keys, int(lens[lo])) // 256 * 256 if s > 1 else 0
+        for b in range(lo + 1, lo + s):
+            k[b, :, :keys], v[b, :, :keys] = k[lo, :, :keys], v[lo, :, :keys]
+            given[b, :keys // page] = -1 if b % 2 else 1 << 30
+    want = bi.batch_invariant_attention(q, k, v, kv_lens=lens.cuda(), mask=mask)
+    call = bi.batch_invariant_quantized_paged_attention if nbits else bi.batch_invariant_shared_prefix_attention
+    got = call(q, kp, vp, given, lens.cuda(), mask=mask, shared_starts=dev(starts), shared_lens=dev(shared))
+    assert torch.equal(got, want), (got.float() - want.float()).abs().amax((1, 2, 3))
+    return q, kp, vp, given, lens.cuda(), dev(starts), dev(shared), want
+
+
+@pytest.mark.parametrize("nbits,dt", [(0, "bf16"), (8, "bf16"), (4, "f16"), (0, "f32"), (8, "f32")])
+@pytest.mark.parametrize("page", [1, 16, 256, 512, 1024])
+@pytest.mark.parametrize("T", [1, 4, 8, 100])
+def test_pages_of_the_first_sequence(nbits, dt, page, T):
+    """Any number of query tokens, pages that hold several splits, groups of one, none and many."""
+    lens = [1030, 700, 40, 1100, 0, 900, 256, 511]
+    _check_sources(dt, nbits, 8, 2, 64, T, page, [3, 1, 4], [600, 512, 1024], lens, "causal", 100 + T + page, lead=1, tail=1)
+    _check_sources(dt, nbits, 3, 3, 64, T, page, [9], [768], lens, None, 200 + T + page)
+
+
+@pytest.mark.parametrize("T", [4, 8, 16, 17])
+@pytest.mark.parametrize("nbits", [0, 8])
+def test_pages_of_the_first_sequence_whichever_kernel(T, nbits):
+    """Token counts to either side of the rules on rows, many sequences."""
+    _check_sources("bf16", nbits, 16, 4, 64, T, 16, [8, 8, 8, 8], [512, 600, 256, 300], [620, 700, 560, 800], "causal", T + nbits)
+
+
+@pytest.mark.parametrize("layout", ["page", "row"])
+@pytest.mark.parametrize("page", [512, 2048])
+def test_splits_inside_pages(layout, page):
+    """Many rows, a prefix that ends inside a page; heads inside rows in memory as well."""
+    _check_sources("bf16", 0, 16, 2, 128, 200, page, [4], [1300], [1500, 2000, 1600, 1400], "causal", page, layout=layout)
+
+
+@pytest.mark.parametrize("nbits", [0, 8])
+def test_captured_many_rows(nbits):
+    """A captured call of many rows with changing groups and tables: every replay has the eager bits."""
+    bi = _bi()
+    cases = [_check_sources("bf16", nbits, 8, 2, 64, 200, 16, sizes, shared, lens, "causal", 7) for sizes, shared, lens in (
+        ([3, 3], [512, 700], [900, 800, 300]), ([6, 0], [256, 9], [900, 333]), ([1, 5], [900, 768], [900, 850, 870]))]
+    q, kp, vp = cases[0][:3]
+    call = bi.batch_invariant_quantized_paged_attention if nbits else bi.batch_invariant_shared_prefix_attention
+    held = [t.clone() for t in cases[0][3:7]]
+    step = lambda: call(q, kp, vp, held[0], held[1], mask="causal", shared_starts=held[2], shared_lens=held[3])
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        step()
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = step()
+    for case in cases + cases[:2]:
+        for h, c in zip(held, case[3:7]):
+            h.copy_(c)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, step()) and torch.equal(out, case[7])

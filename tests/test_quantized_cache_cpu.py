@@ -201,3 +201,39 @@ def test_fake_shapes():
                                              None).shape == out.shape
         pool = torch.empty(9, 2, 16, 64, dtype=dt)
         assert ops.shared_prefix_attention(out, pool, pool, i(2, 5), i(2), 0.125, True, None, i(1)).shape == out.shape
+
+
+def test_shared_pages_of_several_splits():
+    """Many rows behind shared prefixes over plain pages of more than a split: one ratio of strides
+    for K and V, page numbers that stay below 2^31."""
+    lib = _lib.load()
+    q = (1 << 20, 1 << 12, 64)
+
+    def call(k, v, pages=9, page=512, n=BIG):
+        return _pages_call(B=32, Hq=8, Hkv=2, Tq=200, L=4096, bits=0, groups=1, shared=512, page=page, pages=pages,
+                           strides=(*q, *k, *v, *(0,) * 6), n=n)
+
+    heads_out, rows_out = (2 * 512 * 64, 512 * 64, 64), (512 * 128, 64, 128)      # heads around rows, rows around heads
+    assert call(heads_out, rows_out) == -2 and b"layout" in lib.bi_last_error()
+    assert call((1 << 20, 64, 64), (1 << 20, 64, 64), pages=(1 << 31) - 1) == -2
+    assert call((1 << 20, 64, 1 << 51), heads_out) == -2
+    # (what is enough otherwise is a workspace, asked for last)
+    for k, v in ((heads_out, heads_out), (rows_out, rows_out), ((2 * 512 * 64 + 8, 512 * 64, 64), (2 * 512 * 64 + 8, 512 * 64, 64)),
+                 ((1 << 19, 1 << 18, 8), (1 << 21, 64, 32))):
+        assert call(k, v, n=0) == -3, lib.bi_last_error()
+    assert call(heads_out, rows_out, pages=1, n=0) == -3          # one page: its stride does not matter
+    assert call(heads_out, rows_out, page=256, n=0) == -3         # pages of one split
+
+
+def test_workspaces_of_shared_prefixes():
+    lib = _lib.load()
+    f, g = lib.bi_attn_pages_workspace_bytes, lib.bi_attn_pages_workspace_bytes_paged
+    shape = (32, 8, 2, 200, 4096, 64)
+    none = f(*shape, 0, 0, 1, 2)
+    # a table of every sequence's pages (of at most 256 keys), or two words a sequence
+    for page, cols in ((1, 4096), (16, 256), (256, 16), (512, 16), (1 << 20, 16)):
+        assert g(*shape, 0, 0, 1, 2, page) == none
+        assert g(*shape, 3, 0, 1, 2, page) == none + 4 * 32 * cols
+        assert g(*shape, 3, 8, 1, 2, page) == f(*shape, 0, 8, 1, 2) + 8 * 32
+    assert f(*shape, 3, 0, 1, 2) == g(*shape, 3, 0, 1, 2, 1) and g(*shape, 3, 0, 1, 2, 0) == 0
+    assert g(32, 8, 2, 1, 4096, 64, 3, 0, 1, 2, 16) == f(32, 8, 2, 1, 4096, 64, 3, 0, 1, 2)
