@@ -124,7 +124,7 @@ __device__ __forceinline__ void plan_segments(const PagesArgs& a, int32_t* seg, 
       s[1] = lo;
       s[2] = max(hi - lo, 0);
       s[3] = 0;
-      s[4] = hi - lo > 1 && a.nsplit > 1 ? min(want, (int)seg[(int64_t)(a.groups + lo) * kPlanWords]) / kSplit : 0;
+      s[4] = hi - lo > 1 ? min(want, (int)seg[(int64_t)(a.groups + lo) * kPlanWords]) / kSplit : 0;
     }
     __syncthreads();
   }

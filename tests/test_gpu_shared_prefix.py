@@ -305,6 +305,14 @@ def test_splits_inside_pages(layout, page):
     _check_sources("bf16", 0, 16, 2, 128, 200, page, [4], [1300], [1500, 2000, 1600, 1400], "causal", page, layout=layout)
 
 
+@pytest.mark.parametrize("nbits,dt", [(0, "bf16"), (8, "f16"), (4, "bf16"), (0, "f32")])
+@pytest.mark.parametrize("T", [1, 3, 8, 80])
+def test_one_split_is_shared(nbits, dt, T):
+    """A table of one split: the first sequence's pages too."""
+    _check_sources(dt, nbits, 8, 2, 64, T, 16, [3, 4], [256, 300], [256, 100, 0, 256, 256, 255, 3], "causal", T)
+    _check_sources(dt, nbits, 5, 1, 32, T, 64, [6], [256], [256, 100, 0, 256, 1], None, T + 1, tail=1)
+
+
 @pytest.mark.parametrize("nbits", [0, 8])
 def test_captured_many_rows(nbits):
     """A captured call of many rows with changing groups and tables: every replay has the eager bits."""
