@@ -120,13 +120,27 @@ bool bad_shape(int64_t B, int64_t Hq, int64_t Hkv, int64_t Tq, int64_t L, int64_
          Tq > 0x7fffffffLL || L <= 0 || L > 0x7fffffffLL - bi::kSplit || D <= 0 || D > 65536 || groups < 0 || groups > 65535;
 }
 
+bool known(int64_t D, int dtype) {
+  return (D == 32 || D == 64 || D == 96 || D == 128 || D == 192 || D == 256) &&
+         (dtype == BI_BF16 || dtype == BI_F16 || dtype == BI_F32);
+}
+
+// Whether the kernels of few rows can count a call's items, rows and the merge's threads in
+// 32 bits. (Products in an order in which none leaves 64 bits.)
+bool few_fits(int64_t B, int64_t Hq, int64_t Hkv, int64_t Tq, int64_t L, int64_t groups) {
+  const int64_t nsplit = (L + bi::kSplit - 1) / bi::kSplit, rows1 = Tq * (Hq / Hkv);
+  return B * Hq * Tq <= 0x7fffffffLL && rows1 <= 0x7fffffffLL - 16 && B * rows1 <= 0x7fffffffLL - 1024 &&
+         (double)nsplit * Hkv * ((double)B * ((rows1 + 15) / 16) + groups) <= 2e9 &&
+         B * Hq * Tq * nsplit <= ((int64_t)1 << 36) && B * Hq * Tq * 64 <= ((int64_t)1 << 32) - 256;
+}
+
 }  // namespace
 
 extern "C" size_t bi_attn_pages_workspace_bytes_paged(int64_t B, int64_t Hq, int64_t Hkv, int64_t Tq, int64_t L, int64_t D,
                                                       int64_t groups, int bits, int causal, int dtype, int64_t page_size) {
-  if (bad_shape(B, Hq, Hkv, Tq, L, D, groups) || page_size <= 0) return 0;
+  if (bad_shape(B, Hq, Hkv, Tq, L, D, groups) || !known(D, dtype) || page_size <= 0) return 0;
   if (bi::pages_few_rows(B, Hq, Hkv, Tq, L, D, groups, bits, causal, dtype))
-    return partial_bytes(B, Hq, Tq, L, D) + (size_t)(2 + bi::kPlanWords * (groups + B)) * sizeof(int32_t);
+    return !few_fits(B, Hq, Hkv, Tq, L, groups) ? 0 : partial_bytes(B, Hq, Tq, L, D) + (size_t)(2 + bi::kPlanWords * (groups + B)) * sizeof(int32_t);
   const int64_t nb = bits ? dense_slice(B, Hkv, L, D, dtype) : B;
   size_t n = bi_attn_scored_workspace_bytes(nb, Hq, Hkv, Tq, L, D, causal, 0, dtype);
   if (bits) n = std::max(n, bi_attn_scored_workspace_bytes((B - 1) % nb + 1, Hq, Hkv, Tq, L, D, causal, 0, dtype));
@@ -154,9 +168,9 @@ extern "C" int bi_attn_pages(const void* q, const void* k, const void* k_groups,
   if (B < 0 || Hq <= 0 || Hkv <= 0 || Tq <= 0 || L <= 0 || groups < 0)
     return fail(BI_E_INVALID_ARG, "%s: bad shape B=%lld Hq=%lld Hkv=%lld Tq=%lld L=%lld groups=%lld", what, (long long)B,
                 (long long)Hq, (long long)Hkv, (long long)Tq, (long long)L, (long long)groups);
-  if (D != 32 && D != 64 && D != 96 && D != 128 && D != 192 && D != 256)
+  if (!known(D, BI_F32))
     return fail(BI_E_UNSUPPORTED, "%s: head dim %lld (supported: 32, 64, 96, 128, 192, 256)", what, (long long)D);
-  if (dtype != BI_BF16 && dtype != BI_F16 && dtype != BI_F32)
+  if (!known(D, dtype))
     return fail(BI_E_UNSUPPORTED, "%s: unknown dtype %d", what, dtype);
   if (bad_shape(B, Hq, Hkv, Tq, L, D, groups)) return fail(BI_E_UNSUPPORTED, "%s: shape exceeds the grid limits", what);
   if (causal && Tq > L)
@@ -205,6 +219,7 @@ extern "C" int bi_attn_pages(const void* q, const void* k, const void* k_groups,
                 "%s: shared prefixes of many rows over pages of %lld keys need K and V of one layout (page strides %lld, "
                 "%lld, row strides %lld, %lld)", what, (long long)page_size, (long long)strides[3], (long long)strides[6],
                 (long long)strides[5], (long long)strides[8]);
+  if (few && !few_fits(B, Hq, Hkv, Tq, L, groups)) return fail(BI_E_UNSUPPORTED, "%s: grid too large", what);
   const size_t need = bi_attn_pages_workspace_bytes_paged(B, Hq, Hkv, Tq, L, D, groups, bits, causal, dtype, page_size);
   if (need > 0 && (!ws || ws_bytes < need || !aligned16(ws)))
     return fail(BI_E_WORKSPACE, "%s: 16-byte aligned workspace of %zu bytes required, got %zu", what, need,
@@ -258,11 +273,6 @@ extern "C" int bi_attn_pages(const void* q, const void* k, const void* k_groups,
   }
 
   const int64_t nsplit = (L + bi::kSplit - 1) / bi::kSplit, rows1 = Tq * (Hq / Hkv), n = B * Hq * Tq * nsplit;
-  // (items, rows and the merge's threads in 32 bits)
-  if (B * Hq * Tq > 0x7fffffffLL || rows1 > 0x7fffffffLL - 16 || B * rows1 > 0x7fffffffLL - 1024 ||
-      (double)nsplit * Hkv * ((double)B * ((rows1 + 15) / 16) + groups) > 2e9 || n > ((int64_t)1 << 36) ||
-      B * Hq * Tq * 64 > ((int64_t)1 << 32) - 256)
-    return fail(BI_E_UNSUPPORTED, "%s: grid too large", what);
   a.q = q; a.k = k; a.v = v; a.kg = k_groups; a.vg = v_groups;
   a.out = out;
   a.q_sb = strides[0]; a.q_sh = strides[1]; a.q_st = strides[2];

@@ -237,3 +237,19 @@ def test_workspaces_of_shared_prefixes():
         assert g(*shape, 3, 8, 1, 2, page) == f(*shape, 0, 8, 1, 2) + 8 * 32
     assert f(*shape, 3, 0, 1, 2) == g(*shape, 3, 0, 1, 2, 1) and g(*shape, 3, 0, 1, 2, 0) == 0
     assert g(32, 8, 2, 1, 4096, 64, 3, 0, 1, 2, 16) == f(32, 8, 2, 1, 4096, 64, 3, 0, 1, 2)
+
+
+def test_workspaces_of_refused_shapes():
+    """Shapes that the call refuses need nothing; none of their products wraps."""
+    lib = _lib.load()
+    for f, more in ((lib.bi_attn_pages_workspace_bytes, ()), (lib.bi_attn_pages_workspace_bytes_paged, (16,))):
+        for bits in (0, 8):
+            for dtype in (0, 1, 2):                       # 2^63 and 2^64 bytes read back
+                assert f(1, 32768, 32768, 4096, 1 << 30, 65536, 0, bits, 1, dtype, *more) == 0
+            for D in (16, 48, 160, 512, 65536):
+                assert f(1, 4, 2, 200, 512, D, 1, bits, 1, 2, *more) == 0
+            assert f(1, 4, 2, 200, 512, 64, 1, bits, 1, 7, *more) == 0                        # no such type
+            assert f(65535, 1 << 26, 1 << 10, 1, (1 << 31) - 257, 256, 0, bits, 1, 2, *more) == 0   # 2^65 partials
+            assert f(60000, 60000, 60000, 1, 1 << 20, 64, 0, bits, 1, 2, *more) == 0
+    assert _pages_call(B=65535, Hq=1 << 26, Hkv=1 << 10, L=(1 << 31) - 4096, D=256, stride=1 << 28) == -2
+    assert b"grid too large" in lib.bi_last_error()
