@@ -392,10 +392,11 @@ __global__ __launch_bounds__(256, (pages_min_blocks<T, D>())) void attn_pages(Pa
       t = quotient(p, G, a.g_inv);
       h = hk * G + p - t * G;
     };
-    if (n_act == 0) {                                     // (direct, an empty sequence) no keys: zeros
-      for (int i = tid; i < nrows * D; i += 256) {
+    if (n_act == 0) {                                     // (direct, an empty sequence) no keys: zeros in this item's rows
+      const int rows0 = 16 * chunk0, n = min(16 * chunks, nrows - rows0) * D;   // (at most kPlanMostChunks chunks)
+      for (int i = tid; i < n; i += 256) {
         int b, h, t;
-        row_of(i / D, b, h, t);
+        row_of(rows0 + i / D, b, h, t);
         static_cast<T*>(a.out)[(((int64_t)b * a.Hq + h) * a.Tq + t) * D + i % D] = (T)0.0f;
       }
       it = locate(dealt(round, items));

@@ -337,3 +337,25 @@ def test_captured_many_rows(nbits):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, step()) and torch.equal(out, case[7])
+
+
+def test_empty_sequences_of_many_heads():
+    """A sequence without keys, and more values in its rows than 31 bits count: zeros."""
+    bi, g = _bi(), gen(12)
+    kp, vp = _pools(4, 1, 16, 256, "bf16", g, 0)
+    table = torch.zeros(1, 3, dtype=I32, device="cuda")
+    for heads in (40, 5000, 1 << 23):
+        q = torch.ones(1, heads, 1, 256, dtype=torch.bfloat16, device="cuda")
+        torch.full_like(q, float("nan"))                  # (what the result's memory held before)
+        out = bi.batch_invariant_shared_prefix_attention(q, kp, vp, table, dev([0]), shared_lens=300)
+        assert not out.any()
+        del q, out
+
+
+def test_empty_and_short_sequences_of_many_heads():
+    g = gen(13)
+    table, lens, _, _, n = _case([7], [0], [0, 3, 40, 0, 31], 16, g)
+    kp, vp = _pools(n, 1, 16, 64, "f16", g, 0)
+    q = randn((7, 700, 1, 64), torch.float16, g)
+    got, want = _calls(0, q, kp, vp, table.cuda(), lens.cuda(), None, shared_lens=256)
+    assert torch.equal(got, want) and not want[0].any() and want[1].any()
