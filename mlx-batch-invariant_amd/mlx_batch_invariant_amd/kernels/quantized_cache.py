@@ -62,7 +62,8 @@ def quantized_pages(num_pages: int, kv_heads: int, page_size: int, head_dim: int
 
 
 def _format(what: str, bits, group_size, head_dim: int) -> None:
-    if bits not in SUPPORTED_BITS or group_size not in SUPPORTED_GROUPS:
+    whole = hasattr(bits, "__index__") and hasattr(group_size, "__index__")
+    if not whole or bits not in SUPPORTED_BITS or group_size not in SUPPORTED_GROUPS:
         raise ValueError(f"{what}: bits={bits} group_size={group_size} (4 or 8 bits, groups of 32, 64 or 128)")
     if head_dim <= 0 or head_dim % group_size:
         raise ValueError(f"{what}: head dim {head_dim} is no whole number of groups of {group_size}")
@@ -74,16 +75,20 @@ _layouts: dict = {}
 def _pools(what: str, k_pages: QuantizedPages, v_pages: QuantizedPages, dtype=None):
     """Checks a pair of pools; (num_pages, Hkv, page_size, D, the 12 strides). Shapes, strides and types
     that passed once are remembered (a lookup is cheaper than the checks on every step)."""
+    key = None
     if type(k_pages) is QuantizedPages is type(v_pages):
         kc, kg, bits, gs = k_pages
         vc, vg, v_bits, v_gs = v_pages
-        key = (kc.shape, kc.stride(), kg.shape, kg.stride(), vc.shape, vc.stride(), vg.shape, vg.stride(), kc.dtype, kg.dtype,
-               vc.dtype, vg.dtype, bits, gs, v_bits, v_gs, dtype)
-        seen = _layouts.get(key)
+        try:
+            key = (kc.shape, kc.stride(), kg.shape, kg.stride(), vc.shape, vc.stride(), vg.shape, vg.stride(), kc.dtype, kg.dtype,
+                   vc.dtype, vg.dtype, bits, gs, v_bits, v_gs, dtype)
+            if not type(bits) is type(gs) is type(v_bits) is type(v_gs) is int:
+                key = None                                # (8.0 would find what 8 left)
+            seen = _layouts.get(key)
+        except AttributeError:                            # a field that is no tensor: _check_pools names it
+            seen = None
         if seen is not None and not (kc.data_ptr() | kg.data_ptr() | vc.data_ptr() | vg.data_ptr()) & 15:
             return seen
-    else:
-        key = None
     seen = _check_pools(what, k_pages, v_pages, dtype)
     if key is not None:
         if len(_layouts) > 1024:
@@ -96,6 +101,9 @@ def _check_pools(what: str, k_pages: QuantizedPages, v_pages: QuantizedPages, dt
     for p in (k_pages, v_pages):
         if not isinstance(p, QuantizedPages):
             raise ValueError(f"{what}: pools must be QuantizedPages; got {type(p).__name__}")
+        if not isinstance(p.codes, torch.Tensor) or not isinstance(p.groups, torch.Tensor):
+            raise ValueError(f"{what}: a pool's codes and groups must be tensors; got {type(p.codes).__name__} and "
+                             f"{type(p.groups).__name__}")
     codes, groups, bits, gs = k_pages
     if (bits, gs) != v_pages[2:] or codes.shape != v_pages.codes.shape or groups.shape != v_pages.groups.shape:
         raise ValueError(f"{what}: pools of {bits} bits, groups of {gs}, {tuple(codes.shape)} and of "
@@ -103,6 +111,7 @@ def _check_pools(what: str, k_pages: QuantizedPages, v_pages: QuantizedPages, dt
     cs = codes.shape
     D = cs[3] * 8 // bits if len(cs) == 4 and bits in SUPPORTED_BITS else 0
     _format(what, bits, gs, D)
+    _format(what, *v_pages[2:], D)
     if groups.shape != (*cs[:3], D // gs, 2):
         raise ValueError(f"{what}: groups {tuple(groups.shape)} for codes {tuple(cs)} of {bits} bits, groups of {gs}")
     _page_size(what, cs[2])

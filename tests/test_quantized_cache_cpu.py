@@ -253,3 +253,23 @@ def test_workspaces_of_refused_shapes():
             assert f(60000, 60000, 60000, 1, 1 << 20, 64, 0, bits, 1, 2, *more) == 0
     assert _pages_call(B=65535, Hq=1 << 26, Hkv=1 << 10, L=(1 << 31) - 4096, D=256, stride=1 << 28) == -2
     assert b"grid too large" in lib.bi_last_error()
+
+
+@pytest.mark.parametrize("change,match", [
+    (dict(codes=None), "tensors"), (dict(codes=[[0]]), "tensors"), (dict(groups=1.0), "tensors"), (dict(bits="8"), "bits"),
+    (dict(bits=[8]), "bits"), (dict(bits=8.0), "bits"), (dict(group_size=64.0), "bits"), (dict(group_size=None), "bits")])
+def test_pools_of_other_things(change, match):
+    """Fields of the wrong kind are named, also after pools of the same layout have passed."""
+    t, q = torch.zeros(2, 3, dtype=I32), torch.zeros(2, 4, 1, 64)
+    good = [_pool() for _ in range(2)]
+    for calls in range(2):
+        bad = [p._replace(**change) for p in good]
+        for kp, vp in (bad, (bad[0], good[1]), (good[0], bad[1])):
+            with pytest.raises(ValueError, match=match + "|pools"):
+                bi.rope_quantized_cache(**_write(k_pages=kp, v_pages=vp))
+            with pytest.raises(ValueError, match=match + "|pools"):
+                bi.read_quantized_cache(kp, vp, t)
+            with pytest.raises(ValueError, match=match + "|pools"):
+                bi.batch_invariant_quantized_paged_attention(q, kp, vp, t)
+        with pytest.raises(ValueError, match="GPU"):      # (the layout is remembered now)
+            bi.read_quantized_cache(*good, t)
