@@ -736,7 +736,7 @@ __global__ __launch_bounds__(256, (codes_min_blocks<T, D, BITS>())) void attn_co
   constexpr int NG = D / GS;                              // groups of a row
   // Pairs that a wave's dim tiles need: one where they share a group (two tiles from
   // an even one on, four of 64 dims), else one for each or for two of them.
-  constexpr int NS = NJ == 3 ? 3 : NJ == 4 && GS == 32 ? 4 : 1;
+  constexpr int NS = NJ == 3 ? 3 : NJ == 4 && GS == 32 ? 2 : 1;
   __shared__ __attribute__((aligned(1024))) char Vs[kSplit * CT::kRowBytes];
   __shared__ __attribute__((aligned(16))) float vsc[NG][kSplit], vbi[NG][kSplit];   // V's scales (times the codes' factors) and biases
   // (a wave's scales may be too large for that: fp16's are finite times 2^24)
