@@ -335,3 +335,83 @@ def test_noncontiguous_queries_and_lists():
     odd.copy_(q.transpose(1, 2))
     assert torch.equal(bi.batch_invariant_quantized_paged_attention(odd, *args[:2], table.long().cuda(), args[3], mask="causal"), want)
     assert bi.batch_invariant_quantized_paged_attention(odd[:0], kp, vp, table[:0].cuda(), []).shape == (0, 4, 3, 64)
+
+
+def _seen_values(clean, v, lens, T, mask, G):
+    """What comes out where rows see infinities and NaN of v [B, Hkv, L, D]: those, else `clean`."""
+    B, _, L, _ = v.shape
+    reach = lens[:, None] if mask is None else lens[:, None] - T + 1 + torch.arange(T, device=lens.device)
+    seen = (torch.arange(L, device=lens.device) < reach[:, :, None]).expand(B, T, L).float()[:, None]      # [B, 1, T, L]
+    v = v.repeat_interleave(G, 1)
+    up, down, nan = (torch.matmul(seen, x.float()) > 0 for x in (v == float("inf"), v == -float("inf"), v.isnan()))
+    want = clean.clone()
+    want[up & ~down] = float("inf")
+    want[down & ~up] = -float("inf")
+    want[nan | up & down] = float("nan")
+    return want
+
+
+def _same(got, want):
+    return torch.equal(got.isnan(), want.isnan()) and torch.equal(got[~got.isnan()], want[~want.isnan()])
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f16", "f32"])
+@pytest.mark.parametrize("nbits,gs,D", [(8, 64, 64), (8, 32, 96), (4, 32, 64), (4, 64, 128), (4, 32, 256)])
+@pytest.mark.parametrize("L", [256, 512])
+@pytest.mark.parametrize("T,mask,shared", [(1, None, False), (4, "causal", False), (3, "causal", True), (150, "causal", False),
+                                           (150, "causal", True)])
+def test_not_finite_codes(dt, nbits, gs, D, L, T, mask, shared):
+    """Infinite and NaN scales and biases, seen and hidden, of one split and several, few rows and
+    many, behind a shared split too; a scale of 2^101 beside them where the type has it."""
+    bi, g = _bi(), gen(D + T + L + nbits)
+    B, Hq, Hkv, page, inf, nan = 3, 8, 2, 16, float("inf"), float("nan")
+    table, n = _requests(g, B, L, page)
+    if shared:
+        table[1:, :256 // page] = table[0, :256 // page]
+    kp, vp = (random_pool(n, Hkv, page, D, nbits, gs, dt, g) for _ in range(2))
+    q = randn((B, Hq, T, D), DT[dt], g)
+    lens = [256, 160, 230] if L == 256 else [512, 301, 330]
+    at = lambda b, p: (int(table[b, p // page]), p % page)
+    if dt != "f16":
+        page0, row0 = at(0, 7)
+        vp.groups[page0, 0, row0, 0, 0] = 2.0 ** 101
+    lens = torch.tensor(lens, dtype=I32, device="cuda")
+    args = (table.cuda(), lens)
+    more = dict(mask=mask, **(dict(shared_lens=256) if shared else {}))
+    clean = bi.batch_invariant_quantized_paged_attention(q, kp, vp, *args, **more)
+    assert torch.isfinite(clean).all()
+    last = D // gs - 1
+    for b, p, h, group, pair in ((0, int(lens[0]) - 1, 0, 0, (0.01, inf)),       # seen by the last row alone
+                                 (0, 5, 1, last, (0.02, -inf)), (0, 70, 1, 0, (inf, 1.0)), (1, 130, 0, last, (-inf, 0.5)),
+                                 (1, int(lens[1]) - 2, 1, last, (nan, nan)), (2, 3, 1, last, (0.01, inf)),
+                                 (1, int(lens[1]) + 1, 0, 0, (0.01, -inf)), (2, int(lens[2]), 1, 0, (inf, -inf)),   # behind sequences
+                                 (2, int(lens[2]) + 9, 0, last, (nan, 1.0))):
+        pg, row = at(b, p)
+        vp.groups[pg, h, row, group] = torch.tensor(pair)
+        kp_row = kp.groups[pg, h, row]
+        if p >= int(lens[b]) and not shared:
+            kp_row.fill_(nan)                             # K behind a sequence may hold anything too
+    v = bi.read_quantized_cache(kp, vp, args[0])[1]
+    want = _seen_values(clean, v, lens, T, mask, Hq // Hkv)
+    got = bi.batch_invariant_quantized_paged_attention(q, kp, vp, *args, **more)
+    assert not torch.isfinite(want).all() and _same(got, want)
+
+
+@pytest.mark.parametrize("dt", ["bf16", "f32"])
+@pytest.mark.parametrize("T", [1, 6, 200])
+def test_not_finite_in_one_shared_split(dt, T):
+    """Plain pages, a table of one split: the first sequence's hidden and seen values."""
+    bi, g = _bi(), gen(T)
+    B, D, page, inf = 4, 64, 16, float("inf")
+    table, n = _requests(g, 1, 256, page)
+    table = table.expand(B, -1).contiguous()
+    kp, vp = (randn((n, 2, page, D), DT[dt], g) for _ in range(2))
+    q = randn((B, 8, T, D), DT[dt], g)
+    lens = torch.tensor([256, 90, 0, 255], dtype=I32, device="cuda")
+    call = lambda: bi.batch_invariant_shared_prefix_attention(q, kp, vp, table.cuda(), lens, mask="causal", shared_lens=256)
+    clean = call()
+    for p, h, d, x in ((255, 0, 3, inf), (100, 1, 5, -inf), (4, 1, 5, inf), (89, 0, 9, float("nan"))):
+        vp[table[0, p // page], h, p % page, d] = x
+    v = vp[table.cuda().long()].transpose(1, 2).flatten(2, 3)
+    want = _seen_values(clean, v, lens, T, "causal", 4)
+    assert not torch.isfinite(want).all() and _same(call(), want)
