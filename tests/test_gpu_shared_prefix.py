@@ -359,3 +359,22 @@ def test_empty_and_short_sequences_of_many_heads():
     q = randn((7, 700, 1, 64), torch.float16, g)
     got, want = _calls(0, q, kp, vp, table.cuda(), lens.cuda(), None, shared_lens=256)
     assert torch.equal(got, want) and not want[0].any() and want[1].any()
+
+
+def test_slices_behind_a_shared_prefix():
+    """Codes of sequences so wide that they are read back a few at a time: every slice finds the first
+    sequence's pages."""
+    bi, g = _bi(), gen(22)
+    D, page, cols = 256, 256, 1 << 10                    # 2^18 keys: 2 x 128 MiB a head and sequence
+    kp, vp = (random_pool(40, 4, page, D, 8, 64, "bf16", g) for _ in range(2))
+    table = torch.randint(0, 40, (5, cols), generator=g).to(I32)
+    lens = dev([300, 900, 600, 1500, 500])
+    q = randn((5, 16, 280, D), torch.bfloat16, g)
+    given, whole = table.clone(), table.clone()
+    given[2:5, :2] = -1                                   # group of sequences 1 to 4, 700 keys: two whole splits
+    whole[2:5, :2] = table[1, :2]
+    got = bi.batch_invariant_quantized_paged_attention(q, kp, vp, given.cuda(), lens, mask="causal", shared_starts=dev([1, 5]),
+                                                       shared_lens=dev([700]))
+    for b in range(5):
+        want = bi.batch_invariant_quantized_paged_attention(q[b:b + 1], kp, vp, whole[b:b + 1, :6].cuda(), lens[b:b + 1], mask="causal")
+        assert torch.equal(got[b:b + 1], want)
