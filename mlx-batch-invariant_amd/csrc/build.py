@@ -55,11 +55,12 @@ CFLAGS = [
 # tile measured 3-8% slower with it, so the flag stays per file; the fp32
 # attention kernels keep the default (with it one more of them spills).
 #
-# The attention over pages (bi_attn_pages_*) keeps 16-bit kernels of up to 128 dims
-# within 256 registers that way, for two workgroups a CU; split into plain and
-# accumulator registers they spill. Its 192 and 256 dims are sources of their own
-# (bi_attn_pages_wide_*) without the flag: with it the compiler ends with an
-# error on them (ROCm 7.2).
+# The attention over pages, fp32 (bi_attn_pages_f32): the decode kernels of 128 dims
+# take 157 to 168 registers that way and three workgroups a CU, without it 153 to 164
+# and 16 accumulators, two workgroups. Its 16-bit kernels, held to two workgroups a
+# CU or more, use no accumulators either way. 192 and 256 dims are sources of their own
+# (bi_attn_pages_wide_*) without the flag: with it the compiler ends with an error on
+# them (ROCm 7.2).
 #
 # The 4-bit quantized sources use the memory-clause scheduler (device pass
 # only). Its visible change in the decode GEMV is the prologue: every
@@ -75,7 +76,7 @@ _CLAUSE = ["-Xarch_device", "-mllvm=-misched=gcn-max-memory-clause"]
 EXTRA_FLAGS = {
     "bi_attn_bf16": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     "bi_attn_f16": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
-    **{f"bi_attn_pages_{t}": ["-mllvm", "-amdgpu-mfma-vgpr-form"] for t in ("bf16", "f16", "f32")},
+    "bi_attn_pages_f32": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
     **{f"bi_attn_mod_{v}_{t}": ["-mllvm", "-amdgpu-mfma-vgpr-form"]
        for v in ("decode", "rows", "mask", "cap", "bias", "capbias") for t in ("bf16", "f16")},
     "bi_qmm_bf16": _CLAUSE,
