@@ -490,8 +490,9 @@ int bi_read_quantized_cache(const void* k_codes, const void* k_groups, const voi
  * groups > 0: sequences shared_starts[n] .. shared_starts[n + 1] - 1 (device int32
  * [groups + 1], rising; null for one group of all) begin with the same shared_lens[n]
  * keys (device int32 [groups]; null: shared_len for one group). Their whole 256-key
- * splits that the first sequence holds are read from its pages, once for all of the
- * group; a sequence in no group, or alone in one, shares nothing.
+ * splits that the first sequence holds are read from its pages (the others' table
+ * entries there are not read), by calls of few rows once for all of the group; a
+ * sequence in no group, or alone in one, shares nothing.
  * The results are the bits of the plain calls on the same keys (codes: on the rows
  * read back) where q, K and V are finite. Hidden keys take no part whatever their
  * rows hold; a query that sees no key gets zeros; infinities and NaN that a query

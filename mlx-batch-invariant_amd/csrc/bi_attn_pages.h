@@ -272,11 +272,16 @@ struct KRow {
 // rows costs its Q^T, its products and the exchange of maxima and weights. Wave w takes
 // the dims 16 dt, dt = NJ w .. NJ w + NJ - 1, of P.V. (fp32 rows of more than 128 dims: V
 // in two slices, copied for every chunk.) BITS 0: rows of T; 8 or 4: codes.
-// Bound by instructions where many rows share a prefix: a chunk takes a CU about 1.3 us,
-// 48 products a wave (as long as 0.35 us) among some 330 vector instructions and
-// two exchanges; by latency and bytes where they share little. 64 sequences of 32 / 8
-// heads of 128 in bf16 behind 8192 keys, 256 of their own: 63 us with the merge, where
-// every sequence reading its own keys takes 323; without the shared keys 24.
+// Bound by a chunk's chain where many rows share a prefix: it takes a CU about 1.3 us, 48
+// products a wave (as long as 0.35 us) among some 330 vector instructions and two
+// exchanges. 64 sequences behind 8192 keys, up to 512 of their own: 54 us, in which a SIMD
+// issues in 46% of its cycles (vector instructions in 31%), the matrix unit is busy in
+// 11%, and a wave waits for half of its time. By latency and bytes where they share
+// little. 64 sequences of 32 / 8 heads of 128 in bf16 behind 8192 keys, 256 of their own:
+// 63 us with the merge, where every sequence reading its own keys takes 323; without
+// the shared keys 24. Codes that nobody shares take longer here than in attn_codes: 64
+// sequences of up to 8192 keys of their own 269 us in 8 bits and 242 in 4 instead of
+// 150 and 98.
 // Of a second half of the grid that takes its items from the last on, loads beside the
 // others' products, nothing came (57 -> 59 us), nor of waiting for the next rows in front
 // of the stores.
@@ -287,7 +292,9 @@ constexpr int pages_v_slices() {
 }
 // Workgroups per CU that the registers are held to: two where LDS has room for them. (64
 // dims fit three anyway, and held to them are slower, 43 instead of 41 us for 64
-// sequences behind 8192 keys; 32 dims gain, 32 instead of 34.5.)
+// sequences behind 8192 keys; 32 dims gain, 32 instead of 34.5.) Within that only fp32 of
+// 256 dims spills, 36 to 52 registers; scalars, 38 to 156 of them, go to the lanes of
+// vector registers.
 template <typename T, int D>
 constexpr int pages_min_blocks() {
   return sizeof(T) == 4 || D > 128 ? 1 : D > 32 ? 2 : 3;
@@ -666,12 +673,15 @@ __global__ __launch_bounds__(256, (pages_min_blocks<T, D>())) void attn_pages(Pa
 // registers. For P.V wave w takes the dims 16 dt, dt = NJ w .. NJ w + NJ - 1: a
 // transposing LDS read gives a lane the codes of 8 keys (4 bits: 16) of one dim, and
 // each is dequantized once, with its key's pair from LDS.
-// Bound by bytes at 8 bits, by bytes and vector instructions at 4 (an fma, half a
-// rounding pair and some cutting for every value, most of a step's instructions): 64
-// sequences of up to 8192 keys, 32 / 8 heads of 128: 139 to 160 us on different cards for
-// 8 bits in bf16 (572 MB; a copy takes 112), 92 to 100 for 4 bits in fp16 (303 MB, 59).
+// Bound by bytes and latency at 8 bits (a SIMD issues in 66% of its cycles, vector
+// instructions in 48%), by issue at 4 (89% and 63%: an fma, half a rounding pair and some
+// cutting for every value, most of a step's instructions): 64 sequences of up to 8192
+// keys, 32 / 8 heads of 128: 150 us for 8 bits in bf16 (572 MB; a copy takes 112), 98 for 4
+// bits in fp16 (303 MB, 59); cards differ, up to 163 and 111. fp32, 8 bits: 251 (606 MB, 119).
 // Nothing that follows from the lane alone is kept over the items: at 128 registers it
-// goes to scratch memory, and reading it back waits for every copy in flight (97 us).
+// goes to scratch memory, and reading it back waits for every copy in flight (110 instead
+// of 98 us). What is left there, 8 to 12 bytes a lane, is used in rare paths; scalars, 53
+// to 120, go to the lanes of vector registers.
 // Codes converted before they go to LDS took 500 and 459, the next item's codes
 // requested an item ahead, with two workgroups a CU for the registers, 176 and 136.
 // ---------------------------------------------------------------------------

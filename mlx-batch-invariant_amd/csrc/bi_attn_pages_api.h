@@ -52,6 +52,11 @@ int launch_pages(const PagesArgs& a, int bits, hipStream_t st);
 //    sequences are not so few that the others would split their keys too: 32 sequences
 //    67 / 91, 16 in 4 groups 47 / 53, 8 in 2 groups 41 / 37; of 2 chunks 101 / 90.
 //    (fp32: 158 / 147.)
+// It holds for other heads and lengths: codes of 14 / 2 heads of 64, 4000 keys, 56 rows, 32
+// sequences 31 / 69; 8 / 8 of 128, 4000 keys, 16 sequences, 32 rows 45 / 124, 64 rows 62 / 118; 32 / 8
+// of 128, 32768 keys, 16 sequences, 32 rows 239 / 1022; 16-bit rows of 16, 32 sequences in 4 groups
+// behind 256 keys 28 / 38 and behind 8192 100 / 264, 8 / 8 heads behind 2048 43 / 90; of 64 rows, 64
+// sequences in one group behind 8192, 620 / 289.
 inline bool pages_few_rows(int64_t B, int64_t Hq, int64_t Hkv, int64_t Tq, int64_t L, int64_t D, int64_t groups, int bits,
                            int causal, int dtype) {
   if (Tq == 1 || few_rows(B, Hq, Hkv, Tq, L, D, causal, dtype)) return true;

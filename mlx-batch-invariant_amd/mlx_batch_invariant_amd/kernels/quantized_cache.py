@@ -16,7 +16,8 @@ invariances of kernels/attention.py hold over a quantized cache too.
 
 Sequences of a batch that begin with the same keys (an instruction, a document) may
 say so: ``shared_lens`` and ``shared_starts``. The 256-key splits of the shared keys
-are then read once for the rows of the whole group, with the same bits as without.
+are then those of the first sequence's pages, with the same bits as without, and calls
+of few rows read them once for the whole group.
 
 The reference quantizes weights only (mlx_batch_invariant/kernels/quantized.py:33-67)
 and reads one contiguous cache for each sequence (kernels/attention.py:87-254).
@@ -314,7 +315,10 @@ def batch_invariant_quantized_paged_attention(q: torch.Tensor, k_pages: Quantize
     one sequence).
 
     ``shared_lens`` / ``shared_starts``: as in ``batch_invariant_shared_prefix_attention``
-    (None: no sequence shares its prefix).
+    (None: no sequence shares its prefix). Read once where the codes are read, up to 64
+    rows. Own keys take longer then: 64 sequences of up to 8192 keys of which none is
+    shared 269 us instead of 150 in 8 bits, 242 instead of 98 in 4, so give them for
+    prefixes that are long beside what follows.
     """
     what = "batch_invariant_quantized_paged_attention"
     if q.ndim != 4:
@@ -330,8 +334,12 @@ def batch_invariant_quantized_paged_attention(q: torch.Tensor, k_pages: Quantize
 def batch_invariant_shared_prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torch.Tensor,
                                             block_table: torch.Tensor, kv_lens=None, *, shared_lens,
                                             shared_starts=None, scale: float | None = None, mask=None) -> torch.Tensor:
-    """``batch_invariant_paged_attention`` for sequences that share long prefixes,
-    which are read once for all of them; the same bits where q, K and V are finite.
+    """``batch_invariant_paged_attention`` for sequences that share long prefixes; the
+    same bits where q, K and V are finite. Single tokens read a prefix once for all
+    of its group; so do the few rows (tokens x query heads of a kv head) of chunks whose
+    batch does not fill the GPU otherwise, and up to 16 of them in 16-bit types with four sequences
+    or more a group and 128 (sequence, kv head) pairs in the batch. Calls of more rows
+    read it for every 64 rows of a sequence, from the first sequence's pages too.
 
     ``shared_lens`` int32 ``[N]`` and ``shared_starts`` int32 ``[N + 1]``, rising:
     sequences ``shared_starts[n]`` .. ``shared_starts[n + 1] - 1`` begin with the same
@@ -339,7 +347,9 @@ def batch_invariant_shared_prefix_attention(q: torch.Tensor, k_pages: torch.Tens
     whole batch. The whole 256-key splits of those keys, as far as the first sequence
     of the group holds them, come from that sequence's pages (the others' table
     entries there are not read), everything else from each sequence's own. Lengths
-    and starts are read on the GPU, so one captured graph serves changing groups.
+    and starts are read on the GPU, so one captured graph serves changing groups. Calls
+    of many rows over pages of more than 256 keys need K and V pools whose page and row
+    strides have one ratio, as pools of one layout have.
 
     The other arguments are those of ``batch_invariant_paged_attention``: pools
     ``[num_pages, Hkv, page_size, D]`` of q's type with contiguous rows at strides of
