@@ -378,3 +378,16 @@ def test_slices_behind_a_shared_prefix():
     for b in range(5):
         want = bi.batch_invariant_quantized_paged_attention(q[b:b + 1], kp, vp, whole[b:b + 1, :6].cuda(), lens[b:b + 1], mask="causal")
         assert torch.equal(got[b:b + 1], want)
+
+
+@pytest.mark.parametrize("B,groups,Hq,Hkv", [(300, 100, 4, 2), (600, 2, 64, 4), (64, 64, 8, 8)])
+def test_one_split_of_many_sequences(B, groups, Hq, Hkv):
+    """One split: plans that a launch of its own makes, items of several chunks, groups of one."""
+    sizes = [B // groups] * groups
+    g = torch.Generator().manual_seed(B)
+    lens = torch.randint(0, 257, (B,), generator=g)
+    lens[::max(sizes[0], 1)] = 256                        # first sequences hold the split, but for some
+    lens[sizes[0] * (groups // 2)] = 255
+    shared = [256] * groups
+    _check_sources("bf16", 0, Hq, Hkv, 32, 1, 16, sizes, shared, lens.tolist(), "causal", B)
+    _check_sources("f16", 8, Hq, Hkv, 64, 2, 64, sizes, shared, lens.tolist(), "causal", B + 1)
